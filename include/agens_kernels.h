@@ -241,6 +241,58 @@ int ak_wq_chain_chained(void* chain); /* 1: runs as one chained launch, 0: one l
 int ak_wq_chain_destroy(void* chain);
 int ak_wq_chain_status(void);
 
+/* ---------------------------------------------------------------------------------------------- paged key-value cache
+ * No counterpart in the reference's quantized path: what a decode step has between its linears.  A cache is one pool of
+ * `npages` pages of `page` token slots (16, 32, 64, 128 or 256) for `heads` key-value heads of `dim` values (64, 128 or
+ * 256), at `bits` = 16 (bf16), 8 or 4 per value.  A page is ak_kv_page_bytes() long (0: a shape that is refused):
+ *   rows   [head][keys, values][slot] of dim * bits / 8 bytes (8 bits: bytes q + 128; 4 bits: nibbles q + 8, even one low);
+ *   scales [head][slot] pairs of bf16 (keys, values), one per token and head (not at 16 bits); padded to 128 bytes.
+ * Slot s is slot s % page of page s / page.  The value held is q * s with s = bf16(max|x| / Q) and q = rint(x / s) clamped to
+ * +-Q, Q = 127 or 7; a row whose s is below 2^-126 is held as zeros; a row with a NaN or Inf reads back as NaN (quantised).
+ *   ak_kv_write  keys and values of m tokens (bf16, token t at k + t * ldk, heads contiguous; 16-byte aligned, ldk and ldv
+ *                multiples of 8) into slots[t] (device memory).  A slot outside the pool is skipped; two tokens with one
+ *                slot leave either of them;
+ *   ak_kv_read   the converse, bf16(q * s); zeros for a slot outside the pool.  ldk, ldv >= heads * dim.
+ * m = 0 does nothing.  Both are one launch, allocate nothing and can be captured. */
+size_t ak_kv_page_bytes(int bits, int page, int heads, int dim);
+int ak_kv_write(int bits, const void* k, const void* v, int m, long ldk, long ldv, const int* slots, void* pool,
+                int npages, int page, int heads, int dim, void* stream);
+int ak_kv_read(int bits, const void* pool, int npages, int page, int heads, int dim, const int* slots, int m, void* k,
+               void* v, long ldk, long ldv, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- attention over the cache
+ * Attention of the newest tokens of b sequences over their pages.  q and y bf16 [m][heads * dim] (token stride ldq / ldy,
+ * multiples of 8; 16-byte aligned), heads a multiple of kv_heads (query head h reads key-value head h / (heads /
+ * kv_heads)).  Sequence i has the tokens [qstart[i], qstart[i + 1]) of q (qstart NULL: m / b each), lens[i] tokens in the
+ * cache, these new ones included as its last (written before the call), and the pages table[i * ldt ...].  Token t of T sees
+ * the cached tokens before len - T + t + 1 -- itself the last -- except those of pages outside the pool, which count
+ * as not there (a freed page's entry may be -1); lengths past the table's ldt pages end there.  y = softmax(scale * q . k) v
+ * in fp32, rounded once; a row that sees nothing is 0.  lse (may be NULL): fp32 [m][heads], the natural log of the sum of
+ * exponentials (-inf for such a row), to join with attention over other keys.  Tokens of q in no sequence's range are left
+ * alone.  qstart, lens and table are device memory, read by the launch: a captured call follows them from replay to
+ * replay.  Values at slots past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS. */
+#define AK_ATTN_MAX_SEQS 4096
+int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, int npages, int page, int heads,
+                  int kv_heads, int dim, int b, const int* qstart, const int* lens, const int* table, int ldt, float scale,
+                  void* y, long ldy, float* lse, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- verification of drafts
+ * Speculative sampling of b sequences with up to t drafted tokens each: target logits bf16 [b][t + 1][ldt] (row j: after j
+ * drafts), draft logits bf16 [b][t][ldd] of the model that drew the drafts, or NULL for drafts that were not drawn at random
+ * (looked up, or a greedy draft), ids [b][t] the drafts, counts [b] how many each sequence has (NULL: t), u fp32 [b][t + 1]
+ * uniform in [0, 1), temperature fp32 [b] (NULL: 1; 0 or less: greedy), all in device memory.  Draft j is accepted while
+ * u[j] q(x) < p(x), p = softmax(target / temperature), q likewise of the draft (NULL: 1 on x); the next token comes from
+ * max(p - q, 0) after a rejection, else from p, by the inverse of its cumulative sum at u[t]; greedy: from the largest
+ * logit, the lowest token among equal ones.  With t = 0 this draws one token from p.
+ *   tokens [b][t + 1]: the accepted drafts, the next token, then -1;  accepted [b]: how many drafts;
+ *   logp (may be NULL) fp32 [b][t + 1]: log p of each of these tokens (greedy: at temperature 1), 0 where there is none.
+ * NaN logits count as -inf; a row of nothing else rejects its draft and gives the token -1.  Weights are computed in fp32,
+ * their sums in 64 bits in an order that does not depend on b. */
+#define AK_VERIFY_MAX_DRAFTS 127
+int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, const int* ids, const int* counts,
+                   const float* u, const float* temperature, int b, int t, int vocab, int* tokens, int* accepted,
+                   float* logp, void* stream);
+
 /* ---------------------------------------------------------------------------------------------- switches
  * reference: agens_kernels.h:205 / :208 / :211, w4_gemv.cu:3271-3282.  mma: -1 auto (environment AGENS_W4_EXACT), 0 exact
  * fp32 path, 1 default integer-MFMA path.  lean / tma select bit-identical sm90-only variants in the reference;
