@@ -271,7 +271,7 @@ int ak_kv_read(int bits, const void* pool, int npages, int page, int heads, int 
  * exponentials (-inf for such a row), to join with attention over other keys.  Tokens of q in no sequence's range are left
  * alone.  qstart, lens and table are device memory, read by the launch: a captured call follows them from replay to
  * replay.  Values at slots past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS. */
-#define AK_ATTN_MAX_SEQS 4096
+#define AK_ATTN_MAX_SEQS 1024
 int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, int npages, int page, int heads,
                   int kv_heads, int dim, int b, const int* qstart, const int* lens, const int* table, int ldt, float scale,
                   void* y, long ldy, float* lse, void* stream);
