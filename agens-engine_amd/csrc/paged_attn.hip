@@ -5,35 +5,35 @@
 // over the cached tokens j < len - T + t + 1 whose page is held.  exp is taken as exp2 of z * log2(e).
 //
 // Bound by the bytes of the cache: every one is needed once, a few flops each.  So the rows that share a key-value head (its
-// query heads, times the new tokens) are the columns of one MFMA (tiles of 16 rows), and the cached tokens stream:
-//   * a wave takes TPW tokens at a time into registers: S = K Q^T (keys as the A operand: the lane's 16-byte load is a
-//     piece of a row, any split of the row's values over lanes and steps does, so long as the queries are laid out by the
-//     same), the softmax of the running maximum, then O^T += V^T P^T.  The scores leave the first product with the row in
-//     the lane and four tokens in its registers, which is how the second takes its B operand when the tokens of 32 are
-//     numbered accordingly: the weights never change lanes.  The values are loaded as whole row pieces too, and
-//     transposed in the lane: a lane holds eight tokens' pieces of the same values, and pairs of tokens are what a
-//     register of the A operand is;
-//   * eight waves side by side make a chunk, kChunks chunks a part, whose sums the waves then add in LDS in wave order; a
-//     workgroup takes parts from a list over all sequences and heads, the next chunk's loads in flight from the moment
-//     the registers are free.
+// query heads, times the new tokens) are the columns of one MFMA (tiles of 16 rows), and the cached tokens stream through
+// waves that work alone, without LDS exchange or barriers (a workgroup's waves that meet after every few hundred tokens to
+// add up load at once and compute at once, and the memory idles in between: 15 to 30 % of the time):
+//   * a wave takes a chunk of TPW tokens at a time into registers: S = K Q^T (keys as the A operand: the lane's 16-byte load
+//     is a piece of a row, any split of the row's values over lanes and steps does, so long as the queries are laid out by
+//     the same), the softmax of the running maximum, then O^T += V^T P^T.  The scores leave the first product with the row
+//     in the lane and four tokens in its registers, which is how the second takes its B operand when the tokens of 32 are
+//     numbered accordingly: the weights never change lanes.  The values are loaded as whole row pieces too, and transposed
+//     in the lane: a lane holds eight tokens' pieces of the same values, and pairs of tokens are what a register of the A
+//     operand is;
+//   * the next chunk's keys are loaded as soon as the scores are done with theirs, the values likewise.
 //
-// Order of summation.  What a row gives depends on its own tokens only, never on the call: parts lie at fixed places of
-// the sequence, parts are added left to right into blocks of BLOCK parts, blocks left to right; a chunk or part in which a
+// Order of summation.  What a row gives depends on its own tokens only, never on the call: tokens lie in parts of 128, added
+// left to right into blocks of 8 parts, these into groups of 16 blocks, and these left to right; a chunk or part in which a
 // row sees nothing adds an exact nothing.  So T tokens verified in one call have the bits of T one-token calls, in any
-// batch.  Who adds is free: workgroups that hold one part each write it to scratch and the last to arrive adds them
-// (split 0); a workgroup that holds a whole block adds in LDS (split 1), and so does one that holds a whole sequence's
-// head (split 2, which needs no scratch).
+// batch.  Who adds is free (AttnSplit): a wave takes a block and writes its sums, or a part where blocks are too few to keep
+// the memory busy, and a second small kernel adds up; or, where there is no scratch for that, a wave takes a sequence's head.
 #include "agens_kernels.h"
 #include "kv_page.h"
 
 namespace agq {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;
-constexpr int kTable = 64;      // work items known ahead
-constexpr float kEven = 1.1f;   // the longest workgroup's tokens over the average's, for whole sequences
-constexpr int kNowhere = 0x7FFFFF00;  // an offset past any scratch
-constexpr size_t kMaxPartialBytes = (size_t)128 << 20;
+constexpr int kWaves = 4, kThreads = 64 * kWaves;  // of a workgroup; two of them on a CU
+constexpr int kPart = 128, kBlock = 8, kGroup = 16;  // tokens of a part, parts of a block, blocks of a group
+constexpr int kTable = 64;                           // work items that a wave knows ahead
+constexpr size_t kMaxPartialBytes = (size_t)240 << 20;
+
+enum AttnSplit { kByPart, kByBlock, kByHead };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -41,7 +41,6 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct AttnArgs {
   KvShape s;
@@ -51,34 +50,21 @@ struct AttnArgs {
   const uint8_t* pool;
   const int *qstart, *lens, *table;
   long ldq, ldy;
-  int m, tq, b, heads, g, ldt;      // tq: tokens of a sequence without qstart
-  uint32_t g_inv;                   // 2^32 / g, rounded up
+  int m, tq, b, heads, g, ldt;  // tq: tokens of a sequence without qstart
+  uint32_t g_inv;               // 2^32 / g, rounded up
   int page_log2;
   size_t page_bytes, scale_off;
   float scale;
   float* part;  // partial rows: of each D sums, then of each its largest score and sum of weights; then the plan
   int cap;      // that fit
+  int few;      // blocks, below which parts are the work items
 };
-
-// waves of a SIMD
-constexpr int simd_waves(int bits, int d, int nt) { return 2; }
 
 template <int BITS, int D>
 struct Geo {
   static constexpr int RB = D * BITS / 8;                // bytes of a row
-  static constexpr int TPW = BITS == 16 ? (D == 64 ? 64 : 32) : BITS == 8 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;
-  static constexpr int CHUNK = kWaves * TPW;
-  // Parts: four of 256 tokens, so that a short context has some to share out, then of 1024; blocks of 16 parts.
-  static constexpr int PART = 1024, FIRST = 256, FIRSTS = PART / FIRST, BLOCK = 16;
-  static constexpr int kChunks = PART / CHUNK, kFirstChunks = FIRST / CHUNK;
-  static_assert(kFirstChunks >= 1, "");
-  static __host__ __device__ int parts(int len) {  // of len tokens, at least one
-    return len > PART ? FIRSTS + (len - 1) / PART : len > FIRST ? (len + FIRST - 1) / FIRST : 1;
-  }
-  static __device__ __forceinline__ int start(int part) { return part < FIRSTS ? part * FIRST : (part - FIRSTS + 1) * PART; }
-  static __device__ __forceinline__ int chunks(int part) { return part < FIRSTS ? kFirstChunks : kChunks; }
-  static constexpr int NS = TPW / 16, NG = TPW / 32;     // subtiles of 16 tokens, groups of 32
-  static_assert(NS * kChunks <= 64, "");                 // a lane for every subtile of a wave's part
+  static constexpr int TPW = BITS == 16 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;  // tokens of a chunk
+  static constexpr int NS = TPW / 16, NG = TPW / 32;     // its subtiles of 16 tokens, groups of 32
   static constexpr int STEPS = D / 32;                   // MFMAs of a subtile's scores
   static constexpr int KLB = RB >= 64 ? 16 : 8;          // bytes of a key load
   static constexpr int KL = RB / (4 * KLB), KW = KL * KLB / 4;
@@ -86,9 +72,6 @@ struct Geo {
   static constexpr int CH = D / 16;                      // values of a lane's piece of a value row
   static constexpr int VB = RB / 16, VW = VB >= 4 ? VB / 4 : 1;
   static constexpr int kOff = BITS == 8 ? 128 : 24;      // offset of the key codes as the scores' products see them
-  static constexpr int kPasses = D == 256 ? 4 : D == 128 ? 2 : 1;  // in which a tile's sums go through LDS
-  static constexpr int LD = D / kPasses + 4;             // of the LDS rows: the 16 rows of a tile on different banks
-  static constexpr int kSums = kWaves * 16 * LD + 2 * 16 * kWaves;  // floats
   // element j of lane group g4's eight of 32 tokens: the numbering in which the scores leave their product
   static __device__ __forceinline__ int token(int j, int g4) { return (j < 4 ? j : 12 + j) + 4 * g4; }
   // first of the 8 values that lane group g4 contributes to step s
@@ -209,29 +192,37 @@ __device__ __forceinline__ int scan64(int x) {
   return x;
 }
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// a barrier for what is in LDS: it does not wait for global loads in flight
-__device__ __forceinline__ void block_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+// order among a wave's accesses to LDS
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 }
 // a load of the scalar unit: it does not wait for the vector loads in flight
 __device__ __forceinline__ int scalar_load(const int* p) {
   return *(const __attribute__((address_space(4))) int*)(uintptr_t)p;
 }
 
-// A row's running state: largest score (in units of log2), sum of weights, and four of the weighted sums of values.
+__device__ __forceinline__ int parts_of(int len) { return len > kPart ? (len + kPart - 1) / kPart : 1; }
+
+// What two sums are worth side by side: the larger score, and the factors of the first's and the second's sums.
+struct Fold {
+  float m, a, b;
+  __device__ __forceinline__ Fold(float m1, float m2) {
+    m = fmaxf(m1, m2);
+    a = m1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m1 - m);
+    b = m2 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m2 - m);
+  }
+  __device__ __forceinline__ float operator()(float x, float y) const { return fmaf(y, b, x * a); }
+};
+
+// Four values of a row's sums, its largest score (in units of log2) and its sum of weights.
 struct Sums {
   float m = -INFINITY, l = 0.0f;
   float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
   __device__ __forceinline__ void add(const Sums& p) {
-    const float mn = fmaxf(m, p.m);
-    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float b = p.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p.m - mn);
-    l = fmaf(p.l, b, l * a);
+    const Fold f(m, p.m);
+    m = f.m, l = f(l, p.l);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = fmaf(p.o[i], b, o[i] * a);
-    m = mn;
+    for (int i = 0; i < 4; ++i) o[i] = f(o[i], p.o[i]);
   }
 };
 
@@ -239,56 +230,42 @@ struct Sums {
 __device__ __forceinline__ int first_token(const AttnArgs& a, int seq) {
   return a.qstart ? min(max(scalar_load(a.qstart + seq), 0), a.m) : seq * a.tq;
 }
-// a finished row's four values, and its lse
-template <int D>
-__device__ __forceinline__ void finish_row(const AttnArgs& a, const Sums& s, int q0, int head, int row, int c4) {
-  const int t = div_g(a, row), h = head * a.g + row - t * a.g;
-  const size_t tok = (size_t)(q0 + t);
-  const float inv = 1.0f / s.l;
-  uint2 y = make_uint2(0u, 0u);
-  if (s.l != 0.0f) {
-    y.x = (uint32_t)f2bf(s.o[0] * inv) | ((uint32_t)f2bf(s.o[1] * inv) << 16);
-    y.y = (uint32_t)f2bf(s.o[2] * inv) | ((uint32_t)f2bf(s.o[3] * inv) << 16);
-  }
-  *reinterpret_cast<uint2*>(a.y + tok * a.ldy + (size_t)h * D + 4 * c4) = y;
-  if (a.lse && c4 == 0)
-    a.lse[tok * a.heads + h] = s.l == 0.0f ? -INFINITY : (s.m + __log2f(s.l)) * 0.69314718055994531f;
+// where a row of a (sequence, head) goes: its token and query head
+__device__ __forceinline__ void row_place(const AttnArgs& a, int q0, int head, int row, size_t* tok, int* h) {
+  const int t = div_g(a, row);
+  *tok = (size_t)(q0 + t);
+  *h = head * a.g + row - t * a.g;
+}
+__device__ __forceinline__ float row_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
-// What every workgroup works out alike about the launch's sequences: the work list, and where partial rows and counters
-// lie.  The arrays are in LDS, indexed by sequence; the first two are sums over the sequences before.
+// What every workgroup works out alike about the call's sequences: the work list, and where partial rows lie.  The arrays
+// are in LDS, indexed by sequence; the first two are sums over the sequences before.
 struct Plan {
   int *items, *rows;  // work items of one head; partial rows of all heads
-  int *len, *tok;            // cached tokens and new tokens
-  int split, total;          // parts are the work items (0) or sequences' heads (1); of all heads
+  int *len, *tok;     // cached tokens and new tokens
+  int split, total;   // an AttnSplit; work items of all heads
 };
 
-struct Seq {
-  int len, tok, parts, rbs;  // rbs: row blocks
-};
-
-template <class G, int NT>
-__device__ __forceinline__ Seq seq_shape(const AttnArgs& a, int len, int tok) {
-  Seq s;
-  s.len = len;
-  s.tok = tok;
-  s.parts = G::parts(len);
-  const int tiles = (tok * a.g + 15) / 16;
-  s.rbs = (tiles + NT - 1) / NT;
-  return s;
+__device__ __forceinline__ int seq_tiles(const AttnArgs& a, int tok) { return (tok * a.g + 15) >> 4; }
+// pieces that a sequence's head is split into
+__device__ __forceinline__ int seq_pieces(int len, int split) {
+  const int p = parts_of(len);
+  return split == kByPart ? p : split == kByBlock ? (p + kBlock - 1) / kBlock : 1;
 }
-__device__ __forceinline__ int seq_items(const Seq& s, int split) { return s.rbs * (split ? 1 : s.parts); }
-// Partial rows of one head.  (No more than kTooMany are told apart: it is more
-// than fits, and the sums over all sequences stay in 32 bits.)
+// Partial rows of one head.  (No more than kTooMany are told apart: it is more than fits, and the sums over all sequences
+// stay in 32 bits.)
 constexpr int kTooMany = 1 << 20;
 static_assert((long)kTooMany * AK_ATTN_MAX_SEQS < (1l << 31), "");
-__device__ __forceinline__ int seq_rows(const Seq& s, int split, int g) {
-  if (split || s.parts == 1) return 0;
-  return (float)s.tok * (float)g * (float)s.parts >= (float)kTooMany ? kTooMany : s.tok * g * s.parts;
+__device__ __forceinline__ int seq_rows(const AttnArgs& a, int len, int tok, int split) {
+  const int n = seq_pieces(len, split);
+  if (n == 1) return 0;
+  return (float)tok * (float)a.g * (float)n >= (float)kTooMany ? kTooMany : tok * a.g * n;
 }
 
-// Every wave works the plan out, a lane for one sequence or a few in a row.
-template <class G, int NT>
+// Every wave works the plan out, a lane for one sequence or a few in a row.  Blocks are the work items unless they are fewer
+// than `few` and parts fit; heads are where neither fits.
 __device__ __forceinline__ void make_plan(const AttnArgs& a, Plan& p, int* mem) {
   const int lane = threadIdx.x & 63;
   p.items = mem;
@@ -296,74 +273,63 @@ __device__ __forceinline__ void make_plan(const AttnArgs& a, Plan& p, int* mem) 
   p.len = mem + 2 * a.b;
   p.tok = mem + 3 * a.b;
   const int each = (a.b + 63) >> 6, lo = min(a.b, lane * each), hi = min(a.b, lo + each);
-  const bool writes = threadIdx.x < 64;
   int len = -1, tok = 0;
-  auto shape = [&](int i) __attribute__((always_inline)) {
-    if (each > 1 || len < 0) {  // (one sequence a lane stays in registers)
-      tok = a.tq;
-      if (a.qstart) {
-        const int q0 = min(max(a.qstart[i], 0), a.m);
-        tok = min(max(a.qstart[i + 1], q0), a.m) - q0;
-      }
-      len = (int)min((long)max(a.lens[i], 0), (long)a.ldt << a.page_log2);
+  auto load = [&](int i) __attribute__((always_inline)) {
+    if (each == 1 && len >= 0) return;  // (one sequence a lane stays in registers)
+    tok = a.tq;
+    if (a.qstart) {
+      const int q0 = min(max(a.qstart[i], 0), a.m);
+      tok = min(max(a.qstart[i + 1], q0), a.m) - q0;
     }
-    return seq_shape<G, NT>(a, len, tok);
+    len = (int)min((long)max(a.lens[i], 0), min((long)a.ldt << a.page_log2, 0x7FFFF000l));
   };
-  int split = 0;
-  for (;; ++split) {
-    int mine[2] = {0, 0};
+  const float kv = (float)a.s.heads;
+  float fits[2], blocks = 0.0f;
+#pragma unroll
+  for (int split = 0; split < 2; ++split) {
+    int rows = 0, items = 0;
     for (int i = lo; i < hi; ++i) {
-      const Seq s = shape(i);
-      mine[0] += seq_items(s, split);
-      mine[1] = min(mine[1] + seq_rows(s, split, a.g), kTooMany);
+      load(i);
+      rows = min(rows + seq_rows(a, len, tok, split), kTooMany);
+      items = min(items + seq_tiles(a, tok) * seq_pieces(len, split), kTooMany);
     }
-    int at[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) at[i] = scan64(mine[i]);
-    const int all = __builtin_amdgcn_readlane(at[0], 63);
-    const float kv = (float)a.s.heads, rows = (float)__builtin_amdgcn_readlane(at[1], 63) * kv;
-    if (!split) {
-      if (rows > (float)a.cap) continue;
-      // whole sequences also where that keeps all workgroups busy to the end, nearly
-      int units = 0, most = 0;
-      float sum = 0.0f;
-      for (int i = lo; i < hi; ++i) {
-        const Seq s = shape(i);
-        units += s.rbs, most = max(most, s.rbs ? s.len : 0), sum += (float)s.rbs * (float)s.len;
-      }
-      units = __builtin_amdgcn_readlane(scan64(units), 63) * a.s.heads;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) most = max(most, __shfl_xor(most, d)), sum += __shfl_xor(sum, d);
-      const int turns = (units + (int)gridDim.x - 1) / (int)gridDim.x;
-      if (units >= (int)gridDim.x && (float)turns * (float)most * (float)gridDim.x <= kEven * sum * kv) continue;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) at[i] -= mine[i];
-    for (int i = lo; writes && i < hi; ++i) {
-      const Seq s = shape(i);
+    fits[split] = (float)__builtin_amdgcn_readlane(scan64(rows), 63) * kv;
+    blocks = (float)__builtin_amdgcn_readlane(scan64(items), 63) * kv;
+  }
+  const float cap = (float)a.cap;
+  p.split = fits[kByPart] <= cap && blocks < (float)a.few ? kByPart : fits[kByBlock] <= cap ? kByBlock : kByHead;
+  int mine[2] = {0, 0};
+  for (int i = lo; i < hi; ++i) {
+    load(i);
+    mine[0] += seq_tiles(a, tok) * seq_pieces(len, p.split);
+    mine[1] += seq_rows(a, len, tok, p.split);
+  }
+  int at[2] = {scan64(mine[0]), scan64(mine[1])};
+  p.total = __builtin_amdgcn_readlane(at[0], 63) * a.s.heads;
+  at[0] -= mine[0], at[1] -= mine[1];
+  if (threadIdx.x < 64)
+    for (int i = lo; i < hi; ++i) {
+      load(i);
       p.items[i] = at[0], p.rows[i] = at[1] * a.s.heads;
       p.len[i] = len, p.tok[i] = tok;
-      at[0] += seq_items(s, split);
-      at[1] += seq_rows(s, split, a.g);
+      at[0] += seq_tiles(a, tok) * seq_pieces(len, p.split);
+      at[1] += seq_rows(a, len, tok, p.split);
     }
-    p.split = split;
-    p.total = all * a.s.heads;
-    break;
-  }
-  block_sync();
+  __syncthreads();
 }
 
-// One step of a workgroup: a part of a work item.  All of it uniform.
-struct Step {
-  int k, seq, head, rb, part, end, len, tok;  // the workgroup's item k; its parts end at `end` (0: no such item)
+// A wave's work item: pieces [part, end) of parts of a sequence's head, for a tile of 16 rows.  All of it uniform; end 0: no
+// such item.
+struct Item {
+  int k, seq, head, tile, part, end, len, tok;
 };
 
-// Items k .. k + n - 1 of the workgroup into the table, a lane each.
-template <class G, int NT>
-__device__ __forceinline__ void fill_table(const AttnArgs& a, const Plan& p, int* table, int k, int n) {
-  if ((int)threadIdx.x >= n) return;
-  k += (int)threadIdx.x;
-  const long item = (long)blockIdx.x + (long)k * gridDim.x;
+// The wave's items k .. k + 63 into its table, a lane each.
+__device__ __forceinline__ void fill_table(const AttnArgs& a, const Plan& p, int* table, int k, int n, int wave, int waves) {
+  const int lane = threadIdx.x & 63;
+  if (lane >= n) return;
+  k += lane;
+  const long item = (long)wave + (long)k * waves;
   int* const e = table + (k & (kTable - 1)) * 8;
   e[3] = 0;
   if (item >= p.total) return;
@@ -375,25 +341,26 @@ __device__ __forceinline__ void fill_table(const AttnArgs& a, const Plan& p, int
     lo = up ? mid : lo;
     hi = up ? hi : mid;
   }
-  const Seq q = seq_shape<G, NT>(a, p.len[lo], p.tok[lo]);
-  const int rem = at - p.items[lo], u = rem / q.rbs;
+  const int len = p.len[lo], tok = p.tok[lo], tiles = seq_tiles(a, tok), parts = parts_of(len);
+  const int rem = at - p.items[lo], u = rem / tiles;
+  const int per = p.split == kByPart ? 1 : p.split == kByBlock ? kBlock : parts;
   e[0] = lo;
   e[1] = (int)item - at * a.s.heads;
-  e[2] = rem - u * q.rbs;
-  e[3] = p.split ? q.parts : u + 1;
-  e[4] = u;
-  e[5] = q.len;
-  e[6] = q.tok;
+  e[2] = rem - u * tiles;
+  e[3] = min(parts, (u + 1) * per);
+  e[4] = u * per;
+  e[5] = len;
+  e[6] = tok;
 }
-__device__ __forceinline__ void read_step(const int* table, int k, Step& s) {
+__device__ __forceinline__ void read_item(const int* table, int k, Item& s) {
   const int4* const e = reinterpret_cast<const int4*>(table + (k & (kTable - 1)) * 8);
   const int4 x = e[0], y = e[1];
   s.k = k;
-  s.seq = uni(x.x), s.head = uni(x.y), s.rb = uni(x.z), s.end = uni(x.w);
+  s.seq = uni(x.x), s.head = uni(x.y), s.tile = uni(x.z), s.end = uni(x.w);
   s.part = uni(y.x), s.len = uni(y.y), s.tok = uni(y.z);
 }
 
-// A wave's share of a chunk, as it comes from memory.
+// A chunk, as it comes from memory.
 template <int BITS, int D>
 struct Tokens {
   using G = Geo<BITS, D>;
@@ -402,18 +369,18 @@ struct Tokens {
   const uint8_t* base[G::NS];  // page of each subtile
   uint32_t dead;               // subtiles without tokens or page
 
-  // lane i of the result: the page of the wave's subtile i of a part (-1: no tokens there)
-  static __device__ __forceinline__ int load_ids(const AttnArgs& a, const Step& s, int w, int lane) {
-    const int tok = G::start(s.part) + lane / G::NS * G::CHUNK + w * G::TPW + 16 * (lane % G::NS);
+  // lane i of the result: the page of subtile i from token `first` on (-1: no tokens there)
+  static __device__ __forceinline__ int load_ids(const AttnArgs& a, const Item& s, int first, int lane) {
+    const int tok = first + 16 * lane;
     int id = -1;
-    if (lane < G::NS * G::chunks(s.part) && tok < s.len) id = a.table[(size_t)s.seq * a.ldt + (tok >> a.page_log2)];
+    if (tok < min(s.len, s.end * kPart)) id = a.table[(size_t)s.seq * a.ldt + (tok >> a.page_log2)];
     return id;
   }
-  __device__ __forceinline__ void find(const AttnArgs& a, int ids, int chunk) {
+  __device__ __forceinline__ void find(const AttnArgs& a, int ids, int subtile) {
     dead = 0;
 #pragma unroll
     for (int i = 0; i < G::NS; ++i) {
-      int pg = __builtin_amdgcn_readlane(ids, chunk * G::NS + i);
+      int pg = __builtin_amdgcn_readlane(ids, subtile + i);
       if ((unsigned)pg >= (unsigned)a.s.npages) dead |= 1u << i, pg = 0;  // (page 0 is there to be read)
       base[i] = a.pool + a.page_bytes * (uint32_t)pg;
     }
@@ -453,7 +420,7 @@ struct Tokens {
 // Adds the non-finite values (bf16) of the 32 tokens from `first` on that the sequence's first new token does not see, one
 // token at a time, to the rows that see it.  Rare, so the values are read again rather than kept.
 template <int D>
-__device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Step& s, int first, const u32x4 p, int limit,
+__device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s, int first, const u32x4 p, int limit,
                                                int lane, f32x4 (&o)[Geo<16, D>::CH]) {
   using G = Geo<16, D>;
 #pragma unroll 1
@@ -475,196 +442,163 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Step& s,
   }
 }
 
-template <int BITS, int D, int NT>
-__global__ void __launch_bounds__(kThreads, simd_waves(BITS, D, NT)) paged_attn_kernel(const AttnArgs a) {
+template <int BITS, int D, bool HEADS>
+__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs a) {
   using G = Geo<BITS, D>;
+  constexpr int kLevels = HEADS ? 3 : 1;
   extern __shared__ __align__(16) uint8_t lds[];
-  float* const so = reinterpret_cast<float*>(lds);               // [waves][16][LD] the waves' sums
-  float* const sm = so + kWaves * 16 * G::LD;                    // [16][waves] largest scores
-  float* const sl = sm + 16 * kWaves;                            // [16][waves] sums of weights
-  uint4* const sq = reinterpret_cast<uint4*>(so + G::kSums);     // [NT][STEPS][64] the queries as operands
-  Sums* const state = reinterpret_cast<Sums*>(sq + NT * G::STEPS * 64);  // split > 0: [2][NT][16 D / 4] running sums
-  int* const items = reinterpret_cast<int*>(state + 2 * NT * 16 * D / 4);  // [kTable][8]
-  int* const mem = items + kTable * 8;
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), r16 = lane & 15, g4 = lane >> 4;
+  // the wave's running sums: of a block; where it takes whole heads also of a group of blocks, and of the groups
+  f32x4* const held = reinterpret_cast<f32x4*>(lds) + w * kLevels * G::CH * 64 + lane;
+  const int nw = (int)blockDim.x >> 6;
+  int* const tables = reinterpret_cast<int*>(lds + (size_t)nw * kLevels * G::CH * 1024);
+  int* const items = tables + w * kTable * 8;
+  int* const mem = tables + nw * kTable * 8;
 
   Plan plan;
-  make_plan<G, NT>(a, plan, mem);
-  const int split = plan.split, grp = a.g;
-  fill_table<G, NT>(a, plan, items, 0, kTable);
-  if (a.cap && blockIdx.x == 0) {  // for the kernel that joins the parts
+  make_plan(a, plan, mem);
+  if (a.cap && blockIdx.x == 0 && !HEADS) {  // for the kernel that adds up
     int* const out = reinterpret_cast<int*>(a.part + (size_t)a.cap * (D + 2));
-    if (tid == 0) out[0] = split;
+    if (tid == 0) out[0] = plan.split;
     for (int i = tid; i < a.b; i += kThreads)
       out[1 + i] = plan.rows[i], out[1 + a.b + i] = plan.len[i], out[1 + 2 * a.b + i] = plan.tok[i];
   }
-  block_sync();
+  if ((plan.split == kByHead) != HEADS) return;  // the other kernel's
+  const int grp = a.g, waves = (int)gridDim.x * nw, wave = w * (int)gridDim.x + (int)blockIdx.x;
+  fill_table(a, plan, items, 0, kTable, wave, waves);
+  wave_sync();
 
-  // where a (sequence, head)'s partial rows begin
-  auto unit_row = [&](int seq, int head, const Seq& s) __attribute__((always_inline)) {
-    return plan.rows[seq] + head * seq_rows(s, split, grp);
-  };
-  const __amdgpu_buffer_rsrc_t scratch =
-      __builtin_amdgcn_make_buffer_rsrc(a.part, (short)0, (int)(a.cap * (D * 4 + 8)), 0x00020000);
-  const uint32_t ml_at = (uint32_t)a.cap * (D * 4);
-  // A part's sums are kept for a chunk and written by stores that every chunk makes, to places past the scratch's end (where
-  // the hardware drops them) when there is nothing to write.  Memory operations are waited for in order, and by counts that
-  // hold on every path: after a store under a condition the next wait for values would be one for the store to reach memory
-  // too, several microseconds.
-  Sums held[NT * G::kPasses];
-  int held_o[NT * G::kPasses], held_ml[NT * G::kPasses];
-  auto write_held = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < NT * G::kPasses; ++i) {
-      const f32x4 o = {held[i].o[0], held[i].o[1], held[i].o[2], held[i].o[3]};
-      const f32x2 ml = {held[i].m, held[i].l};
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), scratch, held_o[i], 0, 0);
-      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, ml), scratch, held_ml[i], 0, 0);
-      held_o[i] = held_ml[i] = kNowhere;
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < NT * G::kPasses; ++i) held_o[i] = held_ml[i] = kNowhere;
-  Step cur, nxt;  // the part whose chunk is in registers, and the next one
-  read_step(items, 0, cur);
+  Item cur, nxt;
+  read_item(items, 0, cur);
   if (!cur.end) return;
-  read_step(items, 1, nxt);
-  if (cur.part + 1 < cur.end) nxt = cur, ++nxt.part;
+  read_item(items, 1, nxt);
   Tokens<BITS, D> x;
-  int ids = x.load_ids(a, cur, w, lane), next_ids = -1;  // of cur's part, and of nxt's
-
-  // The queries of an item, as operands in LDS: [tile][step][lane] 16 bytes, kQ a thread.  They are asked for before the
-  // item's first keys, and put into LDS when the item before is done.
-  constexpr int kQ = (NT * G::STEPS * 64 + kThreads - 1) / kThreads;
-  uint4 qs[kQ];
-  auto load_queries = [&](const Step& s) __attribute__((always_inline)) {
-    const int rows = s.tok * grp, row0 = s.rb * 16 * NT;
+  uint4 q[G::STEPS];
+  auto load_queries = [&](const Item& s) __attribute__((always_inline)) {
+    size_t tok;
+    int h;
+    row_place(a, first_token(a, s.seq), s.head, min(s.tile * 16 + r16, s.tok * grp - 1), &tok, &h);
+    const uint16_t* const p = a.q + tok * a.ldq + (size_t)h * D;
 #pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      const int n = (tid + i * kThreads) & (NT * G::STEPS * 64 - 1), l = n & 63, step = (n >> 6) % G::STEPS;
-      const int row = min(row0 + (n >> 6) / G::STEPS * 16 + (l & 15), rows - 1), t = div_g(a, row);
-      const int h = s.head * grp + row - t * grp;
-      qs[i] = *reinterpret_cast<const uint4*>(a.q + (size_t)(first_token(a, s.seq) + t) * a.ldq + (size_t)h * D +
-                                              G::dim0(step, l >> 4));
-    }
-  };
-  auto put_queries = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      uint4 v = qs[i];
-      if constexpr (BITS == 4)  // values i and i + 4 share a register
-        v = make_uint4(halves(v.x, v.z, false), halves(v.x, v.z, true), halves(v.y, v.w, false), halves(v.y, v.w, true));
-      if (tid + i * kThreads < NT * G::STEPS * 64) sq[tid + i * kThreads] = v;
-    }
-    block_sync();
+    for (int i = 0; i < G::STEPS; ++i) q[i] = *reinterpret_cast<const uint4*>(p + G::dim0(i, g4));
   };
   const float zscale = a.scale * 1.44269504088896341f;
-  float top[NT], total[NT], ptop[NT], unit[NT];  // of the lane's row: largest score, sum of weights; see the product below
-  f32x4 o[NT][G::CH];
+  float top, total, ptop, unit;  // of the lane's row: largest score, sum of weights; see the product below
+  f32x4 o[G::CH];
   auto clear = [&]() __attribute__((always_inline)) {
+    top = -INFINITY, total = 0.0f, ptop = 0.0f, unit = 1.0f;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      top[n] = -INFINITY, total[n] = 0.0f, ptop[n] = 0.0f, unit[n] = 1.0f;
-#pragma unroll
-      for (int t = 0; t < G::CH; ++t) o[n][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int t = 0; t < G::CH; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   };
   clear();
+  float htop[kLevels], htotal[kLevels];  // of the sums held in LDS; -inf and 0: none yet
+#pragma unroll
+  for (int i = 0; i < kLevels; ++i) htop[i] = -INFINITY, htotal[i] = 0.0f;
+  // the sums at hand into level i's, or the other way round (`back`: level i's are then done with)
+  auto hold = [&](int i, bool back) __attribute__((always_inline)) {
+    const Fold f(htop[i], top);
+    const bool none = htop[i] == -INFINITY && htotal[i] == 0.0f;  // (nothing was ever written there)
+#pragma unroll
+    for (int t = 0; t < G::CH; ++t) {
+      f32x4 h = held[(i * G::CH + t) * 64], n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = none ? 0.0f : h[e];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n[e] = f(h[e], o[t][e]);
+      if (back)
+        o[t] = n;
+      else
+        held[(i * G::CH + t) * 64] = n;
+    }
+    const float l = f(htotal[i], total);
+    htop[i] = back ? -INFINITY : f.m, htotal[i] = back ? 0.0f : l;
+    if (back) top = f.m, total = l;
+  };
 
-  int chunk = 0, at = G::start(cur.part) + w * G::TPW;  // at: the wave's first token of the chunk
-  x.find(a, ids, 0);
-  if (nxt.end) next_ids = x.load_ids(a, nxt, w, lane);
+  // ids: the pages of 64 subtiles from token id0 on, of cur; next_ids of nxt
+  int at = cur.part * kPart, id0 = at;
+  int ids = x.load_ids(a, cur, at, lane), next_ids = -1;
   load_queries(cur);
+  x.find(a, ids, 0);
+  if (nxt.end) next_ids = x.load_ids(a, nxt, nxt.part * kPart, lane);
   x.load_keys(a, cur.head, at, lane, ~0u);
   x.load_values(a, cur.head, at, lane, ~0u);
-  put_queries();
 
   for (;;) {
-    const int len = cur.len, tok = cur.tok, rows = tok * grp, row0 = cur.rb * 16 * NT;
+    const int len = cur.len, tok = cur.tok, rows = tok * grp, row = cur.tile * 16 + r16;
     const uint32_t dead = x.dead;
     const bool masked = dead || at + G::TPW > len - tok + 1;  // slots without a token, or that some row does not see
-    const bool same = chunk + 1 < G::chunks(cur.part) && at - w * G::TPW + G::CHUNK < len;  // the part goes on
+    const int nat0 = at + G::TPW;
+    const bool same = nat0 < min(len, cur.end * kPart);  // the item goes on
     const bool more = same || nxt.end;
     const uint32_t live = more ? ~0u : 0u;
     const int nhead = same ? cur.head : more ? nxt.head : 0;
-    const int nat = same ? at + G::CHUNK : more ? G::start(nxt.part) + w * G::TPW : 0;
+    const int nat = same ? nat0 : more ? nxt.part * kPart : 0;
 
-    // ---- scores: z[n][i][e] of token at + 16 i + 4 g4 + e, row r16 of tile n
-    float z[NT][G::NS][4];
+    // ---- scores: z[i][e] of token at + 16 i + 4 g4 + e, row r16
+    float z[G::NS][4];
     {
-      f32x4 c[NT][G::NS];
+      f32x4 c[G::NS], init = {0.0f, 0.0f, 0.0f, 0.0f};
+      bf16x8 qf[G::STEPS];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        f32x4 init = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < G::STEPS; ++s) {
+        uint4 v = q[s];
+        if constexpr (BITS == 4)  // values i and i + 4 share a register
+          v = make_uint4(halves(v.x, v.z, false), halves(v.x, v.z, true), halves(v.y, v.w, false), halves(v.y, v.w, true));
+        qf[s] = __builtin_bit_cast(bf16x8, v);
         if constexpr (BITS < 16) {  // the codes' offset is taken off first: its product with the queries
           const uint32_t off = 0x00010001u * (BITS == 8 ? 0xC300u : 0xC1C0u);  // -128, -24
           static_assert(G::kOff == (BITS == 8 ? 128 : 24), "");
-#pragma unroll
-          for (int s = 0; s < G::STEPS; ++s)
-            init = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                frag(off, off, off, off), __builtin_bit_cast(bf16x8, sq[(n * G::STEPS + s) * 64 + lane]), init, 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < G::NS; ++i) c[n][i] = init;
-      }
-#pragma unroll
-      for (int s = 0; s < G::STEPS; ++s) {
-        bf16x8 q[NT];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) q[n] = __builtin_bit_cast(bf16x8, sq[(n * G::STEPS + s) * 64 + lane]);
-#pragma unroll
-        for (int i = 0; i < G::NS; ++i) {
-          const bf16x8 k = key_frag<BITS, D>(x.k[i], s);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) c[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, q[n], c[n][i], 0, 0, 0);
+          init = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(off, off, off, off), qf[s], init, 0, 0, 0);
         }
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < G::NS; ++i) c[i] = init;
+#pragma unroll
+      for (int s = 0; s < G::STEPS; ++s)
 #pragma unroll
         for (int i = 0; i < G::NS; ++i)
+          c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key_frag<BITS, D>(x.k[i], s), qf[s], c[i], 0, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) z[n][i][e] = c[n][i][e];
+      for (int i = 0; i < G::NS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[i][e] = c[i][e];
     }
     if (!same) {
-      ids = next_ids;  // (-1 where there is no next part)
+      ids = next_ids, id0 = nat;  // (-1 where there is no next item)
       next_ids = -1;
       if (more) {
-        Step then = nxt;
-        if (nxt.part + 1 < nxt.end)
-          ++then.part;
-        else
-          read_step(items, nxt.k + 1, then);
-        if (then.end) next_ids = x.load_ids(a, then, w, lane);
+        Item then;
+        read_item(items, nxt.k + 1, then);
+        if (then.end) next_ids = x.load_ids(a, then, then.part * kPart, lane);
         load_queries(nxt);
       }
+    } else if (HEADS && nat - id0 == 1024) {
+      ids = x.load_ids(a, cur, nat, lane), id0 = nat;
     }
-    x.find(a, ids, same ? chunk + 1 : 0);
+    x.find(a, ids, (nat - id0) >> 4);
     x.load_keys(a, nhead, nat, lane, live);
-    write_held();
     // ---- softmax of the running maximum
-    u32x4 pk[NT][G::NG] = {};
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (n && row0 + n * 16 >= rows) continue;  // (the tile's sums go nowhere)
-      const int limit = len - tok + 1 + div_g(a, row0 + n * 16 + r16);
+    u32x4 pk[G::NG];
+    {
+      const int limit = len - tok + 1 + div_g(a, row);
       float most = -INFINITY;
 #pragma unroll
       for (int i = 0; i < G::NS; ++i) {
         const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          z[n][i][e] *= BITS == 16 ? zscale : zscale * __uint_as_float(sc[e] << 16);
+          z[i][e] *= BITS == 16 ? zscale : zscale * __uint_as_float(sc[e] << 16);
           if (masked) {
             const int j = at + 16 * i + 4 * g4 + e;
-            if (j >= limit || j >= len || (dead >> i & 1)) z[n][i][e] = -INFINITY;
+            if (j >= limit || j >= len || (dead >> i & 1)) z[i][e] = -INFINITY;
           }
-          most = fmaxf(most, z[n][i][e]);
+          most = fmaxf(most, z[i][e]);
         }
       }
-      most = fmaxf(top[n], max4(most));
-      float f = most == top[n] ? 1.0f : __builtin_amdgcn_exp2f(top[n] - most);  // what the sums so far are worth
-      top[n] = most;
+      most = fmaxf(top, max4(most));
+      float f = most == top ? 1.0f : __builtin_amdgcn_exp2f(top - most);  // what the sums so far are worth
+      top = most;
       const float base = most == -INFINITY ? 0.0f : most;
       float sum = 0.0f, pmost = 0.0f;
 #pragma unroll
@@ -672,40 +606,40 @@ __global__ void __launch_bounds__(kThreads, simd_waves(BITS, D, NT)) paged_attn_
         const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(z[n][i][e] - base);
+          const float p = __builtin_amdgcn_exp2f(z[i][e] - base);
           sum += p;
           if constexpr (BITS == 16) {
-            z[n][i][e] = p;
+            z[i][e] = p;
           } else {  // the codes' weight; where a token is not seen its scale may be anything
-            z[n][i][e] = masked && z[n][i][e] == -INFINITY ? 0.0f : p * __uint_as_float(sc[e] & 0xFFFF0000u);
-            pmost = fmaxf(pmost, z[n][i][e]);
+            z[i][e] = masked && z[i][e] == -INFINITY ? 0.0f : p * __uint_as_float(sc[e] & 0xFFFF0000u);
+            pmost = fmaxf(pmost, z[i][e]);
           }
         }
       }
-      total[n] = fmaf(total[n], f, sum4(sum));
+      total = fmaf(total, f, sum4(sum));
       // The weights are rounded for the product: to bf16 beside bf16 values (the range of the values needs it), to f16,
       // 8 times as fine, beside codes -- in units of a power of two such that the row's largest so far is in [1, 2), so
       // what f16 cannot hold is less than 2^-25 of it.  The sums are in these units.
       if constexpr (BITS < 16) {
-        ptop[n] = fmaxf(ptop[n] * f, max4(pmost));
-        const uint32_t ex = min(max(__float_as_uint(ptop[n]) >> 23, 2u), 252u);
+        ptop = fmaxf(ptop * f, max4(pmost));
+        const uint32_t ex = min(max(__float_as_uint(ptop) >> 23, 2u), 252u);
         const float inv = __uint_as_float((254u - ex) << 23);
-        f *= unit[n] * inv;
-        unit[n] = __uint_as_float(ex << 23);
+        f *= unit * inv;
+        unit = __uint_as_float(ex << 23);
 #pragma unroll
         for (int i = 0; i < G::NS; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            pk[n][i / 2][2 * (i & 1) + e] = pack_f16(z[n][i][2 * e] * inv, z[n][i][2 * e + 1] * inv);
+            pk[i / 2][2 * (i & 1) + e] = pack_f16(z[i][2 * e] * inv, z[i][2 * e + 1] * inv);
       } else {
 #pragma unroll
         for (int i = 0; i < G::NS; ++i)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) pk[n][i / 2][2 * (i & 1) + e] = pack_bf16(z[n][i][2 * e], z[n][i][2 * e + 1]);
+          for (int e = 0; e < 2; ++e) pk[i / 2][2 * (i & 1) + e] = pack_bf16(z[i][2 * e], z[i][2 * e + 1]);
       }
       if (__ballot(f != 1.0f)) {
 #pragma unroll
-        for (int t = 0; t < G::CH; ++t) o[n][t] *= f;
+        for (int t = 0; t < G::CH; ++t) o[t] *= f;
       }
     }
     // ---- values
@@ -736,218 +670,212 @@ __global__ void __launch_bounds__(kThreads, simd_waves(BITS, D, NT)) paged_attn_
 #pragma unroll
     for (int i = 0; i < G::NG; ++i) {
 #pragma unroll
-      for (int t = 0; t < G::CH; ++t) {
-        const u32x4 v = value_frag<BITS, D>(x.v[i], t);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) o[n][t] = weigh<BITS>(v, pk[n][i], o[n][t]);
-      }
+      for (int t = 0; t < G::CH; ++t) o[t] = weigh<BITS>(value_frag<BITS, D>(x.v[i], t), pk[i], o[t]);
       if constexpr (BITS == 16) {
-        if (odd >> i & 1)
-#pragma unroll
-          for (int n = 0; n < NT; ++n)
-            add_non_finite<D>(a, cur, at + 32 * i, pk[n][i], len - tok + 1 + div_g(a, row0 + n * 16 + r16), lane, o[n]);
+        if (odd >> i & 1) add_non_finite<D>(a, cur, at + 32 * i, pk[i], len - tok + 1 + div_g(a, row), lane, o);
       }
     }
     x.load_values(a, nhead, nat, lane, live);
+    const int part = at / kPart;
     at = nat;
+    if (same && at % kPart) continue;
+
+    // ---- the end of a part
+    if constexpr (BITS < 16) {
+#pragma unroll
+      for (int t = 0; t < G::CH; ++t) o[t] *= unit;
+    }
+    if (plan.split != kByPart) {
+      const bool block_ends = !same || (part + 1) % kBlock == 0;
+      hold(0, block_ends);
+      if (HEADS && block_ends) {
+        const bool group_ends = !same || (part + 1) % (kBlock * kGroup) == 0;
+        hold(1, group_ends);
+        if (group_ends) hold(2, !same);
+      }
+    }
     if (same) {
-      ++chunk;
+      clear();
       continue;
     }
-
-    // ---- the end of a part: the waves' sums, in wave order
-    const Seq shape = seq_shape<G, NT>(a, len, tok);
+    // ---- the end of an item: the lane has 4 runs of CH sums of its row
+    if (row < rows) {
+      const int pieces = seq_pieces(len, plan.split);
+      if (pieces > 1) {
+        const int piece = part / (plan.split == kByPart ? 1 : kBlock);
+        const int to = uni(plan.rows[cur.seq]) + cur.head * rows * pieces + piece * rows + cur.tile * 16;
+        // four values of all the tile's rows side by side: what a store writes is in one piece
+        const int n = min(16, rows - cur.tile * 16) * 16;
+        float* const p = a.part + (size_t)to * D + r16 * 16 + g4 * 4;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int tile0 = row0 + n * 16;
-      if (tile0 >= rows) continue;
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int u = 0; u < G::kPasses; ++u) {
-        constexpr int RUN = 4 / G::kPasses;  // of the lane's four runs of CH sums
-        constexpr int C4 = D / G::kPasses / 4;
-        block_sync();  // the rows in LDS are free
-        if (tile0 + r16 < rows) {
-          if (g4 == 0) sm[r16 * kWaves + w] = top[n], sl[r16 * kWaves + w] = total[n];
-          float* const dst = so + (w * 16 + r16) * G::LD + g4 * RUN * G::CH;
+          for (int t = 0; t < G::CH; t += 4)
+            *reinterpret_cast<float4*>(p + (i * G::CH + t) / 4 * n) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
+        if (g4 == 0) reinterpret_cast<float2*>(a.part + (size_t)a.cap * D)[to + r16] = make_float2(top, total);
+      } else {
+        size_t to;
+        int h;
+        row_place(a, first_token(a, cur.seq), cur.head, row, &to, &h);
+        uint16_t* const p = a.y + to * a.ldy + (size_t)h * D + 4 * g4 * G::CH;
+        const float inv = 1.0f / total;
+        const bool none = total == 0.0f;
 #pragma unroll
-          for (int i = 0; i < RUN; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int t = 0; t < G::CH; t += 4) {
-              const int k = u * RUN + i;
-              float4 v;
-              v.x = o[n][t][k] * unit[n], v.y = o[n][t + 1][k] * unit[n];
-              v.z = o[n][t + 2][k] * unit[n], v.w = o[n][t + 3][k] * unit[n];
-              *reinterpret_cast<float4*>(dst + i * G::CH + t) = v;
-            }
-        }
-        block_sync();
-        const int rr = tid / C4, c = tid % C4, grow = tile0 + rr;
-        if (rr >= 16 || grow >= rows) continue;
-        const int c4 = c / (RUN * G::CH / 4) * G::CH + u * (RUN * G::CH / 4) + c % (RUN * G::CH / 4);  // of the row
-        Sums s;
-        float f[kWaves], fl[kWaves];
-#pragma unroll
-        for (int j = 0; j < kWaves; j += 4) {
-          const float4 x4 = *reinterpret_cast<const float4*>(sm + rr * kWaves + j);
-          const float4 l4 = *reinterpret_cast<const float4*>(sl + rr * kWaves + j);
-          f[j] = x4.x, f[j + 1] = x4.y, f[j + 2] = x4.z, f[j + 3] = x4.w;
-          fl[j] = l4.x, fl[j + 1] = l4.y, fl[j + 2] = l4.z, fl[j + 3] = l4.w;
-        }
-#pragma unroll
-        for (int j = 0; j < kWaves; ++j) s.m = fmaxf(s.m, f[j]);
-        const float mx = s.m == -INFINITY ? 0.0f : s.m;
-#pragma unroll
-        for (int j = 0; j < kWaves; ++j) {
-          f[j] = __builtin_amdgcn_exp2f(f[j] - mx);
-          const float4 v = *reinterpret_cast<const float4*>(so + (j * 16 + rr) * G::LD + 4 * c);
-          s.l = fmaf(fl[j], f[j], s.l);
-          s.o[0] = fmaf(v.x, f[j], s.o[0]), s.o[1] = fmaf(v.y, f[j], s.o[1]);
-          s.o[2] = fmaf(v.z, f[j], s.o[2]), s.o[3] = fmaf(v.w, f[j], s.o[3]);
-        }
-        bool done = shape.parts == 1;
-        int to = -1;  // where a partial sum goes
-        if (!split) {
-          if (!done) to = unit_row(cur.seq, cur.head, shape) + cur.part * rows + grow;
-        } else {
-          Sums* const block = state + (n * G::kPasses + u) * 16 * C4 + tid;  // running sums: of the block's parts, of the blocks
-          Sums* const whole = block + NT * 16 * D / 4;
-          Sums b = cur.part % G::BLOCK == 0 ? Sums() : *block;
-          b.add(s);
-          done = cur.part + 1 == cur.end;
-          if (!done && (cur.part + 1) % G::BLOCK) {
-            *block = b;
-            continue;
+          for (int t = 0; t < G::CH; t += 4) {
+            uint2 v;
+            v.x = none ? 0u : (uint32_t)f2bf(o[t][i] * inv) | ((uint32_t)f2bf(o[t + 1][i] * inv) << 16);
+            v.y = none ? 0u : (uint32_t)f2bf(o[t + 2][i] * inv) | ((uint32_t)f2bf(o[t + 3][i] * inv) << 16);
+            *reinterpret_cast<uint2*>(p + i * G::CH + t) = v;
           }
-          s = cur.part < G::BLOCK ? Sums() : *whole;
-          s.add(b);
-          if (!done) *whole = s;
-        }
-        if (to >= 0) {
-          held[n * G::kPasses + u] = s;
-          held_o[n * G::kPasses + u] = to * (D * 4) + 16 * c4;
-          held_ml[n * G::kPasses + u] = c4 ? kNowhere : (int)ml_at + to * 8;
-        } else if (done)
-          finish_row<D>(a, s, first_token(a, cur.seq), cur.head, grow, c4);
+        if (a.lse && g4 == 0) a.lse[to * a.heads + h] = row_lse(top, total);
       }
     }
-    if (!more) break;
-    const bool fresh = nxt.k != cur.k;
+    if (!more) return;
     cur = nxt;
-    if (cur.part + 1 < cur.end) {
-      ++nxt.part;
-    } else {
-      // (items up to cur.k + 2 are read before the next part ends)
-      if (fresh && ((cur.k + 2) & (kTable / 2 - 1)) == 0 && cur.k + 2 >= kTable) {
-        fill_table<G, NT>(a, plan, items, cur.k + 2, kTable / 2);
-        block_sync();
-      }
-      read_step(items, cur.k + 1, nxt);
+    // (items up to cur.k + 2 are read before the next one ends)
+    if (((cur.k + 2) & (kTable / 2 - 1)) == 0 && cur.k + 2 >= kTable) {
+      fill_table(a, plan, items, cur.k + 2, kTable / 2, wave, waves);
+      wave_sync();
     }
-    chunk = 0;
+    read_item(items, cur.k + 1, nxt);
     clear();
-    if (fresh) put_queries();
   }
-  write_held();
 }
 
-// The rows whose parts went to scratch: blocks of parts side by side, then left to right.  A workgroup takes rows of one
-// (sequence, head).
-template <class G, int D>
+// The rows whose pieces went to scratch.  A workgroup takes rows of one (sequence, head); C4 threads side by side a row's
+// values, SIDE such sets the pieces: of blocks, a set adds a group; of parts, a set adds a block, and the first set then
+// the blocks of a group.
+template <int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const AttnArgs a) {
   constexpr int C4 = D / 4, SIDE = kThreads / C4;
-  __shared__ __align__(16) uint8_t lds[SIDE * C4 * sizeof(Sums)];
-  Sums* const side = reinterpret_cast<Sums*>(lds);  // [SIDE][C4]
+  __shared__ __align__(16) uint8_t lds[kGroup * C4 * sizeof(Sums)];
+  Sums* const side = reinterpret_cast<Sums*>(lds);  // [up to kGroup][C4]
   const int* const plan = reinterpret_cast<const int*>(a.part + (size_t)a.cap * (D + 2));
-  if (plan[0]) return;  // nothing was split
-  const int seq = blockIdx.x / a.s.heads, head = blockIdx.x - seq * a.s.heads;
+  const int split = plan[0], seq = blockIdx.x / a.s.heads, head = blockIdx.x - seq * a.s.heads;
   const int first = plan[1 + seq], len = plan[1 + a.b + seq], tok = plan[1 + 2 * a.b + seq];
-  const int parts = G::parts(len), rows = tok * a.g;
-  if (parts == 1) return;
+  const int pieces = seq_pieces(len, split), rows = tok * a.g;
+  if (pieces == 1) return;
   const int c4 = threadIdx.x % C4, s = threadIdx.x / C4, q0 = first_token(a, seq);
-  const float4* const o = reinterpret_cast<const float4*>(a.part) + (size_t)(first + head * rows * parts) * C4 + c4;
-  const float2* const ml = reinterpret_cast<const float2*>(a.part + (size_t)a.cap * D) + first + head * rows * parts;
+  const float* const o = a.part + (size_t)(first + head * rows * pieces) * D;
+  const float2* const ml = reinterpret_cast<const float2*>(a.part + (size_t)a.cap * D) + first + head * rows * pieces;
+  // left to right, n pieces from p0 on
+  auto add = [&](int p0, int n, int row) {
+    constexpr int U = 8;
+    const int tile = row & ~15, place = tile * D + c4 / 4 * min(16, rows - tile) * 16 + (row & 15) * 16 + c4 % 4 * 4;
+    Sums t;
+    for (int i0 = 0; i0 < n; i0 += U) {
+      float4 v[U];
+      float2 w[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const size_t j = (size_t)(p0 + min(i0 + i, n - 1)) * rows;
+        v[i] = *reinterpret_cast<const float4*>(o + j * D + place), w[i] = ml[j + row];
+      }
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (i0 + i < n) {
+          Sums p;
+          p.m = w[i].x, p.l = w[i].y;
+          p.o[0] = v[i].x, p.o[1] = v[i].y, p.o[2] = v[i].z, p.o[3] = v[i].w;
+          t.add(p);
+        }
+    }
+    return t;
+  };
+  const bool fine = split == kByPart;
+  const int step = fine ? kBlock : kGroup;        // pieces of a set's share
+  const int at_once = fine ? kGroup : SIDE;       // shares between two meetings: a group's blocks, or as many groups as sets
   for (int row = blockIdx.y; row < rows; row += gridDim.y) {
     Sums total;
-    for (int from = 0; from < parts; from += SIDE * G::BLOCK) {
-      const int p0 = from + s * G::BLOCK;
-      if (p0 < parts) {
-        const int n = min(G::BLOCK, parts - p0);
-        float4 v[G::BLOCK];
-        float2 w[G::BLOCK];
-#pragma unroll
-        for (int i = 0; i < G::BLOCK; ++i) {
-          const size_t j = (size_t)(p0 + min(i, n - 1)) * rows + row;
-          v[i] = o[j * C4], w[i] = ml[j];
-        }
-        Sums t;
-#pragma unroll
-        for (int i = 0; i < G::BLOCK; ++i)
-          if (i < n) {
-            Sums p;
-            p.m = w[i].x, p.l = w[i].y;
-            p.o[0] = v[i].x, p.o[1] = v[i].y, p.o[2] = v[i].z, p.o[3] = v[i].w;
-            t.add(p);
-          }
-        side[threadIdx.x] = t;
+    for (int from = 0; from < pieces; from += at_once * step) {
+      const int n = min(at_once, (pieces - from + step - 1) / step);
+      for (int i = s; i < n; i += SIDE) {
+        const int p0 = from + i * step;
+        side[i * C4 + c4] = add(p0, min(step, pieces - p0), row);
       }
       __syncthreads();
-      if (s == 0)
-        for (int i = 0; i < SIDE && from + i * G::BLOCK < parts; ++i) total.add(side[i * C4 + c4]);
+      if (s == 0) {
+        if (fine) {
+          Sums g;
+          for (int i = 0; i < n; ++i) g.add(side[i * C4 + c4]);
+          total.add(g);
+        } else {
+          for (int i = 0; i < n; ++i) total.add(side[i * C4 + c4]);
+        }
+      }
       __syncthreads();
     }
-    if (s == 0) finish_row<D>(a, total, q0, head, row, c4);
+    if (s == 0) {
+      size_t to;
+      int h;
+      row_place(a, q0, head, row, &to, &h);
+      const float inv = 1.0f / total.l;
+      uint2 y = make_uint2(0u, 0u);
+      if (total.l != 0.0f) {
+        y.x = (uint32_t)f2bf(total.o[0] * inv) | ((uint32_t)f2bf(total.o[1] * inv) << 16);
+        y.y = (uint32_t)f2bf(total.o[2] * inv) | ((uint32_t)f2bf(total.o[3] * inv) << 16);
+      }
+      *reinterpret_cast<uint2*>(a.y + to * a.ldy + (size_t)h * D + c4 % 4 * (D / 4) + c4 / 4 * 4) = y;
+      if (a.lse && c4 == 0) a.lse[to * a.heads + h] = row_lse(total.m, total.l);
+    }
   }
 }
 
-template <int BITS, int D, int NT>
+template <int BITS, int D>
 int launch(AttnArgs a, hipStream_t s) {
   using G = Geo<BITS, D>;
-  static_assert(G::KW * 4 * 64 == 16 * G::RB, "");
+  static_assert(G::KW * 4 * 64 == 16 * G::RB && kPart % G::TPW == 0 && kBlock * kPart == 64 * 16, "");
+  static_assert(kThreads / (D / 4) <= kGroup, "");
   static const int cus = [] {
     int dev = 0, n = 0;
     if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess)
       return 256;
     return n;
   }();
-  const long max_tokens = (long)a.ldt << a.page_log2;
-  const long parts = G::parts((int)(max_tokens < 0x7FFFFFFF ? max_tokens : 0x7FFFFFFF));
+  const double max_tokens = (double)a.ldt * a.s.page, rows_seq = (double)a.m / a.b * a.g;  // the latter on average
   const double tiles = ((double)(a.qstart ? a.m : a.tq) * a.g + 15) / 16;
-  const double items = (double)a.b * a.s.heads * (double)parts * tiles;
-  const int slots = cus * (simd_waves(BITS, D, NT) * 4 / kWaves);
-  const unsigned grid = items < slots ? (unsigned)items : (unsigned)slots;
+  const double items = (double)a.b * a.s.heads * (max_tokens / kPart + 1) * tiles;  // no more than these
+  const int slots = 2 * cus;
+  // A wave alone streams some 11 GB/s of 16 bits, 9 of 8 and 4 of 4 (128 values a row), limited by its own steps, and the
+  // memory 5.5 TB/s: fewer waves than that leave it idle.  A part's start and end cost about as much as two chunks.
+  a.few = slots * (BITS == 16 ? 3 : BITS == 8 ? 4 : 8) / 2;
+  const unsigned grid = items < (double)slots * kWaves ? (unsigned)((items + kWaves - 1) / kWaves) : (unsigned)slots;
   std::lock_guard<std::mutex> lock(scratch_mutex(s));
-  // partial rows of all sequences at their longest; fewer where that is more than kMaxPartialBytes
+  // Partial rows: those of all blocks at the sequences' longest, and those of as many parts as are ever taken one by one
+  // (the blocks are then few); no more than kMaxPartialBytes.
   const size_t row_bytes = (size_t)D * 4 + 8, plan_bytes = (size_t)(3 * a.b + 1) * 4;
-  double want = parts > 1 ? (double)a.m * a.heads * (double)parts : 0.0;
+  const double by_block = (double)a.m * a.heads * (max_tokens / (kBlock * kPart) + 1);
+  const double by_part = (double)a.m * a.heads * (max_tokens / kPart + 1);
+  const double few = (double)a.few * kBlock * 16;
   const double most = (double)(kMaxPartialBytes / row_bytes);
-  if (want > most) want = most;
-  a.cap = (int)want;
+  double want = max_tokens <= kPart ? 0.0 : by_part < few ? by_part : few < by_block ? by_block : few;
+  const bool all = want <= most;
+  a.cap = (int)(all ? want : most);
   if (a.cap) {
     a.part = reinterpret_cast<float*>(call_scratch(s, (size_t)a.cap * row_bytes + plan_bytes).data);
     if (!a.part) a.cap = 0;
   }
-  const size_t smem = (size_t)(G::kSums + kTable * 8 + 4 * a.b) * 4 + (size_t)NT * G::STEPS * 64 * 16 +
-                      sizeof(Sums) * 2 * NT * 16 * D / 4;
-  hipLaunchKernelGGL((paged_attn_kernel<BITS, D, NT>), dim3(grid), dim3(kThreads), smem, s, a);
+  auto smem = [&](int waves, int levels) {
+    return (size_t)waves * (levels * G::CH * 1024 + kTable * 8 * 4) + (size_t)4 * a.b * 4;
+  };
+  hipLaunchKernelGGL((paged_attn_kernel<BITS, D, false>), dim3(grid), dim3(kThreads), smem(kWaves, 1), s, a);
   if (const int e = (int)hipGetLastError()) return e;
-  if (!a.cap) return 0;
-  const double rows = (double)a.m / a.b * a.g;  // of a (sequence, head), on average
-  hipLaunchKernelGGL((join_kernel<G, D>), dim3((unsigned)(a.b * a.s.heads), rows < 1 ? 1u : rows < 64 ? (unsigned)rows : 64u),
-                     dim3(kThreads), 0, s, a);
-  return (int)hipGetLastError();
-}
-template <int BITS, int D>
-int launch_tiles(const AttnArgs& a, hipStream_t s) {
-  const double tiles = (double)a.m / a.b * a.g / 16;  // of a sequence, on average
-  if constexpr (D <= 128) {
-    if (tiles > 1) return launch<BITS, D, 2>(a, s);
+  if (a.cap) {
+    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.b * a.s.heads), rows_seq < 1 ? 1u : rows_seq < 64 ? (unsigned)rows_seq : 64u),
+                       dim3(kThreads), 0, s, a);
+    if (const int e = (int)hipGetLastError()) return e;
   }
-  return launch<BITS, D, 1>(a, s);
+  if (max_tokens > kPart && (!a.cap || !all)) {  // the pieces may not fit: then this one does the work, by heads
+    hipLaunchKernelGGL((paged_attn_kernel<BITS, D, true>), dim3(2 * grid), dim3(kThreads / 2), smem(kWaves / 2, 3), s, a);
+    return (int)hipGetLastError();
+  }
+  return 0;
 }
 template <int BITS>
 int launch_dim(const AttnArgs& a, hipStream_t s) {
-  return a.s.dim == 64 ? launch_tiles<BITS, 64>(a, s)
-                       : a.s.dim == 128 ? launch_tiles<BITS, 128>(a, s) : launch_tiles<BITS, 256>(a, s);
+  return a.s.dim == 64 ? launch<BITS, 64>(a, s) : a.s.dim == 128 ? launch<BITS, 128>(a, s) : launch<BITS, 256>(a, s);
 }
 
 }  // namespace
