@@ -6,13 +6,47 @@
 // is the inverse of the cumulative sum: the first token whose cumulative weight passes u_t times their sum.  T <= 0 is the
 // greedy limit: a draft is accepted if it is the target's largest logit (the lowest token among equal ones), which is the
 // next token otherwise.  The tokens emitted are then distributed as the target's own (T > 0), or equal to its greedy ones.
+//
+// Bound by the logits' bytes, each read once: verify_rows_kernel gives every workgroup kChunk logits of one row, which it
+// holds in registers for both their largest and the sum of their weights relative to it.  What follows needs little of it:
+//   verify_decide_kernel  puts the chunks of a sequence's rows together and decides on its drafts in order; without draft
+//                         logits it also draws the next token, for which the chunks' sums say in which chunk it lies, and
+//                         only that one is read again;
+//   with draft logits     its workgroups, one a chunk, each come to the same decision and add up their chunk of the
+//                         weights p - q, which are known only now; verify_draw_kernel draws the next token.
+// (Joined by the launches' order: counters and fences between workgroups cost more than a launch here.)
+// Without scratch (a capture before any other call), verify_whole_kernel does all of it in one workgroup a sequence, in the
+// same order, so with the same bits.
+//
+// Weights are fp32 (the hardware's exp2 of the scaled difference to the largest logit), as are the sums of the 16 that a
+// thread holds; all larger sums are 64 bits, in an order that only a row's length decides.
 #include "agens_kernels.h"
 #include "wq_common.h"
+
+#include <cfloat>
 
 namespace agq {
 namespace {
 
-constexpr int kVerThreads = 1024;
+constexpr int kThreads = 256, kWaves = kThreads / 64, kEach = 16, kChunk = kThreads * kEach;
+constexpr int kMaxChunks = kThreads;  // of a row: a thread looks at one
+constexpr int kMaxVocab = kMaxChunks * kChunk;
+static_assert(kMaxVocab == AK_VERIFY_MAX_VOCAB, "the header's limit");
+constexpr size_t kMaxScratch = (size_t)64 << 20;  // of a launch; more sequences take several
+
+// A row, or a chunk of one: its largest logit, the lowest token that has it (-1: nothing above -inf), the sum of the
+// weights relative to it.
+struct RowStat {
+  float top;
+  int best;
+  double total;
+};
+
+// The next token of a sequence is drawn for place j, whose rows' sums are p and q (residual: from p - q).
+struct Decision {
+  int j, residual;
+  RowStat p, q;
+};
 
 struct VerifyArgs {
   const uint16_t *target, *draft;
@@ -22,134 +56,443 @@ struct VerifyArgs {
   int* accepted;
   float* logp;
   long ldt, ldd;
-  int b, t, vocab;
+  int t, vocab, chunks, rows;  // rows: of a sequence, target rows first
+  // scratch
+  RowStat* stats;  // [b][rows][chunks]
+  double* sums;    // [b][chunks]: of max(p - q, 0) in the rejected draft's place
+  Decision* plan;  // [b]
 };
 
-// NaN counts as -inf
-__device__ __forceinline__ float logit(uint16_t b) {
-  const float f = bf2f(b);
-  return f != f ? -INFINITY : f;
-}
-
-struct RowStat {
-  float top;     // largest logit
-  int best;      // its lowest index
-  double total;  // sum of weights
+// What a workgroup shares
+struct Shared {
+  double red[kWaves];
+  int ired[kWaves];
+  double pick_before;
+  RowStat p[kWaves], q[kWaves];
+  int ok[kWaves];
 };
 
-__device__ __forceinline__ float weight(float l, float top, float heat) {
-  return top == -INFINITY ? 0.0f : l == top ? 1.0f : expf((l - top) / heat);
+struct Seq {
+  int id, n;  // n: drafts
+  bool greedy;
+  float heat;
+  // log2(e) / T in two parts: one of 24 bits alone shifts all exponents the same way, so the row's sum by up to 2^-24 times
+  // the mean exponent.  Kept where products with every difference of logits are numbers and -FLT_MAX's exp2 is 0.
+  float scale, scale_lo;
+  float next_u;
+};
+__device__ __forceinline__ Seq seq_of(const VerifyArgs& a, int id) {
+  Seq s;
+  s.id = id;
+  s.n = a.counts ? min(max(a.counts[id], 0), a.t) : a.t;
+  const float temp = a.temp ? a.temp[id] : 1.0f;
+  s.greedy = !(temp > 0.0f);
+  s.heat = s.greedy ? 1.0f : temp;
+  const double scale = fmin(fmax(1.44269504088896340736 / (double)s.heat, 1e-30), (double)FLT_MAX);
+  s.scale = (float)scale;
+  s.scale_lo = (float)(scale - (double)s.scale);
+  s.next_u = a.u[(size_t)id * (a.t + 1) + a.t];
+  return s;
+}
+__device__ __forceinline__ const uint16_t* target_row(const VerifyArgs& a, int seq, int j) {
+  return a.target + ((size_t)seq * (a.t + 1) + j) * a.ldt;
+}
+__device__ __forceinline__ const uint16_t* draft_row(const VerifyArgs& a, int seq, int j) {
+  return a.draft + ((size_t)seq * a.t + j) * a.ldd;
 }
 
-__device__ RowStat row_stat(const uint16_t* row, int vocab, float heat, double* red, int* ired) {
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < vocab; i += kVerThreads) top = fmaxf(top, logit(row[i]));
+// NaN counts as -inf; +inf as a number above every finite bf16, so that differences stay numbers.
+__device__ __forceinline__ float logit(uint32_t b) { return fminf(fmaxf(bf2f((uint16_t)b), -INFINITY), FLT_MAX); }
+// The weight of logit l in a row whose largest is top.
+__device__ __forceinline__ float weight(const Seq& s, float l, float top) {
+  const float d = fmaxf(l - (top == -INFINITY ? 0.0f : top), -FLT_MAX);
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, s.scale, d * s.scale_lo));
+}
+
+// 8 logits from token k on, -inf past the end.  Rows begin at any even address.
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+__device__ __forceinline__ void load8(const uint16_t* row, int k, int vocab, float* l) {
+  if (k + 8 <= vocab) {
+    const u32x4 v = *reinterpret_cast<const u32x4_any*>(row + k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[i] = logit((v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[i] = k + i < vocab ? logit(row[k + i]) : -INFINITY;
+  }
+}
+
+__device__ __forceinline__ double sum16(const float (&w)[kEach]) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) s += w[i];
+  return (double)s;
+}
+
+// The sum over the workgroup, in every thread.
+__device__ __forceinline__ double block_sum(double x, Shared& sh) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) s += sh.red[i];
+  return s;
+}
+
+// A chunk of a row, by a workgroup: thread t holds 8 logits from 8 t on in either half (whole cache lines a wave).
+__device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row, int chunk, int vocab, Shared& sh) {
+  const int t = threadIdx.x, at0 = chunk * kChunk + 8 * t, at1 = at0 + kChunk / 2;
+  float l[kEach];
+  load8(row, at0, vocab, l);
+  load8(row, at1, vocab, l + 8);
+  float mine = l[0];
+#pragma unroll
+  for (int i = 1; i < kEach; ++i) mine = fmaxf(mine, l[i]);
+  float top = mine;
+#pragma unroll
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+  if ((t & 63) == 0) sh.red[t >> 6] = top;
+  if (t == 0) sh.ired[0] = 0x7FFFFFFF;
   __syncthreads();
-  for (int w = 0; w < kVerThreads / 64; ++w) top = fmaxf(top, (float)red[w]);
-  __syncthreads();
-  int best = vocab;
-  double sum = 0.0;
-  for (int i = threadIdx.x; i < vocab; i += kVerThreads) {
-    const float l = logit(row[i]);
-    if (l == top && top > -INFINITY && best == vocab) best = i;
-    sum += weight(l, top, heat);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, (float)sh.red[i]);
+  if (mine == top && top > -INFINITY) {
+    int best = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = kEach - 1; i >= 0; --i)
+      if (l[i] == top) best = (i < 8 ? at0 : at1 - 8) + i;
+    atomicMin(&sh.ired[0], best);
   }
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d), best = min(best, __shfl_xor(best, d));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum, ired[threadIdx.x >> 6] = best;
-  __syncthreads();
-  RowStat r{top, vocab, 0.0};
-  for (int w = 0; w < kVerThreads / 64; ++w) r.total += red[w], r.best = min(r.best, ired[w]);
-  if (r.best == vocab) r.best = -1;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) l[i] = weight(s, l[i], top);
+  const double total = block_sum(sum16(l), sh);
+  return RowStat{top, sh.ired[0] == 0x7FFFFFFF ? -1 : sh.ired[0], total};
+}
+
+// How much a chunk's sum counts in its row: in 64 bits, so that a row's sum is as good as its chunks'.
+__device__ __forceinline__ double chunk_share(const Seq& s, const RowStat& c, float top) {
+  return c.top == -INFINITY ? 0.0 : c.total * exp2((double)(c.top - top) * ((double)s.scale + (double)s.scale_lo));
+}
+
+// A row from its chunks, by one wave.
+__device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int chunks) {
+  const int lane = threadIdx.x & 63;
+  RowStat r{-INFINITY, 0x7FFFFFFF, 0.0};
+  for (int c = lane; c < chunks; c += 64)
+    if (st[c].top > r.top) r.top = st[c].top, r.best = st[c].best;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) {
+    const float m = __shfl_xor(r.top, d);
+    const int i = __shfl_xor(r.best, d);
+    if (m > r.top || (m == r.top && i < r.best)) r.top = m, r.best = i;
+  }
+  if (r.top == -INFINITY) {
+    r.best = -1;
+    return r;
+  }
+  for (int c = lane; c < chunks; c += 64) r.total += chunk_share(s, st[c], r.top);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) r.total += __shfl_xor(r.total, d);
   return r;
 }
 
-__global__ void __launch_bounds__(kVerThreads) spec_verify_kernel(const VerifyArgs a) {
-  __shared__ double red[kVerThreads + 1];
-  __shared__ int ired[kVerThreads / 64], pick;
-  const int seq = blockIdx.x, V = a.vocab;
-  const int n = a.counts ? min(max(a.counts[seq], 0), a.t) : a.t;
-  const float temp = a.temp ? a.temp[seq] : 1.0f;
-  const bool greedy = !(temp > 0.0f);
-  const float heat = greedy ? 1.0f : temp;
-  int* const tok = a.tokens + (size_t)seq * (a.t + 1);
-  float* const lp = a.logp ? a.logp + (size_t)seq * (a.t + 1) : nullptr;
-  for (int j = 0;; ++j) {
-    const uint16_t* const row = a.target + ((size_t)seq * (a.t + 1) + j) * a.ldt;
-    const RowStat P = row_stat(row, V, heat, red, ired);
-    const int x = j < n ? a.ids[(size_t)seq * a.t + j] : -1;
-    const bool known = x >= 0 && x < V;
-    const uint16_t* const drow = a.draft && j < n ? a.draft + ((size_t)seq * a.t + j) * a.ldd : nullptr;
-    RowStat Q{0.0f, 0, 1.0};
-    if (drow && !greedy) Q = row_stat(drow, V, heat, red, ired);
-    if (known) {
-      const double p = P.total > 0 ? weight(logit(row[x]), P.top, heat) / P.total : 0.0;
-      const double q = drow ? (Q.total > 0 ? weight(logit(drow[x]), Q.top, heat) / Q.total : 0.0) : 1.0;
-      if (greedy ? x == P.best : a.u[(size_t)seq * (a.t + 1) + j] * q < p) {
-        if (threadIdx.x == 0) {
-          tok[j] = x;
-          if (lp) lp[j] = (float)((logit(row[x]) == P.top ? 0.0 : (double)(logit(row[x]) - P.top) / heat) - log(P.total));
-        }
-        continue;
-      }
+// The first thread at which the sum of the threads' x (>= 0) passes `at`; the last with any x if rounding lets none pass;
+// -1 without any.  *before: the sum of the threads before it.
+__device__ __forceinline__ int pick_thread(double x, double at, Shared& sh, double* before) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  double inc = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double y = __shfl_up(inc, d);
+    if (lane >= d) inc += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh.red[w] = inc;
+  if (threadIdx.x == 0) sh.ired[0] = 0x7FFFFFFF, sh.ired[1] = -1;
+  __syncthreads();
+  double b = inc - x;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i)
+    if (i < w) b += sh.red[i];
+  if (x > 0.0) {
+    if (b + x > at) atomicMin(&sh.ired[0], (int)threadIdx.x);
+    atomicMax(&sh.ired[1], (int)threadIdx.x);
+  }
+  __syncthreads();
+  const int pick = sh.ired[0] != 0x7FFFFFFF ? sh.ired[0] : sh.ired[1];
+  if ((int)threadIdx.x == pick) sh.pick_before = b;
+  __syncthreads();
+  *before = sh.pick_before;
+  return pick;
+}
+
+// The next token: chunk c weighs share (of thread c); weigh(k, w) gives the weights of the 16 tokens from k on.  -1: none.
+template <class Weigh>
+__device__ __forceinline__ int find_token(const VerifyArgs& a, float u, double share, Weigh weigh, Shared& sh) {
+  const double all = block_sum(share, sh);
+  if (!(all > 0.0)) return -1;
+  double at = (double)u * all, before;
+  const int chunk = pick_thread(share, at, sh, &before);
+  at -= before;
+  const int k = chunk * kChunk + (int)threadIdx.x * kEach;
+  float w[kEach];
+  weigh(k, w);
+  const int who = pick_thread(sum16(w), at, sh, &before);
+  int token = -1;
+  if ((int)threadIdx.x == who) {
+    double c = before;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {  // the last with any weight at worst
+      if (w[i] > 0.0f && c <= at) token = k + i;
+      c += (double)w[i];
     }
-    // the next token: weights p - q of a rejection (p where nothing is left of it), p otherwise
-    if (threadIdx.x == 0) pick = greedy ? P.best : -1;
-    __syncthreads();
-    for (int pass = j < n ? 0 : 1; pass < 2 && pick < 0 && P.total > 0 && !greedy; ++pass) {
-      const int each = (V + kVerThreads - 1) / kVerThreads, lo = min(V, (int)threadIdx.x * each), hi = min(V, lo + each);
-      auto w = [&](int i) {
-        const double p = weight(logit(row[i]), P.top, heat) / P.total;
-        if (pass == 1) return p;
-        const double q = drow ? (Q.total > 0 ? weight(logit(drow[i]), Q.top, heat) / Q.total : 0.0) : (i == x ? 1.0 : 0.0);
-        return p > q ? p - q : 0.0;
+    sh.ired[0] = token;
+  }
+  __syncthreads();
+  return who < 0 ? -1 : sh.ired[0];
+}
+
+// From the target's weights, without token `skip` (-1: all).
+__device__ __forceinline__ int draw_target(const VerifyArgs& a, const Seq& s, int j, const RowStat* st, const RowStat& p,
+                                           int skip, Shared& sh) {
+  const uint16_t* const row = target_row(a, s.id, j);
+  auto weigh = [&](int k, float(&w)[kEach]) {
+    load8(row, k, a.vocab, w);
+    load8(row, k + 8, a.vocab, w + 8);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) w[i] = k + i == skip ? 0.0f : weight(s, w[i], p.top);
+  };
+  const int c = threadIdx.x;
+  double share = c < a.chunks ? chunk_share(s, st[c], p.top) : 0.0;
+  if (skip >= 0) {  // its chunk anew: nothing is left of a difference where the token had nearly all
+    float w[kEach];
+    weigh(skip / kChunk * kChunk + c * kEach, w);
+    const double rest = block_sum(sum16(w), sh);
+    if (c == skip / kChunk) share = rest;
+  }
+  return find_token(a, s.next_u, share, weigh, sh);
+}
+
+// The weights max(p - q, 0) of the 16 tokens from k on, with p and q normalised: in 64 bits, since the two may be close.
+__device__ __forceinline__ void residual16(const VerifyArgs& a, const Seq& s, const Decision& d, const float (&lp)[kEach],
+                                           const float (&lq)[kEach], float (&w)[kEach]) {
+  const double pi = 1.0 / d.p.total, qi = 1.0 / d.q.total;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    w[i] = (float)fmax(weight(s, lp[i], d.p.top) * pi - weight(s, lq[i], d.q.top) * qi, 0.0);
+}
+__device__ __forceinline__ double residual_sum(const VerifyArgs& a, const Seq& s, const Decision& d, int chunk, Shared& sh) {
+  const uint16_t *const p = target_row(a, s.id, d.j), *const q = draft_row(a, s.id, d.j);
+  const int at = chunk * kChunk + 8 * (int)threadIdx.x;
+  float lp[kEach], lq[kEach], w[kEach];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    load8(p, at + h * kChunk / 2, a.vocab, lp + 8 * h);
+    load8(q, at + h * kChunk / 2, a.vocab, lq + 8 * h);
+  }
+  residual16(a, s, d, lp, lq, w);
+  return block_sum(sum16(w), sh);
+}
+
+__device__ __forceinline__ float log_prob(const Seq& s, const RowStat& p, uint16_t bits) {
+  return (float)((double)(logit(bits) - p.top) / (double)s.heat - log(p.total));
+}
+
+// Whether draft j is accepted.  (One lane.)
+__device__ __forceinline__ bool accept(const VerifyArgs& a, const Seq& s, int j, const RowStat& p, const RowStat& q) {
+  const int x = a.ids[(size_t)s.id * a.t + j];
+  if (x < 0 || x >= a.vocab || p.best < 0) return false;
+  if (s.greedy) return x == p.best;
+  double qx = 1.0;
+  if (a.draft) qx = q.best < 0 ? 0.0 : weight(s, logit(draft_row(a, s.id, j)[x]), q.top) / q.total;
+  return a.u[(size_t)s.id * (a.t + 1) + j] * qx < weight(s, logit(target_row(a, s.id, j)[x]), p.top) / p.total;
+}
+__device__ __forceinline__ void put_accepted(const VerifyArgs& a, const Seq& s, int j, const RowStat& p) {
+  const int x = a.ids[(size_t)s.id * a.t + j];
+  a.tokens[(size_t)s.id * (a.t + 1) + j] = x;
+  if (a.logp) a.logp[(size_t)s.id * (a.t + 1) + j] = log_prob(s, p, target_row(a, s.id, j)[x]);
+}
+__device__ __forceinline__ Decision decision(const VerifyArgs& a, const Seq& s, int j, const RowStat& p, const RowStat& q) {
+  return Decision{j, j < s.n && a.draft && !s.greedy && p.best >= 0 && q.best >= 0, p, q};
+}
+
+// Draws and stores the next token and that nothing follows it.  st: the chunks of target row d.j; sum: thread c's chunk of
+// the residual weights, where the decision asks for them.
+__device__ __forceinline__ void finish(const VerifyArgs& a, const Seq& s, const Decision& d, const RowStat* st, double sum,
+                                       Shared& sh) {
+  int token = -1;
+  if (s.greedy || d.p.best < 0) {
+    token = d.p.best;
+  } else {
+    if (d.residual) {
+      const uint16_t *const p = target_row(a, s.id, d.j), *const q = draft_row(a, s.id, d.j);
+      auto weigh = [&](int k, float(&w)[kEach]) {
+        float lp[kEach], lq[kEach];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          load8(p, k + 8 * h, a.vocab, lp + 8 * h);
+          load8(q, k + 8 * h, a.vocab, lq + 8 * h);
+        }
+        residual16(a, s, d, lp, lq, w);
       };
-      double sum = 0.0;
-      for (int i = lo; i < hi; ++i) sum += w(i);
-      red[threadIdx.x + 1] = sum;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        red[0] = 0.0;
-        for (int i = 1; i <= kVerThreads; ++i) red[i] += red[i - 1];
-        if (red[kVerThreads] > 0) {
-          const double at = (double)a.u[(size_t)seq * (a.t + 1) + a.t] * red[kVerThreads];
-          int last = -1;
-          for (int c = 0; c < kVerThreads && pick < 0; ++c) {
-            if (red[c + 1] <= at && c + 1 < kVerThreads) {
-              continue;
-            }
-            double s = red[c];
-            for (int i = c * each; i < min(V, c * each + each); ++i) {
-              const double wi = w(i);
-              s += wi;
-              if (wi > 0) last = i;
-              if (s > at) {
-                pick = i;
-                break;
-              }
-            }
-          }
-          if (pick < 0) pick = last;
-        }
-      }
-      __syncthreads();
+      token = find_token(a, s.next_u, sum, weigh, sh);
+    } else if (d.j < s.n && !a.draft) {  // q was all on this draft
+      const int x = a.ids[(size_t)s.id * a.t + d.j];
+      if (x >= 0 && x < a.vocab) token = draw_target(a, s, d.j, st, d.p, x, sh);
     }
-    if (threadIdx.x == 0) {
-      tok[j] = pick;
-      if (lp)
-        lp[j] = pick < 0 ? 0.0f
-                         : (float)((logit(row[pick]) == P.top ? 0.0 : (double)(logit(row[pick]) - P.top) / heat) -
-                                   log(P.total));
-      for (int i = j + 1; i <= a.t; ++i) {
-        tok[i] = -1;
-        if (lp) lp[i] = 0.0f;
-      }
-      a.accepted[seq] = j;
+    if (token < 0) token = draw_target(a, s, d.j, st, d.p, -1, sh);  // also where nothing is left of p - q
+  }
+  const size_t at = (size_t)s.id * (a.t + 1);
+  for (int i = d.j + (int)threadIdx.x; i <= a.t; i += kThreads) {
+    a.tokens[at + i] = i == d.j ? token : -1;
+    if (a.logp) a.logp[at + i] = i == d.j && token >= 0 ? log_prob(s, d.p, target_row(a, s.id, d.j)[token]) : 0.0f;
+  }
+  if (threadIdx.x == 0) a.accepted[s.id] = d.j;
+}
+
+// One chunk of one row that its sequence's decision may need.
+__global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs a) {
+  __shared__ Shared sh;
+  const int chunk = blockIdx.x, row = blockIdx.y;
+  const Seq s = seq_of(a, blockIdx.z);
+  const bool of_target = row <= a.t;
+  if (of_target ? row > s.n : s.greedy || row - a.t - 1 >= s.n) return;
+  const RowStat r =
+      chunk_stat(s, of_target ? target_row(a, s.id, row) : draft_row(a, s.id, row - a.t - 1), chunk, a.vocab, sh);
+  if (threadIdx.x == 0) a.stats[((size_t)s.id * a.rows + row) * a.chunks + chunk] = r;
+}
+
+// A sequence's drafts in order, as many at a time as the workgroup has waves; then its next token (DRAFT: one chunk of the
+// weights that it may be drawn from).
+template <bool DRAFT>
+__global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArgs a) {
+  __shared__ Shared sh;
+  const int chunk = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const Seq s = seq_of(a, blockIdx.y);
+  const RowStat* const st = a.stats + (size_t)s.id * a.rows * a.chunks;
+  Decision d;
+  for (int j0 = 0;; j0 += kWaves) {
+    const int j = j0 + w;
+    if (j <= s.n) {
+      const RowStat p = row_stat(s, st + (size_t)j * a.chunks, a.chunks);
+      RowStat q = p;
+      if (DRAFT && !s.greedy && j < s.n) q = row_stat(s, st + (size_t)(a.t + 1 + j) * a.chunks, a.chunks);
+      if (lane == 0) sh.p[w] = p, sh.q[w] = q, sh.ok[w] = j < s.n && accept(a, s, j, p, q);
     }
+    __syncthreads();
+    int n = 0;  // place j0 + n is the first that is not an accepted draft (place s.n never is)
+    while (n < kWaves && sh.ok[n]) ++n;
+    if ((!DRAFT || chunk == 0) && lane == 0 && w < n) put_accepted(a, s, j, sh.p[w]);
+    if (n < kWaves) {
+      d = decision(a, s, j0 + n, sh.p[n], sh.q[n]);
+      break;
+    }
+    __syncthreads();
+  }
+  if (!DRAFT) {
+    finish(a, s, d, st + (size_t)d.j * a.chunks, 0.0, sh);
     return;
   }
+  if (chunk == 0 && threadIdx.x == 0) a.plan[s.id] = d;
+  if (!d.residual) return;
+  const double sum = residual_sum(a, s, d, chunk, sh);
+  if (threadIdx.x == 0) a.sums[(size_t)s.id * a.chunks + chunk] = sum;
+}
+
+__global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs a) {
+  __shared__ Shared sh;
+  const Seq s = seq_of(a, blockIdx.x);
+  const Decision d = a.plan[s.id];
+  const int c = threadIdx.x;
+  const double sum = d.residual && c < a.chunks ? a.sums[(size_t)s.id * a.chunks + c] : 0.0;
+  finish(a, s, d, a.stats + ((size_t)s.id * a.rows + d.j) * a.chunks, sum, sh);
+}
+
+// All of a sequence in one workgroup, row after row.
+__global__ void __launch_bounds__(kThreads) verify_whole_kernel(const VerifyArgs a) {
+  __shared__ Shared sh;
+  __shared__ RowStat st[2][kMaxChunks];
+  const Seq s = seq_of(a, blockIdx.x);
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  Decision d;
+  for (int j = 0;; ++j) {
+    const bool drafted = a.draft && !s.greedy && j < s.n;
+    for (int c = 0; c < a.chunks; ++c) {
+      const RowStat r = chunk_stat(s, target_row(a, s.id, j), c, a.vocab, sh);
+      if (threadIdx.x == 0) st[0][c] = r;
+      if (!drafted) continue;
+      const RowStat q = chunk_stat(s, draft_row(a, s.id, j), c, a.vocab, sh);
+      if (threadIdx.x == 0) st[1][c] = q;
+    }
+    __syncthreads();
+    if (w == 0) {
+      const RowStat p = row_stat(s, st[0], a.chunks);
+      const RowStat q = drafted ? row_stat(s, st[1], a.chunks) : p;
+      if (lane == 0) {
+        sh.p[0] = p, sh.q[0] = q, sh.ok[0] = j < s.n && accept(a, s, j, p, q);
+        if (sh.ok[0]) put_accepted(a, s, j, p);
+      }
+    }
+    __syncthreads();
+    if (!sh.ok[0]) {
+      d = decision(a, s, j, sh.p[0], sh.q[0]);
+      break;
+    }
+  }
+  double sum = 0.0;
+  for (int c = 0; d.residual && c < a.chunks; ++c) {
+    const double x = residual_sum(a, s, d, c, sh);
+    if (c == (int)threadIdx.x) sum = x;
+  }
+  finish(a, s, d, st[0], sum, sh);
+}
+
+VerifyArgs from(VerifyArgs a, int seq) {
+  const size_t i = (size_t)seq;
+  a.target += i * (a.t + 1) * a.ldt;
+  if (a.draft) a.draft += i * a.t * a.ldd;
+  if (a.ids) a.ids += i * a.t;
+  if (a.counts) a.counts += i;
+  if (a.temp) a.temp += i;
+  if (a.logp) a.logp += i * (a.t + 1);
+  a.u += i * (a.t + 1), a.tokens += i * (a.t + 1), a.accepted += i;
+  return a;
+}
+
+int launch(VerifyArgs a, int b, hipStream_t st) {
+  a.chunks = (a.vocab + kChunk - 1) / kChunk;
+  a.rows = a.t + 1 + (a.draft ? a.t : 0);
+  const size_t per = (size_t)a.chunks * (a.rows * sizeof(RowStat) + sizeof(double)) + sizeof(Decision);
+  const size_t most = kMaxScratch / per < 65535 ? kMaxScratch / per : 65535;  // (per <= 1.1 MB; a grid's y and z axes)
+  const int each = b < (int)most ? b : (int)most;
+  std::lock_guard<std::mutex> lock(scratch_mutex(st));  // the launches that share the scratch stay together
+  uint8_t* const z = call_scratch(st, per * each).data;
+  if (!z) {
+    hipLaunchKernelGGL(verify_whole_kernel, dim3((unsigned)b), dim3(kThreads), 0, st, a);
+    return (int)hipGetLastError();
+  }
+  a.stats = reinterpret_cast<RowStat*>(z);
+  a.plan = reinterpret_cast<Decision*>(a.stats + (size_t)each * a.rows * a.chunks);
+  a.sums = reinterpret_cast<double*>(a.plan + each);
+  for (int i = 0; i < b; i += each) {
+    const VerifyArgs l = from(a, i);
+    const unsigned n = (unsigned)(b - i < each ? b - i : each), chunks = (unsigned)a.chunks;
+    hipLaunchKernelGGL(verify_rows_kernel, dim3(chunks, (unsigned)a.rows, n), dim3(kThreads), 0, st, l);
+    if (const int e = (int)hipGetLastError()) return e;
+    if (a.draft) {
+      hipLaunchKernelGGL(verify_decide_kernel<true>, dim3(chunks, n), dim3(kThreads), 0, st, l);
+      if (const int e = (int)hipGetLastError()) return e;
+      hipLaunchKernelGGL(verify_draw_kernel, dim3(n), dim3(kThreads), 0, st, l);
+    } else {
+      hipLaunchKernelGGL(verify_decide_kernel<false>, dim3(1, n), dim3(kThreads), 0, st, l);
+    }
+    if (const int e = (int)hipGetLastError()) return e;
+  }
+  return 0;
 }
 
 }  // namespace
@@ -158,13 +501,16 @@ __global__ void __launch_bounds__(kVerThreads) spec_verify_kernel(const VerifyAr
 extern "C" int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, const int* ids,
                               const int* counts, const float* u, const float* temperature, int b, int t, int vocab,
                               int* tokens, int* accepted, float* logp, void* stream) {
-  if (b < 0 || t < 0 || t > AK_VERIFY_MAX_DRAFTS || vocab < 1 || ldt < vocab || (draft && t && ldd < vocab))
+  if (b < 0 || t < 0 || t > AK_VERIFY_MAX_DRAFTS || vocab < 1 || vocab > AK_VERIFY_MAX_VOCAB || ldt < vocab ||
+      (draft && t && ldd < vocab))
     return AK_INVALID;
   if (!b) return 0;
   if (!target || (t && !ids) || !u || !tokens || !accepted) return AK_INVALID;
-  const agq::VerifyArgs a{static_cast<const uint16_t*>(target), t ? static_cast<const uint16_t*>(draft) : nullptr, ids,
-                          counts, u, temperature, tokens, accepted, logp, ldt, ldd, b, t, vocab};
-  hipLaunchKernelGGL(agq::spec_verify_kernel, dim3((unsigned)b), dim3(agq::kVerThreads), 0,
-                     static_cast<hipStream_t>(stream), a);
-  return (int)hipGetLastError();
+  agq::VerifyArgs a{};
+  a.target = static_cast<const uint16_t*>(target);
+  a.draft = t ? static_cast<const uint16_t*>(draft) : nullptr;
+  a.ids = ids, a.counts = counts, a.u = u, a.temp = temperature;
+  a.tokens = tokens, a.accepted = accepted, a.logp = logp;
+  a.ldt = ldt, a.ldd = ldd, a.t = t, a.vocab = vocab;
+  return agq::launch(a, b, static_cast<hipStream_t>(stream));
 }

@@ -289,6 +289,7 @@ int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, in
  * NaN logits count as -inf; a row of nothing else rejects its draft and gives the token -1.  Weights are computed in fp32,
  * their sums in 64 bits in an order that does not depend on b. */
 #define AK_VERIFY_MAX_DRAFTS 127
+#define AK_VERIFY_MAX_VOCAB 1048576
 int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, const int* ids, const int* counts,
                    const float* u, const float* temperature, int b, int t, int vocab, int* tokens, int* accepted,
                    float* logp, void* stream);
