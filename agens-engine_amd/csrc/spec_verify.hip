@@ -67,7 +67,7 @@ struct VerifyArgs {
 struct Shared {
   double red[kWaves];
   int ired[kWaves];
-  double pick_before;
+  double before[kWaves];
   RowStat p[kWaves], q[kWaves];
   int ok[kWaves];
 };
@@ -156,34 +156,51 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
   __syncthreads();
   if ((t & 63) == 0) sh.red[t >> 6] = top;
-  if (t == 0) sh.ired[0] = 0x7FFFFFFF;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) top = fmaxf(top, (float)sh.red[i]);
+  // the lowest token with it: in the first half before the second, there in the first wave, lane and place
+  int best0 = -1, best1 = -1;
   if (mine == top && top > -INFINITY) {
-    int best = 0x7FFFFFFF;
 #pragma unroll
-    for (int i = kEach - 1; i >= 0; --i)
-      if (l[i] == top) best = (i < 8 ? at0 : at1 - 8) + i;
-    atomicMin(&sh.ired[0], best);
+    for (int i = 7; i >= 0; --i) {
+      if (l[i] == top) best0 = at0 + i;
+      if (l[i + 8] == top) best1 = at1 + i;
+    }
+  }
+  const uint64_t in0 = __ballot(best0 >= 0), in1 = __ballot(best1 >= 0);
+  if (in0 | in1) {
+    const int best = __shfl(in0 ? best0 : best1, __builtin_ctzll(in0 ? in0 : in1));
+    if ((t & 63) == 0) sh.ired[t >> 6] = best;
+  } else if ((t & 63) == 0) {
+    sh.ired[t >> 6] = 0x7FFFFFFF;
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i) l[i] = weight(s, l[i], top);
   const double total = block_sum(sum16(l), sh);
-  return RowStat{top, sh.ired[0] == 0x7FFFFFFF ? -1 : sh.ired[0], total};
+  int best = sh.ired[0];
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) best = min(best, sh.ired[i]);
+  return RowStat{top, best == 0x7FFFFFFF ? -1 : best, total};
 }
 
-// How much a chunk's sum counts in its row: in 64 bits, so that a row's sum is as good as its chunks'.
+// How much a chunk's sum counts in its row.
 __device__ __forceinline__ double chunk_share(const Seq& s, const RowStat& c, float top) {
-  return c.top == -INFINITY ? 0.0 : c.total * exp2((double)(c.top - top) * ((double)s.scale + (double)s.scale_lo));
+  return c.total * (double)weight(s, c.top, top);
 }
 
 // A row from its chunks, by one wave.
 __device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int chunks) {
   const int lane = threadIdx.x & 63;
-  RowStat r{-INFINITY, 0x7FFFFFFF, 0.0};
-  for (int c = lane; c < chunks; c += 64)
-    if (st[c].top > r.top) r.top = st[c].top, r.best = st[c].best;
+  RowStat c[kMaxChunks / 64], r{-INFINITY, 0x7FFFFFFF, 0.0};
+#pragma unroll
+  for (int i = 0; i < kMaxChunks / 64; ++i) {
+    c[i] = RowStat{-INFINITY, 0x7FFFFFFF, 0.0};
+    if (lane + 64 * i < chunks) c[i] = st[lane + 64 * i];
+  }
+#pragma unroll
+  for (int i = 0; i < kMaxChunks / 64; ++i)
+    if (c[i].top > r.top) r.top = c[i].top, r.best = c[i].best;
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const float m = __shfl_xor(r.top, d);
@@ -194,7 +211,8 @@ __device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int
     r.best = -1;
     return r;
   }
-  for (int c = lane; c < chunks; c += 64) r.total += chunk_share(s, st[c], r.top);
+#pragma unroll
+  for (int i = 0; i < kMaxChunks / 64; ++i) r.total += chunk_share(s, c[i], r.top);
 #pragma unroll
   for (int d = 32; d; d >>= 1) r.total += __shfl_xor(r.total, d);
   return r;
@@ -212,21 +230,23 @@ __device__ __forceinline__ int pick_thread(double x, double at, Shared& sh, doub
   }
   __syncthreads();
   if (lane == 63) sh.red[w] = inc;
-  if (threadIdx.x == 0) sh.ired[0] = 0x7FFFFFFF, sh.ired[1] = -1;
   __syncthreads();
   double b = inc - x;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i)
     if (i < w) b += sh.red[i];
-  if (x > 0.0) {
-    if (b + x > at) atomicMin(&sh.ired[0], (int)threadIdx.x);
-    atomicMax(&sh.ired[1], (int)threadIdx.x);
+  const uint64_t past = __ballot(x > 0.0 && b + x > at), any = __ballot(x > 0.0);
+  const int mine = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : -1;  // of the wave
+  if (lane == mine) sh.before[w] = b;
+  if (lane == 0) sh.ired[w] = mine < 0 ? -1 : 64 * w + mine, sh.ok[w] = past != 0;
+  __syncthreads();
+  int pick = -1;
+  for (int i = 0; i < kWaves; ++i) {
+    if (sh.ired[i] < 0) continue;
+    pick = sh.ired[i], *before = sh.before[i];
+    if (sh.ok[i]) break;
   }
   __syncthreads();
-  const int pick = sh.ired[0] != 0x7FFFFFFF ? sh.ired[0] : sh.ired[1];
-  if ((int)threadIdx.x == pick) sh.pick_before = b;
-  __syncthreads();
-  *before = sh.pick_before;
   return pick;
 }
 
