@@ -101,12 +101,24 @@ __device__ __forceinline__ const uint16_t* draft_row(const VerifyArgs& a, int se
   return a.draft + ((size_t)seq * a.t + j) * a.ldd;
 }
 
-// NaN counts as -inf; +inf as a number above every finite bf16, so that differences stay numbers.
-__device__ __forceinline__ float logit(uint32_t b) { return fminf(fmaxf(bf2f((uint16_t)b), -INFINITY), FLT_MAX); }
-// The weight of logit l in a row whose largest is top.
+// The weight of logit l in a row whose largest is top (not +inf).  The clamp takes a masked logit's -inf, and NaN, to a
+// difference whose weight is 0.
 __device__ __forceinline__ float weight(const Seq& s, float l, float top) {
   const float d = fmaxf(l - (top == -INFINITY ? 0.0f : top), -FLT_MAX);
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, s.scale, d * s.scale_lo));
+}
+// Of any row: where the largest is +inf, all that are it weigh the same.
+__device__ __forceinline__ float any_weight(const Seq& s, float l, float top) {
+  return top == INFINITY ? (l == top ? 1.0f : 0.0f) : weight(s, l, top);
+}
+__device__ __forceinline__ void weigh16(const Seq& s, float top, float (&l)[kEach]) {
+  if (top == INFINITY) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) l[i] = l[i] == top ? 1.0f : 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) l[i] = weight(s, l[i], top);
+  }
 }
 
 // 8 logits from token k on, -inf past the end.  Rows begin at any even address.
@@ -115,10 +127,10 @@ __device__ __forceinline__ void load8(const uint16_t* row, int k, int vocab, flo
   if (k + 8 <= vocab) {
     const u32x4 v = *reinterpret_cast<const u32x4_any*>(row + k);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) l[i] = logit((v[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
+    for (int i = 0; i < 8; ++i) l[i] = __uint_as_float(i & 1 ? v[i >> 1] & 0xFFFF0000u : v[i >> 1] << 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) l[i] = k + i < vocab ? logit(row[k + i]) : -INFINITY;
+    for (int i = 0; i < 8; ++i) l[i] = k + i < vocab ? bf2f(row[k + i]) : -INFINITY;
   }
 }
 
@@ -129,10 +141,55 @@ __device__ __forceinline__ double sum16(const float (&w)[kEach]) {
   return (double)s;
 }
 
+// Over the lanes of a wave, by DPP (an LDS exchange takes several times as long): x of the lane `ctrl` names, `none` where
+// there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t x, uint32_t none) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)none, (int)x, CTRL, ROWS, 0xF, false);
+}
+// op over the lanes up to each one: row_shr 1, 2, 4, 8 within the rows of 16, then the rows' last lanes
+template <class T, class Op>
+__device__ __forceinline__ T wave_scan(T x, Op op) {
+  x = op.template step<0x111, 0xF>(x);
+  x = op.template step<0x112, 0xF>(x);
+  x = op.template step<0x114, 0xF>(x);
+  x = op.template step<0x118, 0xF>(x);
+  x = op.template step<0x142, 0xA>(x);  // row_bcast 15
+  return op.template step<0x143, 0xC>(x);  // row_bcast 31
+}
+struct Add {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ double step(double x) const {
+    const uint64_t v = (uint64_t)__double_as_longlong(x);
+    return x + __longlong_as_double((long long)((uint64_t)dpp<CTRL, ROWS>((uint32_t)(v >> 32), 0) << 32 |
+                                                dpp<CTRL, ROWS>((uint32_t)v, 0)));
+  }
+};
+struct Max {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ float step(float x) const {
+    return fmaxf(x, __uint_as_float(dpp<CTRL, ROWS>(__float_as_uint(x), 0xFF800000u)));
+  }
+};
+struct Min {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ int step(int x) const {
+    return min(x, (int)dpp<CTRL, ROWS>((uint32_t)x, 0x7FFFFFFFu));
+  }
+};
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)x, 63); }
+__device__ __forceinline__ double wave_sum(double x) {
+  const uint64_t v = (uint64_t)__double_as_longlong(wave_scan(x, Add()));
+  return __longlong_as_double((long long)((uint64_t)last_lane((uint32_t)(v >> 32)) << 32 | last_lane((uint32_t)v)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __uint_as_float(last_lane(__float_as_uint(wave_scan(x, Max()))));
+}
+__device__ __forceinline__ int wave_min(int x) { return (int)last_lane((uint32_t)wave_scan(x, Min())); }
+
 // The sum over the workgroup, in every thread.
 __device__ __forceinline__ double block_sum(double x, Shared& sh) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d);
+  x = wave_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = x;
   __syncthreads();
@@ -151,9 +208,7 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
   float mine = l[0];
 #pragma unroll
   for (int i = 1; i < kEach; ++i) mine = fmaxf(mine, l[i]);
-  float top = mine;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  float top = wave_max(mine);
   __syncthreads();
   if ((t & 63) == 0) sh.red[t >> 6] = top;
   __syncthreads();
@@ -175,8 +230,7 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
   } else if ((t & 63) == 0) {
     sh.ired[t >> 6] = 0x7FFFFFFF;
   }
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) l[i] = weight(s, l[i], top);
+  weigh16(s, top, l);
   const double total = block_sum(sum16(l), sh);
   int best = sh.ired[0];
 #pragma unroll
@@ -186,7 +240,7 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
 
 // How much a chunk's sum counts in its row.
 __device__ __forceinline__ double chunk_share(const Seq& s, const RowStat& c, float top) {
-  return c.total * (double)weight(s, c.top, top);
+  return c.total * (double)any_weight(s, c.top, top);
 }
 
 // A row from its chunks, by one wave.
@@ -201,20 +255,13 @@ __device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int
 #pragma unroll
   for (int i = 0; i < kMaxChunks / 64; ++i)
     if (c[i].top > r.top) r.top = c[i].top, r.best = c[i].best;
-#pragma unroll
-  for (int d = 32; d; d >>= 1) {
-    const float m = __shfl_xor(r.top, d);
-    const int i = __shfl_xor(r.best, d);
-    if (m > r.top || (m == r.top && i < r.best)) r.top = m, r.best = i;
-  }
-  if (r.top == -INFINITY) {
-    r.best = -1;
-    return r;
-  }
+  const float mine = r.top;
+  r.top = wave_max(mine);
+  r.best = r.top == -INFINITY ? -1 : wave_min(mine == r.top ? r.best : 0x7FFFFFFF);
+  if (r.best < 0) return r;
 #pragma unroll
   for (int i = 0; i < kMaxChunks / 64; ++i) r.total += chunk_share(s, c[i], r.top);
-#pragma unroll
-  for (int d = 32; d; d >>= 1) r.total += __shfl_xor(r.total, d);
+  r.total = wave_sum(r.total);
   return r;
 }
 
@@ -222,12 +269,7 @@ __device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int
 // -1 without any.  *before: the sum of the threads before it.
 __device__ __forceinline__ int pick_thread(double x, double at, Shared& sh, double* before) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double inc = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const double y = __shfl_up(inc, d);
-    if (lane >= d) inc += y;
-  }
+  const double inc = wave_scan(x, Add());
   __syncthreads();
   if (lane == 63) sh.red[w] = inc;
   __syncthreads();
@@ -283,8 +325,10 @@ __device__ __forceinline__ int draw_target(const VerifyArgs& a, const Seq& s, in
   auto weigh = [&](int k, float(&w)[kEach]) {
     load8(row, k, a.vocab, w);
     load8(row, k + 8, a.vocab, w + 8);
+    weigh16(s, p.top, w);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) w[i] = k + i == skip ? 0.0f : weight(s, w[i], p.top);
+    for (int i = 0; i < kEach; ++i)
+      if (k + i == skip) w[i] = 0.0f;
   };
   const int c = threadIdx.x;
   double share = c < a.chunks ? chunk_share(s, st[c], p.top) : 0.0;
@@ -298,12 +342,14 @@ __device__ __forceinline__ int draw_target(const VerifyArgs& a, const Seq& s, in
 }
 
 // The weights max(p - q, 0) of the 16 tokens from k on, with p and q normalised: in 64 bits, since the two may be close.
-__device__ __forceinline__ void residual16(const VerifyArgs& a, const Seq& s, const Decision& d, const float (&lp)[kEach],
-                                           const float (&lq)[kEach], float (&w)[kEach]) {
+__device__ __forceinline__ void residual16(const VerifyArgs& a, const Seq& s, const Decision& d, float (&lp)[kEach],
+                                           float (&lq)[kEach], float (&w)[kEach]) {
+  weigh16(s, d.p.top, lp);
+  weigh16(s, d.q.top, lq);
   const double pi = 1.0 / d.p.total, qi = 1.0 / d.q.total;
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
-    w[i] = (float)fmax(weight(s, lp[i], d.p.top) * pi - weight(s, lq[i], d.q.top) * qi, 0.0);
+    w[i] = (float)fmax(lp[i] * pi - lq[i] * qi, 0.0);
 }
 __device__ __forceinline__ double residual_sum(const VerifyArgs& a, const Seq& s, const Decision& d, int chunk, Shared& sh) {
   const uint16_t *const p = target_row(a, s.id, d.j), *const q = draft_row(a, s.id, d.j);
@@ -319,7 +365,8 @@ __device__ __forceinline__ double residual_sum(const VerifyArgs& a, const Seq& s
 }
 
 __device__ __forceinline__ float log_prob(const Seq& s, const RowStat& p, uint16_t bits) {
-  return (float)((double)(logit(bits) - p.top) / (double)s.heat - log(p.total));
+  const float l = bf2f(bits);
+  return (float)((l == p.top ? 0.0 : (double)(l - p.top) / (double)s.heat) - log(p.total));
 }
 
 // Whether draft j is accepted.  (One lane.)
@@ -328,8 +375,8 @@ __device__ __forceinline__ bool accept(const VerifyArgs& a, const Seq& s, int j,
   if (x < 0 || x >= a.vocab || p.best < 0) return false;
   if (s.greedy) return x == p.best;
   double qx = 1.0;
-  if (a.draft) qx = q.best < 0 ? 0.0 : weight(s, logit(draft_row(a, s.id, j)[x]), q.top) / q.total;
-  return a.u[(size_t)s.id * (a.t + 1) + j] * qx < weight(s, logit(target_row(a, s.id, j)[x]), p.top) / p.total;
+  if (a.draft) qx = q.best < 0 ? 0.0 : any_weight(s, bf2f(draft_row(a, s.id, j)[x]), q.top) / q.total;
+  return a.u[(size_t)s.id * (a.t + 1) + j] * qx < any_weight(s, bf2f(target_row(a, s.id, j)[x]), p.top) / p.total;
 }
 __device__ __forceinline__ void put_accepted(const VerifyArgs& a, const Seq& s, int j, const RowStat& p) {
   const int x = a.ids[(size_t)s.id * a.t + j];
