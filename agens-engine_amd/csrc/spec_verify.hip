@@ -243,15 +243,23 @@ __device__ __forceinline__ double chunk_share(const Seq& s, const RowStat& c, fl
   return c.total * (double)any_weight(s, c.top, top);
 }
 
-// A row from its chunks, by one wave.
-__device__ __forceinline__ RowStat row_stat(const Seq& s, const RowStat* st, int chunks) {
+// A row from its chunks, by one wave: their loads (the lane's chunks), then the rest.
+struct Chunks {
+  RowStat c[kMaxChunks / 64];
+};
+__device__ __forceinline__ Chunks load_chunks(const RowStat* st, int chunks) {
   const int lane = threadIdx.x & 63;
-  RowStat c[kMaxChunks / 64], r{-INFINITY, 0x7FFFFFFF, 0.0};
+  Chunks x;
 #pragma unroll
   for (int i = 0; i < kMaxChunks / 64; ++i) {
-    c[i] = RowStat{-INFINITY, 0x7FFFFFFF, 0.0};
-    if (lane + 64 * i < chunks) c[i] = st[lane + 64 * i];
+    x.c[i] = RowStat{-INFINITY, 0x7FFFFFFF, 0.0};
+    if (lane + 64 * i < chunks) x.c[i] = st[lane + 64 * i];
   }
+  return x;
+}
+__device__ __forceinline__ RowStat row_stat(const Seq& s, const Chunks& x) {
+  const RowStat(&c)[kMaxChunks / 64] = x.c;
+  RowStat r{-INFINITY, 0x7FFFFFFF, 0.0};
 #pragma unroll
   for (int i = 0; i < kMaxChunks / 64; ++i)
     if (c[i].top > r.top) r.top = c[i].top, r.best = c[i].best;
@@ -369,14 +377,27 @@ __device__ __forceinline__ float log_prob(const Seq& s, const RowStat& p, uint16
   return (float)((l == p.top ? 0.0 : (double)(l - p.top) / (double)s.heat) - log(p.total));
 }
 
-// Whether draft j is accepted.  (One lane.)
-__device__ __forceinline__ bool accept(const VerifyArgs& a, const Seq& s, int j, const RowStat& p, const RowStat& q) {
-  const int x = a.ids[(size_t)s.id * a.t + j];
-  if (x < 0 || x >= a.vocab || p.best < 0) return false;
-  if (s.greedy) return x == p.best;
+// What the decision on draft j needs besides the sums: loaded before they are there.
+struct Draft {
+  int x;
+  float u, lp, lq;
+};
+__device__ __forceinline__ Draft load_draft(const VerifyArgs& a, const Seq& s, int j) {
+  Draft d{a.ids[(size_t)s.id * a.t + j], a.u[(size_t)s.id * (a.t + 1) + j], -INFINITY, -INFINITY};
+  if (d.x >= 0 && d.x < a.vocab) {
+    d.lp = bf2f(target_row(a, s.id, j)[d.x]);
+    if (a.draft) d.lq = bf2f(draft_row(a, s.id, j)[d.x]);
+  } else {
+    d.x = -1;
+  }
+  return d;
+}
+__device__ __forceinline__ bool accept(const VerifyArgs& a, const Seq& s, const Draft& d, const RowStat& p, const RowStat& q) {
+  if (d.x < 0 || p.best < 0) return false;
+  if (s.greedy) return d.x == p.best;
   double qx = 1.0;
-  if (a.draft) qx = q.best < 0 ? 0.0 : any_weight(s, bf2f(draft_row(a, s.id, j)[x]), q.top) / q.total;
-  return a.u[(size_t)s.id * (a.t + 1) + j] * qx < any_weight(s, bf2f(target_row(a, s.id, j)[x]), p.top) / p.total;
+  if (a.draft) qx = q.best < 0 ? 0.0 : any_weight(s, d.lq, q.top) / q.total;
+  return d.u * qx < any_weight(s, d.lp, p.top) / p.total;
 }
 __device__ __forceinline__ void put_accepted(const VerifyArgs& a, const Seq& s, int j, const RowStat& p) {
   const int x = a.ids[(size_t)s.id * a.t + j];
@@ -445,10 +466,12 @@ __global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArg
   for (int j0 = 0;; j0 += kWaves) {
     const int j = j0 + w;
     if (j <= s.n) {
-      const RowStat p = row_stat(s, st + (size_t)j * a.chunks, a.chunks);
-      RowStat q = p;
-      if (DRAFT && !s.greedy && j < s.n) q = row_stat(s, st + (size_t)(a.t + 1 + j) * a.chunks, a.chunks);
-      if (lane == 0) sh.p[w] = p, sh.q[w] = q, sh.ok[w] = j < s.n && accept(a, s, j, p, q);
+      const bool drafted = DRAFT && !s.greedy && j < s.n;
+      const Chunks pc = load_chunks(st + (size_t)j * a.chunks, a.chunks);
+      const Chunks qc = load_chunks(st + (size_t)(drafted ? a.t + 1 + j : j) * a.chunks, DRAFT ? a.chunks : 0);
+      const Draft x = j < s.n ? load_draft(a, s, j) : Draft{-1, 0.0f, 0.0f, 0.0f};
+      const RowStat p = row_stat(s, pc), q = drafted ? row_stat(s, qc) : p;
+      if (lane == 0) sh.p[w] = p, sh.q[w] = q, sh.ok[w] = accept(a, s, x, p, q);
     }
     __syncthreads();
     int n = 0;  // place j0 + n is the first that is not an accepted draft (place s.n never is)
@@ -497,10 +520,11 @@ __global__ void __launch_bounds__(kThreads) verify_whole_kernel(const VerifyArgs
     }
     __syncthreads();
     if (w == 0) {
-      const RowStat p = row_stat(s, st[0], a.chunks);
-      const RowStat q = drafted ? row_stat(s, st[1], a.chunks) : p;
+      const RowStat p = row_stat(s, load_chunks(st[0], a.chunks));
+      const RowStat q = drafted ? row_stat(s, load_chunks(st[1], a.chunks)) : p;
+      const Draft x = j < s.n ? load_draft(a, s, j) : Draft{-1, 0.0f, 0.0f, 0.0f};
       if (lane == 0) {
-        sh.p[0] = p, sh.q[0] = q, sh.ok[0] = j < s.n && accept(a, s, j, p, q);
+        sh.p[0] = p, sh.q[0] = q, sh.ok[0] = accept(a, s, x, p, q);
         if (sh.ok[0]) put_accepted(a, s, j, p);
       }
     }
