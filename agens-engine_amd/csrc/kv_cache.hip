@@ -3,9 +3,10 @@
 // Quantisation of a row x of dim values (one token, one head, keys or values), Q = 127 (8 bits) or 7 (4 bits):
 //   s = bf16(max|x| / Q), q = rint(x / s) clamped to +-Q, the value held is q * s.
 // The codes are those of the rounded scale that readers multiply with, so the rounding of s costs no accuracy beyond the
-// clamped end (x / s <= Q (1 + 2^-9), less than half a step).  x / s is the fp32 quotient: bf16 over bf16 is never close
-// enough to a half for that rounding to move rint, so the codes are those of exact arithmetic.  A row whose s would lie
-// below 2^-126 is held as zeros; one with a non-finite value gets the scale NaN and reads back as NaN.
+// clamped end (x / s <= Q (1 + 2^-9), less than half a step).  The codes are those of exact arithmetic: two bf16's quotient is
+// a half or at least 2^-11 from one, and q0 = x * (1 / s), q0 + (x - q0 s) / s is right to the last bit where it is a half.
+// (Without a division: 16384 tokens of 8 heads 34 -> TIME us.)  A row whose s would lie below 2^-126 is held as zeros; one
+// with a non-finite value gets the scale NaN and reads back as NaN.
 //
 // Both kernels are streams: dim / 8 lanes take the keys and the values of one (token, head), 16 bytes of bf16 a lane each;
 // the largest magnitude is found by lane exchanges.  Consecutive groups take consecutive tokens of one head, whose
@@ -24,7 +25,7 @@ struct KvArgs {
   long ldk, ldv;
   const int* slots;
   uint8_t* pool;
-  int m;
+  int m, page_log2;
 };
 
 struct KvPlace {
@@ -33,8 +34,8 @@ struct KvPlace {
 };
 __device__ __forceinline__ KvPlace place(const KvArgs& a, int slot, int head) {
   const KvShape& s = a.s;
-  uint8_t* const pg = a.pool + s.bytes() * (size_t)(slot / s.page);
-  const size_t off = slot % s.page;
+  uint8_t* const pg = a.pool + s.bytes() * (size_t)(slot >> a.page_log2);
+  const size_t off = slot & (s.page - 1);
   KvPlace p;
   p.krow = pg + s.plane() * (2 * (size_t)head) + off * s.row_bytes();
   p.vrow = p.krow + s.plane();
@@ -52,8 +53,12 @@ __device__ __forceinline__ uint32_t row_amax(const uint4 x) {
     const uint32_t lo = w[i] & 0x7FFFu, hi = (w[i] >> 16) & 0x7FFFu;
     m = max(m, max(lo, hi));
   }
-#pragma unroll
-  for (int d = LANES / 2; d; d >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
+  auto with = [&](int other) { m = max(m, (uint32_t)other); };
+  with(__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true));   // quad_perm [1, 0, 3, 2]
+  with(__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true));   // quad_perm [2, 3, 0, 1]
+  with(__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true));  // row_half_mirror
+  if constexpr (LANES >= 16) with(__builtin_amdgcn_mov_dpp((int)m, 0x140, 0xF, 0xF, true));  // row_mirror
+  if constexpr (LANES >= 32) with(__shfl_xor((int)m, 16));
   return m;
 }
 
@@ -66,52 +71,66 @@ __device__ __forceinline__ uint64_t quantise8(const uint4 x, uint32_t amax, uint
   if (sb < 0x0080u) sb = 0;             // below 2^-126
   if (amax >= 0x7F80u) sb = 0x7FC0u;    // a NaN or Inf in the row
   *sbits = sb;
-  const float s = bf2f(sb);
+  const bool held = sb != 0 && sb != 0x7FC0u;
+  const float up = sb < 0x2000u ? 0x1p64f : 1.0f;  // where x - q0 s would lose bits below 2^-149
+  const float s = held ? bf2f(sb) * up : 1.0f, r = __builtin_amdgcn_rcpf(s);
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint64_t out = 0;
+  uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float f = bf2f((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu);
-    float q = rintf(f / s);
-    q = fminf(fmaxf(q, -Q), Q);  // (also takes NaN, of a zero or NaN scale, to a code)
-    const int code = sb == 0 || sb == 0x7FC0u ? kOff : (int)q + kOff;
-    out |= (uint64_t)(uint32_t)code << (BITS * i);
+    const float f = bf2f((w[i >> 1] >> (16 * (i & 1))) & 0xFFFFu) * up;
+    float q = f * r;
+    q = __builtin_fmaf(__builtin_fmaf(-q, s, f), r, q);
+    q = fminf(fmaxf(q, -Q), Q);
+    c[i] = __float_as_uint(q + (0x1.8p23f + (float)kOff));  // rounds to the even of two; the integer is in the low bits
+  }
+  uint64_t out = 0;
+  if constexpr (BITS == 8) {
+    uint32_t h[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      h[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[4 * i + 3], c[4 * i + 2], 0x0C0C0400u),
+                                   __builtin_amdgcn_perm(c[4 * i + 1], c[4 * i], 0x0C0C0400u), 0x05040100u);
+    out = held ? (uint64_t)h[1] << 32 | h[0] : 0x8080808080808080ull;
+  } else {
+    uint32_t h = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h |= (c[i] & 15u) << (4 * i);
+    out = held ? h : 0x88888888u;
   }
   return out;
 }
 
 template <int BITS, int D>
-__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvArgs a, long groups) {
+__global__ void __launch_bounds__(kKvThreads) kv_write_kernel(const KvArgs a) {
   constexpr int LANES = D / 8;
   const int l = threadIdx.x % LANES;
-  for (long g = (long)blockIdx.x * (kKvThreads / LANES) + threadIdx.x / LANES; g < groups;
-       g += (long)gridDim.x * (kKvThreads / LANES)) {
-    const int t = (int)(g % a.m), head = (int)(g / a.m);
-    const int slot = a.slots[t];
-    if (slot < 0 || slot / a.s.page >= a.s.npages) continue;  // (whole groups of lanes)
-    const uint4 k = *reinterpret_cast<const uint4*>(a.k + (size_t)t * a.ldk + head * D + l * 8);
-    const uint4 v = *reinterpret_cast<const uint4*>(a.v + (size_t)t * a.ldv + head * D + l * 8);
-    const KvPlace p = place(a, slot, head);
-    if constexpr (BITS == 16) {
-      reinterpret_cast<uint4*>(p.krow)[l] = k;
-      reinterpret_cast<uint4*>(p.vrow)[l] = v;
+  const int t = (int)blockIdx.x * (kKvThreads / LANES) + threadIdx.x / LANES, head = blockIdx.y;
+  if (t >= a.m) return;
+  const int slot = a.slots[t];
+  if (slot < 0 || slot >> a.page_log2 >= a.s.npages) return;  // (whole groups of lanes)
+  const uint4 k = *reinterpret_cast<const uint4*>(a.k + (size_t)t * a.ldk + head * D + l * 8);
+  const uint4 v = *reinterpret_cast<const uint4*>(a.v + (size_t)t * a.ldv + head * D + l * 8);
+  const KvPlace p = place(a, slot, head);
+  if constexpr (BITS == 16) {
+    reinterpret_cast<uint4*>(p.krow)[l] = k;
+    reinterpret_cast<uint4*>(p.vrow)[l] = v;
+  } else {
+    uint32_t ks, vs;
+    const uint64_t kc = quantise8<BITS>(k, row_amax<LANES>(k), &ks);
+    const uint64_t vc = quantise8<BITS>(v, row_amax<LANES>(v), &vs);
+    if constexpr (BITS == 8) {
+      reinterpret_cast<uint64_t*>(p.krow)[l] = kc;
+      reinterpret_cast<uint64_t*>(p.vrow)[l] = vc;
     } else {
-      uint32_t ks, vs;
-      const uint64_t kc = quantise8<BITS>(k, row_amax<LANES>(k), &ks);
-      const uint64_t vc = quantise8<BITS>(v, row_amax<LANES>(v), &vs);
-      if constexpr (BITS == 8) {
-        reinterpret_cast<uint64_t*>(p.krow)[l] = kc;
-        reinterpret_cast<uint64_t*>(p.vrow)[l] = vc;
-      } else {
-        reinterpret_cast<uint32_t*>(p.krow)[l] = (uint32_t)kc;
-        reinterpret_cast<uint32_t*>(p.vrow)[l] = (uint32_t)vc;
-      }
-      if (l == 0) *p.pair = ks | (vs << 16);
+      reinterpret_cast<uint32_t*>(p.krow)[l] = (uint32_t)kc;
+      reinterpret_cast<uint32_t*>(p.vrow)[l] = (uint32_t)vc;
     }
+    if (l == 0) *p.pair = ks | (vs << 16);
   }
 }
 
-// codes -> 8 packed bf16 values q * s, rounded once
+// codes -> 8 packed bf16 values q * s, rounded once (the product is exact in fp32)
 template <int BITS>
 __device__ __forceinline__ uint4 dequantise8(uint64_t c, float s) {
   uint32_t w[4];
@@ -120,8 +139,8 @@ __device__ __forceinline__ uint4 dequantise8(uint64_t c, float s) {
     uint32_t r = 0;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int code = (int)((c >> (BITS * (2 * i + e))) & ((1u << BITS) - 1)) - (1 << (BITS - 1));
-      r |= (uint32_t)f2bf((float)code * s) << (16 * e);
+      const uint32_t code = (uint32_t)(c >> (BITS * (2 * i + e))) & ((1u << BITS) - 1);
+      r |= (uint32_t)f2bf(((float)code - (float)(1 << (BITS - 1))) * s) << (16 * e);
     }
     w[i] = r;
   }
@@ -129,48 +148,44 @@ __device__ __forceinline__ uint4 dequantise8(uint64_t c, float s) {
 }
 
 template <int BITS, int D>
-__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvArgs a, long groups) {
+__global__ void __launch_bounds__(kKvThreads) kv_read_kernel(const KvArgs a) {
   constexpr int LANES = D / 8;
   const int l = threadIdx.x % LANES;
-  for (long g = (long)blockIdx.x * (kKvThreads / LANES) + threadIdx.x / LANES; g < groups;
-       g += (long)gridDim.x * (kKvThreads / LANES)) {
-    const int t = (int)(g % a.m), head = (int)(g / a.m);
-    const int slot = a.slots[t];
-    uint4 k = make_uint4(0, 0, 0, 0), v = k;
-    if (slot >= 0 && slot / a.s.page < a.s.npages) {
-      const KvPlace p = place(a, slot, head);
-      if constexpr (BITS == 16) {
-        k = reinterpret_cast<const uint4*>(p.krow)[l];
-        v = reinterpret_cast<const uint4*>(p.vrow)[l];
+  const int t = (int)blockIdx.x * (kKvThreads / LANES) + threadIdx.x / LANES, head = blockIdx.y;
+  if (t >= a.m) return;
+  const int slot = a.slots[t];
+  uint4 k = make_uint4(0, 0, 0, 0), v = k;
+  if (slot >= 0 && slot >> a.page_log2 < a.s.npages) {
+    const KvPlace p = place(a, slot, head);
+    if constexpr (BITS == 16) {
+      k = reinterpret_cast<const uint4*>(p.krow)[l];
+      v = reinterpret_cast<const uint4*>(p.vrow)[l];
+    } else {
+      const uint32_t pair = *p.pair;
+      uint64_t kc, vc;
+      if constexpr (BITS == 8) {
+        kc = reinterpret_cast<const uint64_t*>(p.krow)[l];
+        vc = reinterpret_cast<const uint64_t*>(p.vrow)[l];
       } else {
-        const uint32_t pair = *p.pair;
-        uint64_t kc, vc;
-        if constexpr (BITS == 8) {
-          kc = reinterpret_cast<const uint64_t*>(p.krow)[l];
-          vc = reinterpret_cast<const uint64_t*>(p.vrow)[l];
-        } else {
-          kc = reinterpret_cast<const uint32_t*>(p.krow)[l];
-          vc = reinterpret_cast<const uint32_t*>(p.vrow)[l];
-        }
-        k = dequantise8<BITS>(kc, bf2f(pair & 0xFFFFu));
-        v = dequantise8<BITS>(vc, bf2f(pair >> 16));
+        kc = reinterpret_cast<const uint32_t*>(p.krow)[l];
+        vc = reinterpret_cast<const uint32_t*>(p.vrow)[l];
       }
+      k = dequantise8<BITS>(kc, bf2f(pair & 0xFFFFu));
+      v = dequantise8<BITS>(vc, bf2f(pair >> 16));
     }
-    *reinterpret_cast<uint4*>(a.k + (size_t)t * a.ldk + head * D + l * 8) = k;
-    *reinterpret_cast<uint4*>(a.v + (size_t)t * a.ldv + head * D + l * 8) = v;
   }
+  *reinterpret_cast<uint4*>(a.k + (size_t)t * a.ldk + head * D + l * 8) = k;
+  *reinterpret_cast<uint4*>(a.v + (size_t)t * a.ldv + head * D + l * 8) = v;
 }
 
 template <bool WRITE, int BITS, int D>
 int launch(const KvArgs& a, hipStream_t s) {
   constexpr int per = kKvThreads / (D / 8);
-  const long groups = (long)a.m * a.s.heads;
-  long grid = (groups + per - 1) / per;
-  if (grid > 65536) grid = 65536;
+  const dim3 grid((unsigned)((a.m - 1) / per + 1), (unsigned)a.s.heads);
   if constexpr (WRITE)
-    hipLaunchKernelGGL((kv_write_kernel<BITS, D>), dim3((unsigned)grid), dim3(kKvThreads), 0, s, a, groups);
+    hipLaunchKernelGGL((kv_write_kernel<BITS, D>), grid, dim3(kKvThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((kv_read_kernel<BITS, D>), dim3((unsigned)grid), dim3(kKvThreads), 0, s, a, groups);
+    hipLaunchKernelGGL((kv_read_kernel<BITS, D>), grid, dim3(kKvThreads), 0, s, a);
   return (int)hipGetLastError();
 }
 template <bool WRITE, int BITS>
@@ -208,7 +223,7 @@ extern "C" int ak_kv_write(int bits, const void* k, const void* v, int m, long l
     return AK_INVALID;
   const agq::KvArgs a{s,     const_cast<uint16_t*>(static_cast<const uint16_t*>(k)),
                       const_cast<uint16_t*>(static_cast<const uint16_t*>(v)), ldk, ldv, slots,
-                      static_cast<uint8_t*>(pool), m};
+                      static_cast<uint8_t*>(pool), m, __builtin_ctz((unsigned)page)};
   return agq::launch_bits<true>(a, static_cast<hipStream_t>(stream));
 }
 
@@ -222,6 +237,6 @@ extern "C" int ak_kv_read(int bits, const void* pool, int npages, int page, int 
       !agq::aligned16(pool))
     return AK_INVALID;
   const agq::KvArgs a{s,   static_cast<uint16_t*>(k), static_cast<uint16_t*>(v), ldk, ldv, slots,
-                      const_cast<uint8_t*>(static_cast<const uint8_t*>(pool)), m};
+                      const_cast<uint8_t*>(static_cast<const uint8_t*>(pool)), m, __builtin_ctz((unsigned)page)};
   return agq::launch_bits<false>(a, static_cast<hipStream_t>(stream));
 }
