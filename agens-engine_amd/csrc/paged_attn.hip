@@ -521,8 +521,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
   load_queries(cur);
   x.find(a, ids, 0);
   if (nxt.end) next_ids = x.load_ids(a, nxt, nxt.part * kPart, lane);
+  // (in this order also here: the wait for the keys is the same instruction for the first chunk and all later ones)
   x.load_keys(a, cur.head, at, lane, ~0u);
+  __builtin_amdgcn_sched_barrier(0);
   x.load_values(a, cur.head, at, lane, ~0u);
+  __builtin_amdgcn_sched_barrier(0);
 
   for (;;) {
     const int len = cur.len, tok = cur.tok, rows = tok * grp, row = cur.tile * 16 + r16;
