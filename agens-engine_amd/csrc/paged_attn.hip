@@ -39,6 +39,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
@@ -71,7 +72,6 @@ struct Geo {
   static constexpr int EPL = KLB * 8 / BITS;             // values of a key load
   static constexpr int CH = D / 16;                      // values of a lane's piece of a value row
   static constexpr int VB = RB / 16, VW = VB >= 4 ? VB / 4 : 1;
-  static constexpr int kOff = BITS == 8 ? 128 : 24;      // offset of the key codes as the scores' products see them
   // element j of lane group g4's eight of 32 tokens: the numbering in which the scores leave their product
   static __device__ __forceinline__ int token(int j, int g4) { return (j < 4 ? j : 12 + j) + 4 * g4; }
   // first of the 8 values that lane group g4 contributes to step s
@@ -88,38 +88,40 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f32x2 x = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
 }
-// 1024 + n as the f16 with n in its low bits, less the offset: a code, exactly
-__device__ __forceinline__ uint32_t code_f16(uint32_t n, float offset) {
-  const _Float16 o = (_Float16)(-1024.0f - offset);
-  const f16x2 x = __builtin_bit_cast(f16x2, n | 0x64006400u) + f16x2{o, o};
-  return __builtin_bit_cast(uint32_t, x);
-}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, bool high) {  // (a's half, b's half)
   return __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
 }
-__device__ __forceinline__ bf16x8 frag(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  const u32x4 v = {a, b, c, d};
-  return __builtin_bit_cast(bf16x8, v);
+
+// Codes as operands.  A code n in the low bits of 16 is the f16 n 2^-24, a subnormal that the matrix unit takes as it is: eight
+// bits cost one byte permutation for two values, four bits a mask, where a conversion to bf16 took three instructions.  The
+// second of a byte's nibbles stays where it is, as 16 n.  So the queries are f16 too, in units of a power of two for each
+// row.  The offset of the keys' codes comes off the scores' sums; that of the values off every value, since a sum whose
+// heavy tokens hold zeros is to be as exact as any.
+template <int BITS>
+__device__ __forceinline__ u32x4 minus_offset() {  // -128 2^-24, or -8 2^-24 and 16 times that
+  const uint32_t even = BITS == 8 ? 0x80808080u : 0x80088008u, odd = 0x80808080u;
+  return u32x4{even, odd, even, odd};
 }
-__device__ __forceinline__ float ubyte(uint32_t w, int i) { return (float)((w >> (8 * i)) & 255u); }
 
 // the keys of step s (8 values of a row) as an operand
 template <int BITS, int D>
-__device__ __forceinline__ bf16x8 key_frag(const uint32_t (&k)[Geo<BITS, D>::KW], int s) {
-  if constexpr (BITS == 16) return frag(k[4 * s], k[4 * s + 1], k[4 * s + 2], k[4 * s + 3]);
+__device__ __forceinline__ u32x4 key_frag(const uint32_t (&k)[Geo<BITS, D>::KW], int s) {
+  if constexpr (BITS == 16) return u32x4{k[4 * s], k[4 * s + 1], k[4 * s + 2], k[4 * s + 3]};
   if constexpr (BITS == 8) {
     const uint32_t a = k[2 * s], b = k[2 * s + 1];
-    return frag(pack_bf16(ubyte(a, 0), ubyte(a, 1)), pack_bf16(ubyte(a, 2), ubyte(a, 3)),
-                pack_bf16(ubyte(b, 0), ubyte(b, 1)), pack_bf16(ubyte(b, 2), ubyte(b, 3)));
+    return u32x4{__builtin_amdgcn_perm(0, a, 0x0C010C00u), __builtin_amdgcn_perm(0, a, 0x0C030C02u),
+                 __builtin_amdgcn_perm(0, b, 0x0C010C00u), __builtin_amdgcn_perm(0, b, 0x0C030C02u)};
   }
-  // a nibble in the upper bits of 16.0's mantissa is 16 + it; values i and i + 4 share a register (the queries are put
-  // likewise)
-  const uint32_t w = k[s];
-  return frag(((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-              ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u);
+  const uint32_t w = k[s], u = w >> 8;  // values i and i + 4 share a register (the queries are put likewise)
+  return u32x4{w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u};
 }
 
-// Value tt of the lane's pieces of 8 tokens as an operand: bf16, or the codes as f16.
+__device__ __forceinline__ uint32_t less_offset(uint32_t n, uint32_t offset) {
+  const f16x2 x = __builtin_bit_cast(f16x2, n) - __builtin_bit_cast(f16x2, offset * 0x10001u);
+  return __builtin_bit_cast(uint32_t, x);
+}
+// Value tt of the lane's pieces of 8 tokens as an operand: bf16, or q 2^-24 (of 4 bits 16 times that where tt is odd).
 template <int BITS, int D>
 __device__ __forceinline__ u32x4 value_frag(const uint32_t (&v)[8][Geo<BITS, D>::VW], int tt) {
   u32x4 r;
@@ -129,21 +131,21 @@ __device__ __forceinline__ u32x4 value_frag(const uint32_t (&v)[8][Geo<BITS, D>:
       r[a] = halves(v[2 * a][tt / 2], v[2 * a + 1][tt / 2], tt & 1);
     } else if constexpr (BITS == 8) {
       const uint32_t sel = 0x0C040C00u + 0x00010001u * (uint32_t)(tt % 4);  // (0, second's byte, 0, first's byte)
-      r[a] = code_f16(__builtin_amdgcn_perm(v[2 * a + 1][tt / 4], v[2 * a][tt / 4], sel), 128.0f);
+      r[a] = less_offset(__builtin_amdgcn_perm(v[2 * a + 1][tt / 4], v[2 * a][tt / 4], sel), 128);
     } else {
       const uint32_t w = halves(v[2 * a][tt / 8], v[2 * a + 1][tt / 8], tt % 8 >= 4);
-      r[a] = code_f16((w >> (4 * (tt % 4))) & 0x000F000Fu, 8.0f);
+      r[a] = less_offset((tt % 4 < 2 ? w : w >> 8) & (tt % 2 ? 0x00F000F0u : 0x000F000Fu), tt % 2 ? 128 : 8);
     }
   }
   return r;
 }
-// values times weights
+// a product of bf16 operands, or of f16 ones beside codes
 template <int BITS>
-__device__ __forceinline__ f32x4 weigh(const u32x4 v, const u32x4 p, const f32x4 c) {
+__device__ __forceinline__ f32x4 product(const u32x4 x, const u32x4 y, const f32x4 c) {
   if constexpr (BITS == 16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v), __builtin_bit_cast(bf16x8, p), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, y), c, 0, 0, 0);
   else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, v), __builtin_bit_cast(f16x8, p), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, x), __builtin_bit_cast(f16x8, y), c, 0, 0, 0);
 }
 
 template <int BYTES>
@@ -436,7 +438,7 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s,
     for (int t = 0; t < G::CH; ++t) {
       const uint32_t v = row[(lane & 15) * G::CH + t];
       const bool use = mine && (v & 0x7F80u) == 0x7F80u;
-      const f32x4 sum = weigh<16>(u32x4{use ? v : 0u, 0u, 0u, 0u}, u32x4{mine ? w : 0u, 0u, 0u, 0u}, o[t]);
+      const f32x4 sum = product<16>(u32x4{use ? v : 0u, 0u, 0u, 0u}, u32x4{mine ? w : 0u, 0u, 0u, 0u}, o[t]);
       if (at < limit) o[t] = sum;
     }
   }
@@ -482,7 +484,44 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
 #pragma unroll
     for (int i = 0; i < G::STEPS; ++i) q[i] = *reinterpret_cast<const uint4*>(p + G::dim0(i, g4));
   };
-  const float zscale = a.scale * 1.44269504088896341f;
+  // (the smallest normal number in place of 0: a masked score's -inf times it is -inf)
+  const float zscale = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
+  float zs;  // of the lane's row: scores in units of log2, of the products below
+  // The queries of a new item as an operand: its sign takes the scale's.  Beside codes they are f16 with the row's largest in
+  // [2^14, 2^15): what f16 does not hold of the others is less than 2^-38 of it.
+  auto lay_queries = [&]() __attribute__((always_inline)) {
+    zs = zscale;
+    const bool minus = a.scale < 0.0f;
+    if constexpr (BITS == 16) {
+      if (minus)
+#pragma unroll
+        for (int s = 0; s < G::STEPS; ++s)
+          q[s].x ^= 0x80008000u, q[s].y ^= 0x80008000u, q[s].z ^= 0x80008000u, q[s].w ^= 0x80008000u;
+    } else {
+      u16x2 m = {0, 0};
+#pragma unroll
+      for (int s = 0; s < G::STEPS; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, word(q[s], i) & 0x7FFF7FFFu));
+      const float most = max4(__uint_as_float((uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16));
+      const uint32_t ex = min(max(__float_as_uint(most) >> 23, 14u), 244u);
+      const float f = __uint_as_float(((268u - ex) << 23) | (minus ? 0x80000000u : 0u));
+      zs *= __uint_as_float((ex + 10u) << 23);
+#pragma unroll
+      for (int s = 0; s < G::STEPS; ++s) {
+        uint4 v = q[s];
+        if constexpr (BITS == 4)  // values i and i + 4 share a register
+          v = make_uint4(halves(v.x, v.z, false), halves(v.x, v.z, true), halves(v.y, v.w, false), halves(v.y, v.w, true));
+        uint32_t r[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float g = BITS == 4 && i % 2 ? f * 0.0625f : f;  // (those codes are 16 times as large)
+          r[i] = pack_f16(__uint_as_float(word(v, i) << 16) * g, __uint_as_float(word(v, i) & 0xFFFF0000u) * g);
+        }
+        q[s] = make_uint4(r[0], r[1], r[2], r[3]);
+      }
+    }
+  };
   float top, total, ptop, unit;  // of the lane's row: largest score, sum of weights; see the product below
   f32x4 o[G::CH];
   auto clear = [&]() __attribute__((always_inline)) {
@@ -527,6 +566,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
   x.load_values(a, cur.head, at, lane, ~0u);
   __builtin_amdgcn_sched_barrier(0);
 
+  bool fresh = true;  // the first chunk of an item
   for (;;) {
     const int len = cur.len, tok = cur.tok, rows = tok * grp, row = cur.tile * 16 + r16;
     const uint32_t dead = x.dead;
@@ -541,32 +581,27 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
     // ---- scores: z[i][e] of token at + 16 i + 4 g4 + e, row r16
     float z[G::NS][4];
     {
+      if (fresh) lay_queries();
       f32x4 c[G::NS], init = {0.0f, 0.0f, 0.0f, 0.0f};
-      bf16x8 qf[G::STEPS];
+      u32x4 qf[G::STEPS];
 #pragma unroll
       for (int s = 0; s < G::STEPS; ++s) {
-        uint4 v = q[s];
-        if constexpr (BITS == 4)  // values i and i + 4 share a register
-          v = make_uint4(halves(v.x, v.z, false), halves(v.x, v.z, true), halves(v.y, v.w, false), halves(v.y, v.w, true));
-        qf[s] = __builtin_bit_cast(bf16x8, v);
-        if constexpr (BITS < 16) {  // the codes' offset is taken off first: its product with the queries
-          const uint32_t off = 0x00010001u * (BITS == 8 ? 0xC300u : 0xC1C0u);  // -128, -24
-          static_assert(G::kOff == (BITS == 8 ? 128 : 24), "");
-          init = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(off, off, off, off), qf[s], init, 0, 0, 0);
-        }
+        qf[s] = u32x4{q[s].x, q[s].y, q[s].z, q[s].w};
+        if constexpr (BITS < 16)  // the offset's product with the queries comes off first
+          init = product<BITS>(minus_offset<BITS>(), qf[s], init);
       }
 #pragma unroll
       for (int i = 0; i < G::NS; ++i) c[i] = init;
 #pragma unroll
       for (int s = 0; s < G::STEPS; ++s)
 #pragma unroll
-        for (int i = 0; i < G::NS; ++i)
-          c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key_frag<BITS, D>(x.k[i], s), qf[s], c[i], 0, 0, 0);
+        for (int i = 0; i < G::NS; ++i) c[i] = product<BITS>(key_frag<BITS, D>(x.k[i], s), qf[s], c[i]);
 #pragma unroll
       for (int i = 0; i < G::NS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[i][e] = c[i][e];
     }
+    fresh = !same;
     if (!same) {
       ids = next_ids, id0 = nat;  // (-1 where there is no next item)
       next_ids = -1;
@@ -591,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
         const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          z[i][e] *= BITS == 16 ? zscale : zscale * __uint_as_float(sc[e] << 16);
+          if constexpr (BITS < 16) z[i][e] *= __uint_as_float(sc[e] << 16);
           if (masked) {
             const int j = at + 16 * i + 4 * g4 + e;
             if (j >= limit || j >= len || (dead >> i & 1)) z[i][e] = -INFINITY;
@@ -599,7 +634,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
           most = fmaxf(most, z[i][e]);
         }
       }
-      most = fmaxf(top, max4(most));
+      most = max4(most);
+      most = fmaxf(top, most == -INFINITY ? most : most * zs);
       float f = most == top ? 1.0f : __builtin_amdgcn_exp2f(top - most);  // what the sums so far are worth
       top = most;
       const float base = most == -INFINITY ? 0.0f : most;
@@ -609,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
         const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(z[i][e] - base);
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][e], zs, -base));
           sum += p;
           if constexpr (BITS == 16) {
             z[i][e] = p;
@@ -673,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
 #pragma unroll
     for (int i = 0; i < G::NG; ++i) {
 #pragma unroll
-      for (int t = 0; t < G::CH; ++t) o[t] = weigh<BITS>(value_frag<BITS, D>(x.v[i], t), pk[i], o[t]);
+      for (int t = 0; t < G::CH; ++t) o[t] = product<BITS>(value_frag<BITS, D>(x.v[i], t), pk[i], o[t]);
       if constexpr (BITS == 16) {
         if (odd >> i & 1) add_non_finite<D>(a, cur, at + 32 * i, pk[i], len - tok + 1 + div_g(a, row), lane, o);
       }
@@ -686,7 +722,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs 
     // ---- the end of a part
     if constexpr (BITS < 16) {
 #pragma unroll
-      for (int t = 0; t < G::CH; ++t) o[t] *= unit;
+      for (int t = 0; t < G::CH; ++t) o[t] = o[t] * (BITS == 4 && t % 2 ? 0x1p20f : 0x1p24f) * unit;
     }
     if (plan.split != kByPart) {
       const bool block_ends = !same || (part + 1) % kBlock == 0;
