@@ -28,7 +28,7 @@
 namespace agq {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves;  // of a workgroup; two of them on a CU
+constexpr int kWaves = 4, kThreads = 64 * kWaves;  // of a workgroup
 constexpr int kPart = 128, kBlock = 8, kGroup = 16;  // tokens of a part, parts of a block, blocks of a group
 constexpr int kTable = 64;                           // work items that a wave knows ahead
 constexpr size_t kMaxPartialBytes = (size_t)240 << 20;
@@ -64,6 +64,9 @@ struct AttnArgs {
 template <int BITS, int D>
 struct Geo {
   static constexpr int RB = D * BITS / 8;                // bytes of a row
+  // workgroups on a CU: with rows of 512 bytes a wave needs more than half of the registers (two with their spills: 32
+  // contexts of 4096 in bf16 of width 256 451 us, one 184)
+  static constexpr int PER_CU = RB == 512 ? 1 : 2;
   static constexpr int TPW = BITS == 16 ? (D == 64 ? 64 : 32) : D == 256 ? 32 : 64;  // tokens of a chunk
   static constexpr int NS = TPW / 16, NG = TPW / 32;     // its subtiles of 16 tokens, groups of 32
   static constexpr int STEPS = D / 32;                   // MFMAs of a subtile's scores
@@ -445,7 +448,7 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s,
 }
 
 template <int BITS, int D, bool HEADS>
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_kernel(const AttnArgs a) {
   using G = Geo<BITS, D>;
   constexpr int kLevels = HEADS ? 3 : 1;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -876,7 +879,7 @@ int launch(AttnArgs a, hipStream_t s) {
   const double max_tokens = (double)a.ldt * a.s.page, rows_seq = (double)a.m / a.b * a.g;  // the latter on average
   const double tiles = ((double)(a.qstart ? a.m : a.tq) * a.g + 15) / 16;
   const double items = (double)a.b * a.s.heads * (max_tokens / kPart + 1) * tiles;  // no more than these
-  const int slots = 2 * cus;
+  const int slots = G::PER_CU * cus;
   // A wave alone streams some 11 GB/s of 16 bits, 9 of 8 and 4 of 4 (128 values a row), limited by its own steps, and the
   // memory 5.5 TB/s: fewer waves than that leave it idle.  A part's start and end cost about as much as two chunks.
   a.few = slots * (BITS == 16 ? 3 : BITS == 8 ? 4 : 8) / 2;
