@@ -525,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
       }
     }
   };
-  float top, total, ptop, unit;  // of the lane's row: largest score, sum of weights; see the product below
+  // of the lane's row: largest score, sum of weights (until the end of a part, of the lane's own tokens); see the product
+  float top, total, ptop, unit;
   f32x4 o[G::CH];
   auto clear = [&]() __attribute__((always_inline)) {
     top = -INFINITY, total = 0.0f, ptop = 0.0f, unit = 1.0f;
@@ -533,28 +534,32 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
     for (int t = 0; t < G::CH; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   };
   clear();
-  float htop[kLevels], htotal[kLevels];  // of the sums held in LDS; -inf and 0: none yet
+  float htop[kLevels], htotal[kLevels];  // of the sums held in LDS
+  // The sums at hand into level i's (`first`: in their place), or the other way round (`back`: level i's are then done with).
+  auto hold = [&](int i, bool first, bool back) __attribute__((always_inline)) {
+    if (first) {
+      if (back) return;
 #pragma unroll
-  for (int i = 0; i < kLevels; ++i) htop[i] = -INFINITY, htotal[i] = 0.0f;
-  // the sums at hand into level i's, or the other way round (`back`: level i's are then done with)
-  auto hold = [&](int i, bool back) __attribute__((always_inline)) {
+      for (int t = 0; t < G::CH; ++t) held[(i * G::CH + t) * 64] = o[t];
+      htop[i] = top, htotal[i] = total;
+      return;
+    }
     const Fold f(htop[i], top);
-    const bool none = htop[i] == -INFINITY && htotal[i] == 0.0f;  // (nothing was ever written there)
 #pragma unroll
     for (int t = 0; t < G::CH; ++t) {
-      f32x4 h = held[(i * G::CH + t) * 64], n;
+      f32x4 h = held[(i * G::CH + t) * 64];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = none ? 0.0f : h[e];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) n[e] = f(h[e], o[t][e]);
+      for (int e = 0; e < 4; ++e) h[e] = f(h[e], o[t][e]);
       if (back)
-        o[t] = n;
+        o[t] = h;
       else
-        held[(i * G::CH + t) * 64] = n;
+        held[(i * G::CH + t) * 64] = h;
     }
     const float l = f(htotal[i], total);
-    htop[i] = back ? -INFINITY : f.m, htotal[i] = back ? 0.0f : l;
-    if (back) top = f.m, total = l;
+    if (back)
+      top = f.m, total = l;
+    else
+      htop[i] = f.m, htotal[i] = l;
   };
 
   // ids: the pages of 64 subtiles from token id0 on, of cur; next_ids of nxt
@@ -626,19 +631,21 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
       float most = -INFINITY;
 #pragma unroll
       for (int i = 0; i < G::NS; ++i) {
-        const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
+        uint32_t* const sc[4] = {&x.sc[i].x, &x.sc[i].y, &x.sc[i].z, &x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (BITS < 16) z[i][e] *= __uint_as_float(sc[e] << 16);
+          if constexpr (BITS < 16) z[i][e] *= __uint_as_float(*sc[e] << 16);
           if (masked) {
             const int j = at + 16 * i + 4 * g4 + e;
-            if (j >= limit || j >= len || (dead >> i & 1)) z[i][e] = -INFINITY;
+            const bool gone = j >= limit || j >= len || (dead >> i & 1);
+            if (gone) z[i][e] = -INFINITY;
+            if constexpr (BITS < 16)  // (where a token is not seen its scale may be anything)
+              if (gone) *sc[e] = 0;
           }
           most = fmaxf(most, z[i][e]);
         }
       }
-      most = max4(most);
-      most = fmaxf(top, most == -INFINITY ? most : most * zs);
+      most = fmaxf(top, max4(most) * zs);
       float f = most == top ? 1.0f : __builtin_amdgcn_exp2f(top - most);  // what the sums so far are worth
       top = most;
       const float base = most == -INFINITY ? 0.0f : most;
@@ -652,13 +659,13 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
           sum += p;
           if constexpr (BITS == 16) {
             z[i][e] = p;
-          } else {  // the codes' weight; where a token is not seen its scale may be anything
-            z[i][e] = masked && z[i][e] == -INFINITY ? 0.0f : p * __uint_as_float(sc[e] & 0xFFFF0000u);
+          } else {  // the codes' weight
+            z[i][e] = p * __uint_as_float(sc[e] & 0xFFFF0000u);
             pmost = fmaxf(pmost, z[i][e]);
           }
         }
       }
-      total = fmaf(total, f, sum4(sum));
+      total = fmaf(total, f, sum);
       // The weights are rounded for the product: to bf16 beside bf16 values (the range of the values needs it), to f16,
       // 8 times as fine, beside codes -- in units of a power of two such that the row's largest so far is in [1, 2), so
       // what f16 cannot hold is less than 2^-25 of it.  The sums are in these units.
@@ -723,17 +730,19 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
     if (same && at % kPart) continue;
 
     // ---- the end of a part
+    total = sum4(total);
     if constexpr (BITS < 16) {
 #pragma unroll
       for (int t = 0; t < G::CH; ++t) o[t] = o[t] * (BITS == 4 && t % 2 ? 0x1p20f : 0x1p24f) * unit;
     }
     if (plan.split != kByPart) {
       const bool block_ends = !same || (part + 1) % kBlock == 0;
-      hold(0, block_ends);
+      hold(0, part % kBlock == 0, block_ends);
       if (HEADS && block_ends) {
-        const bool group_ends = !same || (part + 1) % (kBlock * kGroup) == 0;
-        hold(1, group_ends);
-        if (group_ends) hold(2, !same);
+        const int block = part / kBlock;
+        const bool group_ends = !same || (block + 1) % kGroup == 0;
+        hold(1, block % kGroup == 0, group_ends);
+        if (group_ends) hold(2, block < kGroup, !same);
       }
     }
     if (same) {
