@@ -448,7 +448,7 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s,
 }
 
 template <int BITS, int D, bool HEADS>
-__global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D>::PER_CU)) paged_attn_kernel(const AttnArgs a) {
   using G = Geo<BITS, D>;
   constexpr int kLevels = HEADS ? 3 : 1;
   extern __shared__ __align__(16) uint8_t lds[];
@@ -535,31 +535,24 @@ __global__ void __launch_bounds__(kThreads, (Geo<BITS, D>::PER_CU)) paged_attn_k
   };
   clear();
   float htop[kLevels], htotal[kLevels];  // of the sums held in LDS
-  // The sums at hand into level i's (`first`: in their place), or the other way round (`back`: level i's are then done with).
+  // Level i's sums, unless these are the first for it, and the sums at hand together; held there again unless they are wanted
+  // `back`.
   auto hold = [&](int i, bool first, bool back) __attribute__((always_inline)) {
-    if (first) {
-      if (back) return;
+    if (!first) {
+      const Fold f(htop[i], top);
+#pragma unroll
+      for (int t = 0; t < G::CH; ++t) {
+        const f32x4 h = held[(i * G::CH + t) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][e] = f(h[e], o[t][e]);
+      }
+      total = f(htotal[i], total), top = f.m;
+    }
+    if (!back) {
 #pragma unroll
       for (int t = 0; t < G::CH; ++t) held[(i * G::CH + t) * 64] = o[t];
       htop[i] = top, htotal[i] = total;
-      return;
     }
-    const Fold f(htop[i], top);
-#pragma unroll
-    for (int t = 0; t < G::CH; ++t) {
-      f32x4 h = held[(i * G::CH + t) * 64];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) h[e] = f(h[e], o[t][e]);
-      if (back)
-        o[t] = h;
-      else
-        held[(i * G::CH + t) * 64] = h;
-    }
-    const float l = f(htotal[i], total);
-    if (back)
-      top = f.m, total = l;
-    else
-      htop[i] = f.m, htotal[i] = l;
   };
 
   // ids: the pages of 64 subtiles from token id0 on, of cur; next_ids of nxt
