@@ -892,7 +892,8 @@ int launch(AttnArgs a, hipStream_t s) {
   const size_t row_bytes = (size_t)D * 4 + 8, plan_bytes = (size_t)(3 * a.b + 1) * 4;
   const double by_block = (double)a.m * a.heads * (max_tokens / (kBlock * kPart) + 1);
   const double by_part = (double)a.m * a.heads * (max_tokens / kPart + 1);
-  const double few = (double)a.few * kBlock * 16;
+  const double most_rows = (double)(a.qstart ? a.m : a.tq) * a.g;  // of a sequence's head
+  const double few = (double)a.few * kBlock * (most_rows < 16 ? most_rows : 16);
   const double most = (double)(kMaxPartialBytes / row_bytes);
   double want = max_tokens <= kPart ? 0.0 : by_part < few ? by_part : few < by_block ? by_block : few;
   const bool all = want <= most;
