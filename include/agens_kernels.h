@@ -251,9 +251,9 @@ int ak_wq_chain_status(void);
  * +-Q, Q = 127 or 7; a row whose s is below 2^-126 is held as zeros; a row with a NaN or Inf reads back as NaN (quantised).
  *   ak_kv_write  keys and values of m tokens (bf16, token t at k + t * ldk, heads contiguous; 16-byte aligned, ldk and ldv
  *                multiples of 8) into slots[t] (device memory).  A slot outside the pool is skipped; two tokens with one
- *                slot leave either of them;
+ *                slot leave any mix of them;
  *   ak_kv_read   the converse, bf16(q * s); zeros for a slot outside the pool.  ldk, ldv >= heads * dim.
- * m = 0 does nothing.  Both are one launch, allocate nothing and can be captured. */
+ * m = 0 does nothing.  Both only launch, allocate nothing and can be captured. */
 size_t ak_kv_page_bytes(int bits, int page, int heads, int dim);
 int ak_kv_write(int bits, const void* k, const void* v, int m, long ldk, long ldv, const int* slots, void* pool,
                 int npages, int page, int heads, int dim, void* stream);
@@ -270,7 +270,13 @@ int ak_kv_read(int bits, const void* pool, int npages, int page, int heads, int 
  * in fp32, rounded once; a row that sees nothing is 0.  lse (may be NULL): fp32 [m][heads], the natural log of the sum of
  * exponentials (-inf for such a row), to join with attention over other keys.  Tokens of q in no sequence's range are left
  * alone.  qstart, lens and table are device memory, read by the launch: a captured call follows them from replay to
- * replay.  Values at slots past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS. */
+ * replay.  Values at slots past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS;
+ * m * (heads / kv_heads)^2 below 2^32.
+ * A token's bits do not depend on the call: T tokens in one call, in any batch, give what T calls of one token give.
+ * Where ldt * page is above 128, partial sums lie in library scratch (above; inside a capture the graph's own): 4 * dim + 8
+ * bytes for each row (token and query head) and each 1024 cached tokens that the table has room for, or for each 128 where
+ * the sequences are few (up to 32 MB with 8 rows a key-value head in 8 bits); 240 MB at most.  Without it, or beyond it, a
+ * wave takes all of a sequence's head: the same bits, slower. */
 #define AK_ATTN_MAX_SEQS 1024
 int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, int npages, int page, int heads,
                   int kv_heads, int dim, int b, const int* qstart, const int* lens, const int* table, int ldt, float scale,
@@ -287,7 +293,9 @@ int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, in
  *   tokens [b][t + 1]: the accepted drafts, the next token, then -1;  accepted [b]: how many drafts;
  *   logp (may be NULL) fp32 [b][t + 1]: log p of each of these tokens (greedy: at temperature 1), 0 where there is none.
  * NaN logits count as -inf; a row of nothing else rejects its draft and gives the token -1.  Weights are computed in fp32,
- * their sums in 64 bits in an order that does not depend on b. */
+ * the sums of more than 16 of them in 64 bits, in an order that does not depend on b.  Rows need no alignment beyond bf16's.
+ * Library scratch (above; inside a capture the graph's own): 16 bytes for each 4096 logits, 64 MB at most; without it one
+ * workgroup takes a sequence, with the same bits. */
 #define AK_VERIFY_MAX_DRAFTS 127
 #define AK_VERIFY_MAX_VOCAB 1048576
 int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, const int* ids, const int* counts,
