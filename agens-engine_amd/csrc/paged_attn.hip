@@ -447,20 +447,84 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s,
   }
 }
 
-template <int BITS, int D, bool HEADS>
-__global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D>::PER_CU)) paged_attn_kernel(const AttnArgs a) {
+// MODE: which work items, and so what becomes of their sums.  Parts or blocks, which a plan lists; heads, likewise; or, where
+// no sequence is longer than a block, a workgroup for a sequence's head and tile, its waves a part each, which meet in LDS.
+enum AttnMode { kListed, kHeads, kShort };
+template <int BITS, int D, int MODE>
+__global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
+                                  MODE == kShort || (MODE == kHeads && D == 256) ? 1 : (Geo<BITS, D>::PER_CU))
+    paged_attn_kernel(const AttnArgs a) {
   using G = Geo<BITS, D>;
+  constexpr bool HEADS = MODE == kHeads, SHORT = MODE == kShort;
   constexpr int kLevels = HEADS ? 3 : 1;
   extern __shared__ __align__(16) uint8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6), r16 = lane & 15, g4 = lane >> 4;
   // the wave's running sums: of a block; where it takes whole heads also of a group of blocks, and of the groups
   f32x4* const held = reinterpret_cast<f32x4*>(lds) + w * kLevels * G::CH * 64 + lane;
   const int nw = (int)blockDim.x >> 6;
+  f32x4* const meet = reinterpret_cast<f32x4*>(lds);  // kShort: each wave's sums, then its rows' tops and totals
+  float2* const meet_ml = reinterpret_cast<float2*>(lds + (size_t)nw * G::CH * 1024);
   int* const tables = reinterpret_cast<int*>(lds + (size_t)nw * kLevels * G::CH * 1024);
   int* const items = tables + w * kTable * 8;
   int* const mem = tables + nw * kTable * 8;
 
   Plan plan;
+  const int grp = a.g;
+  Item cur, nxt;
+  int waves = 0, wave = 0;  // kListed, kHeads
+  auto next_item = [&](int k, Item& s) __attribute__((always_inline)) {
+    if constexpr (SHORT) {  // its part of one tile after the other
+      s = cur;
+      s.k = k, s.tile = (int)blockIdx.y + k * (int)gridDim.y;
+      s.part = w, s.end = s.tile < seq_tiles(a, s.tok) && w < parts_of(s.len) ? w + 1 : 0;
+    } else {
+      read_item(items, k, s);
+    }
+  };
+  // The tile's sums of all parts, left to right, and its outputs: a wave takes every nw-th of the lanes' values.
+  auto meet_up = [&](int tile) __attribute__((always_inline)) {
+    __syncthreads();
+    const int rows = cur.tok * grp, row = tile * 16 + r16, parts = parts_of(cur.len);
+    size_t to;
+    int h;
+    row_place(a, first_token(a, cur.seq), cur.head, min(row, rows - 1), &to, &h);
+    uint16_t* const y = a.y + to * a.ldy + (size_t)h * D + 4 * g4 * G::CH;
+    for (int t = w; t < G::CH; t += nw) {
+      Sums sum;
+      for (int p = 0; p < parts; ++p) {
+        const f32x4 v = meet[(p * G::CH + t) * 64 + lane];
+        Sums s;
+        s.m = meet_ml[p * 16 + r16].x, s.l = meet_ml[p * 16 + r16].y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.o[i] = v[i];
+        sum.add(s);
+      }
+      const float inv = 1.0f / sum.l;
+      if (row < rows) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i * G::CH + t] = sum.l == 0.0f ? (uint16_t)0 : f2bf(sum.o[i] * inv);
+        if (t == 0 && a.lse && g4 == 0) a.lse[to * a.heads + h] = row_lse(sum.m, sum.l);
+      }
+    }
+    __syncthreads();
+  };
+  if constexpr (SHORT) {
+    plan.split = kByPart;
+    cur.seq = (int)blockIdx.x / a.s.heads, cur.head = (int)blockIdx.x - cur.seq * a.s.heads;
+    cur.tok = a.tq;
+    if (a.qstart) {
+      const int q0 = first_token(a, cur.seq);
+      cur.tok = min(max(scalar_load(a.qstart + cur.seq + 1), q0), a.m) - q0;
+    }
+    cur.len = (int)min((long)max(scalar_load(a.lens + cur.seq), 0), (long)a.ldt << a.page_log2);
+    next_item(0, cur);
+    next_item(1, nxt);
+    if (!cur.end) {  // no such part
+      if (parts_of(cur.len) == 1) return;
+      for (int tile = blockIdx.y; tile < seq_tiles(a, cur.tok); tile += gridDim.y) meet_up(tile);
+      return;
+    }
+  } else {
   make_plan(a, plan, mem);
   if (a.cap && blockIdx.x == 0 && !HEADS) {  // for the kernel that adds up
     int* const out = reinterpret_cast<int*>(a.part + (size_t)a.cap * (D + 2));
@@ -469,14 +533,14 @@ __global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D
       out[1 + i] = plan.rows[i], out[1 + a.b + i] = plan.len[i], out[1 + 2 * a.b + i] = plan.tok[i];
   }
   if ((plan.split == kByHead) != HEADS) return;  // the other kernel's
-  const int grp = a.g, waves = (int)gridDim.x * nw, wave = w * (int)gridDim.x + (int)blockIdx.x;
+  waves = (int)gridDim.x * nw, wave = w * (int)gridDim.x + (int)blockIdx.x;
   fill_table(a, plan, items, 0, kTable, wave, waves);
   wave_sync();
 
-  Item cur, nxt;
   read_item(items, 0, cur);
   if (!cur.end) return;
   read_item(items, 1, nxt);
+  }
   Tokens<BITS, D> x;
   uint4 q[G::STEPS];
   auto load_queries = [&](const Item& s) __attribute__((always_inline)) {
@@ -608,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D
       next_ids = -1;
       if (more) {
         Item then;
-        read_item(items, nxt.k + 1, then);
+        next_item(nxt.k + 1, then);
         if (then.end) next_ids = x.load_ids(a, then, then.part * kPart, lane);
         load_queries(nxt);
       }
@@ -743,9 +807,14 @@ __global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D
       continue;
     }
     // ---- the end of an item: the lane has 4 runs of CH sums of its row
-    if (row < rows) {
+    if (SHORT && parts_of(len) > 1) {
+#pragma unroll
+      for (int t = 0; t < G::CH; ++t) meet[(w * G::CH + t) * 64 + lane] = o[t];
+      if (g4 == 0) meet_ml[w * 16 + r16] = make_float2(top, total);
+      meet_up(cur.tile);
+    } else if (row < rows) {
       const int pieces = seq_pieces(len, plan.split);
-      if (pieces > 1) {
+      if (!SHORT && pieces > 1) {
         const int piece = part / (plan.split == kByPart ? 1 : kBlock);
         const int to = uni(plan.rows[cur.seq]) + cur.head * rows * pieces + piece * rows + cur.tile * 16;
         // four values of all the tile's rows side by side: what a store writes is in one piece
@@ -779,11 +848,12 @@ __global__ void __launch_bounds__(kThreads, HEADS && D == 256 ? 1 : (Geo<BITS, D
     if (!more) return;
     cur = nxt;
     // (items up to cur.k + 2 are read before the next one ends)
-    if (((cur.k + 2) & (kTable / 2 - 1)) == 0 && cur.k + 2 >= kTable) {
-      fill_table(a, plan, items, cur.k + 2, kTable / 2, wave, waves);
-      wave_sync();
-    }
-    read_item(items, cur.k + 1, nxt);
+    if constexpr (!SHORT)
+      if (((cur.k + 2) & (kTable / 2 - 1)) == 0 && cur.k + 2 >= kTable) {
+        fill_table(a, plan, items, cur.k + 2, kTable / 2, wave, waves);
+        wave_sync();
+      }
+    next_item(cur.k + 1, nxt);
     clear();
   }
 }
@@ -884,6 +954,15 @@ int launch(AttnArgs a, hipStream_t s) {
   const int slots = G::PER_CU * cus;
   // A wave alone streams some 11 GB/s of 16 bits, 9 of 8 and 4 of 4 (128 values a row), limited by its own steps, and the
   // memory 5.5 TB/s: fewer waves than that leave it idle.  A part's start and end cost about as much as two chunks.
+  if constexpr (G::PER_CU == 2) {
+    if (max_tokens <= kBlock * kPart) {
+      const int parts = (int)((max_tokens + kPart - 1) / kPart);
+      const double t = a.qstart ? rows_seq / 16 : ((double)a.tq * a.g + 15) / 16;
+      hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kShort>), dim3((unsigned)(a.b * a.s.heads), t < 1 ? 1u : t < 1024 ? (unsigned)t : 1024u),
+                         dim3(64 * (unsigned)parts), (size_t)parts * (G::CH * 1024 + 128), s, a);
+      return (int)hipGetLastError();
+    }
+  }
   a.few = slots * (BITS == 16 ? 3 : BITS == 8 ? 4 : 8) / 2;
   const unsigned grid = items < (double)slots * kWaves ? (unsigned)((items + kWaves - 1) / kWaves) : (unsigned)slots;
   std::lock_guard<std::mutex> lock(scratch_mutex(s));
@@ -905,7 +984,7 @@ int launch(AttnArgs a, hipStream_t s) {
   auto smem = [&](int waves, int levels) {
     return (size_t)waves * (levels * G::CH * 1024 + kTable * 8 * 4) + (size_t)4 * a.b * 4;
   };
-  hipLaunchKernelGGL((paged_attn_kernel<BITS, D, false>), dim3(grid), dim3(kThreads), smem(kWaves, 1), s, a);
+  hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kListed>), dim3(grid), dim3(kThreads), smem(kWaves, 1), s, a);
   if (const int e = (int)hipGetLastError()) return e;
   if (a.cap) {
     hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.b * a.s.heads), rows_seq < 1 ? 1u : rows_seq < 64 ? (unsigned)rows_seq : 64u),
@@ -913,7 +992,7 @@ int launch(AttnArgs a, hipStream_t s) {
     if (const int e = (int)hipGetLastError()) return e;
   }
   if (max_tokens > kPart && (!a.cap || !all)) {  // the pieces may not fit: then this one does the work, by heads
-    hipLaunchKernelGGL((paged_attn_kernel<BITS, D, true>), dim3(2 * grid), dim3(kThreads / 2), smem(kWaves / 2, 3), s, a);
+    hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kHeads>), dim3(2 * grid), dim3(kThreads / 2), smem(kWaves / 2, 3), s, a);
     return (int)hipGetLastError();
   }
   return 0;
