@@ -954,11 +954,17 @@ int launch(AttnArgs a, hipStream_t s) {
   const int slots = G::PER_CU * cus;
   // A wave alone streams some 11 GB/s of 16 bits, 9 of 8 and 4 of 4 (128 values a row), limited by its own steps, and the
   // memory 5.5 TB/s: fewer waves than that leave it idle.  A part's start and end cost about as much as two chunks.
+  // Short contexts: in one launch, a workgroup for a sequence's head.  Measured with 8 key-value heads in 8 bits (us; the two
+  // launches below): 1 sequence of 100 tokens 7.8 (11.1), of 600 11.1 (12.8), of 900 13.9 (13.4); 64 of 400 18 (27), 96 of
+  // 900 46 (55), 128 of 900 61 (59), 256 of 900 121 (95); 1000 of 100 61 (88).  So while its waves are no more than three times
+  // what the GPU holds -- beyond that the waves of a list, which load their next item beside the present one, do better --
+  // or where a sequence is one part.
   if constexpr (G::PER_CU == 2) {
-    if (max_tokens <= kBlock * kPart) {
-      const int parts = (int)((max_tokens + kPart - 1) / kPart);
-      const double t = a.qstart ? rows_seq / 16 : ((double)a.tq * a.g + 15) / 16;
-      hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kShort>), dim3((unsigned)(a.b * a.s.heads), t < 1 ? 1u : t < 1024 ? (unsigned)t : 1024u),
+    const double parts = ceil(max_tokens / kPart);
+    const double t = a.qstart ? rows_seq / 16 : ((double)a.tq * a.g + 15) / 16;  // tiles of a sequence, on average
+    const unsigned ty = t < 1 ? 1u : t < 1024 ? (unsigned)t : 1024u;
+    if (parts <= 1 || (parts <= kBlock && (double)a.b * a.s.heads * ty * parts <= 3.0 * slots * kWaves)) {
+      hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kShort>), dim3((unsigned)(a.b * a.s.heads), ty),
                          dim3(64 * (unsigned)parts), (size_t)parts * (G::CH * 1024 + 128), s, a);
       return (int)hipGetLastError();
     }
