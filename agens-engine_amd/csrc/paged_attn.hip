@@ -6,8 +6,8 @@
 //
 // Bound by the bytes of the cache: every one is needed once, a few flops each.  So the rows that share a key-value head (its
 // query heads, times the new tokens) are the columns of one MFMA (tiles of 16 rows), and the cached tokens stream through
-// waves that work alone, without LDS exchange or barriers (a workgroup's waves that meet after every few hundred tokens to
-// add up load at once and compute at once, and the memory idles in between: 15 to 30 % of the time):
+// waves that work alone, without LDS exchange or barriers (workgroups of 8 waves that meet in LDS after each 1024 tokens: 12
+// sequences of up to 6007 tokens with one key-value head 24 us instead of 15, 8 of 6000 with 4 drafts 43 instead of 36):
 //   * a wave takes a chunk of TPW tokens at a time into registers: S = K Q^T (keys as the A operand: the lane's 16-byte load
 //     is a piece of a row, any split of the row's values over lanes and steps does, so long as the queries are laid out by
 //     the same), the softmax of the running maximum, then O^T += V^T P^T.  The scores leave the first product with the row
@@ -22,6 +22,13 @@
 // row sees nothing adds an exact nothing.  So T tokens verified in one call have the bits of T one-token calls, in any
 // batch.  Who adds is free (AttnSplit): a wave takes a block and writes its sums, or a part where blocks are too few to keep
 // the memory busy, and a second small kernel adds up; or, where there is no scratch for that, a wave takes a sequence's head.
+// Contexts of up to one block need neither plan nor second kernel: the waves of a workgroup take a part each (kShort).
+//
+// Measured (heads of 128 values, 40 query heads on 8): one context of 131072 tokens in bf16 93 us, 5.7 TB/s of the cache; 64 of
+// 8192 in 8 bits 195 us, 5.6; 16 of up to 32768 in 4 bits 114 us, 4.6, where unpacking, some 400 instructions a chunk, is
+// what the waves wait for; one of 777 tokens 13 us, of 100 8 us: a launch, a wave's loads one after the other (page table,
+// then rows), and its chunks.  8 drafts of 4 sequences (40 rows a key-value head, three tiles) 44 us: each tile loads and
+// unpacks the tokens anew.  512 tokens on 8192: 372 us, 230 TFLOP/s.
 #include "agens_kernels.h"
 #include "kv_page.h"
 
@@ -59,6 +66,7 @@ struct AttnArgs {
   float* part;  // partial rows: of each D sums, then of each its largest score and sum of weights; then the plan
   int cap;      // that fit
   int few;      // blocks, below which parts are the work items
+  int cus;
 };
 
 template <int BITS, int D>
@@ -533,7 +541,9 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
       out[1 + i] = plan.rows[i], out[1 + a.b + i] = plan.len[i], out[1 + 2 * a.b + i] = plan.tok[i];
   }
   if ((plan.split == kByHead) != HEADS) return;  // the other kernel's
-  waves = (int)gridDim.x * nw, wave = w * (int)gridDim.x + (int)blockIdx.x;
+  // Items go to one wave of every CU before a second, and to one of every SIMD before a second: workgroup i is on CU i % cus.
+  const int turn = (int)blockIdx.x / a.cus, base = turn * a.cus;
+  waves = (int)gridDim.x * nw, wave = base * nw + w * min(a.cus, (int)gridDim.x - base) + (int)blockIdx.x - base;
   fill_table(a, plan, items, 0, kTable, wave, waves);
   wave_sync();
 
@@ -952,8 +962,7 @@ int launch(AttnArgs a, hipStream_t s) {
   const double tiles = ((double)(a.qstart ? a.m : a.tq) * a.g + 15) / 16;
   const double items = (double)a.b * a.s.heads * (max_tokens / kPart + 1) * tiles;  // no more than these
   const int slots = G::PER_CU * cus;
-  // A wave alone streams some 11 GB/s of 16 bits, 9 of 8 and 4 of 4 (128 values a row), limited by its own steps, and the
-  // memory 5.5 TB/s: fewer waves than that leave it idle.  A part's start and end cost about as much as two chunks.
+  a.cus = cus;
   // Short contexts: in one launch, a workgroup for a sequence's head.  Measured with 8 key-value heads in 8 bits (us; the two
   // launches below): 1 sequence of 100 tokens 7.8 (11.1), of 600 11.1 (12.8), of 900 13.9 (13.4); 64 of 400 18 (27), 96 of
   // 900 46 (55), 128 of 900 61 (59), 256 of 900 121 (95); 1000 of 100 61 (88).  So while its waves are no more than three times
@@ -969,7 +978,10 @@ int launch(AttnArgs a, hipStream_t s) {
       return (int)hipGetLastError();
     }
   }
-  a.few = slots * (BITS == 16 ? 3 : BITS == 8 ? 4 : 8) / 2;
+  // A wave streams 9 to 11 GB/s (128 values a row in 8 and 16 bits), limited by its own steps, so with few blocks parts go to
+  // more waves, though their starts, ends and partial rows cost as much again.  Measured (us, blocks and parts): in bf16 576
+  // blocks 52 and 58; in 8 bits 256 54 and 24, 576 71 and 44, 1024 94 and 122; in 4 bits 1024 69 and 75.
+  a.few = slots * (BITS == 16 ? 2 : BITS == 8 ? 3 : 4) / 2;
   const unsigned grid = items < (double)slots * kWaves ? (unsigned)((items + kWaves - 1) / kWaves) : (unsigned)slots;
   std::lock_guard<std::mutex> lock(scratch_mutex(s));
   // Partial rows: those of all blocks at the sequences' longest, and those of as many parts as are ever taken one by one

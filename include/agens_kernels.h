@@ -275,7 +275,7 @@ int ak_kv_read(int bits, const void* pool, int npages, int page, int heads, int 
  * A token's bits do not depend on the call: T tokens in one call, in any batch, give what T calls of one token give.
  * Where ldt * page is above 128, partial sums lie in library scratch (above; inside a capture the graph's own): 4 * dim + 8
  * bytes for each row (token and query head) and each 1024 cached tokens that the table has room for, or for each 128 where
- * the sequences are few (up to 32 MB with 8 rows a key-value head in 8 bits); 240 MB at most.  Without it, or beyond it, a
+ * the sequences are few (up to 26 MB with 8 rows a key-value head of 128 values in 8 bits); 240 MB at most.  Without it, or beyond it, a
  * wave takes all of a sequence's head: the same bits, slower. */
 #define AK_ATTN_MAX_SEQS 1024
 int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, int npages, int page, int heads,
