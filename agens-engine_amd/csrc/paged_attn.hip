@@ -561,13 +561,13 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
 #pragma unroll
     for (int i = 0; i < G::STEPS; ++i) q[i] = *reinterpret_cast<const uint4*>(p + G::dim0(i, g4));
   };
-  // (the smallest normal number in place of 0: a masked score's -inf times it is -inf)
-  const float zscale = fmaxf(fabsf(a.scale) * 1.44269504088896341f, 1.17549435e-38f);
-  float zs;  // of the lane's row: scores in units of log2, of the products below
+  // of the lane's row: scores in units of log2, of the products below (the smallest normal number in place of 0: a masked
+  // score's -inf times it is -inf)
+  float zs;
   // The queries of a new item as an operand: its sign takes the scale's.  Beside codes they are f16 with the row's largest in
   // [2^14, 2^15): what f16 does not hold of the others is less than 2^-38 of it.
   auto lay_queries = [&]() __attribute__((always_inline)) {
-    zs = zscale;
+    zs = fabsf(a.scale) * 1.44269504088896341f;
     const bool minus = a.scale < 0.0f;
     if constexpr (BITS == 16) {
       if (minus)
@@ -598,6 +598,7 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
         q[s] = make_uint4(r[0], r[1], r[2], r[3]);
       }
     }
+    zs = fmaxf(zs, 1.17549435e-38f);
   };
   // of the lane's row: largest score, sum of weights (until the end of a part, of the lane's own tokens); see the product
   float top, total, ptop, unit;

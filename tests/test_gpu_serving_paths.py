@@ -133,3 +133,12 @@ def test_queries_of_any_size(bits, size):
     b.scale /= size
     y2, e2 = b.device().run()
     assert np.array_equal(y, y2) and np.array_equal(e, e2)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_small_queries_without_a_scale(bits):
+    """Scores too small for any number: the mean of the values that a row sees."""
+    b = Batch(8, bits, 16, 10, 2, 128, [300, 5], [3, 2])
+    b.q = f2bf_array((np.asarray(b.q, dtype=np.uint32) << 16).view(np.float32).ravel() * np.float32(2.0 ** -100)).reshape(b.q.shape)
+    b.scale = 0.0
+    b.check()
