@@ -1051,5 +1051,9 @@ extern "C" int ak_paged_attn(int bits, const void* q, int m, long ldq, const voi
   a.page_bytes = s.bytes();
   a.scale_off = s.scale_off();
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return bits == 16 ? agq::launch_dim<16>(a, st) : bits == 8 ? agq::launch_dim<8>(a, st) : agq::launch_dim<4>(a, st);
+  try {  // (the scratch's bookkeeping allocates host memory)
+    return bits == 16 ? agq::launch_dim<16>(a, st) : bits == 8 ? agq::launch_dim<8>(a, st) : agq::launch_dim<4>(a, st);
+  } catch (...) {
+    return AK_OOM;
+  }
 }

@@ -608,5 +608,9 @@ extern "C" int ak_spec_verify(const void* target, long ldt, const void* draft, l
   a.ids = ids, a.counts = counts, a.u = u, a.temp = temperature;
   a.tokens = tokens, a.accepted = accepted, a.logp = logp;
   a.ldt = ldt, a.ldd = ldd, a.t = t, a.vocab = vocab;
-  return agq::launch(a, b, static_cast<hipStream_t>(stream));
+  try {  // (the scratch's bookkeeping allocates host memory)
+    return agq::launch(a, b, static_cast<hipStream_t>(stream));
+  } catch (...) {
+    return AK_OOM;
+  }
 }

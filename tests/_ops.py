@@ -1,5 +1,5 @@
 """Bindings and 64-bit restatements (numpy) of the operators between the linears: the paged key-value cache, attention over
-it and the verification of drafts.  Test infrastructure: the checker."""
+it and the verification of drafts.  Test infrastructure: the oracle."""
 import ctypes
 
 import numpy as np

@@ -70,7 +70,15 @@ def test_verify_refusals():
     assert f(b=0, target=None) == 0
 
 
-# ------------------------------------------------------------------------------------------------ the checker itself
+def test_limits():
+    K = ops()
+    assert K.ak_spec_verify(P, 1 << 21, None, 0, None, None, P, None, 1, 0, (1 << 20) + 1, P, P, None, None) == 1
+    # 1025 sequences; rows of 256 heads whose numbers do not divide exactly
+    assert K.ak_paged_attn(8, P, 1025, 128, P, 4, 16, 1, 1, 128, 1025, None, P, P, 1, 1.0, P, 128, None, None) == 1
+    assert K.ak_paged_attn(8, P, 65536, 32768, P, 4, 16, 256, 1, 128, 1, None, P, P, 1, 1.0, P, 32768, None, None) == 1
+
+
+# ------------------------------------------------------------------------------------------------ the oracle itself
 def test_quantise_definition():
     x = f2bf_array(np.array([[127.0, 2.5, 3.5, -0.5] + [0.0] * 4, [7.0, 1.0, -3.0, 0.25] + [0.0] * 4], dtype=np.float32))
     c, s = quantise(x[:1], 8)
@@ -85,7 +93,7 @@ def test_quantise_definition():
     assert bf16_rn(1 + 2.0 ** -8) == 0x3F80 and bf16_rn(1 + 2.0 ** -8 + 2.0 ** -40) == 0x3F81
 
 
-def test_attention_checker_of_one_key():
+def test_attention_oracle_of_one_key():
     rng = np.random.default_rng(0)
     q = f2bf_array(rng.standard_normal((1, 2, 64)).astype(np.float32))
     k, v = rng.standard_normal((1, 1, 64)), rng.standard_normal((1, 1, 64))
@@ -93,7 +101,7 @@ def test_attention_checker_of_one_key():
     assert np.allclose(y[0], v[0]) and np.allclose(lse[0], bf2f_array(q)[0].astype(np.float64) @ k[0, 0] * 0.5)
 
 
-def test_verify_checker_emits_the_targets_distribution():
+def test_verify_oracle_emits_the_targets_distribution():
     """Speculative sampling leaves the target's distribution unchanged: over a grid of uniform numbers the first token's
     frequencies are p, whatever the draft."""
     target = f2bf_array(np.log(np.array([[0.5, 0.25, 0.15, 0.1]] * 2, dtype=np.float32)))
