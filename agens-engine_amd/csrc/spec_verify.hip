@@ -65,6 +65,7 @@ struct VerifyArgs {
   // scratch
   RowStat* stats;  // [b][rows][chunks]
   double* sums;    // [b][chunks]: of max(p - q, 0) in the rejected draft's place
+  double* rest;    // [b][t], without draft logits: the sum of the draft's chunk without the draft
   Decision* plan;  // [b]
 };
 
@@ -205,7 +206,9 @@ __device__ __forceinline__ double block_sum(double x, Shared& sh) {
 }
 
 // A chunk of a row, by a workgroup: thread t holds 8 logits from 8 t on in either half (whole cache lines a wave).
-__device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row, int chunk, int vocab, Shared& sh) {
+// Where it holds token `skip`, its sum without that token also goes to *rest.
+__device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row, int chunk, int vocab, int skip, double* rest,
+                                              Shared& sh) {
   const int t = threadIdx.x, at0 = chunk * kChunk + 8 * t, at1 = at0 + kChunk / 2;
   float l[kEach];
   load8(row, at0, vocab, l);
@@ -240,7 +243,20 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
   int best = sh.ired[0];
 #pragma unroll
   for (int i = 1; i < kWaves; ++i) best = min(best, sh.ired[i]);
+  if (skip >= 0 && skip / kChunk == chunk) {  // (summed anew: nothing is left of a difference where it has nearly all)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if ((i < 8 ? at0 : at1 - 8) + i == skip) l[i] = 0.0f;
+    const double x = block_sum(sum16(l), sh);
+    if (t == 0) *rest = x;
+  }
   return RowStat{top, best == 0x7FFFFFFF ? -1 : best, total};
+}
+// The draft that its row's weights are drawn without if it is rejected (-1: none): with nothing else known of the draft model.
+__device__ __forceinline__ int lone_draft(const VerifyArgs& a, const Seq& s, int j) {
+  if (a.draft || s.greedy || j >= s.n) return -1;
+  const int x = a.ids[(size_t)s.id * a.t + j];
+  return x < a.vocab ? x : -1;
 }
 
 // How much a chunk's sum counts in its row.
@@ -331,9 +347,9 @@ __device__ __forceinline__ int find_token(const VerifyArgs& a, float u, double s
   return who < 0 ? -1 : sh.ired[0];
 }
 
-// From the target's weights, without token `skip` (-1: all).
+// From the target's weights, without token `skip` (-1: all), where its chunk's sum is `rest`.
 __device__ __forceinline__ int draw_target(const VerifyArgs& a, const Seq& s, int j, const RowStat* st, const RowStat& p,
-                                           int skip, Shared& sh) {
+                                           int skip, double rest, Shared& sh) {
   const uint16_t* const row = target_row(a, s.id, j);
   auto weigh = [&](int k, float(&w)[kEach]) {
     load8(row, k, a.vocab, w);
@@ -344,14 +360,10 @@ __device__ __forceinline__ int draw_target(const VerifyArgs& a, const Seq& s, in
       if (k + i == skip) w[i] = 0.0f;
   };
   const int c = threadIdx.x;
-  double share = c < a.chunks ? chunk_share(s, st[c], p.top) : 0.0;
-  if (skip >= 0) {  // its chunk anew: nothing is left of a difference where the token had nearly all
-    float w[kEach];
-    weigh(skip / kChunk * kChunk + c * kEach, w);
-    const double rest = block_sum(sum16(w), sh);
-    if (c == skip / kChunk) share = rest;
-  }
-  return find_token(a, s.next_u, share, weigh, sh);
+  RowStat mine{-INFINITY, -1, 0.0};
+  if (c < a.chunks) mine = st[c];
+  if (skip >= 0 && c == skip / kChunk) mine.total = rest;
+  return find_token(a, s.next_u, chunk_share(s, mine, p.top), weigh, sh);
 }
 
 // The weights max(p - q, 0) of the 16 tokens from k on, with p and q normalised: in 64 bits, since the two may be close.
@@ -414,9 +426,9 @@ __device__ __forceinline__ Decision decision(const VerifyArgs& a, const Seq& s, 
 }
 
 // Draws and stores the next token and that nothing follows it.  st: the chunks of target row d.j; sum: thread c's chunk of
-// the residual weights, where the decision asks for them.
+// the residual weights, where the decision asks for them; rest: see draw_target, of a rejected lone_draft.
 __device__ __forceinline__ void finish(const VerifyArgs& a, const Seq& s, const Decision& d, const RowStat* st, double sum,
-                                       Shared& sh) {
+                                       double rest, Shared& sh) {
   int token = -1;
   if (s.greedy || d.p.best < 0) {
     token = d.p.best;
@@ -433,11 +445,11 @@ __device__ __forceinline__ void finish(const VerifyArgs& a, const Seq& s, const 
         residual16(a, s, d, lp, lq, w);
       };
       token = find_token(a, s.next_u, sum, weigh, sh);
-    } else if (d.j < s.n && !a.draft) {  // q was all on this draft
-      const int x = a.ids[(size_t)s.id * a.t + d.j];
-      if (x >= 0 && x < a.vocab) token = draw_target(a, s, d.j, st, d.p, x, sh);
+    } else {
+      const int x = lone_draft(a, s, d.j);
+      if (x >= 0) token = draw_target(a, s, d.j, st, d.p, x, rest, sh);
     }
-    if (token < 0) token = draw_target(a, s, d.j, st, d.p, -1, sh);  // also where nothing is left of p - q
+    if (token < 0) token = draw_target(a, s, d.j, st, d.p, -1, 0.0, sh);  // also where nothing is left of p - q
   }
   const size_t at = (size_t)s.id * (a.t + 1);
   for (int i = d.j + (int)threadIdx.x; i <= a.t; i += kThreads) {
@@ -455,7 +467,8 @@ __global__ void __launch_bounds__(kThreads) verify_rows_kernel(const VerifyArgs 
   const bool of_target = row <= a.t;
   if (of_target ? row > s.n : s.greedy || row - a.t - 1 >= s.n) return;
   const RowStat r =
-      chunk_stat(s, of_target ? target_row(a, s.id, row) : draft_row(a, s.id, row - a.t - 1), chunk, a.vocab, sh);
+      chunk_stat(s, of_target ? target_row(a, s.id, row) : draft_row(a, s.id, row - a.t - 1), chunk, a.vocab,
+                 of_target ? lone_draft(a, s, row) : -1, a.rest + (size_t)s.id * a.t + row, sh);
   if (threadIdx.x == 0) a.stats[((size_t)s.id * a.rows + row) * a.chunks + chunk] = r;
 }
 
@@ -489,7 +502,7 @@ __global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArg
     __syncthreads();
   }
   if (!DRAFT) {
-    finish(a, s, d, st + (size_t)d.j * a.chunks, 0.0, sh);
+    finish(a, s, d, st + (size_t)d.j * a.chunks, 0.0, d.j < s.n ? a.rest[(size_t)s.id * a.t + d.j] : 0.0, sh);
     return;
   }
   if (chunk == 0 && threadIdx.x == 0) a.plan[s.id] = d;
@@ -501,26 +514,27 @@ __global__ void __launch_bounds__(kThreads) verify_decide_kernel(const VerifyArg
 __global__ void __launch_bounds__(kThreads) verify_draw_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
   const Seq s = seq_of(a, blockIdx.x);
-  const Decision d = a.plan[s.id];
   const int c = threadIdx.x;
-  const double sum = d.residual && c < a.chunks ? a.sums[(size_t)s.id * a.chunks + c] : 0.0;
-  finish(a, s, d, a.stats + ((size_t)s.id * a.rows + d.j) * a.chunks, sum, sh);
+  const double sum = c < a.chunks ? a.sums[(size_t)s.id * a.chunks + c] : 0.0;  // (nothing yet, and unused, without a residual)
+  const Decision d = a.plan[s.id];
+  finish(a, s, d, a.stats + ((size_t)s.id * a.rows + d.j) * a.chunks, sum, 0.0, sh);
 }
 
 // All of a sequence in one workgroup, row after row.
 __global__ void __launch_bounds__(kThreads) verify_whole_kernel(const VerifyArgs a) {
   __shared__ Shared sh;
   __shared__ RowStat st[2][kMaxChunks];
+  __shared__ double rest;
   const Seq s = seq_of(a, blockIdx.x);
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   Decision d;
   for (int j = 0;; ++j) {
     const bool drafted = a.draft && !s.greedy && j < s.n;
     for (int c = 0; c < a.chunks; ++c) {
-      const RowStat r = chunk_stat(s, target_row(a, s.id, j), c, a.vocab, sh);
+      const RowStat r = chunk_stat(s, target_row(a, s.id, j), c, a.vocab, lone_draft(a, s, j), &rest, sh);
       if (threadIdx.x == 0) st[0][c] = r;
       if (!drafted) continue;
-      const RowStat q = chunk_stat(s, draft_row(a, s.id, j), c, a.vocab, sh);
+      const RowStat q = chunk_stat(s, draft_row(a, s.id, j), c, a.vocab, -1, nullptr, sh);
       if (threadIdx.x == 0) st[1][c] = q;
     }
     __syncthreads();
@@ -544,7 +558,7 @@ __global__ void __launch_bounds__(kThreads) verify_whole_kernel(const VerifyArgs
     const double x = residual_sum(a, s, d, c, sh);
     if (c == (int)threadIdx.x) sum = x;
   }
-  finish(a, s, d, st[0], sum, sh);
+  finish(a, s, d, st[0], sum, rest, sh);
 }
 
 VerifyArgs from(VerifyArgs a, int seq) {
@@ -562,7 +576,7 @@ VerifyArgs from(VerifyArgs a, int seq) {
 int launch(VerifyArgs a, int b, hipStream_t st) {
   a.chunks = (a.vocab + kChunk - 1) / kChunk;
   a.rows = a.t + 1 + (a.draft ? a.t : 0);
-  const size_t per = (size_t)a.chunks * (a.rows * sizeof(RowStat) + sizeof(double)) + sizeof(Decision);
+  const size_t per = (size_t)a.chunks * (a.rows * sizeof(RowStat) + sizeof(double)) + sizeof(Decision) + a.t * sizeof(double);
   const size_t most = kMaxScratch / per < 65535 ? kMaxScratch / per : 65535;  // (per <= 1.1 MB; a grid's y and z axes)
   const int each = b < (int)most ? b : (int)most;
   std::lock_guard<std::mutex> lock(scratch_mutex(st));  // the launches that share the scratch stay together
@@ -574,6 +588,7 @@ int launch(VerifyArgs a, int b, hipStream_t st) {
   a.stats = reinterpret_cast<RowStat*>(z);
   a.plan = reinterpret_cast<Decision*>(a.stats + (size_t)each * a.rows * a.chunks);
   a.sums = reinterpret_cast<double*>(a.plan + each);
+  a.rest = a.sums + (size_t)each * a.chunks;
   for (int i = 0; i < b; i += each) {
     const VerifyArgs l = from(a, i);
     const unsigned n = (unsigned)(b - i < each ? b - i : each), chunks = (unsigned)a.chunks;
