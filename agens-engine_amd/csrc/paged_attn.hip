@@ -533,23 +533,23 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
       return;
     }
   } else {
-  make_plan(a, plan, mem);
-  if (a.cap && blockIdx.x == 0 && !HEADS) {  // for the kernel that adds up
-    int* const out = reinterpret_cast<int*>(a.part + (size_t)a.cap * (D + 2));
-    if (tid == 0) out[0] = plan.split;
-    for (int i = tid; i < a.b; i += kThreads)
-      out[1 + i] = plan.rows[i], out[1 + a.b + i] = plan.len[i], out[1 + 2 * a.b + i] = plan.tok[i];
-  }
-  if ((plan.split == kByHead) != HEADS) return;  // the other kernel's
-  // Items go to one wave of every CU before a second, and to one of every SIMD before a second: workgroup i is on CU i % cus.
-  const int turn = (int)blockIdx.x / a.cus, base = turn * a.cus;
-  waves = (int)gridDim.x * nw, wave = base * nw + w * min(a.cus, (int)gridDim.x - base) + (int)blockIdx.x - base;
-  fill_table(a, plan, items, 0, kTable, wave, waves);
-  wave_sync();
+    make_plan(a, plan, mem);
+    if (a.cap && blockIdx.x == 0 && !HEADS) {  // for the kernel that adds up
+      int* const out = reinterpret_cast<int*>(a.part + (size_t)a.cap * (D + 2));
+      if (tid == 0) out[0] = plan.split;
+      for (int i = tid; i < a.b; i += kThreads)
+        out[1 + i] = plan.rows[i], out[1 + a.b + i] = plan.len[i], out[1 + 2 * a.b + i] = plan.tok[i];
+    }
+    if ((plan.split == kByHead) != HEADS) return;  // the other kernel's
+    // Items go to one wave of every CU before a second, and to one of every SIMD before a second: workgroup i is on CU i % cus.
+    const int turn = (int)blockIdx.x / a.cus, base = turn * a.cus;
+    waves = (int)gridDim.x * nw, wave = base * nw + w * min(a.cus, (int)gridDim.x - base) + (int)blockIdx.x - base;
+    fill_table(a, plan, items, 0, kTable, wave, waves);
+    wave_sync();
 
-  read_item(items, 0, cur);
-  if (!cur.end) return;
-  read_item(items, 1, nxt);
+    read_item(items, 0, cur);
+    if (!cur.end) return;
+    read_item(items, 1, nxt);
   }
   Tokens<BITS, D> x;
   uint4 q[G::STEPS];
@@ -1006,8 +1006,8 @@ int launch(AttnArgs a, hipStream_t s) {
   hipLaunchKernelGGL((paged_attn_kernel<BITS, D, kListed>), dim3(grid), dim3(kThreads), smem(kWaves, 1), s, a);
   if (const int e = (int)hipGetLastError()) return e;
   if (a.cap) {
-    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.b * a.s.heads), rows_seq < 1 ? 1u : rows_seq < 64 ? (unsigned)rows_seq : 64u),
-                       dim3(kThreads), 0, s, a);
+    const unsigned rows = rows_seq < 1 ? 1u : rows_seq < 64 ? (unsigned)rows_seq : 64u;
+    hipLaunchKernelGGL((join_kernel<D>), dim3((unsigned)(a.b * a.s.heads), rows), dim3(kThreads), 0, s, a);
     if (const int e = (int)hipGetLastError()) return e;
   }
   if (max_tokens > kPart && (!a.cap || !all)) {  // the pieces may not fit: then this one does the work, by heads

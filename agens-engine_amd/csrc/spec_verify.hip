@@ -19,9 +19,9 @@
 // same order, so with the same bits.
 //
 // Measured: 32 sequences of 5 looked-up drafts, 152064 logits (58 MB) 23 us: rows 16, 3.6 TB/s (a wave instead of a workgroup
-// for 4096 logits, without barriers: the same), decision and draw 9, a chain of dependent loads; one sequence with 4 drafts and
-// their logits 14 us, of which rows 4, decision 5, draw 4.  (LDS atomics for the picks cost 5 us each, exchanges through LDS
-// instead of DPP 2.)
+// for 4096 logits, without barriers, or 32 logits a thread: no faster), decision and draw 8, a chain of dependent loads; one
+// sequence with 4 drafts and their logits 14 us, of which rows 4, decision 5, draw 4.  (LDS atomics for the picks cost 5 us
+// each, exchanges through LDS instead of DPP 2.)
 //
 // Weights are fp32 (the hardware's exp2 of the scaled difference to the largest logit), as are the sums of the 16 that a
 // thread holds; all larger sums are 64 bits, in an order that only a row's length decides.
