@@ -83,8 +83,9 @@ struct Seq {
   bool greedy;
   float heat;
   // log2(e) / T in two parts: one of 24 bits alone shifts all exponents the same way, so the row's sum by up to 2^-24 times
-  // the mean exponent.  Kept where products with every difference of logits are numbers and -FLT_MAX's exp2 is 0.
+  // the mean exponent.  T counts as at least fp32's smallest normal number, and as 1.44e30 at most.
   float scale, scale_lo;
+  float least;  // a difference of logits whose weight is 0 (2^-300), as is that of all below: its products are numbers at any T
   float next_u;
 };
 __device__ __forceinline__ Seq seq_of(const VerifyArgs& a, int id) {
@@ -94,9 +95,11 @@ __device__ __forceinline__ Seq seq_of(const VerifyArgs& a, int id) {
   const float temp = a.temp ? a.temp[id] : 1.0f;
   s.greedy = !(temp > 0.0f);
   s.heat = s.greedy ? 1.0f : temp;
-  const double scale = fmin(fmax(1.44269504088896340736 / (double)s.heat, 1e-30), (double)FLT_MAX);
+  const float heat = fminf(fmaxf(s.heat, FLT_MIN), 1.44e30f);
+  const double scale = 1.44269504088896340736 / (double)heat;
   s.scale = (float)scale;
   s.scale_lo = (float)(scale - (double)s.scale);
+  s.least = -208.0f * heat;
   s.next_u = a.u[(size_t)id * (a.t + 1) + a.t];
   return s;
 }
@@ -110,7 +113,7 @@ __device__ __forceinline__ const uint16_t* draft_row(const VerifyArgs& a, int se
 // The weight of logit l in a row whose largest is top (not +inf).  The clamp takes a masked logit's -inf, and NaN, to a
 // difference whose weight is 0.
 __device__ __forceinline__ float weight(const Seq& s, float l, float top) {
-  const float d = fmaxf(l - (top == -INFINITY ? 0.0f : top), -FLT_MAX);
+  const float d = fmaxf(l - (top == -INFINITY ? 0.0f : top), s.least);
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, s.scale, d * s.scale_lo));
 }
 // Of any row: where the largest is +inf, all that are it weigh the same.
