@@ -397,6 +397,12 @@ __device__ __forceinline__ float log_prob(const Seq& s, const RowStat& p, uint16
   return (float)((l == p.top ? 0.0 : (double)(l - p.top) / (double)s.heat) - log(p.total));
 }
 
+// The weight of one token, also below what fp32 holds: two that are both too small for it still compare.
+__device__ __forceinline__ double token_weight(const Seq& s, float l, float top) {
+  const float w = any_weight(s, l, top);
+  return w >= 0x1p-100f || !(l > -INFINITY) || top == INFINITY ? (double)w : exp((double)(l - top) / (double)s.heat);
+}
+
 // What the decision on draft j needs besides the sums: loaded before they are there.
 struct Draft {
   int x;
@@ -416,8 +422,8 @@ __device__ __forceinline__ bool accept(const VerifyArgs& a, const Seq& s, const 
   if (d.x < 0 || p.best < 0) return false;
   if (s.greedy) return d.x == p.best;
   double qx = 1.0;
-  if (a.draft) qx = q.best < 0 ? 0.0 : any_weight(s, d.lq, q.top) / q.total;
-  return d.u * qx < any_weight(s, d.lp, p.top) / p.total;
+  if (a.draft) qx = q.best < 0 ? 0.0 : token_weight(s, d.lq, q.top) / q.total;
+  return d.u * qx < token_weight(s, d.lp, p.top) / p.total;
 }
 __device__ __forceinline__ void put_accepted(const VerifyArgs& a, const Seq& s, int j, const RowStat& p) {
   const int x = a.ids[(size_t)s.id * a.t + j];

@@ -59,6 +59,21 @@ def test_cold(vocab, drafted, masks):
             assert (np.abs(got[2][i] - lp) <= 1e-5).all(), temp[i]
 
 
+@pytest.mark.parametrize("masks", [False, True])
+@pytest.mark.parametrize("vocab", [300, 8193])
+@pytest.mark.parametrize("drafted", [True, False])
+def test_low(vocab, drafted, masks):
+    target, draft, ids, u, temp, b, t = scene(vocab, ORDINARY, 6, masks)
+    args = (target, draft if drafted else None, ids, None, u, temp, b, t)
+    got = run(*args[:6], b, t, vocab)
+    compare(got, *args, least=0.8)
+    for i in range(b):
+        tok, acc, lp, near = verify64(target[i], args[1][i] if drafted else None, ids[i], t, np.float32(u[i]),
+                                      float(np.float32(temp[i])), t)
+        if not near:
+            assert (np.abs(got[2][i] - lp) <= 1e-5 * (1 + np.abs(lp)))[lp > -50].all(), temp[i]
+
+
 def test_small_logits_and_a_small_temperature():
     """The weights are those of (l - largest) / T, however small both are."""
     rng = np.random.default_rng(7)
