@@ -331,7 +331,7 @@ __device__ __forceinline__ int find_token(const VerifyArgs& a, float u, double s
   if (!(all > 0.0)) return -1;
   double at = (double)u * all, before;
   const int chunk = pick_thread(share, at, sh, &before);
-  at -= before;
+  at = fmax(at - before, 0.0);  // (the chunks before may sum to a rounding more than they did one by one)
   const int k = chunk * kChunk + (int)threadIdx.x * kEach;
   float w[kEach];
   weigh(k, w);
@@ -340,8 +340,8 @@ __device__ __forceinline__ int find_token(const VerifyArgs& a, float u, double s
   if ((int)threadIdx.x == who) {
     double c = before;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {  // the last with any weight at worst
-      if (w[i] > 0.0f && c <= at) token = k + i;
+    for (int i = 0; i < kEach; ++i) {  // the last with any weight at worst; likewise the first
+      if (w[i] > 0.0f && (token < 0 || c <= at)) token = k + i;
       c += (double)w[i];
     }
     sh.ired[0] = token;
