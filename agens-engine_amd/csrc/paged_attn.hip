@@ -741,7 +741,7 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
         ptop = fmaxf(ptop * f, max4(pmost));
         const uint32_t ex = min(max(__float_as_uint(ptop) >> 23, 2u), 252u);
         const float inv = __uint_as_float((254u - ex) << 23);
-        f *= unit * inv;
+        f = f * unit * inv;  // (in this order a number whatever the two units: f is 0 where inv is far beyond 1 / unit)
         unit = __uint_as_float(ex << 23);
 #pragma unroll
         for (int i = 0; i < G::NS; ++i)
