@@ -14,7 +14,9 @@
 //     in the lane and four tokens in its registers, which is how the second takes its B operand when the tokens of 32 are
 //     numbered accordingly: the weights never change lanes.  The values are loaded as whole row pieces too, and transposed
 //     in the lane: a lane holds eight tokens' pieces of the same values, and pairs of tokens are what a register of the A
-//     operand is;
+//     operand is.  A weight meets the values as two operands that add up to it (split_bf16, split_f16): rounded to one, equal
+//     weights all move the same way and the outputs by up to 2^-9 of the values, beyond their own rounding (two cost nothing
+//     in bf16 and 8 bits; 16 contexts of 32768 in 4 bits 118 -> 123 us);
 //   * the next chunk's keys are loaded as soon as the scores are done with theirs, the values likewise.
 //
 // Order of summation.  What a row gives depends on its own tokens only, never on the call: tokens lie in parts of 128, added
@@ -98,6 +100,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const f32x2 x = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, f16x2));
+}
+// Two weights x >= 0 as two operands that add up to them.  In bf16, 16 bits of each: `hi` is the largest bf16 below x, so what
+// is left for `lo` is above 0 too (down to x = 2^-117), and both products with an infinite value are that infinity.  In f16, 22
+// bits of each times `unit`, a power of two.
+struct Split {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Split split_bf16(float x0, float x1) {
+  const uint32_t a = __builtin_elementwise_sub_sat(__float_as_uint(x0), 1u);
+  const uint32_t b = __builtin_elementwise_sub_sat(__float_as_uint(x1), 1u);
+  return {__builtin_amdgcn_perm(b, a, 0x07060302u),
+          pack_bf16(x0 - __uint_as_float(a & 0xFFFF0000u), x1 - __uint_as_float(b & 0xFFFF0000u))};
+}
+__device__ __forceinline__ Split split_f16(float x0, float x1, float unit) {
+  const auto h = __builtin_amdgcn_cvt_pkrtz(x0 * unit, x1 * unit);
+  return {__builtin_bit_cast(uint32_t, h),
+          pack_f16(__builtin_fmaf(x0, unit, -(float)h[0]), __builtin_fmaf(x1, unit, -(float)h[1]))};
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 __device__ __forceinline__ uint32_t halves(uint32_t a, uint32_t b, bool high) {  // (a's half, b's half)
@@ -433,8 +452,8 @@ struct Tokens {
 // Adds the non-finite values (bf16) of the 32 tokens from `first` on that the sequence's first new token does not see, one
 // token at a time, to the rows that see it.  Rare, so the values are read again rather than kept.
 template <int D>
-__device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s, int first, const u32x4 p, int limit,
-                                               int lane, f32x4 (&o)[Geo<16, D>::CH]) {
+__device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s, int first, const u32x4 hi, const u32x4 lo,
+                                               int limit, int lane, f32x4 (&o)[Geo<16, D>::CH]) {
   using G = Geo<16, D>;
 #pragma unroll 1
   for (int at = max(first, s.len - s.tok + 1); at < min(first + 32, s.len); ++at) {
@@ -444,12 +463,16 @@ __device__ __forceinline__ void add_non_finite(const AttnArgs& a, const Item& s,
         a.pool + a.page_bytes * (size_t)pg + (size_t)((2 * s.head + 1) * a.s.page + (at & (a.s.page - 1))) * G::RB);
     const int n = at - first, j = (n >> 4) * 4 + (n & 3);  // element j of lane group (n % 16) / 4
     const bool mine = lane >> 4 == (n & 15) >> 2;
-    const uint32_t w2 = j < 2 ? p.x : j < 4 ? p.y : j < 6 ? p.z : p.w, w = (j & 1) ? w2 >> 16 : w2 & 0xFFFFu;
+    auto weight = [&](const u32x4 p) {
+      const uint32_t w2 = j < 2 ? p.x : j < 4 ? p.y : j < 6 ? p.z : p.w;
+      return u32x4{!mine ? 0u : (j & 1) ? w2 >> 16 : w2 & 0xFFFFu, 0u, 0u, 0u};
+    };
 #pragma unroll
     for (int t = 0; t < G::CH; ++t) {
       const uint32_t v = row[(lane & 15) * G::CH + t];
       const bool use = mine && (v & 0x7F80u) == 0x7F80u;
-      const f32x4 sum = product<16>(u32x4{use ? v : 0u, 0u, 0u, 0u}, u32x4{mine ? w : 0u, 0u, 0u, 0u}, o[t]);
+      const u32x4 x{use ? v : 0u, 0u, 0u, 0u};
+      const f32x4 sum = product<16>(x, weight(lo), product<16>(x, weight(hi), o[t]));
       if (at < limit) o[t] = sum;
     }
   }
@@ -693,7 +716,7 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
     x.find(a, ids, (nat - id0) >> 4);
     x.load_keys(a, nhead, nat, lane, live);
     // ---- softmax of the running maximum
-    u32x4 pk[G::NG];
+    u32x4 pk[G::NG], pl[G::NG];
     {
       const int limit = len - tok + 1 + div_g(a, row);
       float most = -INFINITY;
@@ -734,26 +757,24 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
         }
       }
       total = fmaf(total, f, sum);
-      // The weights are rounded for the product: to bf16 beside bf16 values (the range of the values needs it), to f16,
-      // 8 times as fine, beside codes -- in units of a power of two such that the row's largest so far is in [1, 2), so
-      // what f16 cannot hold is less than 2^-25 of it.  The sums are in these units.
+      // The weights meet the values as two operands (Split), so that they keep what the sum of weights has of them.  Beside codes
+      // they are in units of a power of two such that the row's largest so far is in [2^14, 2^15): what f16 cannot hold is
+      // less than 2^-39 of it.  The sums are in these units.
+      float inv = 1.0f;
       if constexpr (BITS < 16) {
         ptop = fmaxf(ptop * f, max4(pmost));
-        const uint32_t ex = min(max(__float_as_uint(ptop) >> 23, 2u), 252u);
-        const float inv = __uint_as_float((254u - ex) << 23);
+        const uint32_t ex = min(max(__float_as_uint(ptop) >> 23, 15u), 252u);
+        inv = __uint_as_float((268u - ex) << 23);
         f = f * unit * inv;  // (in this order a number whatever the two units: f is 0 where inv is far beyond 1 / unit)
-        unit = __uint_as_float(ex << 23);
-#pragma unroll
-        for (int i = 0; i < G::NS; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            pk[i / 2][2 * (i & 1) + e] = pack_f16(z[i][2 * e] * inv, z[i][2 * e + 1] * inv);
-      } else {
-#pragma unroll
-        for (int i = 0; i < G::NS; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) pk[i / 2][2 * (i & 1) + e] = pack_bf16(z[i][2 * e], z[i][2 * e + 1]);
+        unit = __uint_as_float((ex - 14u) << 23);
       }
+#pragma unroll
+      for (int i = 0; i < G::NS; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const Split w = BITS == 16 ? split_bf16(z[i][2 * e], z[i][2 * e + 1]) : split_f16(z[i][2 * e], z[i][2 * e + 1], inv);
+          pk[i / 2][2 * (i & 1) + e] = w.hi, pl[i / 2][2 * (i & 1) + e] = w.lo;
+        }
       if (__ballot(f != 1.0f)) {
 #pragma unroll
         for (int t = 0; t < G::CH; ++t) o[t] *= f;
@@ -787,9 +808,15 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
 #pragma unroll
     for (int i = 0; i < G::NG; ++i) {
 #pragma unroll
-      for (int t = 0; t < G::CH; ++t) o[t] = product<BITS>(value_frag<BITS, D>(x.v[i], t), pk[i], o[t]);
+      for (int t = 0; t < G::CH; t += 2) {
+        const u32x4 v = value_frag<BITS, D>(x.v[i], t), v1 = value_frag<BITS, D>(x.v[i], t + 1);
+        o[t] = product<BITS>(v, pk[i], o[t]);
+        o[t + 1] = product<BITS>(v1, pk[i], o[t + 1]);
+        o[t] = product<BITS>(v, pl[i], o[t]);
+        o[t + 1] = product<BITS>(v1, pl[i], o[t + 1]);
+      }
       if constexpr (BITS == 16) {
-        if (odd >> i & 1) add_non_finite<D>(a, cur, at + 32 * i, pk[i], len - tok + 1 + div_g(a, row), lane, o);
+        if (odd >> i & 1) add_non_finite<D>(a, cur, at + 32 * i, pk[i], pl[i], len - tok + 1 + div_g(a, row), lane, o);
       }
     }
     x.load_values(a, nhead, nat, lane, live);

@@ -266,12 +266,13 @@ int ak_kv_read(int bits, const void* pool, int npages, int page, int heads, int 
  * kv_heads)).  Sequence i has the tokens [qstart[i], qstart[i + 1]) of q (qstart NULL: m / b each), lens[i] tokens in the
  * cache, these new ones included as its last (written before the call), and the pages table[i * ldt ...].  Token t of T sees
  * the cached tokens before len - T + t + 1 -- itself the last -- except those of pages outside the pool, which count
- * as not there (a freed page's entry may be -1); lengths past the table's ldt pages end there.  y = softmax(scale * q . k) v
- * in fp32, rounded once; a row that sees nothing is 0.  lse (may be NULL): fp32 [m][heads], the natural log of the sum of
- * exponentials (-inf for such a row), to join with attention over other keys.  Tokens of q in no sequence's range are left
- * alone.  qstart, lens and table are device memory, read by the launch: a captured call follows them from replay to
- * replay.  Values at slots past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS;
- * m * (heads / kv_heads)^2 below 2^32.
+ * as not there (a freed page's entry may be -1); lengths past the table's ldt pages end there.  y = softmax(scale * q
+ * . k) v in fp32 (the weights keep 16 bits beside bf16 values, 22 beside codes), rounded once; a row that sees
+ * nothing is 0.  lse (may be NULL): fp32 [m][heads], the natural log of the sum of exponentials (-inf for such a
+ * row), to join with attention over other keys.  Tokens of q in no sequence's range are left alone.  qstart, lens and
+ * table are device memory, read by the launch: a captured call follows them from replay to replay.  Values at slots
+ * past a row's last token have no effect on it, whatever they hold.  b up to AK_ATTN_MAX_SEQS; m * (heads /
+ * kv_heads)^2 below 2^32.
  * A token's bits do not depend on the call: T tokens in one call, in any batch, give what T calls of one token give.
  * Where ldt * page is above 128, partial sums lie in library scratch (above; inside a capture the graph's own): 4 * dim + 8
  * bytes for each row (token and query head) and each 1024 cached tokens that the table has room for, or for each 128 where

@@ -9,6 +9,8 @@ of rounding them, so 2u a step there):
                keep 16 bits at least, their sums take a step for each of a part's 128 tokens, 8 parts, 16 blocks and the
                context's groups of blocks: (2^-16 + steps * 2u) sum p |v|; then its own rounding, half of bf16's last place;
   lse          sum p_j (dz_j + ez_j), a step u for each of a lane's 32 tokens of a part, parts, blocks and groups, its rounding."""
+import types
+
 import numpy as np
 
 from _lib import f2bf_array, bf2f_array
@@ -83,7 +85,7 @@ class Scene(Batch):
                 sc[pg, :, off, part] = s.view(np.uint8).reshape(n, self.kv, 2)
 
     def device(self):
-        self.pool = self  # (Batch.device takes the bytes from here)
+        self.pool = types.SimpleNamespace(mem=self.mem)  # (where Batch.device looks for them)
         return super().device()
 
     def expect(self):
