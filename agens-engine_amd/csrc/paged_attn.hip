@@ -1024,7 +1024,7 @@ int launch(AttnArgs a, hipStream_t s) {
   const bool all = want <= most;
   a.cap = (int)(all ? want : most);
   if (a.cap) {
-    a.part = reinterpret_cast<float*>(call_scratch(s, (size_t)a.cap * row_bytes + plan_bytes).data);
+    a.part = reinterpret_cast<float*>(call_scratch(s, (size_t)a.cap * row_bytes + plan_bytes, ScratchOf::kOperators).data);
     if (!a.part) a.cap = 0;
   }
   auto smem = [&](int waves, int levels) {

@@ -589,7 +589,7 @@ int launch(VerifyArgs a, int b, hipStream_t st) {
   const size_t most = kMaxScratch / per < 65535 ? kMaxScratch / per : 65535;  // (per <= 1.1 MB; a grid's y and z axes)
   const int each = b < (int)most ? b : (int)most;
   std::lock_guard<std::mutex> lock(scratch_mutex(st));  // the launches that share the scratch stay together
-  uint8_t* const z = call_scratch(st, per * each).data;
+  uint8_t* const z = call_scratch(st, per * each, ScratchOf::kOperators).data;
   if (!z) {
     hipLaunchKernelGGL(verify_whole_kernel, dim3((unsigned)b), dim3(kThreads), 0, st, a);
     return (int)hipGetLastError();

@@ -19,6 +19,12 @@
 // up, calls are captured in the form without scratch.  (The split-K launches of the small-M kernels work in stream_scratch
 // under a capture as well, as the reference's do: graphs with such launches captured from one stream run in order.)
 //
+// The operators between the linears (attention, verification) have a reserve of their own: attention's pieces are 16 MB and
+// more (64 sequences with room for 131072 tokens 172 MB), and a graph for every batch size would leave the linears nothing.
+// It gets another 256 MB, up to 4 GB, whenever one of these calls outside a capture finds too little left to be captured
+// itself: who makes each call once before capturing it has it captured in the form with scratch.  A captured call that
+// finds no room there may take from the first half of the linears' reserve.
+//
 // A caller that must not allocate (ak_wq_gemv_kt_multi_noalloc) installs a fixed buffer for the calling thread first:
 // then both functions return that buffer when it is large enough and null otherwise, and never allocate.
 #include "wq_scratch.h"
@@ -39,19 +45,52 @@ struct Buf {
 };
 
 constexpr size_t kCounters = 4096, kReserve = (size_t)256 << 20;
-struct Reserve {
+// Left besides a call's own piece, for a smaller call of the same capture that comes first (verification: 64 MB at most).
+constexpr size_t kMargin = (size_t)64 << 20;
+constexpr size_t kMaxChunks = 16;  // of the operators' reserve
+struct Chunk {
   uint8_t* p = nullptr;
-  size_t used = 0;
-  bool tried = false;
+  size_t bytes = 0, used = 0;
+};
+struct Reserve {
+  std::vector<Chunk> chunks;
+  bool failed = false;  // to allocate: not tried again
+  // a piece that leaves `keep` of its chunk, or null
+  uint8_t* take(size_t bytes, size_t keep) {
+    for (Chunk& c : chunks)
+      if (c.bytes - c.used >= bytes + keep) {
+        c.used += bytes;
+        return c.p + c.used - bytes;
+      }
+    return nullptr;
+  }
+  // Room for a captured call of `bytes`, in as many chunks as `most`.  Not under a capture.
+  void provide(size_t bytes, size_t most) {
+    for (const Chunk& c : chunks)
+      if (c.bytes - c.used >= bytes) return;
+    if (failed || chunks.size() >= most) return;
+    Chunk c;
+    c.bytes = bytes > kReserve ? bytes : kReserve;
+    void* p = nullptr;
+    if (hipMalloc(&p, c.bytes) == hipSuccess && hipMemset(p, 0, c.bytes) == hipSuccess &&
+        hipDeviceSynchronize() == hipSuccess) {
+      c.p = static_cast<uint8_t*>(p);
+      chunks.push_back(c);
+    } else {
+      if (p) (void)hipFree(p);
+      (void)hipGetLastError();
+      failed = true;
+    }
+  }
 };
 
 struct Pool {
   std::mutex mu;
   std::map<std::tuple<int, hipStream_t, uint64_t>, Buf> bufs;  // (device, stream, thread_of(stream))
   std::vector<std::pair<int, Buf>> idle;                       // (device, buffer) of threads that ended
-  std::map<int, Reserve> reserve;                              // by device
+  std::map<std::pair<int, ScratchOf>, Reserve> reserve;        // by device
   // (device, stream, thread_of(stream), capture) -> the piece its calls share
-  std::map<std::tuple<int, hipStream_t, uint64_t, unsigned long long>, Buf> pieces;
+  std::map<std::tuple<int, hipStream_t, uint64_t, unsigned long long, ScratchOf>, Buf> pieces;
 };
 
 Pool& pool() {
@@ -148,7 +187,7 @@ void* stream_scratch(hipStream_t s, size_t bytes) {
   return replace_with({p, want, false});
 }
 
-CallScratch call_scratch(hipStream_t s, size_t bytes) {
+CallScratch call_scratch(hipStream_t s, size_t bytes, ScratchOf of) {
   CallScratch c;
   auto in = [&](void* p) {
     if (p) c.cnt = static_cast<int*>(p), c.data = static_cast<uint8_t*>(p) + kCounters;
@@ -169,31 +208,20 @@ CallScratch call_scratch(hipStream_t s, size_t bytes) {
   if (cs == hipStreamCaptureStatusNone) {
     void* const z = stream_scratch(s, bytes);
     std::lock_guard<std::mutex> lock(P.mu);
-    Reserve& r = P.reserve[dev];
-    if (z && !r.tried) {
-      r.tried = true;
-      void* p = nullptr;
-      if (hipMalloc(&p, kReserve) == hipSuccess && hipMemset(p, 0, kReserve) == hipSuccess &&
-          hipDeviceSynchronize() == hipSuccess) {
-        r.p = static_cast<uint8_t*>(p);
-      } else {
-        if (p) (void)hipFree(p);
-        (void)hipGetLastError();
-      }
-    }
+    if (z) P.reserve[{dev, ScratchOf::kLinears}].provide(0, 1);
+    if (z && of == ScratchOf::kOperators) P.reserve[{dev, of}].provide(bytes + kMargin, kMaxChunks);
     return in(z);
   }
   if (cs != hipStreamCaptureStatusActive) return c;
   const uint64_t thread = thread_of(s);
   std::lock_guard<std::mutex> lock(P.mu);
-  const std::tuple<int, hipStream_t, uint64_t, unsigned long long> key{dev, s, thread, id};
+  const std::tuple<int, hipStream_t, uint64_t, unsigned long long, ScratchOf> key{dev, s, thread, id, of};
   const auto it = P.pieces.find(key);
   if (it != P.pieces.end() && it->second.bytes >= bytes) return in(it->second.p);
-  Reserve& r = P.reserve[dev];
   bytes = (bytes + 4095) & ~(size_t)4095;
-  if (!r.p || kReserve - r.used < bytes) return c;
-  void* const p = r.p + r.used;
-  r.used += bytes;
+  uint8_t* p = P.reserve[{dev, of}].take(bytes, 0);
+  if (!p && of == ScratchOf::kOperators) p = P.reserve[{dev, ScratchOf::kLinears}].take(bytes, kReserve / 2);
+  if (!p) return c;
   P.pieces[key] = {p, bytes, true};  // (a smaller piece of the capture stays with its earlier calls)
   return in(p);
 }

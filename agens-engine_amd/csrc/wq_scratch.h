@@ -28,11 +28,13 @@ void* stream_scratch(hipStream_t s, size_t bytes);
 constexpr size_t kMaxCallScratch = (size_t)256 << 20;
 
 // The same for a call that may be captured: 4 KB of counters (zero between launches) and `bytes` of data that no other
-// stream and no other graph works in; null pointers without it.
+// stream and no other graph works in; null pointers without it.  Captured calls of the linears and of the operators between
+// them (attention, verification) take it from reserves of their own, so that neither uses up the other's.
+enum class ScratchOf { kLinears, kOperators };
 struct CallScratch {
   int* cnt = nullptr;
   uint8_t* data = nullptr;
 };
-CallScratch call_scratch(hipStream_t s, size_t bytes);
+CallScratch call_scratch(hipStream_t s, size_t bytes, ScratchOf of = ScratchOf::kLinears);
 
 }  // namespace agq

@@ -22,10 +22,12 @@
  *     the GEMM work in a piece of a 256 MB reserve per device (allocated with the first call outside a capture that
  *     needs scratch, on any stream) that belongs to the captured graph: it may run beside other graphs and beside calls
  *     on the stream it was captured from (not beside itself).  Without a reserve, or with too little of it left, they
- *     take a launch that needs no scratch (the GEMV: same results; the GEMM: k not split).  The split-K launches of the
- *     one- to 16-token kernels at group 128, which some calls of more tokens take in chunks of 16, work in the captured
- *     stream's own scratch (if it has any): run graphs that hold such launches in order with each other and with calls
- *     on that stream.
+ *     take a launch that needs no scratch (the GEMV: same results; the GEMM: k not split).  Attention over the cache and
+ *     verification of drafts have such a reserve of their own: 256 MB with the first of these calls outside a capture, and
+ *     another 256 MB, 4 GB at most, whenever such a call finds too little left to be captured itself.  The split-K
+ *     launches of the one- to 16-token kernels at group 128, which some calls of more tokens take in chunks of 16, work
+ *     in the captured stream's own scratch (if it has any): run graphs that hold such launches in order with each other
+ *     and with calls on that stream.
  */
 #pragma once
 #include <stddef.h>
