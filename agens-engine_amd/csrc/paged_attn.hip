@@ -34,6 +34,8 @@
 #include "agens_kernels.h"
 #include "kv_page.h"
 
+#include <cfloat>
+
 namespace agq {
 namespace {
 
@@ -584,8 +586,8 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
 #pragma unroll
     for (int i = 0; i < G::STEPS; ++i) q[i] = *reinterpret_cast<const uint4*>(p + G::dim0(i, g4));
   };
-  // of the lane's row: scores in units of log2, of the products below (the smallest normal number in place of 0: a masked
-  // score's -inf times it is -inf)
+  // of the lane's row: scores in units of log2, of the products below (the smallest normal number in place of 0, the largest in
+  // that of infinity: a masked score's -inf times it is -inf, 0 times it is 0)
   float zs;
   // The queries of a new item as an operand: its sign takes the scale's.  Beside codes they are f16 with the row's largest in
   // [2^14, 2^15): what f16 does not hold of the others is less than 2^-38 of it.
@@ -604,9 +606,9 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
 #pragma unroll
         for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, word(q[s], i) & 0x7FFF7FFFu));
       const float most = max4(__uint_as_float((uint32_t)(m[0] > m[1] ? m[0] : m[1]) << 16));
-      const uint32_t ex = min(max(__float_as_uint(most) >> 23, 14u), 244u);
+      const uint32_t ex = min(max(__float_as_uint(most) >> 23, 14u), 254u), past = ex > 244u ? ex - 244u : 0u;
       const float f = __uint_as_float(((268u - ex) << 23) | (minus ? 0x80000000u : 0u));
-      zs *= __uint_as_float((ex + 10u) << 23);
+      zs = zs * __uint_as_float((ex - past + 10u) << 23) * __uint_as_float((127u + past) << 23);  // 2^(ex - 117)
 #pragma unroll
       for (int s = 0; s < G::STEPS; ++s) {
         uint4 v = q[s];
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
         q[s] = make_uint4(r[0], r[1], r[2], r[3]);
       }
     }
-    zs = fmaxf(zs, 1.17549435e-38f);
+    zs = fminf(fmaxf(zs, FLT_MIN), FLT_MAX);
   };
   // of the lane's row: largest score, sum of weights (until the end of a part, of the lane's own tokens); see the product
   float top, total, ptop, unit;
@@ -746,7 +748,7 @@ __global__ void __launch_bounds__(MODE == kShort ? kBlock * 64 : kThreads,
         const uint32_t sc[4] = {x.sc[i].x, x.sc[i].y, x.sc[i].z, x.sc[i].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(z[i][e], zs, -base));
+          const float p = __builtin_amdgcn_exp2f(z[i][e] * zs - base);  // (not fused: 0 at the top, however large)
           sum += p;
           if constexpr (BITS == 16) {
             z[i][e] = p;

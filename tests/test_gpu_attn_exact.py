@@ -160,6 +160,37 @@ def test_values_of_any_size(bits, first, then):
     assert (np.abs(e - wl) <= tl).all()
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("power", [-110, 100, 118, 119, 120, 123])
+def test_queries_and_scales_far_from_one(bits, power):
+    """Queries times a power of two with a scale divided by it: the same scores."""
+    if bits == 16 and power == 123:
+        pytest.skip("q . k itself, some 2^5 times the power, leaves fp32")
+    a = Scene(12, bits, 16, 5, 1, 128, [300, 37], [2, 1], 1.0).device()
+    y, e = a.run()
+    a.q = bf16(bf2f_array(a.q) * np.float32(2.0 ** power))
+    assert np.isfinite(bf2f_array(a.q)).all()
+    a.scale /= 2.0 ** power
+    y2, e2 = a.run()
+    assert np.array_equal(y, y2) and np.array_equal(e, e2)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("power,scale", [(124, 0.088), (-10, 3.0e38), (0, 1e30)])
+def test_scores_at_the_end_of_fp32(bits, power, scale):
+    """A row whose best score leads by far, up to where scores leave fp32: that token's value."""
+    a = Scene(13, bits, 16, 1, 1, 128, [100], [1], 1.0)
+    q = np.where(np.arange(128) % 2, 1.0, -1.0) * 2.0 ** power
+    a.q = bf16(q).reshape(1, 1, 128)
+    a.k[0] = bf16(np.full((100, 1, 128), 0.0))
+    a.k[0][41, 0, :4] = bf16(q[:4] * 2.0 ** -power * 2.0 ** -9)
+    a.scale = scale
+    a.fill()
+    y, _ = a.device().run()
+    from _ops import held
+    assert np.array_equal(y[0, 0], bf16(held(a.v[0], bits)[41, 0]))
+
+
 @pytest.mark.parametrize("drafts", [1, 3])
 def test_infinite_values(drafts):
     """In bf16 an infinite value of a token that a row sees makes that output infinite, both signs nothing."""
