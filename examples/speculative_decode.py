@@ -112,9 +112,9 @@ class Model:
         self.head = torch.randint(-127, 128, (VOCAB, HIDDEN), generator=g, dtype=torch.int8).to(DEV)
         self.head_scale = torch.full((VOCAB,), 0.02 / HIDDEN ** 0.5, device=DEV)
 
-    def __call__(self, tokens, pos, slots, lens, table, caches):
-        """Logits [m][VOCAB] of tokens [m] (each sequence's side by side) at positions pos, cached at slots; lens: of the
-        sequences, these tokens included."""
+    def __call__(self, tokens, pos, slots, lens, table, caches, head=True):
+        """Logits [m][VOCAB] (if `head`) of tokens [m] (each sequence's side by side) at positions pos, cached at slots; lens:
+        of the sequences, these tokens included."""
         m = len(tokens)
         x = self.embed[tokens.long()]
         for (qkv, out, gate_up, down), cache in zip(self.layers, caches):
@@ -123,6 +123,8 @@ class Model:
             cache.write(y[:, HEADS:], y[:, HEADS + KV_HEADS:], slots)
             x = x + out(cache.attend(y[:, :HEADS], lens, table))
             x = x + down.of_silu(gate_up(norm(x)))
+        if not head:
+            return None
         x = norm(x)
         logits = torch.empty((m, VOCAB), dtype=torch.bfloat16, device=DEV)
         check(L.ak_i8_gemv(x.data_ptr(), self.head.data_ptr(), self.head_scale.data_ptr(), logits.data_ptr(), m, VOCAB, HIDDEN,
@@ -145,20 +147,18 @@ def decode(model, prompts, count, drafts, bits):
     table = torch.randperm(b * need, device=DEV).to(torch.int32).view(b, need)
     caches = [Cache(bits, b * need) for _ in range(LAYERS)]
 
-    def forward(tokens, first):  # tokens [b][n], the first of each at position first[i]
+    def forward(tokens, first, head=True):  # tokens [b][n], the first of each at position first[i]
         n = len(tokens[0])
         pos = torch.tensor([p + j for p in first for j in range(n)], dtype=torch.int32, device=DEV)
         seq = torch.arange(b, device=DEV).repeat_interleave(n)
         slots = table[seq, (pos // PAGE).long()] * PAGE + pos % PAGE
         lens = torch.tensor([p + n for p in first], dtype=torch.int32, device=DEV)
         flat = torch.tensor(tokens, dtype=torch.int32, device=DEV).reshape(-1)
-        return model(flat, pos, slots, lens, table, caches)
+        return model(flat, pos, slots, lens, table, caches, head)
 
     history = [list(p) for p in prompts]
-    done = [0] * b  # tokens in the cache
-    for j in range(len(prompts[0]) - 1):  # (prompts of one length, a token at a time)
-        forward([[h[j]] for h in history], done)
-        done = [d + 1 for d in done]
+    forward([h[:-1] for h in history], [0] * b, head=False)  # (prompts of one length, all but the last token in one call)
+    done = [len(h) - 1 for h in history]  # tokens in the cache
     u = torch.zeros((b, t + 1), device=DEV)
     cold = torch.zeros((b,), device=DEV)  # greedy
     emitted = torch.empty((b, t + 1), dtype=torch.int32, device=DEV)
