@@ -11,7 +11,8 @@
 // Both kernels are streams: dim / 8 lanes take the keys and the values of one (token, head), 16 bytes of bf16 a lane each;
 // the largest magnitude is found by lane exchanges.  Consecutive groups of a workgroup take consecutive tokens of one head,
 // whose slots are usually consecutive, so that a wave writes whole lines of the page.  Measured with 16384 tokens of 8 heads
-// of 128 in 8 bits: written in 24 us, 101 MB at 4.2 TB/s, and read in 17, 5.9 TB/s; one token 3 us, a launch.
+// of 128, six such in turn: written in 27, 22 and 20 us in 16, 8 and 4 bits (134, 101 and 84 MB: 4.9, 4.6 and 4.2 TB/s), read in
+// 27, 24 and 24 (4.9, 4.2 and 3.5); one token 3 us, a launch.
 #include "agens_kernels.h"
 #include "kv_page.h"
 

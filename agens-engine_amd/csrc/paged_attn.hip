@@ -26,11 +26,11 @@
 // the memory busy, and a second small kernel adds up; or, where there is no scratch for that, a wave takes a sequence's head.
 // Contexts of up to one block need neither plan nor second kernel: the waves of a workgroup take a part each (kShort).
 //
-// Measured (heads of 128 values, 40 query heads on 8): one context of 131072 tokens in bf16 93 us, 5.7 TB/s of the cache; 64 of
-// 8192 in 8 bits 195 us, 5.6; 16 of up to 32768 in 4 bits 114 us, 4.6, where unpacking, some 400 instructions a chunk, is
+// Measured (heads of 128 values, 40 query heads on 8): one context of 131072 tokens in bf16 89 us, 6.0 TB/s of the cache; 64 of
+// 8192 in 8 bits 196 us, 5.6; 16 of up to 32768 in 4 bits 126 us, 4.2, where unpacking, some 400 instructions a chunk, is
 // what the waves wait for; one of 777 tokens 13 us, of 100 8 us: a launch, a wave's loads one after the other (page table,
-// then rows), and its chunks.  8 drafts of 4 sequences (40 rows a key-value head, three tiles) 44 us: each tile loads and
-// unpacks the tokens anew.  512 tokens on 8192: 372 us, 230 TFLOP/s.
+// then rows), and its chunks.  8 drafts of 4 sequences (40 rows a key-value head, three tiles) 42 us in 8 bits, 53 in bf16: each
+// tile loads and unpacks the tokens anew.  512 tokens on 8192: 380 us in 8 bits, 220 TFLOP/s; in bf16 580, 145.
 #include "agens_kernels.h"
 #include "kv_page.h"
 

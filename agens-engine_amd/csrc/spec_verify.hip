@@ -18,7 +18,7 @@
 // Without scratch (a capture before any other call), verify_whole_kernel does all of it in one workgroup a sequence, in the
 // same order, so with the same bits.
 //
-// Measured: 32 sequences of 5 looked-up drafts, 152064 logits (58 MB) 23 us: rows 16, 3.6 TB/s (a wave instead of a workgroup
+// Measured: 32 sequences of 5 looked-up drafts, 152064 logits (58 MB) 22 us: rows 16, 3.7 TB/s (a wave instead of a workgroup
 // for 4096 logits, without barriers, or 32 logits a thread: no faster), decision and draw 8, a chain of dependent loads; one
 // sequence with 4 drafts and their logits 14 us, of which rows 4, decision 5, draw 4.  (LDS atomics for the picks cost 5 us
 // each, exchanges through LDS instead of DPP 2.)

@@ -289,7 +289,7 @@ int ak_paged_attn(int bits, const void* q, int m, long ldq, const void* pool, in
  * Speculative sampling of b sequences with up to t drafted tokens each: target logits bf16 [b][t + 1][ldt] (row j: after j
  * drafts), draft logits bf16 [b][t][ldd] of the model that drew the drafts, or NULL for drafts that were not drawn at random
  * (looked up, or a greedy draft), ids [b][t] the drafts, counts [b] how many each sequence has (NULL: t), u fp32 [b][t + 1]
- * uniform in [0, 1), temperature fp32 [b] (NULL: 1; 0 or less: greedy), all in device memory.  Draft j is accepted while
+ * uniform in [0, 1), temperature fp32 [b] (NULL: 1; 0 or less: greedy; at most 1.44e30), all in device memory.  Draft j is accepted while
  * u[j] q(x) < p(x), p = softmax(target / temperature), q likewise of the draft (NULL: 1 on x); the next token comes from
  * max(p - q, 0) after a rejection, else from p, by the inverse of its cumulative sum at u[t]; greedy: from the largest
  * logit, the lowest token among equal ones.  With t = 0 this draws one token from p.
