@@ -160,12 +160,10 @@ def test_values_of_any_size(bits, first, then):
     assert (np.abs(e - wl) <= tl).all()
 
 
-@pytest.mark.parametrize("bits", [16, 8, 4])
-@pytest.mark.parametrize("power", [-110, 100, 118, 119, 120, 123])
+# (in bf16 q . k is summed before the scale, and leaves fp32 at 2^123 times these queries)
+@pytest.mark.parametrize("bits,power", [(b, p) for b in (16, 8, 4) for p in (-110, 100, 118, 119, 120, 123) if b < 16 or p < 123])
 def test_queries_and_scales_far_from_one(bits, power):
     """Queries times a power of two with a scale divided by it: the same scores."""
-    if bits == 16 and power == 123:
-        pytest.skip("q . k itself, some 2^5 times the power, leaves fp32")
     a = Scene(12, bits, 16, 5, 1, 128, [300, 37], [2, 1], 1.0).device()
     y, e = a.run()
     a.q = bf16(bf2f_array(a.q) * np.float32(2.0 ** power))
