@@ -1,0 +1,275 @@
+// Rotary positions: queries and keys turned by their tokens' positions, alone or on the way into the cache's pages.
+//
+//   pair j of a head (values j and j + rot / 2, or 2j and 2j + 1) turns by pos * freqs[j]:
+//   x' = mag (x cos - y sin), y' = mag (y cos + x sin), values from `rot` on stay.
+//
+// Angles, their sines and cosines, and the products are 64 bits, rounded once to bf16: in 32 bits an angle of a far position
+// (10^6 radians) is off by 0.03, and products off by a rounding now and then put a value on the other side of a bf16 border,
+// which then moves a code in the cache.  The 64-bit vector rate of this GPU is half its 32-bit rate, and the kernels wait for
+// memory.
+//
+// A workgroup takes a few tokens: it works out their sines and cosines once, into LDS, for all heads.  Then every group of
+// dim / 8 lanes (a power of two: 80 values take 16 lanes, 10 of them at work) takes one head of one token, 16 bytes a lane; a
+// lane loads its pairs' other halves itself, which are in the same lines.  A head stays within one wave's instructions, so
+// that rotating in place is safe: all of its loads come before its stores.
+#include <math.h>
+
+#include "agens_kernels.h"
+#include "kv_codes.h"
+
+namespace agq {
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+  const uint16_t *q, *k, *v;
+  uint16_t* y;
+  long ldq, ldk, ldv, ldy;
+  const int *pos, *slots;
+  const double* freqs;
+  double mag;
+  uint8_t* pool;
+  KvShape s;
+  int page_log2, m, heads, dim, rot, tokens;  // tokens: of a workgroup
+};
+
+// cos and sin of a = pos * f.  a = n pi / 2 + r: the product's rounding and pi's bits past 53 go into r; then Taylor's series
+// for |r| <= pi / 4 up to r^16 (the next terms are below 2^-53 of the value).
+__device__ __forceinline__ double2 turn(int pos, double f) {
+  const double p = (double)pos, a = p * f, lost = __builtin_fma(p, f, -a);
+  const double n = __builtin_rint(a * 0.63661977236758134308);
+  double r = __builtin_fma(-n, 1.57079632679489655800, a);
+  r = __builtin_fma(-n, 6.12323399573676603587e-17, r) + lost;
+  const double z = r * r;
+  double s = -1.0 / 1307674368000.0, c = 1.0 / 20922789888000.0;
+  s = __builtin_fma(s, z, 1.0 / 6227020800.0);
+  s = __builtin_fma(s, z, -1.0 / 39916800.0);
+  s = __builtin_fma(s, z, 1.0 / 362880.0);
+  s = __builtin_fma(s, z, -1.0 / 5040.0);
+  s = __builtin_fma(s, z, 1.0 / 120.0);
+  s = __builtin_fma(s, z, -1.0 / 6.0);
+  s = __builtin_fma(s * z, r, r);
+  c = __builtin_fma(c, z, -1.0 / 87178291200.0);
+  c = __builtin_fma(c, z, 1.0 / 479001600.0);
+  c = __builtin_fma(c, z, -1.0 / 3628800.0);
+  c = __builtin_fma(c, z, 1.0 / 40320.0);
+  c = __builtin_fma(c, z, -1.0 / 720.0);
+  c = __builtin_fma(c, z, 1.0 / 24.0);
+  c = __builtin_fma(c, z, -0.5);
+  c = __builtin_fma(c, z, 1.0);
+  const int quarter = (int)(n - 4.0 * __builtin_floor(n * 0.25));
+  const double u = quarter & 1 ? s : c, v = quarter & 1 ? c : s;
+  return make_double2(quarter == 1 || quarter == 2 ? -u : u, quarter & 2 ? -v : v);
+}
+
+// 64 bits -> the nearest bf16.  The step over 32 bits keeps as its last bit whether anything was cut off, so the second
+// rounding sees the side of a border that the value is on.
+__device__ __forceinline__ uint32_t d2bf(double d) {
+  const uint64_t u = (uint64_t)__double_as_longlong(d);
+  uint32_t lo = (uint32_t)u;
+  lo = (lo & 0xE0000000u) | ((lo & 0x1FFFFFFFu) ? 0x20000000u : 0u);
+  return f2bf((float)__longlong_as_double((long long)((u & 0xFFFFFFFF00000000ull) | lo)));
+}
+
+__device__ __forceinline__ uint32_t value(const uint4& x, int i) {
+  const uint32_t w = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;
+  return i & 1 ? w >> 16 : w & 0xFFFFu;
+}
+
+// Where pair j of a token lies among its sines and cosines: lanes whose pairs begin EACH apart read side by side.
+template <int EACH>
+__device__ __forceinline__ int spot(int j, int pairs) {
+  return (j % EACH) * ((pairs + EACH - 1) / EACH) + j / EACH;
+}
+__host__ __device__ inline int spots(int pairs) { return (pairs + 7) / 8 * 8; }
+
+// The lane's 8 values of a row, rotated.  LAYOUT: 0 halves with rot % 16 == 0, 1 halves, 2 neighbours.
+template <int LAYOUT>
+__device__ __forceinline__ uint4 rotated(const RopeArgs& a, const uint16_t* row, int lane, const double2* cs) {
+  uint4 x = *reinterpret_cast<const uint4*>(row + 8 * lane);
+  const int at = 8 * lane, half = a.rot / 2;
+  if (at >= a.rot) return x;
+  uint32_t out[8];
+  if constexpr (LAYOUT == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double u = bf2f(value(x, 2 * i)), v = bf2f(value(x, 2 * i + 1));
+      const double2 t = cs[spot<4>(min(at / 2 + i, half - 1), half)];
+      out[2 * i] = d2bf(__builtin_fma(u, t.x, -(v * t.y)));
+      out[2 * i + 1] = d2bf(__builtin_fma(v, t.x, u * t.y));
+    }
+  } else {
+    uint4 o = x;
+    if constexpr (LAYOUT == 0) o = *reinterpret_cast<const uint4*>(row + (at < half ? at + half : at - half));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = min(at + i, a.rot - 1);
+      const bool low = e < half;
+      const int j = low ? e : e - half;
+      const uint32_t other = LAYOUT == 0 ? value(o, i) : row[low ? e + half : j];
+      const double u = bf2f(value(x, i)), v = bf2f(other);
+      const double2 t = cs[spot<8>(j, half)];
+      out[i] = d2bf(__builtin_fma(u, t.x, low ? -(v * t.y) : v * t.y));
+    }
+  }
+  if constexpr (LAYOUT != 0) {  // a lane across rot's end
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (at + i >= a.rot) out[i] = value(x, i);
+  }
+  return make_uint4(out[0] | out[1] << 16, out[2] | out[3] << 16, out[4] | out[5] << 16, out[6] | out[7] << 16);
+}
+
+// One row of keys or values (part 0 or 1) into its slot.
+template <int BITS, int D>
+__device__ __forceinline__ void store_row(const RopeArgs& a, const uint4 x, int slot, int head, int part, int lane) {
+  const KvPlace p = kv_place(a.s, a.pool, a.page_log2, slot, head);
+  uint8_t* const row = part ? p.vrow : p.krow;
+  if constexpr (BITS == 16) {
+    reinterpret_cast<uint4*>(row)[lane] = x;
+  } else {
+    uint32_t s;
+    const uint64_t c = quantise8<BITS>(x, row_amax<D / 8>(x), &s);
+    if constexpr (BITS == 8)
+      reinterpret_cast<uint64_t*>(row)[lane] = c;
+    else
+      reinterpret_cast<uint32_t*>(row)[lane] = (uint32_t)c;
+    if (lane == 0) reinterpret_cast<uint16_t*>(p.pair)[part] = (uint16_t)s;
+  }
+}
+
+// BITS 0: heads of q alone.  Otherwise heads of q, then keys, then values of every token.
+template <int BITS, int D, int LAYOUT>
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a, int lanes_log2) {
+  extern __shared__ double2 cs[];  // [tokens][spots(rot / 2)]
+  const int first = blockIdx.x * a.tokens, n = min(a.tokens, a.m - first), half = a.rot / 2, per = spots(half);
+  for (int e = threadIdx.x; e < n * half; e += kRopeThreads) {
+    const int t = e / half, j = e - t * half;
+    const double2 v = turn(max(a.pos[first + t], 0), a.freqs[j]);
+    cs[t * per + (LAYOUT == 2 ? spot<4>(j, half) : spot<8>(j, half))] = make_double2(v.x * a.mag, v.y * a.mag);
+  }
+  __syncthreads();
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), groups = kRopeThreads >> lanes_log2;
+  const int rows = BITS ? a.heads + 2 * a.s.heads : a.heads;
+  for (int e = threadIdx.x >> lanes_log2; e < n * rows; e += groups) {
+    const int lt = e / rows, h = e - lt * rows, t = first + lt;
+    if (a.pos[t] < 0 || 8 * lane >= a.dim) continue;
+    const double2* const c = cs + lt * per;
+    if (h < a.heads) {
+      const size_t off = (size_t)h * a.dim;
+      const uint4 r = rotated<LAYOUT>(a, a.q + t * a.ldq + off, lane, c);
+      *reinterpret_cast<uint4*>(a.y + t * a.ldy + off + 8 * lane) = r;
+    } else if constexpr (BITS != 0) {
+      const int slot = a.slots[t], part = h >= a.heads + a.s.heads, kh = h - a.heads - (part ? a.s.heads : 0);
+      if (slot < 0 || slot >> a.page_log2 >= a.s.npages) continue;  // (whole groups of lanes)
+      const uint4 x = part ? *reinterpret_cast<const uint4*>(a.v + t * a.ldv + (size_t)kh * D + 8 * lane)
+                           : rotated<LAYOUT>(a, a.k + t * a.ldk + (size_t)kh * D, lane, c);
+      store_row<BITS, D>(a, x, slot, kh, part, lane);
+    }
+  }
+}
+
+template <int BITS, int D, int LAYOUT>
+int launch(RopeArgs a, hipStream_t s) {
+  int lanes_log2 = 0;
+  while ((8 << lanes_log2) < a.dim) ++lanes_log2;
+  const int rows = BITS ? a.heads + 2 * a.s.heads : a.heads;
+  // tokens of a workgroup: three rounds of its lanes, while their sines and cosines fit 16 KB
+  const int per = spots(a.rot / 2) * 16;
+  int tokens = 3 * (kRopeThreads >> lanes_log2) / rows;
+  tokens = tokens < 1 ? 1 : tokens;
+  while (tokens > 1 && tokens * per > 16384) --tokens;
+  a.tokens = tokens;
+  const int m = a.m, most = (1 << 23) * (tokens < 64 ? tokens : 64);  // of a launch: its lanes are counted in 32 bits
+  for (int t = 0; t < m; t += a.m) {
+    a.m = m - t < most ? m - t : most;
+    hipLaunchKernelGGL((rope_kernel<BITS, D, LAYOUT>), dim3((unsigned)((a.m - 1) / tokens + 1)), dim3(kRopeThreads),
+                       (size_t)tokens * per, s, a, lanes_log2);
+    if (const int e = (int)hipGetLastError()) return e;
+    a.q += a.m * a.ldq, a.k += a.m * a.ldk, a.v += a.m * a.ldv, a.y += a.m * a.ldy, a.pos += a.m;
+    if (BITS) a.slots += a.m;
+  }
+  return 0;
+}
+template <int BITS, int D>
+int launch_layout(const RopeArgs& a, int interleaved, hipStream_t s) {
+  return interleaved ? launch<BITS, D, 2>(a, s) : a.rot % 16 ? launch<BITS, D, 1>(a, s) : launch<BITS, D, 0>(a, s);
+}
+template <int BITS>
+int launch_dim(const RopeArgs& a, int interleaved, hipStream_t s) {
+  return a.dim == 64 ? launch_layout<BITS, 64>(a, interleaved, s)
+                     : a.dim == 128 ? launch_layout<BITS, 128>(a, interleaved, s) : launch_layout<BITS, 256>(a, interleaved, s);
+}
+
+bool rows_ok(const void* p, long ld, int m, long width, bool written) {
+  return p && aligned16(p) && ld >= 0 && ld % 8 == 0 && (!written || m <= 1 || ld >= width);
+}
+bool turn_ok(const int* pos, const double* freqs, int rot, int dim, int interleaved, float mag) {
+  return pos && freqs && rot >= 2 && rot <= dim && rot % 2 == 0 && (interleaved == 0 || interleaved == 1) && isfinite(mag);
+}
+
+}  // namespace
+}  // namespace agq
+
+extern "C" int ak_rope(const void* x, long ldx, void* y, long ldy, int m, int heads, int dim, const int* pos,
+                       const double* freqs, int rot, int interleaved, float mag, void* stream) {
+  if (m < 0 || heads < 1 || heads > 4096 || dim < 8 || dim > 512 || dim % 8) return AK_INVALID;
+  if (!m) return 0;
+  const long width = (long)heads * dim;
+  if (!agq::rows_ok(x, ldx, m, width, false) || !agq::rows_ok(y, ldy, m, width, true) ||
+      !agq::turn_ok(pos, freqs, rot, dim, interleaved, mag) || (x == y && m > 1 && ldx != ldy))
+    return AK_INVALID;
+  agq::RopeArgs a{};
+  a.q = static_cast<const uint16_t*>(x), a.y = static_cast<uint16_t*>(y), a.ldq = ldx, a.ldy = ldy;
+  a.pos = pos, a.freqs = freqs, a.mag = (double)mag, a.m = m, a.heads = heads, a.dim = dim, a.rot = rot;
+  return agq::launch_layout<0, 0>(a, interleaved, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ak_rope_kv_write(int bits, const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* y,
+                                long ldy, int m, int heads, const int* pos, const double* freqs, int rot, int interleaved,
+                                float mag, const int* slots, void* pool, int npages, int page, int kv_heads, int dim,
+                                void* stream) {
+  const agq::KvShape s{bits, page, kv_heads, dim, npages};
+  if (!s.valid() || m < 0 || npages < 1 || heads < 1 || heads > 4096) return AK_INVALID;
+  if (!m) return 0;
+  const long width = (long)heads * dim, kv = (long)kv_heads * dim;
+  if (!agq::rows_ok(q, ldq, m, width, false) || !agq::rows_ok(y, ldy, m, width, true) ||
+      !agq::rows_ok(k, ldk, m, kv, false) || !agq::rows_ok(v, ldv, m, kv, false) ||
+      !agq::turn_ok(pos, freqs, rot, dim, interleaved, mag) || (q == y && m > 1 && ldq != ldy) || !slots || !pool ||
+      !agq::aligned16(pool))
+    return AK_INVALID;
+  agq::RopeArgs a{};
+  a.q = static_cast<const uint16_t*>(q), a.k = static_cast<const uint16_t*>(k), a.v = static_cast<const uint16_t*>(v);
+  a.y = static_cast<uint16_t*>(y), a.ldq = ldq, a.ldk = ldk, a.ldv = ldv, a.ldy = ldy;
+  a.pos = pos, a.slots = slots, a.freqs = freqs, a.mag = (double)mag, a.pool = static_cast<uint8_t*>(pool), a.s = s;
+  a.page_log2 = __builtin_ctz((unsigned)page), a.m = m, a.heads = heads, a.dim = dim, a.rot = rot;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return bits == 16 ? agq::launch_dim<16>(a, interleaved, st)
+                    : bits == 8 ? agq::launch_dim<8>(a, interleaved, st) : agq::launch_dim<4>(a, interleaved, st);
+}
+
+// Host only.  Bands: pair j makes trained * f / 2 pi turns over the trained context; pairs of more than `fast` keep their
+// frequency, pairs of fewer than `slow` have it divided, and those between are mixed in proportion.
+extern "C" int ak_rope_freqs(double theta, int rot, int scaling, double factor, long trained, double slow, double fast,
+                             double* freqs, float* mag) {
+  if (!(theta > 0) || !isfinite(theta) || rot < 2 || rot % 2 || !freqs || !mag || scaling < AK_ROPE_PLAIN ||
+      scaling > AK_ROPE_BANDS)
+    return AK_INVALID;
+  if (scaling != AK_ROPE_PLAIN && (!(factor >= 1) || !isfinite(factor))) return AK_INVALID;
+  if (scaling == AK_ROPE_BASE && rot < 4) return AK_INVALID;
+  if (scaling == AK_ROPE_BANDS && (trained < 1 || !(slow >= 0) || !(fast > slow) || !isfinite(fast))) return AK_INVALID;
+  if (scaling == AK_ROPE_BASE) theta *= pow(factor, (double)rot / (rot - 2));
+  for (int j = 0; j < rot / 2; ++j) {
+    double f = pow(theta, -2.0 * j / rot);
+    if (scaling == AK_ROPE_LINEAR) f /= factor;
+    if (scaling == AK_ROPE_BANDS) {
+      const double turns = (double)trained * f / 6.28318530717958647692;
+      const double keep = fmin(fmax((turns - slow) / (fast - slow), 0.0), 1.0);
+      f *= keep + (1.0 - keep) / factor;
+    }
+    freqs[j] = f;
+  }
+  *mag = scaling == AK_ROPE_BANDS ? (float)(0.1 * log(factor) + 1.0) : 1.0f;
+  return 0;
+}

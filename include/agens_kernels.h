@@ -305,6 +305,92 @@ int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, co
                    const float* u, const float* temperature, int b, int t, int vocab, int* tokens, int* accepted,
                    float* logp, void* stream);
 
+/* ---------------------------------------------------------------------------------------------- pages for a batch
+ * What a step needs before its linears, built where the lengths are: the cache pages of b sequences' new tokens, off a free
+ * list, and these tokens' ranges, positions and slots.  Sequence i has cached[i] tokens in the cache, held[i] pages in
+ * table[i * ldt ...], and counts[i] new tokens; drop[i] (drop may be NULL) other than 0: it has ended, its pages go to the end of
+ * the free list, in order, and the row begins anew with counts[i] tokens.  Missing pages come off the end of the list, in the
+ * order of the sequences.  A sequence that does not fit its ldt pages, or whose range passes m, is refused, as is one whose
+ * pages are not all there, and then every later one that wants any; it keeps what it had.  free_pages [npages] with
+ * free_count[0] pages in it; NULL: the table's pages are taken as they are (held, held_out, free_count, free_out unused).
+ *   lens [b]       cached and new tokens (refused: cached);       held_out [b], free_out [1]   as held and free_count, after;
+ *   qstart [b + 1] the ranges of the new tokens, side by side (ak_paged_attn's; at most m);       refused [b]  0 or 1;
+ *   pos [m], slots [m]   position of each token, and its slot (ak_kv_write's); -1 past the last and for refused sequences, and
+ *                  the slot alone where the table holds no page of the pool.
+ * All arrays are device memory, and the results may be the inputs' own arrays (lens as cached, held_out as held, free_out as
+ * free_count); no other two may overlap.  Negative counts, lengths and pages count as 0.  b * ldt up to 2^30, npages * page
+ * below 2^31.  Only launches, allocates nothing, can be captured: a captured step follows counts from replay to replay. */
+#define AK_PLAN_MAX_SEQS 1024
+#define AK_PLAN_MAX_TOKENS 1048576
+int ak_kv_plan(int b, int m, const int* counts, const int* drop, const int* cached, const int* held,
+               const int* free_count, int* free_pages, int npages, int page, int* table, int ldt, int* lens, int* held_out,
+               int* free_out, int* qstart, int* pos, int* slots, int* refused, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- rotary positions
+ * Heads of bf16 turned by their tokens' positions.  Pair j < rot / 2 of a head is values j and j + rot / 2 (interleaved 0), or
+ * 2j and 2j + 1 (1); with the angle c = pos[t] * freqs[j] (radians, fp64, device memory)
+ *   x' = mag * (x cos c - y sin c),  y' = mag * (y cos c + x sin c),
+ * computed in 64 bits and rounded once; values from rot on (even, up to dim) stay.  Negative frequencies turn back.  Tokens
+ * with a negative position are left alone.  Positions and frequencies up to a product of 2^31.
+ *   ak_rope   heads of x (token t at x + t * ldx, heads contiguous; 16-byte aligned, multiples of 8) to y, which may be x (with
+ *             the same stride) but overlap it in no other way.  dim a multiple of 8 up to 512, heads up to 4096;
+ *   ak_rope_kv_write   q to y likewise, the keys turned, and keys and values into slots (the paged cache's): what ak_rope of q,
+ *             ak_rope of k and ak_kv_write leave, bit for bit, in one launch and without the turned keys' way through memory;
+ *   ak_rope_freqs      host memory, no device: freqs[j] = theta^(-2j / rot) and *mag = 1, for contexts `factor` times the
+ *             trained one: LINEAR divides all by factor; BASE takes theta * factor^(rot / (rot - 2)); BANDS divides those that
+ *             make fewer than `slow` turns in `trained` tokens, leaves those of more than `fast`, mixes those between in
+ *             proportion, and gives *mag = 0.1 ln factor + 1. */
+#define AK_ROPE_PLAIN 0
+#define AK_ROPE_LINEAR 1
+#define AK_ROPE_BASE 2
+#define AK_ROPE_BANDS 3
+int ak_rope_freqs(double theta, int rot, int scaling, double factor, long trained, double slow, double fast, double* freqs,
+                  float* mag);
+int ak_rope(const void* x, long ldx, void* y, long ldy, int m, int heads, int dim, const int* pos, const double* freqs,
+            int rot, int interleaved, float mag, void* stream);
+int ak_rope_kv_write(int bits, const void* q, long ldq, const void* k, long ldk, const void* v, long ldv, void* y, long ldy,
+                     int m, int heads, const int* pos, const double* freqs, int rot, int interleaved, float mag,
+                     const int* slots, void* pool, int npages, int page, int kv_heads, int dim, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- sampling
+ * One token of each of b rows of logits (bf16 [b][ld]).  With p = softmax(logits / temperature) and the tokens in order of
+ * falling logit, the lower token first among equal ones: top_k keeps the first top_k; top_p the fewest of these, from the front,
+ * whose p reach top_p of the sum of theirs (one at least); min_p drops those with p below min_p times the largest.  The token is
+ * the first, in order of tokens, at which the cumulative p of those kept passes u times their sum.  temperature [b] (NULL: 1; 0
+ * or less: greedy, the largest logit; more than 1.44e30 counts as that), top_k [b] (NULL, or 0 or less, or vocab and more: off), top_p [b]
+ * (NULL, or 1 and more: off), min_p [b] (NULL, or 0 and less: off), u [b] uniform in [0, 1), all in device memory.
+ * logp (may be NULL): log p of the token before any filter (greedy: at temperature 1).  NaN logits count as -inf; a row of
+ * nothing else gives the token -1 and logp 0.  Without filters the tokens are ak_spec_verify's with t = 0, but for roundings.
+ * Weights are fp32; sums of what filters keep count whole 2^-42 of the largest weight, so a token below that is not drawn.
+ * Rows need no alignment beyond bf16's.  Library scratch (above; inside a capture the graph's own): 2064 bytes for each 16384
+ * logits, 64 MB at most; without it one workgroup takes a row, with the same tokens. */
+#define AK_SAMPLE_MAX_VOCAB 1048576
+int ak_sample(const void* logits, long ld, const float* temperature, const int* top_k, const float* top_p,
+              const float* min_p, const float* u, int b, int vocab, int* tokens, float* logp, void* stream);
+
+/* ---------------------------------------------------------------------------------------------- low-rank adapters
+ * Adapters of many requests beside a shared linear: y_t = base_t + scale[a] * B_a (A_a x_t) for token t of adapter a = ids[t];
+ * tokens with ids[t] outside [0, adapters) have none, and y_t = base_t.  Up to 4 segments that share x, as in
+ * ak_wq_gemv_kt_multi: a bf16 [adapters][nseg * rank][k], segment i's rank rows after those before it; b[i] bf16
+ * [adapters][n[i]][rank]; rank a multiple of 8 up to AK_LORA_MAX_RANK (pad with zeros), k a multiple of 8; x bf16 [m] rows of
+ * stride ldx (a multiple of 8); a, b[i] and x 16-byte aligned; y[i] and base[i] bf16 of row stride ldy[i] (0, or ldy NULL:
+ * n[i]).  base (the linear's outputs) NULL, or base[i] the same as y[i]: added in place; they may overlap in no other way.
+ * scale [adapters] fp32 in device memory (NULL: 1).  Sums are fp32; A x is rounded to 16 bits before B, y once to bf16; a
+ * token's bits do not depend on the other tokens.
+ * ak_lora_plan groups the tokens by adapter, once for all linears of a step, into `plan`: 16-byte aligned device memory of
+ * ak_lora_plan_bytes(m, adapters, nseg * rank, k) bytes, the most over these linears (0: refused).  It also holds what
+ * ak_lora_add's launches hand on, so calls with one plan must follow one another; ak_lora_add with other m or adapters than
+ * the plan's leaves y alone.  Only launches, allocates nothing, can be captured. */
+#define AK_LORA_MAX_RANK 128
+#define AK_LORA_MAX_ADAPTERS 4096
+#define AK_LORA_MAX_TOKENS 1048576
+#define AK_LORA_MAX_INPUTS 16777216 /* and output rows */
+size_t ak_lora_plan_bytes(int m, int adapters, int ranks, int k);
+int ak_lora_plan(const int* ids, int m, int adapters, void* plan, void* stream);
+int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, int adapters, int rank, const void* a,
+                const float* scale, int nseg, const void* const* b, const void* const* base, void* const* y, const int* n,
+                const int* ldy, void* stream);
+
 /* ---------------------------------------------------------------------------------------------- switches
  * reference: agens_kernels.h:205 / :208 / :211, w4_gemv.cu:3271-3282.  mma: -1 auto (environment AGENS_W4_EXACT), 0 exact
  * fp32 path, 1 default integer-MFMA path.  lean / tma select bit-identical sm90-only variants in the reference;

@@ -1,0 +1,280 @@
+"""Sampling (ak_sample) on the GPU, against 64 bits (numpy, test infrastructure).
+
+Tokens are compared exactly except where a decision of the 64-bit evaluation lies within 1e-5 of its threshold; the log
+probabilities within 2^-20 of 1 + |log p| per unit of (largest logit difference / temperature): a logit difference is exact in
+fp32, its quotient and exponential are rounded."""
+import ctypes
+import os
+import subprocess
+import sys
+
+import numpy as np
+import pytest
+
+from _lib import check, Dev, f2bf_array, bf2f_array
+from _ops import Stream, Graph
+from _step import step, sample64
+
+pytestmark = pytest.mark.gpu
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+class Rows:
+    """b rows of logits and their settings (None: the argument is left out)."""
+
+    def __init__(self, bits, temp=None, top_k=None, top_p=None, min_p=None, u=None, pad=0):
+        self.bits = bits
+        self.b, self.vocab = bits.shape
+        self.ld = self.vocab + pad
+        mem = np.full((self.b, self.ld), 0x7F7F, dtype=np.uint16)  # between the rows: never to be chosen
+        mem[:, :self.vocab] = bits
+        full = lambda v, t: None if v is None else np.broadcast_to(np.asarray(v, dtype=t), (self.b,)).copy()  # noqa: E731
+        self.temp, self.top_k = full(temp, np.float32), full(top_k, np.int32)
+        self.top_p, self.min_p = full(top_p, np.float32), full(min_p, np.float32)
+        self.u = full(0.5 if u is None else u, np.float32)
+        dev = lambda v: None if v is None else Dev.of(v)  # noqa: E731
+        self.L = Dev.of(mem)
+        self.d = [dev(v) for v in (self.temp, self.top_k, self.top_p, self.min_p, self.u)]
+        self.tok, self.lp = Dev.of(np.full(self.b + 1, 99, dtype=np.int32)), Dev.of(np.full(self.b + 1, 99, dtype=np.float32))
+
+    def call(self, stream=None, logp=True):
+        return step().ak_sample(self.L.p, self.ld, *[x.p if x else None for x in self.d], self.b, self.vocab, self.tok.p,
+                                self.lp.p if logp else None, stream)
+
+    def got(self):
+        check(step().ak_synchronize())
+        t, l = self.tok.get(np.int32, self.b + 1), self.lp.get(np.float32, self.b + 1)
+        assert t[self.b] == 99 and l[self.b] == 99
+        return t[:self.b], l[:self.b]
+
+    def run(self):
+        check(self.call())
+        return self.got()
+
+    def compare(self, got, least=0.9, tol=1e-5):
+        tok, lp = got
+        sure = 0
+        for i in range(self.b):
+            v = lambda x, off: off if x is None else x[i]  # noqa: E731
+            heat = min(float(v(self.temp, 1.0)), 1.44e30)  # (more counts as that)
+            want, wl, near = sample64(self.bits[i], heat, int(v(self.top_k, 0)), float(v(self.top_p, 1.0)),
+                                      float(v(self.min_p, 0.0)), float(self.u[i]), tol)
+            if near:
+                continue
+            sure += 1
+            assert tok[i] == want, (i, tok[i], want, heat, v(self.top_k, 0), v(self.top_p, 1), v(self.min_p, 0), self.u[i])
+            l = bf2f_array(self.bits[i]).astype(np.float64)
+            spread = np.ptp(l[np.isfinite(l)]) / (heat if heat > 0 else 1.0) if np.isfinite(l).any() else 0.0
+            assert abs(lp[i] - wl) <= 2.0 ** -20 * (1 + abs(wl)) * (1 + spread)
+        assert sure >= int(least * self.b)
+
+
+def logits(rng, b, vocab, spread=2.0, peaks=8):
+    x = rng.standard_normal((b, vocab)) * spread
+    for r in x:
+        r[rng.integers(0, vocab, peaks)] += 6 + 6 * rng.random(peaks)
+    return f2bf_array(x.astype(np.float32).ravel()).reshape(b, vocab)
+
+
+def settings(rng, b, vocab):
+    pick = lambda p, x, off: np.where(rng.random(b) < p, x, off)  # noqa: E731
+    return dict(temp=pick(0.9, 0.2 + 1.5 * rng.random(b), 0.0), top_k=pick(0.5, np.exp(rng.random(b) * np.log(vocab + 1)), 0).astype(int),
+                top_p=pick(0.6, rng.random(b), 1.0), min_p=pick(0.4, 10.0 ** -(4 * rng.random(b)), 0.0), u=rng.random(b))
+
+
+@pytest.mark.parametrize("peaks", [0, 8])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 64, 1000, 1003, 4099, 16384, 16385, 33000, 152064])
+def test_against_64_bits(vocab, peaks):
+    rng = np.random.default_rng(vocab + peaks)
+    b = 12 if vocab > 20000 else 60
+    x = Rows(logits(rng, b, vocab, peaks=min(peaks, vocab)), pad=vocab % 5, **settings(rng, b, vocab))
+    x.compare(x.run(), least=0.7)
+
+
+@pytest.mark.parametrize("one", ["top_k", "top_p", "min_p", None])
+def test_each_filter_alone(one):
+    rng = np.random.default_rng(7)
+    b, vocab = 40, 5000
+    s = settings(rng, b, vocab)
+    s = {"u": s["u"], **({one: dict(top_k=rng.integers(1, 300, b), top_p=0.3 + 0.6 * rng.random(b),
+                                    min_p=0.2 * rng.random(b))[one]} if one else {})}
+    x = Rows(logits(rng, b, vocab), **s)
+    x.compare(x.run())
+
+
+def test_flat_rows_whose_border_is_far_down():
+    """Logits around 0 of either sign: what is kept reaches keys far below the largest's."""
+    rng = np.random.default_rng(9)
+    b, vocab = 48, 40000
+    x = f2bf_array((rng.standard_normal((b, vocab)) * 0.7).astype(np.float32).ravel()).reshape(b, vocab)
+    top_k = np.where(np.arange(b) % 3 == 0, rng.integers(10000, 40000, b), 0)
+    top_p = np.where(np.arange(b) % 3 == 1, 0.9 + 0.0999 * rng.random(b), 1.0)
+    min_p = np.where(np.arange(b) % 3 == 2, 0.01 * rng.random(b), 0.0)
+    r = Rows(x, None, top_k, top_p, min_p, rng.random(b))
+    # exponents below 16 are off by 2^-20 at most, weights and their sums by 2^-20 ln 2 and a step: 8e-7.  (Decisions are 1 / 40000
+    # apart: 1e-5 on either side would leave the half of them out.)
+    r.compare(r.run(), least=0.7, tol=2e-6)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-3, 1.0, 1e30])
+def test_rows_of_any_size(scale):
+    rng = np.random.default_rng(3)
+    b, vocab = 24, 3001
+    x = f2bf_array((rng.standard_normal((b, vocab)) * scale).astype(np.float32).ravel()).reshape(b, vocab)
+    x[::2] |= 0x8000  # all below 0
+    s = settings(rng, b, vocab)
+    s["temp"] = s["temp"] * scale
+    r = Rows(x, **s)
+    r.compare(r.run(), least=0.7)
+
+
+def test_equal_logits():
+    """All weights alike: sums are exact, so the token is known to the last one.  The lowest tokens are kept."""
+    vocab, b = 20000, 9
+    x = np.full((b, vocab), f2bf_array(np.array([-3.0], dtype=np.float32))[0])
+    top_k = [0, 1, 777, 777, 0, 0, 0, 0, 777]
+    top_p = [1, 1, 1, 0.5, 0.25, 0.0, 1, 1, 1]
+    min_p = [0, 0, 0, 0, 0, 0, 1.0, 0.5, 0.0]
+    u = np.float32([0.75, 0.99, 0.5, 0.5, 0.5, 0.99, 0.25, 1 - 2.0 ** -24, 1 - 2.0 ** -24])
+    tok, lp = Rows(x, None, top_k, top_p, min_p, u).run()
+    # kept: all, 1, 777, 389 (388.5 of 777 reached), 5000, 1, all, all, 777
+    assert tok.tolist() == [15000, 0, 388, 194, 2500, 0, 5000, 19999, 776]  # (u times 20000 is 0.0012 below it)
+    assert np.allclose(lp, -np.log(vocab), atol=1e-6)
+
+
+def test_zeros_of_either_sign_are_equal():
+    x = np.full((3, 400), f2bf_array(np.array([-9.0], dtype=np.float32))[0])
+    x[:, 10:20:2], x[:, 11:20:2] = 0x8000, 0x0000
+    tok, _ = Rows(x, [0.0, 1.0, 1.0], [0, 3, 3], None, None, [0.5, 0.5, 0.99]).run()
+    assert tok.tolist() == [10, 11, 12]
+
+
+def test_masked_infinite_and_empty_rows():
+    rng = np.random.default_rng(6)
+    vocab = 30000
+    x = logits(rng, 9, vocab)
+    x[0] = 0xFF80                      # nothing above -inf
+    x[1] = 0x7FC0                      # NaN alone
+    x[2], x[2, 17] = 0xFF80, 0xC000    # one token left
+    x[3, 100], x[3, 29000] = 0x7F80, 0x7F80   # +inf twice
+    x[4, ::2] = 0x7FC1                 # NaN counts as -inf
+    x[5] = 0xFF80
+    x[5, 5:40] = f2bf_array(np.arange(35).astype(np.float32) * 0.1)
+    x[6] = 0xFF7F                      # the type's lowest value
+    x[7], x[7, 29999] = 0xFF7F, 0x7F7F
+    x[8] = 0xFF80
+    x[8, 3], x[8, 4] = 0xFF7F, 0xFF7E
+    for k, p, m in ((0, 1.0, 0.0), (5, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.1), (28000, 0.999, 1e-6)):
+        r = Rows(x, 0.8, k, p, m, 0.6)
+        with np.errstate(over="ignore"):
+            tok, lp = r.run()
+        assert tok[0] == -1 and tok[1] == -1 and lp[0] == 0 and lp[1] == 0
+        assert tok[2] == 17 and lp[2] == 0
+        assert tok[3] == (29000 if k != 1 else 100) and abs(lp[3] + np.log(2)) < 1e-6
+        assert tok[4] % 2 == 1 and 5 <= tok[5] < 40 and tok[7] == 29999 and tok[8] in (3, 4)
+        for i in (4, 5):
+            want, wl, near = sample64(x[i], float(np.float32(0.8)), k, p, m, 0.6)
+            assert near or (tok[i] == want and abs(lp[i] - wl) < 1e-4)
+    tok, _ = Rows(x, 0.0, 3, 0.5, 0.1, 0.6).run()
+    assert tok[:4].tolist() == [-1, -1, 17, 100] and tok[6] == 0
+
+
+def test_settings_out_of_their_ranges():
+    """NaN and what is beyond a filter's range: off, or the most it can do."""
+    rng = np.random.default_rng(8)
+    nan, inf = float("nan"), float("inf")
+    x = logits(rng, 1, 900).repeat(12, 0)
+    r = Rows(x, [1, 1, 1, 1, 1, 1, 1, 1, nan, -1, 1e-45, 3e38], [-5, 900, 2 ** 31 - 1, 0, 0, 0, 0, 0, 0, 0, 0, 0],
+             [nan, inf, 2, -1, 1, 1, 1, 1, 1, 1, 1, 1], [0, 0, 0, 0, nan, -1, 2, inf, 0, 0, 0, 0], 0.7)
+    tok, _ = r.run()
+    free, best = sample64(x[0], 1.0, 0, 1.0, 0.0, 0.7)[0], int(bf2f_array(x[0]).argmax())
+    assert tok.tolist()[:11] == [free, free, free, best, free, free, best, best, best, best, best]
+    assert abs(tok[11] - 630) <= 1  # all tokens alike
+
+
+def test_draws_follow_the_distribution():
+    """Over a grid of u the tokens come as often as their renormalised weights say, to one grid step."""
+    rng = np.random.default_rng(10)
+    n = 2000
+    row = logits(rng, 1, 50, spread=1.0, peaks=0)
+    x = Rows(row.repeat(n, 0), 0.7, 20, 0.95, 0.02, (np.arange(n) + 0.5) / n)
+    tok, _ = x.run()
+    l = bf2f_array(row[0]).astype(np.float64)
+    p = np.exp((l - l.max()) / np.float32(0.7))
+    p /= p.sum()
+    order = np.argsort(-l, kind="stable")[:20]
+    upto = np.cumsum(p[order])
+    order = order[:int((upto < np.float32(0.95) * upto[-1]).sum()) + 1]
+    order = order[p[order] >= np.float32(0.02) * p.max()]
+    w = np.zeros(50)
+    w[order] = p[order] / p[order].sum()
+    assert np.abs(np.bincount(tok, minlength=50) / n - w).max() <= 1.01 / n
+
+
+def test_without_filters_as_verification_draws():
+    rng = np.random.default_rng(11)
+    b, vocab = 32, 152064
+    x = Rows(logits(rng, b, vocab, peaks=30), 0.5 + rng.random(b), u=rng.random(b))
+    tok, lp = x.run()
+    T, A, LP = Dev(4 * b), Dev(4 * b), Dev(4 * b)
+    check(step().ak_spec_verify(x.L.p, x.ld, None, 0, None, None, x.d[4].p, x.d[0].p, b, 0, vocab, T.p, A.p, LP.p, None))
+    check(step().ak_synchronize())
+    assert np.array_equal(tok, T.get(np.int32, b)) and np.allclose(lp, LP.get(np.float32, b), atol=1e-5)
+
+
+def test_many_rows_unaligned_and_without_logp():
+    """More rows than a launch's scratch holds; rows at odd addresses."""
+    rng = np.random.default_rng(12)
+    b, vocab = 33000, 33
+    x = Rows(logits(rng, b, vocab, peaks=3), pad=2, **settings(rng, b, vocab))
+    tok, lp = x.run()
+    for i in rng.integers(0, b, 300):
+        want, wl, near = sample64(x.bits[i], float(x.temp[i]), int(x.top_k[i]), float(x.top_p[i]), float(x.min_p[i]), float(x.u[i]))
+        assert near or tok[i] == want
+    check(x.call(logp=False))
+    assert np.array_equal(x.got()[0], tok)
+
+
+def test_a_row_gives_the_same_alone():
+    rng = np.random.default_rng(13)
+    b, vocab = 20, 60001
+    s = settings(rng, b, vocab)
+    bits = logits(rng, b, vocab, peaks=0)
+    tok, lp = Rows(bits, **s).run()
+    for i in range(0, b, 3):
+        t, l = Rows(bits[i:i + 1], **{k: v[i:i + 1] for k, v in s.items()}).run()
+        assert t[0] == tok[i] and l[0] == lp[i]
+
+
+def captured_before_any_call():
+    """In a process of its own, whose library has no scratch: the form without it, then the form with it."""
+    rng = np.random.default_rng(14)
+    x = [Rows(logits(rng, 40, v, peaks=p), **settings(rng, 40, v)) for v, p in ((3000, 8), (50001, 0), (50001, 20))]
+    s = Stream()
+    graphs = [Graph(s, r.call) for r in x]
+    plain = []
+    for g in graphs:
+        g.launch()
+    s.sync()
+    plain = [r.got() for r in x]
+    for r, (t, l) in zip(x, plain):
+        t2, l2 = r.run()
+        assert np.array_equal(t, t2) and np.array_equal(l, l2)
+        r.compare((t, l), least=0.7)
+    graphs = [Graph(s, r.call) for r in x]
+    for _ in range(3):
+        for r, g, (t, l) in zip(x, graphs, plain):
+            check(step().ak_memcpy_h2d(r.tok.p, ctypes.c_void_p(np.full(40, 5, dtype=np.int32).ctypes.data), 160))
+            g.launch()
+            s.sync()
+            t2, l2 = r.got()
+            assert np.array_equal(t, t2) and np.array_equal(l, l2)
+            check(r.call())
+    print("captured: the same")
+
+
+def test_captured_without_and_with_scratch():
+    r = subprocess.run([sys.executable, "-c", "import test_gpu_sample as t; t.captured_before_any_call()"], cwd=HERE,
+                       capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr
