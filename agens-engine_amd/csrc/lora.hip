@@ -5,7 +5,7 @@
 //   lora_down_kernel   s = A x of 16 tokens at a time on MFMA (bf16, sums in fp32), one wave a chunk of kChunk inputs;
 //   lora_up_kernel     adds up the chunks' parts, and y = y0 + B (scale s): s enters the MFMA as two bf16 operands, which hold
 //                      16 bits of it (one alone would move y by 2^-9 of what is added).
-// The chunks' parts are added up first by eights, then from left to right, whoever does it: a token's bits do not depend on
+// The chunks' parts are added up first by fours, then from left to right, whoever does it: a token's bits do not depend on
 // the other tokens of the call.
 #include "agens_kernels.h"
 #include "wq_common.h"
@@ -16,7 +16,7 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTile = 64, kChunk = 512, kGroup = 8;
+constexpr int kTile = 64, kChunk = 512, kGroup = 4;
 constexpr int kPlanThreads = 1024;
 
 struct Tile {
@@ -30,7 +30,7 @@ struct PlanView {
   PlanHead* head;
   Tile* tiles;
   int* order;
-  float* parts;  // [chunks][m][ranks]
+  float* parts;  // [groups of chunks][m][ranks]
 };
 __host__ __device__ inline int max_tiles(int m, int adapters) {
   const long t = (long)m / kTile + (m < adapters + 1 ? m : adapters + 1);
@@ -55,16 +55,43 @@ __device__ __forceinline__ int adapter_of(const int* ids, int t, int adapters) {
   return a >= 0 && a < adapters ? a : adapters;  // (the last group: none)
 }
 
-// Counts the adapters' tokens, gives each adapter its places and tiles, then the tokens their places.
+// The next places of the lanes' keys (in: this lane has one).  A wave of one prompt's tokens takes them all at once.
+__device__ __forceinline__ int next_place(int* n, int key, bool in) {
+  const int lane = threadIdx.x & 63, k = __builtin_amdgcn_readfirstlane(key);
+  if (__all(in && key == k)) {
+    int base = 0;
+    if (lane == 0) base = atomicAdd(&n[k], 64);
+    return __builtin_amdgcn_readfirstlane(base) + lane;
+  }
+  return in ? atomicAdd(&n[key], 1) : 0;
+}
+
+// Counts the adapters' tokens, gives each adapter its places and tiles, then the tokens their places.  Up to kPlanEach tokens a
+// thread keep the place among their adapter's that the count gave them.
+constexpr int kPlanEach = 4;  // tokens of a thread at a time
 __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int* ids, int m, int adapters, void* plan) {
   extern __shared__ int n[];  // [adapters + 1] counts, then the next free places
   __shared__ int red[2][kPlanThreads / 64], base[2];
   const PlanView p = view(plan, m, adapters);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int key[kPlanEach], place[kPlanEach];
+  const bool once = m <= kPlanEach * kPlanThreads;
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      const int t = t0 + tid + i * kPlanThreads;
+      key[i] = t < m ? adapter_of(ids, t, adapters) : -1;
+    }
+  };
+  load(0);
   for (int i = tid; i <= adapters; i += kPlanThreads) n[i] = 0;
   if (tid == 0) base[0] = base[1] = 0;
   __syncthreads();
-  for (int t = tid; t < m; t += kPlanThreads) atomicAdd(&n[adapter_of(ids, t, adapters)], 1);
+  for (int t0 = 0; t0 < m; t0 += kPlanEach * kPlanThreads) {
+    if (t0) load(t0);
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) place[i] = next_place(n, key[i], key[i] >= 0);
+  }
   __syncthreads();
   for (int i0 = 0; i0 <= adapters; i0 += kPlanThreads) {
     const int i = i0 + tid, count = i <= adapters ? n[i] : 0, tiles = (count + kTile - 1) / kTile;
@@ -84,7 +111,17 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int* ids,
     if (tid == kPlanThreads - 1) base[0] = at + count, base[1] = tile + tiles;
     __syncthreads();
   }
-  for (int t = tid; t < m; t += kPlanThreads) p.order[atomicAdd(&n[adapter_of(ids, t, adapters)], 1)] = t;
+  for (int t0 = 0; t0 < m; t0 += kPlanEach * kPlanThreads) {
+    if (!once) load(t0);
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      if (!once)
+        place[i] = next_place(n, key[i], key[i] >= 0);
+      else if (key[i] >= 0)
+        place[i] += n[key[i]];
+      if (key[i] >= 0) p.order[place[i]] = t0 + tid + i * kPlanThreads;
+    }
+  }
   if (tid == 0) *p.head = PlanHead{m, adapters, base[1], 0};
 }
 
@@ -97,129 +134,321 @@ struct LoraArgs {
   uint16_t* y[kMaxSegs];
   int n[kMaxSegs], ldy[kMaxSegs], end[kMaxSegs];  // end: of the segments' blocks of output rows
   long ldx;
-  int m, adapters, k, rank, ranks, nseg, each;  // each: chunks of a part
+  int m, adapters, k, rank, ranks, nseg;
+  int parts;           // of the sums A x: one for each kGroup chunks
+  int rows, wide;      // output rows of a workgroup; bit i: segment i's rows of y and y0 are 16-byte aligned
 };
 
+__device__ __forceinline__ uint4 load_if(bool in, const uint16_t* p) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (in) v = *reinterpret_cast<const uint4*>(p);
+  return v;
+}
 __device__ __forceinline__ bf16x8 frag(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// One wave: 16 tokens of a tile (grid x: tile, sixteen), up to 64 ranks (z), the chunks of one part (y).
-__global__ void __launch_bounds__(64) lora_down_kernel(const LoraArgs a) {
-  const PlanView p = view(a.plan, a.m, a.adapters);
-  const int tile = blockIdx.x / (kTile / 16), sub = blockIdx.x % (kTile / 16);
+// A tile of a plan that was made for this call; count 0 past the last.  (Both loads go out at once.)
+__device__ __forceinline__ Tile tile_of(const PlanView& p, const LoraArgs& a, int i) {
   const PlanHead head = *p.head;
-  if (head.m != a.m || head.adapters != a.adapters || tile >= head.tiles) return;
-  const Tile t = p.tiles[tile];
+  Tile t = p.tiles[i];
+  if (head.m != a.m || head.adapters != a.adapters || i >= head.tiles) t.count = 0;
+  return t;
+}
+// The token in place i of a tile, the last one's for places past it.
+__device__ __forceinline__ int token_of(const PlanView& p, const Tile& t, int i) { return p.order[t.start + min(i, t.count - 1)]; }
+
+// Few tokens: a workgroup takes 16 tokens of a tile (grid x), a group of chunks (y) and 16 ranks (z), a wave a chunk, all of whose
+// loads go out before its first product.  (z: the tiles' first sixteens before the second, which most tiles do not have.)
+__global__ void __launch_bounds__(64 * kGroup) lora_down_few_kernel(const LoraArgs a) {
+  constexpr int kSteps = kChunk / 32;
+  __shared__ f32x4 sums[kGroup][64];
+  const PlanView p = view(a.plan, a.m, a.adapters);
+  const Tile t = tile_of(p, a, blockIdx.x);
+  const int blocks = (a.ranks + 15) / 16, sub = blockIdx.z / blocks, r0 = (blockIdx.z - sub * blocks) * 16;
   if (t.adapter < 0 || 16 * sub >= t.count) return;
-  const int lane = threadIdx.x, col = lane & 15, quad = lane >> 4;
-  const int token = p.order[t.start + min(16 * sub + col, t.count - 1)];
-  const int r0 = blockIdx.z * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const int r = r0 + col, k0 = (blockIdx.y * kGroup + wave) * kChunk + 8 * quad;
+  const uint16_t* const w = a.a + ((size_t)t.adapter * a.ranks + min(r, a.ranks - 1)) * a.k;
+  const int token = token_of(p, t, 16 * sub + col);
   const uint16_t* const x = a.x + token * a.ldx;
-  const uint16_t* const w = a.a + (size_t)t.adapter * a.ranks * a.k;
-  f32x4 part[4] = {}, acc[4] = {};
-  const int first = blockIdx.y * a.each, last = min(first + a.each, (a.k + kChunk - 1) / kChunk);
-  for (int c = first; c < last; ++c) {
-    f32x4 now[4] = {};
-    const int end = min((c + 1) * kChunk, a.k);
-    for (int k = c * kChunk + 8 * quad; k - 8 * quad < end; k += 32) {
-      const bool in = k < end;
-      const uint4 xv = in ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
+  uint4 av[kSteps], xv[kSteps];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + 16 * i + col;
-        const uint4 av = in && r < a.ranks ? *reinterpret_cast<const uint4*>(w + (size_t)r * a.k + k) : make_uint4(0, 0, 0, 0);
-        now[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(av), frag(xv), now[i], 0, 0, 0);
-      }
+  for (int i = 0; i < kSteps; ++i) av[i] = load_if(r < a.ranks && k0 + 32 * i < a.k, w + k0 + 32 * i);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) xv[i] = load_if(k0 + 32 * i < a.k, x + k0 + 32 * i);
+  f32x4 acc = {};
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(av[i]), frag(xv[i]), acc, 0, 0, 0);
+  sums[wave][lane] = acc;
+  __syncthreads();
+  const int row = r0 + 4 * quad, here = min((a.k - 1) / kChunk + 1 - (int)blockIdx.y * kGroup, kGroup);
+  if (wave || 16 * sub + col >= t.count || row >= a.ranks) return;
+  f32x4 part = {};
+#pragma unroll
+  for (int j = 0; j < kGroup; ++j)
+    if (j < here) part += sums[j][lane];
+  *reinterpret_cast<f32x4*>(p.parts + ((size_t)blockIdx.y * a.m + token) * a.ranks + row) = part;
+}
+
+// Many tokens: a workgroup takes a tile (grid x), a group of chunks (y) and 16 RT ranks (z), 16 tokens a wave.  The weights go
+// through LDS, kStage inputs at a time, for all four waves; the next stage's loads are in flight during a stage's products.
+constexpr int kStage = 256, kStageSteps = kStage / 32, kRow = kStage * 2 + 16;  // a row's bytes: 16 more, for the banks
+template <int RT>
+__global__ void __launch_bounds__(256, 2) lora_down_many_kernel(const LoraArgs a) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][16 * RT * kRow];
+  const PlanView p = view(a.plan, a.m, a.adapters);
+  const Tile t = tile_of(p, a, blockIdx.x);
+  if (t.adapter < 0 || t.count == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4, sub = tid >> 6;
+  const int r0 = blockIdx.z * 16 * RT;
+  const int token = token_of(p, t, 16 * sub + col);
+  const uint16_t* const x = a.x + token * a.ldx;
+  const bool mine = 16 * sub < t.count;
+  const uint16_t* const w = a.a + (size_t)t.adapter * a.ranks * a.k;
+  const int first = blockIdx.y * kGroup * kChunk, last = min(first + kGroup * kChunk, a.k);
+  uint4 an[2 * RT], xn[kStageSteps], xv[kStageSteps];
+  auto fetch = [&](int k) {
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+      const int r = r0 + (tid >> 5) + 8 * i, kk = k + 8 * (tid & 31);
+      an[i] = load_if(r < a.ranks && kk < last, w + (size_t)r * a.k + kk);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      part[i] += now[i];
-      if (c % kGroup == kGroup - 1 || c == last - 1) acc[i] += part[i], part[i] = f32x4{};
+    for (int i = 0; i < kStageSteps; ++i) {
+      const int kk = k + 32 * i + 8 * quad;
+      xn[i] = load_if(mine && kk < last, x + kk);
+    }
+  };
+  fetch(first);
+  f32x4 now[RT] = {}, sum[RT] = {};
+  int buf = 0;
+  for (int k = first; k < last; k += kStage, buf ^= 1) {
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i)
+      *reinterpret_cast<uint4*>(lds[buf] + ((tid >> 5) + 8 * i) * kRow + 16 * (tid & 31)) = an[i];
+#pragma unroll
+    for (int i = 0; i < kStageSteps; ++i) xv[i] = xn[i];
+    if (k + kStage < last) fetch(k + kStage);
+    __syncthreads();  // (the buffer written next was read before this barrier)
+    if (mine) {
+#pragma unroll
+      for (int i = 0; i < kStageSteps; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+          const uint4 av = *reinterpret_cast<const uint4*>(lds[buf] + (16 * j + col) * kRow + 64 * i + 16 * quad);
+          now[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(av), frag(xv[i]), now[j], 0, 0, 0);
+        }
+      if ((k + kStage) % kChunk == 0 || k + kStage >= last) {
+#pragma unroll
+        for (int j = 0; j < RT; ++j) sum[j] += now[j], now[j] = f32x4{};
+      }
     }
   }
   if (16 * sub + col >= t.count) return;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = r0 + 16 * i + 4 * quad;
-    if (r < a.ranks) *reinterpret_cast<f32x4*>(p.parts + ((size_t)blockIdx.y * a.m + token) * a.ranks + r) = acc[i];
+  for (int j = 0; j < RT; ++j) {
+    const int r = r0 + 16 * j + 4 * quad;
+    if (r < a.ranks) *reinterpret_cast<f32x4*>(p.parts + ((size_t)blockIdx.y * a.m + token) * a.ranks + r) = sum[j];
   }
 }
 
-// A workgroup: a tile's tokens and 256 output rows of a segment, 64 a wave.
-constexpr int kUpRows = 256;
-__global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
-  extern __shared__ uint16_t sv[];  // [hi, lo][kTile][rank + 8]
-  const PlanView p = view(a.plan, a.m, a.adapters);
-  const PlanHead head = *p.head;
-  if (head.m != a.m || head.adapters != a.adapters || (int)blockIdx.y >= head.tiles) return;
-  const Tile t = p.tiles[blockIdx.y];
-  int seg = 0;
-  while (seg < a.nseg - 1 && (int)blockIdx.x >= a.end[seg]) ++seg;
-  const int n0 = ((int)blockIdx.x - (seg ? a.end[seg - 1] : 0)) * kUpRows, n = a.n[seg];
-  const long ldy = a.ldy[seg];
-  const uint16_t* const y0 = a.y0[seg];
-  uint16_t* const y = a.y[seg];
-  if (t.adapter < 0) {
-    if (y0 == y) return;
-    for (int e = threadIdx.x; e < t.count * kUpRows; e += 256) {
-      const size_t row = (size_t)p.order[t.start + e / kUpRows] * ldy;
-      const int c = n0 + e % kUpRows;
-      if (c < n) y[row + c] = y0[row + c];
-    }
-    return;
+// Four sums: their parts from left to right, kBatch loads at a time.
+constexpr int kBatch = 8;
+__device__ __forceinline__ f32x4 add_parts(const float* at, int parts, size_t step) {
+  f32x4 s = {};
+  for (int c = 0; c < parts; c += kBatch) {
+    f32x4 x[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) x[j] = *reinterpret_cast<const f32x4*>(at + min(c + j, parts - 1) * step);
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (c + j < parts) s += x[j];
   }
-  const int stride = a.rank + 8, parts = (a.k + kChunk * a.each - 1) / (kChunk * a.each);
-  const float scale = a.scale ? a.scale[t.adapter] : 1.0f;
-  for (int e = threadIdx.x; e < kTile * a.rank; e += 256) {
-    const int i = e / a.rank, r = e - i * a.rank;
-    float s = 0.0f;
-    if (i < t.count) {
-      const float* const at = p.parts + (size_t)p.order[t.start + i] * a.ranks + seg * a.rank + r;
-      float part = 0.0f;
-      for (int c = 0; c < parts; ++c) {
-        part += at[(size_t)c * a.m * a.ranks];
-        if (a.each > 1 || c % kGroup == kGroup - 1 || c == parts - 1) s += part, part = 0.0f;
+  return s;
+}
+
+// 16 outputs of a token, 8 from c on and 8 from c + 32 on: y = y0 + acc.  (A wave's 16-byte pieces of a token are neighbours:
+// with 16 outputs side by side in a lane no faster than 16 side by side, but fewer partial lines.)  WIDE: both 16-byte aligned and all within the row.
+template <bool WIDE>
+__device__ __forceinline__ void load_out(const uint16_t* y0, int c, int n, uint32_t (&v)[8]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h, c += 32) {
+    if constexpr (WIDE) {
+      const uint4 p = *reinterpret_cast<const uint4*>(y0 + c);
+      v[4 * h] = p.x, v[4 * h + 1] = p.y, v[4 * h + 2] = p.z, v[4 * h + 3] = p.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t x = c + i < n ? y0[c + i] : 0;
+        v[4 * h + i / 2] = i & 1 ? v[4 * h + i / 2] | x << 16 : x;
       }
     }
-    s *= scale;
-    const uint32_t hi = f2bf(s);
-    const float rest = s - bf2f(hi);
-    sv[i * stride + r] = (uint16_t)hi;
-    sv[(kTile + i) * stride + r] = fabsf(s) < INFINITY && fabsf(bf2f(hi)) < INFINITY ? f2bf(rest) : 0;
   }
-  __syncthreads();
-  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, wn = n0 + 64 * ((int)threadIdx.x >> 6);
-  if (wn >= n) return;
-  const uint16_t* const w = a.b[seg] + (size_t)t.adapter * n * a.rank;
-  // row of the tile's i-th product that lane col reads: four of them leave a lane 16 neighbouring outputs
-  for (int sub = 0; 16 * sub < t.count; ++sub) {
+}
+template <bool WIDE>
+__device__ __forceinline__ void store_out(uint16_t* y, int c, int n, const uint32_t (&v)[8], const f32x4 (&acc)[4]) {
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    o[i] = (uint32_t)f2bf(bf2f(v[i] & 0xFFFFu) + acc[i / 2][2 * (i & 1)]) |
+           (uint32_t)f2bf(bf2f(v[i] >> 16) + acc[i / 2][2 * (i & 1) + 1]) << 16;
+#pragma unroll
+  for (int h = 0; h < 2; ++h, c += 32) {
+    if constexpr (WIDE) {
+      *reinterpret_cast<uint4*>(y + c) = make_uint4(o[4 * h], o[4 * h + 1], o[4 * h + 2], o[4 * h + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c + i < n) y[c + i] = (uint16_t)(o[4 * h + i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// 64 output rows of a segment by one wave, for all tokens of a tile: KS steps of 32 ranks.  v: the outputs before.
+template <int KS, bool WIDE>
+__device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int seg, int wn, const uint16_t* sv, int stride,
+                                        const uint4 (&bv)[KS][4], const int (&tok)[kTile / 16], uint32_t (&v)[kTile / 16][8]) {
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, n = a.n[seg], c = wn + 8 * quad;
+  uint16_t* const y = a.y[seg];
+  const long ldy = a.ldy[seg];
+#pragma unroll
+  for (int sub = 0; sub < kTile / 16; ++sub) {
+    if (16 * sub >= t.count) break;
     f32x4 acc[4] = {};
-    for (int k = 0; k < a.rank; k += 32) {
-      const int kk = k + 8 * quad;
-      const bool in = kk < a.rank;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const int kk = 32 * s + 8 * quad;
       uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-      if (in) {
+      if (kk < a.rank) {
         hi = *reinterpret_cast<const uint4*>(sv + (16 * sub + col) * stride + kk);
         lo = *reinterpret_cast<const uint4*>(sv + (kTile + 16 * sub + col) * stride + kk);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = wn + 16 * (col >> 2) + 4 * i + (col & 3);
-        const uint4 b = in && row < n ? *reinterpret_cast<const uint4*>(w + (size_t)row * a.rank + kk) : make_uint4(0, 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(b), frag(lo), acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(b), frag(hi), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[s][i]), frag(lo), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[s][i]), frag(hi), acc[i], 0, 0, 0);
       }
     }
-    if (16 * sub + col < t.count) {
-      const size_t at = (size_t)p.order[t.start + 16 * sub + col] * ldy;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int c = wn + 16 * quad + 4 * i + j;
-          if (c < n) y[at + c] = f2bf(bf2f(y0[at + c]) + acc[i][j]);
-        }
-    }
+    if (16 * sub + col < t.count) store_out<WIDE>(y + tok[sub] * ldy, c, n, v[sub], acc);
   }
+}
+
+// Pieces [c0, c0 + width) of a tile's rows, eight in flight a thread.
+template <class T>
+__device__ __forceinline__ void copy_rows(const PlanView& p, const Tile& t, const void* from, void* to, int c0, int width, long ld) {
+  const T* const src = static_cast<const T*>(from) + c0;
+  T* const dst = static_cast<T*>(to) + c0;
+  const int all = t.count * width;
+  for (int e0 = threadIdx.x; e0 < all; e0 += 8 * 256) {
+    T v[8];
+    long at[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = min(e0 + 256 * i, all - 1), row = e / width;
+      at[i] = token_of(p, t, row) * ld + (e - row * width);
+      v[i] = src[at[i]];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (e0 + 256 * i < all) dst[at[i]] = v[i];
+  }
+}
+
+// A workgroup: a tile's tokens (grid y) and a.rows output rows of a segment (x), 64 at a time a wave.
+constexpr int kUpRows = 256;
+template <int KS>
+__global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [hi, lo][kTile][rank + 8]
+  const PlanView p = view(a.plan, a.m, a.adapters);
+  const Tile t = tile_of(p, a, blockIdx.y);
+  if (t.count == 0) return;
+  int seg = 0;
+  while (seg < a.nseg - 1 && (int)blockIdx.x >= a.end[seg]) ++seg;
+  const int n = a.n[seg], n0 = ((int)blockIdx.x - (seg ? a.end[seg - 1] : 0)) * a.rows, n1 = min(n0 + a.rows, n);
+  const long ldy = a.ldy[seg];
+  const uint16_t* const y0 = a.y0[seg];
+  uint16_t* const y = a.y[seg];
+  if (t.adapter < 0) {  // no products
+    if (y0 != y) {
+      if ((a.wide >> seg & 1) && (n1 - n0) % 8 == 0)
+        copy_rows<u32x4>(p, t, y0, y, n0 / 8, (n1 - n0) / 8, ldy / 8);
+      else
+        copy_rows<uint16_t>(p, t, y0, y, n0, n1 - n0, ldy);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, stride = a.rank + 8, subs = (t.count + 15) / 16;
+  const uint16_t* const w = a.b[seg] + (size_t)t.adapter * n * a.rank;
+  // row of B for lane col of product i: the four products leave a lane 16 neighbouring outputs of a token
+  auto load_b = [&](int wn, uint4(&bv)[KS][4]) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = wn + 32 * (i >> 1) + 8 * (col >> 2) + 4 * (i & 1) + (col & 3), kk = 32 * s + 8 * quad;
+        bv[s][i] = load_if(kk < a.rank && row < n, w + (size_t)row * a.rank + kk);
+      }
+  };
+  // the first rows' weights and outputs are on their way while the parts are added up
+  uint4 bv[KS][4];
+  uint32_t v[kTile / 16][8];
+  int wn = n0 + 64 * ((int)threadIdx.x >> 6);
+  int tok[kTile / 16];
+#pragma unroll
+  for (int i = 0; i < kTile / 16; ++i) tok[i] = token_of(p, t, 16 * i + col);
+  const bool wide = a.wide >> seg & 1;
+  auto load_y = [&](int wn) {
+    const bool full = wide && wn + 64 <= n;
+#pragma unroll
+    for (int i = 0; i < kTile / 16; ++i) {
+      if (16 * i >= t.count) break;
+      if (full)
+        load_out<true>(y0 + tok[i] * ldy, wn + 8 * quad, n, v[i]);
+      else
+        load_out<false>(y0 + tok[i] * ldy, wn + 8 * quad, n, v[i]);
+    }
+  };
+  load_b(wn, bv);
+  load_y(wn);
+  const float scale = a.scale ? a.scale[t.adapter] : 1.0f;
+  const size_t step = (size_t)a.m * a.ranks;
+  const int fours = a.rank / 4;
+  for (int e = threadIdx.x; e < 16 * subs * fours; e += 256) {  // 4 ranks of a token; kBatch of their parts at a time
+    const int i = e / fours, r = 4 * (e - i * fours);
+    const float* const at = p.parts + (size_t)token_of(p, t, i) * a.ranks + seg * a.rank + r;
+    const f32x4 s = add_parts(at, a.parts, step);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float f = i < t.count ? s[j] * scale : 0.0f;
+      hi[j] = f2bf(f);
+      lo[j] = (hi[j] & 0x7FFFu) < 0x7F80u ? f2bf(f - bf2f(hi[j])) : 0;  // (nothing beside infinities and NaN)
+    }
+    *reinterpret_cast<uint2*>(sv + i * stride + r) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
+    *reinterpret_cast<uint2*>(sv + (kTile + i) * stride + r) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+  }
+  __syncthreads();
+  for (; wn < n1; wn += kUpRows) {
+    const bool full = wide && wn + 64 <= n;
+    if (wn >= n0 + kUpRows) {
+      load_b(wn, bv);
+      load_y(wn);
+    }
+    if (full)
+      up_rows<KS, true>(a, t, seg, wn, sv, stride, bv, tok, v);
+    else
+      up_rows<KS, false>(a, t, seg, wn, sv, stride, bv, tok, v);
+  }
+}
+
+template <int RT>
+void down_many(const LoraArgs& l, unsigned tiles, hipStream_t s) {
+  hipLaunchKernelGGL(lora_down_many_kernel<RT>,
+                     dim3(tiles, (unsigned)l.parts, (unsigned)((l.ranks - 1) / (16 * RT) + 1)), dim3(256),
+                     0, s, l);
+}
+template <int KS>
+void up(const LoraArgs& l, unsigned blocks, unsigned tiles, hipStream_t s) {
+  hipLaunchKernelGGL(lora_up_kernel<KS>, dim3(blocks, tiles), dim3(256), (size_t)2 * kTile * (l.rank + 8) * 2, s, l);
 }
 
 bool sizes_ok(int m, int adapters) {
@@ -233,7 +462,7 @@ extern "C" size_t ak_lora_plan_bytes(int m, int adapters, int ranks, int k) {
   if (!agq::sizes_ok(m, adapters) || ranks < 8 || ranks % 8 || ranks > AK_LORA_MAX_RANK * agq::kMaxSegs || k < 8 || k % 8 ||
       k > AK_LORA_MAX_INPUTS)
     return 0;
-  return agq::parts_at(m, adapters) + (size_t)agq::chunks_of(k) * m * ranks * sizeof(float);
+  return agq::parts_at(m, adapters) + (size_t)((agq::chunks_of(k) - 1) / agq::kGroup + 1) * m * ranks * sizeof(float);
 }
 
 extern "C" int ak_lora_plan(const int* ids, int m, int adapters, void* plan, void* stream) {
@@ -253,7 +482,6 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
   if (!m) return 0;
   if (odd(plan) || odd(x) || odd(a) || ldx < 0 || ldx % 8) return AK_INVALID;
   agq::LoraArgs l{};
-  int blocks = 0;
   for (int i = 0; i < nseg; ++i) {
     const int ld = ldy && ldy[i] ? ldy[i] : n[i];
     if (n[i] < 1 || n[i] > AK_LORA_MAX_INPUTS || odd(b[i]) || !y[i] || (base && !base[i]) || (m > 1 && ld < n[i])) return AK_INVALID;
@@ -261,18 +489,39 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
     l.y[i] = static_cast<uint16_t*>(y[i]);
     l.y0[i] = base ? static_cast<const uint16_t*>(base[i]) : l.y[i];
     l.n[i] = n[i], l.ldy[i] = ld;
-    l.end[i] = blocks += (n[i] - 1) / agq::kUpRows + 1;
+    if (ld % 8 == 0 && !odd(l.y[i]) && !odd(l.y0[i])) l.wide |= 1 << i;
   }
   l.plan = plan, l.x = static_cast<const uint16_t*>(x), l.a = static_cast<const uint16_t*>(a), l.scale = scale;
   l.ldx = ldx, l.m = m, l.adapters = adapters, l.k = k, l.rank = rank, l.ranks = rank * nseg, l.nseg = nseg;
-  const int tiles = agq::max_tiles(m, adapters), chunks = agq::chunks_of(k);
-  l.each = 1;
+  const unsigned tiles = (unsigned)agq::max_tiles(m, adapters);
+  const int chunks = agq::chunks_of(k);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(agq::lora_down_kernel, dim3((unsigned)tiles * (agq::kTile / 16), (unsigned)((chunks - 1) / l.each + 1),
-                                                 (unsigned)((l.ranks - 1) / 64 + 1)),
-                     dim3(64), 0, s, l);
+  // Tiles of 64 tokens and ranks read less, sixteens keep more of the GPU at work: 256 tokens of 27648 inputs and 64 ranks 36 us by
+  // tiles and 42 by sixteens, 1024 of 5120 and 16 ranks 27 and 21, 2048 of 5120 and 48 ranks 44 and 45.
+  l.parts = (chunks - 1) / agq::kGroup + 1;
+  const bool many = (long)((m - 1) / agq::kTile + 1) * l.parts >= 52;
+  if (!many)
+    hipLaunchKernelGGL(agq::lora_down_few_kernel, dim3(tiles, (unsigned)l.parts, ((unsigned)(l.ranks - 1) / 16 + 1) * (agq::kTile / 16)),
+                       dim3(64 * agq::kGroup), 0, s, l);
+  else if (l.ranks <= 16)
+    agq::down_many<1>(l, tiles, s);
+  else if (l.ranks <= 32)
+    agq::down_many<2>(l, tiles, s);
+  else
+    agq::down_many<4>(l, tiles, s);
   if (const int e = (int)hipGetLastError()) return e;
-  hipLaunchKernelGGL(agq::lora_up_kernel, dim3((unsigned)blocks, (unsigned)tiles), dim3(256),
-                     (size_t)2 * agq::kTile * (rank + 8) * 2, s, l);
+  // a workgroup adds up its tile's parts anew: more rows each where there are workgroups enough
+  l.rows = agq::kUpRows;
+  long rows = 0;
+  for (int i = 0; i < nseg; ++i) rows += n[i];
+  while (l.rows < 4 * agq::kUpRows && (long)tiles * rows / (2 * l.rows) >= 1024) l.rows *= 2;
+  int blocks = 0;
+  for (int i = 0; i < nseg; ++i) l.end[i] = blocks += (n[i] - 1) / l.rows + 1;
+  if (rank <= 32)
+    agq::up<1>(l, (unsigned)blocks, tiles, s);
+  else if (rank <= 64)
+    agq::up<2>(l, (unsigned)blocks, tiles, s);
+  else
+    agq::up<4>(l, (unsigned)blocks, tiles, s);
   return (int)hipGetLastError();
 }
