@@ -7,29 +7,54 @@
 //
 // A logit has 16 bits, so equal ones are many and its bits, made to ascend with the value (`key`), index everything: a
 // histogram of a row's keys holds all counts, and all weights as counts times the weight of a key.  The weights enter sums as
-// whole numbers of 2^-42 of the largest, 2^20 of which fit 64 bits: sums are exact, in any order, so which way they were
+// whole numbers of 2^-40 of the largest (2^20 of them fit 64 bits, 2^12 a double's 53): sums are exact, in any order, so which way they were
 // reached does not show in the tokens.
 //
-//   sample_keys_kernel   a chunk of 16384 logits a workgroup: its largest, its lowest token with that, the sum of its weights
-//                        (16 in 32 bits, then 64), and how often each of the kWindow keys up to its largest occurs;
-//   sample_draw_kernel   a row a workgroup: the chunks' windows, shifted to the row's largest key, give the border of what is
-//                        kept, and what each chunk has of it; then the chunk that the draw falls into is read again.  Where
-//                        the border is below the window, it goes over the row itself, kWide keys at a time.
-// Without scratch sample_draw_kernel takes the chunks' statistics itself and does without their windows: the same tokens.
+//   sample_keys_kernel   a chunk of 4096 logits a workgroup, held in registers: its largest, its lowest token with that, the
+//                        sum of its weights (16 in 32 bits, then 64), and how often each of the kWindow keys up to its
+//                        largest occurs;
+//   sample_draw_kernel   a row a workgroup: the chunks' windows, shifted to the row's largest key and summed, give the border of
+//                        what is kept (one scan of counts and weights serves top-k and top-p, since top-p's border is not
+//                        behind top-k's), and what each chunk has of it; then the chunk that the draw falls into is read again.
+//                        A window goes down to 2^-8 of a positive largest logit; where the border is below it, the row's
+//                        keys are counted anew, all at once, and the chunks' shares summed up in another pass.
+// Both wait: for loads, and for each other's barriers.  Without scratch sample_draw_kernel takes the chunks' statistics itself
+// and does without their windows: the same tokens.
 #include "agens_kernels.h"
 #include "logits.h"
 
 namespace agq {
 namespace {
 
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kEach = 16, kChunk = kThreads * kEach;
-constexpr int kMaxChunks = 64;  // of a row: a lane of a wave each
+constexpr int kEach = 16, kGroupThreads = 256, kChunk = kGroupThreads * kEach;
+constexpr int kDraw = 512, kWaves = kDraw / 64, kGroups = kDraw / kGroupThreads;
+constexpr int kMaxChunks = 256, kLaneChunks = kMaxChunks / 64;  // of a row
 static_assert(kMaxChunks * kChunk == AK_SAMPLE_MAX_VOCAB, "the header's limit");
-constexpr int kWindow = 1024, kWide = 8 * kThreads;
+constexpr int kWindow = 1024;
+static_assert(kWindow == 2 * kDraw && kChunk == 8 * kDraw, "two bins of the window and eight logits of a chunk a thread");
+// Bins of all keys that matter: kSpan from the largest down, zero's, and the rest up from the least with any weight.
+constexpr int kSpan = 8192, kBins = 2 * kSpan, kBinsEach = kBins / kDraw;
 constexpr float kMaxHeat = 1.44e30f;  // (see heat_of)
-constexpr float kUnit = 0x1p42f;
+constexpr float kUnit = 0x1p40f;
 constexpr size_t kMaxScratch = (size_t)64 << 20;
-constexpr uint32_t kLowest = 0x007F;  // key of -inf, and of NaN
+constexpr uint32_t kLowest = 0x007F, kHighest = 0xFF80;  // keys of -inf and inf
+constexpr uint32_t kZero = 0x8000, kMinusZero = 0x7FFF;
+
+// 8 logits from token k on as pairs of bits, -inf past the end.
+__device__ __forceinline__ u32x4 load_bits(const uint16_t* row, int k, int vocab) {
+  u32x4 v;
+  if (k + 8 <= vocab) {
+    v = *reinterpret_cast<const u32x4_any*>(row + k);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = (k + 2 * i < vocab ? row[k + 2 * i] : 0xFF80u) | (k + 2 * i + 1 < vocab ? row[k + 2 * i + 1] : 0xFF80u) << 16;
+  }
+  return v;
+}
+__device__ __forceinline__ float value(const u32x4& v, int i) {
+  return __uint_as_float(i & 1 ? v[i >> 1] & 0xFFFF0000u : v[i >> 1] << 16);
+}
 
 struct ChunkStat {
   float top;
@@ -46,79 +71,77 @@ struct SampleArgs {
   float* logp;
   int b, vocab, chunks;
   ChunkStat* stats;  // [b][chunks]
-  uint16_t* counts;  // [b][chunks][kWindow]: key of the chunk's largest - i
+  uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys first_key - i
 };
 
+// Keys of two logits: their bits, all inverted where the sign is set, else the sign alone.  -0 has a key of its own, kMinusZero,
+// which counts as kZero; NaN are above +inf's key or below -inf's, and never counted.
+__device__ __forceinline__ uint32_t two_keys(uint32_t bits) {
+  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+  const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, bits) >> 15);
+  return bits ^ (sign | 0x80008000u);
+}
 __device__ __forceinline__ uint32_t key_of(uint32_t bits) {
-  if ((bits & 0x7FFFu) > 0x7F80u) return kLowest;  // NaN
-  if (bits == 0x8000u) bits = 0;                   // -0 equals 0
-  return bits & 0x8000u ? 0xFFFFu - bits : bits + 0x8000u;
+  const uint32_t key = two_keys(bits & 0xFFFFu) & 0xFFFFu;
+  return key > kHighest ? kLowest : max(key == kMinusZero ? kZero : key, kLowest);
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
   return bf2f(key & 0x8000u ? key - 0x8000u : 0xFFFFu - key);
 }
 __device__ __forceinline__ uint32_t key_of_value(float l) { return key_of(__float_as_uint(l) >> 16); }
+// A window's first key: the largest, or the one above it, so that windows are shifted by whole pairs.
+__device__ __forceinline__ uint32_t first_key(float top) { return key_of_value(top) | 1u; }
 
-// in whole numbers of 2^-42
-__device__ __forceinline__ uint64_t units(float w) { return (uint64_t)(w * kUnit); }
+// in whole numbers of 2^-40
+__device__ __forceinline__ uint64_t units(float w) {
+  const float x = w * kUnit, hi = __builtin_truncf(x * 0x1p-32f);
+  return (uint64_t)(uint32_t)hi << 32 | (uint32_t)__builtin_fmaf(hi, -0x1p32f, x);
+}
 __device__ __forceinline__ float key_weight(const Heat& s, uint32_t key, float top) {
   return any_weight(s, logit_of(key), top);
 }
 
-struct Shared {
-  double red[kWaves], before[kWaves];
-  uint64_t sum[kWaves];
-  int ired[kWaves], ok[kWaves];
-  uint64_t mass[kMaxChunks];  // of the chunks: what is kept
-  uint32_t at_border[kMaxChunks];
-  uint32_t bins[kWide];
-  uint32_t next;  // the largest key below the window
-  uint64_t border;
-  int chunk;
-  double at;
+struct AddUnits {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ uint64_t step(uint64_t x) const {
+    return x + ((uint64_t)dpp<CTRL, ROWS>((uint32_t)(x >> 32), 0) << 32 | dpp<CTRL, ROWS>((uint32_t)x, 0));
+  }
+};
+struct AddCounts {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ uint32_t step(uint32_t x) const {
+    return x + dpp<CTRL, ROWS>(x, 0);
+  }
+};
+__device__ __forceinline__ uint64_t last_lane64(uint64_t x) {
+  return (uint64_t)last_lane((uint32_t)(x >> 32)) << 32 | last_lane((uint32_t)x);
+}
+__device__ __forceinline__ uint64_t units_sum(uint64_t x) { return last_lane64(wave_scan(x, AddUnits())); }
+__device__ __forceinline__ uint32_t counts_sum(uint32_t x) { return last_lane(wave_scan(x, AddCounts())); }
+
+// What kGroupThreads threads share over a chunk
+struct Group {
+  double red[kGroupThreads / 64];
+  int best[kGroupThreads / 64];
 };
 
-template <class T>
-__device__ __forceinline__ T shfl_up64(T x, int d) {
-  return (T)__shfl_up((unsigned long long)x, d);
-}
-// The sum over the threads up to this one; *total over all.
-__device__ __forceinline__ uint64_t scan(uint64_t x, Shared& sh, uint64_t* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int d = 1; d < 64; d *= 2) {
-    const uint64_t y = shfl_up64(x, d);
-    if (lane >= d) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) sh.sum[w] = x;
-  __syncthreads();
-  uint64_t all = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) {
-    if (i < w) x += sh.sum[i];
-    all += sh.sum[i];
-  }
-  *total = all;
-  return x;
-}
-
-// A chunk: see ChunkStat.  bins: where to count its keys (kWindow, zeros), or null.
-__device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* row, int chunk, int vocab, uint32_t* bins,
-                                                Shared& sh) {
-  const int t = threadIdx.x, at0 = chunk * kChunk + 8 * t, at1 = at0 + kChunk / 2;
+// A chunk, by a group of kGroupThreads threads: see ChunkStat.  bins: where to count its keys (kWindow + 1 zeros), or null.  All
+// threads of the workgroup come here together; a chunk past the last is empty.
+__device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* row, int chunk, int vocab, uint32_t* bins, Group& g) {
+  const int t = threadIdx.x % kGroupThreads, w = t >> 6, at0 = chunk * kChunk + 8 * t, at1 = at0 + kChunk / 2;
+  const u32x4 v[2] = {load_bits(row, at0, vocab), load_bits(row, at1, vocab)};
   float l[kEach];
-  load8(row, at0, vocab, l);
-  load8(row, at1, vocab, l + 8);
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) l[i] = value(v[i >> 3], i & 7);
   float mine = l[0];
 #pragma unroll
   for (int i = 1; i < kEach; ++i) mine = fmaxf(mine, l[i]);
-  const float wtop = wave_max(mine);
+  float top = wave_max(mine);
   __syncthreads();
-  if ((t & 63) == 0) sh.red[t >> 6] = wtop;
+  if ((t & 63) == 0) g.red[w] = top;
   __syncthreads();
-  float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) top = fmaxf(top, (float)sh.red[i]);
+  for (int i = 0; i < kGroupThreads / 64; ++i) top = fmaxf(top, (float)g.red[i]);
   int best = 0x7FFFFFFF;
   if (mine == top && top > -INFINITY) {
 #pragma unroll
@@ -127,36 +150,50 @@ __device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* r
   }
   best = wave_min(best);
   if (bins && top > -INFINITY) {
-    const uint32_t high = key_of_value(top);
+    const uint32_t first = first_key(top), span = min((uint32_t)kWindow + 1, first - kLowest);  // (-inf weighs nothing)
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const uint32_t key = key_of_value(l[i]), d = high - key;
-      if (d < kWindow && key != kLowest) atomicAdd(&bins[d], 1u);  // (-inf weighs nothing)
+    for (int i = 0; i < kEach / 2; ++i) {
+      const uint32_t keys = two_keys(v[i >> 2][i & 3]), d0 = first - (keys & 0xFFFFu), d1 = first - (keys >> 16);
+      if (d0 < span) atomicAdd(&bins[d0], 1u);
+      if (d1 < span) atomicAdd(&bins[d1], 1u);
     }
   }
   float sum = 0.0f;
+  if (top == INFINITY) {
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) sum += any_weight(s, l[i], top);
+    for (int i = 0; i < kEach; ++i) sum += l[i] == top ? 1.0f : 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += weight(s, l[i], top);
+  }
   const double wsum = wave_sum((double)sum);
   __syncthreads();
-  if ((t & 63) == 0) sh.red[t >> 6] = wsum, sh.ired[t >> 6] = best;
+  if ((t & 63) == 0) g.red[w] = wsum, g.best[w] = best;
   __syncthreads();
   ChunkStat r{top, 0x7FFFFFFF, 0.0};
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) r.total += sh.red[i], r.best = min(r.best, sh.ired[i]);
+  for (int i = 0; i < kGroupThreads / 64; ++i) r.total += g.red[i], r.best = min(r.best, g.best[i]);
   if (r.best == 0x7FFFFFFF) r.best = -1;
   return r;
 }
 
-__global__ void __launch_bounds__(kThreads) sample_keys_kernel(const SampleArgs a) {
-  __shared__ Shared sh;
-  const int chunk = blockIdx.x, id = blockIdx.y;
+__global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const SampleArgs a) {
+  __shared__ Group g;
+  __shared__ __attribute__((aligned(16))) uint32_t bins[kWindow + 1];  // (one more: -0 behind 0)
+  const int chunk = blockIdx.x, id = blockIdx.y, t = threadIdx.x;
   const Heat s = heat_of(a.temp ? a.temp[id] : 1.0f);
-  sh.bins[threadIdx.x] = 0;  // (a barrier follows before the first count)
-  const ChunkStat r = chunk_stat(s, a.logits + (size_t)id * a.ld, chunk, a.vocab, sh.bins, sh);
+  *reinterpret_cast<uint4*>(bins + 4 * t) = make_uint4(0, 0, 0, 0);  // (a barrier follows before the first count)
+  if (t == 0) bins[kWindow] = 0;
+  const ChunkStat r = chunk_stat(s, a.logits + (size_t)id * a.ld, chunk, a.vocab, bins, g);
   const size_t at = (size_t)id * a.chunks + chunk;
-  if (threadIdx.x == 0) a.stats[at] = r;
-  a.counts[at * kWindow + threadIdx.x] = (uint16_t)sh.bins[threadIdx.x];
+  if (t == 0) {
+    a.stats[at] = r;
+    const uint32_t d = first_key(r.top) - kZero;  // the counts of -0
+    if (r.top >= 0.0f && d < kWindow) bins[d] += bins[d + 1], bins[d + 1] = 0;
+  }
+  __syncthreads();
+  const uint4 n = *reinterpret_cast<const uint4*>(bins + 4 * t);
+  *reinterpret_cast<uint2*>(a.counts + at * (kWindow / 2) + 2 * t) = make_uint2(n.x | n.y << 16, n.z | n.w << 16);
 }
 
 // What is kept: keys above `key` and the first `n` tokens with it, of weights from `least` on.
@@ -164,335 +201,578 @@ struct Border {
   uint32_t key, n;
   float least;
 };
+struct Shared {
+  Group g[kGroups];
+  ChunkStat stats[kMaxChunks];  // without scratch
+  uint32_t count[kWaves];
+  uint64_t mass[kWaves];
+  double sum[kWaves];
+  uint32_t same[kWaves];
+  Border border;
+  uint64_t border_mass;  // in front of it, its own tokens included
+  uint32_t between;
+  uint64_t kept[kMaxChunks];  // the chunks' weights above the border's key
+  uint32_t equal[kMaxChunks]; // and their tokens with it
+  uint64_t weight[kWindow + 2];  // of the window's keys; the last two are 0
+  uint32_t bins[kBins];
+};
 
 struct Row {
   Heat s;
   const uint16_t* logits;
-  const ChunkStat* stats;   // (in LDS)
-  const uint16_t* counts;   // null: none
+  const uint32_t* counts;  // null: none
   float top;
   int best, vocab, chunks;
   double total;
-  uint32_t high;            // key of top
+  uint32_t first;  // first_key(top)
+  uint32_t least;  // the lowest key that weighs anything
+  uint32_t low;    // the first key of the bins past zero's
+  bool straight;   // or the bins go on below kSpan without a gap, and without a bin for zero alone
 };
 
-// Keys high - first, high - first - 1, ...: how often they occur.  `each` of them a thread, in its place of n.
-// The chunks' windows:
-__device__ __forceinline__ uint32_t count_window(const Row& r) {
-  uint32_t n = 0;
-  for (int c = 0; c < r.chunks; ++c) {
-    const float top = r.stats[c].top;
-    if (top == -INFINITY) continue;
-    const int i = (int)threadIdx.x - (int)(r.high - key_of_value(top));
-    if (i >= 0) n += r.counts[(size_t)c * kWindow + i];
+// Bins in order: two of the window a thread, or kBinsEach of all keys'.
+template <bool WIDE>
+struct Bins {
+  static constexpr int kCount = WIDE ? kBinsEach : 2;
+  uint32_t n[WIDE ? 1 : 2];
+  __device__ __forceinline__ uint32_t count(const Shared& sh, int i) const {
+    if constexpr (WIDE)
+      return sh.bins[threadIdx.x * kBinsEach + i];
+    else
+      return n[i];
   }
-  return n;
-}
-// the row itself, into sh.bins; sh.next: the largest key below
-__device__ __forceinline__ void count_wide(const Row& r, uint32_t high, Shared& sh) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < kWide; i += kThreads) sh.bins[i] = 0;
-  if (threadIdx.x == 0) sh.next = 0;
-  __syncthreads();
-  uint32_t next = 0;
-  for (int k = 8 * threadIdx.x; k < r.vocab; k += 8 * kThreads) {
-    float l[8];
-    load8(r.logits, k, r.vocab, l);
+  __device__ __forceinline__ uint32_t key(const Row& r, int i) const {
+    const int at = (int)threadIdx.x * kCount + i;
+    if (!WIDE || at < kSpan || r.straight) return r.first - at;
+    return at == kSpan ? kZero : r.low - (at - kSpan - 1);
+  }
+  __device__ __forceinline__ uint64_t mass(const Row& r, const Shared& sh, int i) const {
+    const uint32_t m = count(sh, i);
+    return m ? m * units(key_weight(r.s, key(r, i), r.top)) : 0;
+  }
+};
+
+// The two bins of the chunks' windows.
+__device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&first)[kLaneChunks]) {
+  Bins<false> b{{0, 0}};
+  for (int c0 = 0; c0 < r.chunks; c0 += 40) {
+    uint32_t v[40];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t key = key_of_value(l[i]);
-      const int d = (int)high - (int)key;
-      if (d < 0 || key == kLowest) continue;
-      if (d < kWide)
-        atomicAdd(&sh.bins[d], 1u);
-      else
-        next = max(next, key);
+    for (int j = 0; j < 40; ++j) {
+      const int c = min(c0 + j, r.chunks - 1);
+      uint32_t f = first[0];
+#pragma unroll
+      for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
+      const int at = (int)threadIdx.x - (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63)) / 2;
+      v[j] = 0;
+      if (at >= 0 && c0 + j < r.chunks) v[j] = r.counts[(size_t)c * (kWindow / 2) + at];
     }
+#pragma unroll
+    for (int j = 0; j < 40; ++j) b.n[0] += v[j] & 0xFFFFu, b.n[1] += v[j] >> 16;
   }
-  if (next) atomicMax(&sh.next, next);
-  __syncthreads();
+  return b;
 }
 
-// The place in the order where a sum reaches `goal` (> 0): over counts (by_weight false) or weights; tokens past `limit` (a
-// border) count as not there.  key 0: nowhere.  Whole workgroup; the same in every thread.
-__device__ Border find(const Row& r, bool by_weight, uint64_t goal, const Border& limit, Shared& sh) {
-  uint64_t done = 0;
-  const bool quick = r.counts != nullptr;
-  uint32_t high = r.high;
-  for (bool first = quick;; first = false) {
-    const int each = first ? 1 : kWide / kThreads;
-    uint32_t n[kWide / kThreads];
-    if (first) {
-      n[0] = count_window(r);
+// All keys of the row that weigh anything, into sh.bins; `window`: what is known already, or null.  False: some are between the
+// bins.
+template <bool STRAIGHT>
+__device__ __forceinline__ bool count_keys(const Row& r, uint32_t from, Shared& sh) {
+  const uint32_t top = r.first - from, span = (STRAIGHT ? r.first - r.least + 1 : kSpan) - from, all = r.first - r.least + 1 - from;
+  bool between = false;
+  auto add = [&](uint32_t key) {
+    const uint32_t d = top - key;
+    if constexpr (STRAIGHT) {
+      if (d < span) atomicAdd(&sh.bins[from + d], 1u);
     } else {
-      count_wide(r, high, sh);
-      for (int i = 0; i < each; ++i) n[i] = sh.bins[threadIdx.x * each + i];
-    }
-    uint64_t mine = 0;
-    const uint32_t k0 = high - threadIdx.x * each;
-    auto amount = [&](int i) {  // of key k0 - i
-      const uint32_t key = k0 - i;
-      uint32_t m = n[i];
-      if (!m) return (uint64_t)0;
-      if (key < limit.key) m = 0;
-      if (key == limit.key) m = min(m, limit.n);
-      return by_weight ? m * units(key_weight(r.s, key, r.top)) : (uint64_t)m;
-    };
-    for (int i = 0; i < each; ++i) mine += amount(i);
-    uint64_t total;
-    const uint64_t upto = scan(mine, sh, &total);
-    if (done + total >= goal) {
-      uint64_t sum = done + upto - mine;
-      if (sum < goal && sum + mine >= goal) {
-        for (int i = 0; i < each; ++i) {
-          const uint64_t w = amount(i);
-          if (sum + w >= goal) {
-            const uint64_t one = by_weight ? units(key_weight(r.s, k0 - i, r.top)) : 1;
-            sh.border = (uint64_t)((goal - sum + one - 1) / one) << 32 | (k0 - i);
-            break;
-          }
-          sum += w;
-        }
+      const uint32_t e = r.low - key;
+      const bool second = e < kSpan - 1;
+      if (d < span || second) {
+        atomicAdd(&sh.bins[second ? kSpan + 1 + e : from + d], 1u);
+      } else if (d < all) {  // hardly ever
+        if ((key == kZero || key == kMinusZero) && r.first - kZero >= kSpan)
+          atomicAdd(&sh.bins[kSpan], 1u);
+        else
+          between = true;
       }
-      __syncthreads();
-      const uint64_t b = sh.border;
-      __syncthreads();
-      return Border{(uint32_t)b, (uint32_t)(b >> 32), limit.least};
     }
-    done += total;
-    if (first) {  // the next window begins below this one
-      if (high < kWindow) return Border{0, 0, limit.least};
-      high -= kWindow;
-    } else {
-      high = sh.next;
-      __syncthreads();
-      if (!high) return Border{0, 0, limit.least};
-    }
+  };
+  for (int k0 = 8 * threadIdx.x; k0 < r.vocab; k0 += 4 * 8 * kDraw) {
+    u32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = load_bits(r.logits, min(k0 + j * 8 * kDraw, r.vocab), r.vocab);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t keys = two_keys(v[j][i]);
+        add(keys & 0xFFFFu);
+        add(keys >> 16);
+      }
   }
+  return between;
+}
+// The bin of a key that has one.
+__device__ __forceinline__ uint32_t bin_of(const Row& r, uint32_t key) {
+  return r.straight || r.first - key < kSpan ? r.first - key : kSpan + 1 + r.low - key;
+}
+// Whether 0 and -0 have neighbouring bins.
+__device__ __forceinline__ bool zeros_in(const Row& r) {
+  return r.first >= kZero && r.least <= kMinusZero && (r.straight || r.first - kMinusZero < kSpan || kZero <= r.low);
+}
+__device__ __forceinline__ bool count_all(Row& r, const Bins<false>* window, Shared& sh) {
+  // what lies 31 T below the largest weighs less than 2^-44; a key less, since the value loses its low bits
+  const float heat = fminf(fmaxf(r.s.heat, FLT_MIN), kMaxHeat);
+  r.least = r.top == INFINITY ? r.first - 1 : max((int)key_of_value(r.top - 31.0f * heat), (int)kLowest + 2) - 1;
+  r.low = r.least + (kSpan - 2);
+  r.straight = r.low + kSpan >= r.first;
+  const uint32_t from = window ? kWindow : 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins / 4; i += kDraw) reinterpret_cast<uint4*>(sh.bins)[i] = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) sh.between = 0;
+  __syncthreads();
+  if (window) sh.bins[2 * threadIdx.x] = window->n[0], sh.bins[2 * threadIdx.x + 1] = window->n[1];
+  if (r.straight ? count_keys<true>(r, from, sh) : count_keys<false>(r, from, sh)) sh.between = 1;
+  __syncthreads();
+  if (threadIdx.x == 0 && zeros_in(r)) {  // -0 counts as 0 (in the window, both are counted)
+    const uint32_t zero = bin_of(r, kZero);
+    if (zero >= from) sh.bins[zero] += sh.bins[zero + 1];
+    if (zero + 1 >= from) sh.bins[zero + 1] = 0;
+  }
+  __syncthreads();
+  return sh.between == 0;
 }
 
-// Each chunk's part of what is kept, to sh.mass, and how many tokens with the border's key it may keep, to sh.at_border.
-__device__ void chunk_masses(const Row& r, const Border& b, Shared& sh) {
+struct Sums {
+  uint32_t count, own_count, counts;  // in front of the thread's bins; in them; all
+  uint64_t mass, own_mass, masses;
+};
+template <bool WIDE>
+__device__ __forceinline__ Sums sum_bins(const Row& r, const Bins<WIDE>& b, Shared& sh) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  // whether the chunks' windows hold all that is kept
-  const bool quick = r.counts && r.high >= kWindow &&
-                     (b.key > r.high - kWindow || key_weight(r.s, r.high - kWindow, r.top) < b.least);
+  uint32_t n = 0;
+  uint64_t m = 0;
+  for (int j = 0; j < b.kCount; ++j) {
+    const int i = WIDE ? (j + lane) % b.kCount : j;  // (every lane another bank)
+    n += b.count(sh, i), m += b.mass(r, sh, i);
+  }
+  const uint32_t upto = wave_scan(n, AddCounts());
+  const uint64_t mass = wave_scan(m, AddUnits());
+  if (lane == 63) sh.count[w] = upto, sh.mass[w] = mass;
   __syncthreads();
-  if (quick) {
-    for (int c = w; c < r.chunks; c += kWaves) {
-      const float top = r.stats[c].top;
-      const int shift = top == -INFINITY ? kWindow : (int)(r.high - key_of_value(top));
-      uint64_t sum = 0;
-      uint32_t same = 0;
-      for (int j = lane; j < kWindow; j += 64) {
-        const uint32_t key = r.high - j;
-        if (j < shift || key < b.key) continue;
-        const uint32_t n = r.counts[(size_t)c * kWindow + j - shift];
-        if (!n) continue;
-        if (key == b.key) {
-          same = n;
-          continue;
-        }
-        const float x = key_weight(r.s, key, r.top);
-        if (x >= b.least) sum += n * units(x);
+  Sums s{upto - n, n, 0, mass - m, m, 0};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) s.count += sh.count[i], s.mass += sh.mass[i];
+    s.counts += sh.count[i], s.masses += sh.mass[i];
+  }
+  return s;
+}
+
+// The borders of top-k (k > 0) and top-p (p < 1) among bins that hold all in front of them.  False: these do not.
+template <bool WIDE>
+__device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, float p, Border& out, Shared& sh) {
+  const Sums s = sum_bins(r, b, sh);
+  double all = r.total * (double)kUnit;
+  bool found = false;
+  if (k > 0 && s.counts >= (uint32_t)k) {
+    uint32_t n = s.count;
+    uint64_t m = s.mass;
+    for (int i = 0; i < b.kCount && n < (uint32_t)k && s.count + s.own_count >= (uint32_t)k; ++i) {
+      const uint32_t x = b.count(sh, i);
+      if (n + x >= (uint32_t)k) {
+        const uint32_t key = b.key(r, i);
+        sh.border = Border{key, (uint32_t)k - n, 0.0f};
+        sh.border_mass = m + ((uint32_t)k - n) * units(key_weight(r.s, key, r.top));
       }
-      for (int d = 32; d; d /= 2) {
-        sum += (uint64_t)__shfl_xor((unsigned long long)sum, d);
-        same += __shfl_xor(same, d);
-      }
-      if (lane == 0) sh.mass[c] = sum, sh.at_border[c] = same;
+      n += x, m += b.mass(r, sh, i);
     }
     __syncthreads();
-  } else {
-    for (int c = 0; c < r.chunks; ++c) {
-      uint64_t sum = 0;
-      int same = 0;
-      for (int h = 0; h < 2; ++h) {
-        float l[8];
-        load8(r.logits, c * kChunk + h * kChunk / 2 + 8 * threadIdx.x, r.vocab, l);
+    out.key = sh.border.key, out.n = sh.border.n;
+    all = (double)sh.border_mass;
+    found = true;
+  } else if (k > 0 && !WIDE) {
+    return false;
+  }
+  if (p < 1.0f) {
+    const double want = ceil((double)fmaxf(p, 0.0f) * all);
+    const uint64_t goal = want > 1.0 ? (uint64_t)want : 1;
+    if (s.masses < goal) return found;
+    __syncthreads();  // (border was read)
+    uint64_t m = s.mass;
+    for (int i = 0; i < b.kCount && m < goal && s.mass + s.own_mass >= goal; ++i) {
+      const uint64_t x = b.mass(r, sh, i);
+      if (m + x >= goal) {
+        const uint32_t key = b.key(r, i);
+        const uint64_t one = units(key_weight(r.s, key, r.top));
+        sh.border = Border{key, (uint32_t)((goal - m + one - 1) / one), 0.0f};
+      }
+      m += x;
+    }
+    __syncthreads();
+    // (top-k's own border where a rounding of the goal would go past it)
+    if (!found || sh.border.key > out.key || (sh.border.key == out.key && sh.border.n < out.n)) out.key = sh.border.key, out.n = sh.border.n;
+    found = true;
+  }
+  return found;
+}
+
+// Each chunk's weights above the border's key and its tokens with it, to sh.kept and sh.equal: from the windows;
+__device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, const uint32_t (&first)[kLaneChunks], Shared& sh) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
 #pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t key = r.first - (2 * t + i);
+    const float x = key_weight(r.s, key, r.top);
+    sh.weight[2 * t + i] = key > b.key && x >= b.least ? units(x) : 0;
+  }
+  if (t < 2) sh.weight[kWindow + t] = 0;
+  __syncthreads();
+  // a wave kAt chunks at a time, lane by lane two neighbouring bins, 128 a step; steps past the border are not loaded
+  constexpr int kAt = 5, kSteps = kWindow / 128;
+  for (int c0 = w; c0 < r.chunks; c0 += kAt * kWaves) {
+    uint32_t pair[kAt][kSteps];
+    int shift[kAt], border[kAt];  // border: the chunk's bin of the border's key
+#pragma unroll
+    for (int a = 0; a < kAt; ++a) {
+      const int c = min(c0 + a * kWaves, r.chunks - 1);
+      uint32_t f = first[0];
+#pragma unroll
+      for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
+      shift[a] = (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
+      border[a] = (int)(r.first - b.key) - shift[a];
+      const int last = min(border[a], kWindow - 1 - shift[a]);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        pair[a][j] = 0;
+        if (128 * j <= last) pair[a][j] = r.counts[(size_t)c * (kWindow / 2) + 64 * j + lane];
+      }
+    }
+    uint64_t sum[kAt];
+    uint32_t same[kAt];
+#pragma unroll
+    for (int a = 0; a < kAt; ++a) {
+      sum[a] = 0, same[a] = 0;
+      const int last = min(border[a], kWindow - 1 - shift[a]);
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        if (128 * j > last) break;
+        const int at = 128 * j + 2 * lane, in = min(at + shift[a], kWindow);  // (past the window the weights are 0)
+        sum[a] += (pair[a][j] & 0xFFFFu) * sh.weight[in] + (pair[a][j] >> 16) * sh.weight[in + 1];
+        if (at == (border[a] & ~1)) same[a] = pair[a][j] >> (16 * (border[a] & 1)) & 0xFFFFu;
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < kAt; ++a) sum[a] = units_sum(sum[a]), same[a] = counts_sum(same[a]);
+#pragma unroll
+    for (int a = 0; a < kAt; ++a)
+      if (lane == 0 && c0 + a * kWaves < r.chunks)
+        sh.kept[c0 + a * kWaves] = sum[a], sh.equal[c0 + a * kWaves] = b.key ? same[a] : 0;
+  }
+  __syncthreads();
+}
+// and from the row: a wave adds up a chunk's, in whole units, so exactly.  (Weights looked up in LDS by key instead: no faster.)
+template <bool INF>
+__device__ __forceinline__ void chunk_masses_of(const Row& r, const Border& b, Shared& sh) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const float border = b.key ? logit_of(b.key) : -INFINITY;
+  for (int c = w; c < r.chunks; c += kWaves) {
+    u32x4 v[kChunk / 512];
+#pragma unroll
+    for (int j = 0; j < kChunk / 512; ++j) v[j] = load_bits(r.logits, min(c * kChunk + 512 * j + 8 * lane, r.vocab), r.vocab);
+    double sum = 0.0;
+    uint32_t same = 0;
+#pragma unroll
+    for (int j = 0; j < kChunk / 512; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float l = value(v[j], i), x = INF ? (l == r.top ? 1.0f : 0.0f) : weight(r.s, l, r.top);
+        sum += (double)(l > border && x >= b.least ? __builtin_truncf(x * kUnit) : 0.0f);
+        same += l == border;
+      }
+    sum = wave_sum(sum), same = counts_sum(same);
+    if (lane == 0) sh.kept[c] = (uint64_t)sum, sh.equal[c] = b.key ? same : 0;
+  }
+}
+__device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, Shared& sh) {
+  __syncthreads();
+  if (r.top == INFINITY)
+    chunk_masses_of<true>(r, b, sh);
+  else
+    chunk_masses_of<false>(r, b, sh);
+  __syncthreads();
+}
+
+// Keys of a row that has some between the bins: down from the largest, kBins at a time and over empty stretches at once, first to
+// top-k's border, then to top-p's.  Slow, for rows with logits of 2^-58 of the largest and less.
+__device__ __attribute__((noinline)) Border find_slowly(Row r, int k, float p, Border out, Shared& sh) {
+  const uint32_t top = r.first;
+  r.straight = true;
+  double all = r.total * (double)kUnit;
+  bool found = false;
+  for (int turn = k > 0 ? 0 : 1; turn < (p < 1.0f ? 2 : 1); ++turn) {
+    const double want = turn ? ceil((double)fmaxf(p, 0.0f) * all) : (double)k;
+    const uint64_t goal = want > 1.0 ? (uint64_t)want : 1;
+    uint32_t counts = 0;
+    uint64_t masses = 0;
+    r.first = top;
+    for (;;) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < kBins; i += kDraw) sh.bins[i] = 0;
+      if (threadIdx.x == 0) sh.between = 0;
+      __syncthreads();
+      uint32_t next = 0;
+      for (int k0 = 8 * threadIdx.x; k0 < r.vocab; k0 += 8 * kDraw) {
+        float l[8];
+        load8(r.logits, k0, r.vocab, l);
         for (int i = 0; i < 8; ++i) {
           const uint32_t key = key_of_value(l[i]);
-          same += key == b.key;
-          if (key <= b.key) continue;
-          const float x = key_weight(r.s, key, r.top);
-          if (x >= b.least) sum += units(x);
+          if (key > r.first || key == kLowest) continue;
+          if (r.first - key < kBins)
+            atomicAdd(&sh.bins[r.first - key], 1u);
+          else
+            next = max(next, key);
         }
       }
-      uint64_t total, equal;
-      scan(sum, sh, &total);
-      scan((uint64_t)same, sh, &equal);
-      if (threadIdx.x == 0) sh.mass[c] = total, sh.at_border[c] = (uint32_t)equal;
+      if (next) atomicMax(&sh.between, next);
+      __syncthreads();
+      const Bins<true> b{};
+      const Sums s = sum_bins(r, b, sh);
+      if ((turn ? masses + s.masses : (uint64_t)counts + s.counts) >= goal) {
+        uint32_t n = counts + s.count;
+        uint64_t m = masses + s.mass;
+        for (int i = 0; i < kBinsEach && (turn ? m : n) < goal; ++i) {
+          const uint32_t x = b.count(sh, i), key = b.key(r, i);
+          const uint64_t one = x ? units(key_weight(r.s, key, r.top)) : 0;
+          if ((turn ? m + x * one : (uint64_t)n + x) >= goal) {
+            const uint32_t take = turn ? (uint32_t)((goal - m + one - 1) / one) : (uint32_t)goal - n;
+            sh.border = Border{key, take, 0.0f};
+            sh.border_mass = m + take * one;
+          }
+          n += x, m += x * one;
+        }
+        __syncthreads();
+        if (!found || sh.border.key > out.key || (sh.border.key == out.key && sh.border.n < out.n))
+          out.key = sh.border.key, out.n = sh.border.n;
+        all = (double)sh.border_mass;
+        found = true;
+        break;
+      }
+      counts += s.counts, masses += s.masses;
+      r.first = sh.between;
+      if (!r.first) break;
     }
-    __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    const float x = b.key ? key_weight(r.s, b.key, r.top) : 0.0f;
-    uint32_t left = x >= b.least ? b.n : 0;
-    for (int c = 0; c < r.chunks; ++c) {
-      const uint32_t n = min(sh.at_border[c], left);
-      left -= n;
-      sh.at_border[c] = n;
-      sh.mass[c] += n * units(x);
-    }
-  }
-  __syncthreads();
+  return out;
 }
 
-// The first thread at which the sum of the threads' x (>= 0) passes `at`, the last with any x if none does, -1 without any;
-// *before: the sum of the threads before it.
-__device__ __forceinline__ int pick_thread(double x, double at, Shared& sh, double* before) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const double inc = wave_scan(x, Add());
-  __syncthreads();
-  if (lane == 63) sh.red[w] = inc;
-  __syncthreads();
-  double b = inc - x;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i)
-    if (i < w) b += sh.red[i];
-  const uint64_t past = __ballot(x > 0.0 && b + x > at), any = __ballot(x > 0.0);
-  const int mine = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : -1;
-  if (lane == mine) sh.before[w] = b;
-  if (lane == 0) sh.ired[w] = mine < 0 ? -1 : 64 * w + mine, sh.ok[w] = past != 0;
-  __syncthreads();
-  int pick = -1;
-  for (int i = 0; i < kWaves; ++i) {
-    if (sh.ired[i] < 0) continue;
-    pick = sh.ired[i], *before = sh.before[i];
-    if (sh.ok[i]) break;
+__device__ __forceinline__ void store(const SampleArgs& a, int id, const Row& r, int token) {
+  a.tokens[id] = token;
+  if (!a.logp) return;
+  float lp = 0.0f;
+  if (token >= 0) {
+    const float l = bf2f(r.logits[token]);
+    lp = (float)((l == r.top ? 0.0 : (double)(l - r.top) / (double)fminf(r.s.heat, kMaxHeat)) - log(r.total));
   }
-  __syncthreads();
-  return pick;
+  a.logp[id] = lp;
 }
 
-// The token of a chunk at which the kept weights pass `at`; n: how many tokens with the border's key it may keep.
-__device__ __forceinline__ int draw_in(const Row& r, int chunk, const Border& b, uint32_t n, double at, Shared& sh) {
-  const int k = chunk * kChunk + kEach * (int)threadIdx.x;
-  float l[kEach];
+// The token of a chunk at which the kept weights pass `at`; n: how many tokens with the border's key it may keep.  Its thread
+// stores it.
+__device__ __forceinline__ void draw_in(const SampleArgs& a, int id, const Row& r, int chunk, const Border& b, uint32_t n, double at,
+                                        Shared& sh) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, k = chunk * kChunk + 8 * t;
+  float l[8], x[8];
   load8(r.logits, k, r.vocab, l);
-  load8(r.logits, k + 8, r.vocab, l + 8);
-  int same = 0;
+  uint32_t rank = 0;
+  if (b.key) {
+    uint32_t same = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) same += key_of_value(l[i]) == b.key;
-  uint64_t all;
-  uint64_t rank = scan((uint64_t)same, sh, &all) - same;
+    for (int i = 0; i < 8; ++i) same += key_of_value(l[i]) == b.key;
+    const uint32_t upto = wave_scan(same, AddCounts());
+    if (lane == 63) sh.same[w] = upto;
+    __syncthreads();
+    rank = upto - same;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i)
+      if (i < w) rank += sh.same[i];
+  }
   float sum = 0.0f;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
+  for (int i = 0; i < 8; ++i) {
     const uint32_t key = key_of_value(l[i]);
-    const float x = any_weight(r.s, l[i], r.top);
-    bool keep = key > b.key && x >= b.least;
-    if (key == b.key) keep = rank++ < n;
-    l[i] = keep ? x : 0.0f;
-    sum += l[i];
+    x[i] = any_weight(r.s, l[i], r.top);
+    bool keep = key > b.key && x[i] >= b.least;
+    if (b.key && key == b.key) keep = rank++ < n;
+    x[i] = keep ? x[i] : 0.0f;
+    sum += x[i];
   }
-  double before;
-  const int who = pick_thread((double)sum, at, sh, &before);
-  if (who < 0) return -1;
-  if ((int)threadIdx.x == who) {
-    int token = -1;
-    double c = before;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (l[i] > 0.0f && (token < 0 || c <= at)) token = k + i;
-      c += (double)l[i];
-    }
-    sh.ired[0] = token;
-  }
+  const double mine = (double)sum, upto = wave_scan(mine, Add());
+  if (lane == 63) sh.sum[w] = upto;
   __syncthreads();
-  return sh.ired[0];
+  // the first wave that passes `at`, the last with any weight if none does; in it the lane likewise, and there the token
+  double before = 0.0, c = 0.0;
+  int wave = -1;
+  bool past = false;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const double s = sh.sum[i];
+    if (!past && s > 0.0) wave = i, before = c, past = c + s > at;
+    c += s;
+  }
+  if (wave < 0) wave = 0;  // (not with any weight in the chunk)
+  if (w != wave) return;
+  const double to = before + upto, from = to - mine;
+  const uint64_t over = __ballot(mine > 0.0 && to > at), any = __ballot(mine > 0.0);
+  if (lane != (over ? __builtin_ctzll(over) : any ? 63 - __builtin_clzll(any) : 0)) return;
+  int token = r.best;
+  bool have = false;
+  c = from;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (x[i] > 0.0f && (!have || c <= at)) token = k + i, have = true;
+    c += (double)x[i];
+  }
+  store(a, id, r, token);
 }
 
-__global__ void __launch_bounds__(kThreads) sample_draw_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) {
   __shared__ Shared sh;
-  __shared__ ChunkStat st[kMaxChunks];
-  const int id = blockIdx.x, t = threadIdx.x;
+  const int id = blockIdx.x, t = threadIdx.x, lane = t & 63;
   Row r;
   r.s = heat_of(a.temp ? a.temp[id] : 1.0f);
   r.logits = a.logits + (size_t)id * a.ld;
   r.vocab = a.vocab, r.chunks = a.chunks;
-  r.counts = a.counts ? a.counts + (size_t)id * a.chunks * kWindow : nullptr;
-  if (a.stats) {
-    if (t < a.chunks) st[t] = a.stats[(size_t)id * a.chunks + t];
-  } else {
-    for (int c = 0; c < a.chunks; ++c) {
-      const ChunkStat x = chunk_stat(r.s, r.logits, c, a.vocab, nullptr, sh);
-      if (t == 0) st[c] = x;
+  r.counts = a.counts ? a.counts + (size_t)id * a.chunks * (kWindow / 2) : nullptr;
+  const int k = a.top_k ? a.top_k[id] : 0;
+  const float p = a.top_p ? a.top_p[id] : 1.0f, least = a.min_p ? a.min_p[id] : 0.0f, u = a.u[id];
+  if (!a.stats) {
+    for (int c0 = 0; c0 < a.chunks; c0 += kGroups) {
+      const int c = c0 + t / kGroupThreads;
+      const ChunkStat x = chunk_stat(r.s, r.logits, min(c, a.chunks), a.vocab, nullptr, sh.g[t / kGroupThreads]);
+      if (t % kGroupThreads == 0 && c < a.chunks) sh.stats[c] = x;
     }
+    __syncthreads();
   }
-  __syncthreads();
-  r.stats = st;
-  r.top = -INFINITY, r.best = -1, r.total = 0.0;
-  for (int c = 0; c < a.chunks; ++c)
-    if (st[c].top > r.top) r.top = st[c].top, r.best = st[c].best;
-  for (int c = 0; c < a.chunks; ++c) r.total += st[c].total * (double)any_weight(r.s, st[c].top, r.top);
-  int token = r.best;
-  if (!r.s.greedy && r.best >= 0) {
-    r.high = key_of_value(r.top);
-    const int k = a.top_k ? a.top_k[id] : 0;
-    const float p = a.top_p ? a.top_p[id] : 1.0f, least = a.min_p ? a.min_p[id] : 0.0f;
-    Border b{0, 0, least > 0.0f ? fminf(least, 1.0f) : 0.0f};
-    bool limited = b.least > 0.0f;
-    if (k > 0 && k < a.vocab) {
-      b = find(r, false, (uint64_t)k, b, sh);
-      limited |= b.key != 0;
+  // every wave by itself: the row from its chunks (lane by lane, then over the lanes)
+  const ChunkStat* const stats = a.stats ? a.stats + (size_t)id * a.chunks : sh.stats;
+  ChunkStat st[kLaneChunks];
+  uint32_t first[kLaneChunks];
+  r.top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) {
+    st[i] = ChunkStat{-INFINITY, -1, 0.0};
+    if (lane + 64 * i < a.chunks) st[i] = stats[lane + 64 * i];
+  }
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) r.top = fmaxf(r.top, st[i].top), first[i] = first_key(st[i].top);
+  r.top = wave_max(r.top);
+  if (r.top == -INFINITY) {
+    if (t == 0) {
+      a.tokens[id] = -1;
+      if (a.logp) a.logp[id] = 0.0f;
     }
-    if (p < 1.0f) {
-      double all = r.total * (double)kUnit;
-      if (b.key) {
-        chunk_masses(r, Border{b.key, b.n, 0.0f}, sh);
-        uint64_t sum = 0;
-        for (int c = 0; c < a.chunks; ++c) sum += sh.mass[c];
-        all = (double)sum;
-        __syncthreads();
-      }
-      const double goal = (double)fmaxf(p, 0.0f) * all;
-      const Border q = find(r, true, goal > 1.0 ? (uint64_t)ceil(goal) : 1, b, sh);
-      if (q.key) b = q, limited = true;
-    }
-    const float u = a.u[id];
-    double at = 0.0, before = 0.0;
+    return;
+  }
+  double share[kLaneChunks], total = 0.0;
+  int best = 0x7FFFFFFF;
+#pragma unroll
+  for (int i = kLaneChunks - 1; i >= 0; --i) {
+    if (st[i].top == r.top) best = st[i].best;
+    share[i] = st[i].total * (double)any_weight(r.s, st[i].top, r.top);
+  }
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) total += share[i];
+  r.total = wave_sum(total);
+  r.best = wave_min(best);
+  r.first = first_key(r.top);
+  if (r.s.greedy) {
+    if (t == 0) store(a, id, r, r.best);
+    return;
+  }
+  const int limit = k > 0 && k < a.vocab ? k : 0;
+  Border b{0, 0, least > 0.0f ? fminf(least, 1.0f) : 0.0f};
+  if (!limit && !(p < 1.0f) && b.least == 0.0f) {  // no filter: the chunk from their own sums
+    double at = (double)u * r.total, before = 0.0, c = 0.0;
     int chunk = -1;
-    if (limited) {
-      chunk_masses(r, b, sh);
-      uint64_t all = 0, sum = 0;
-      for (int c = 0; c < a.chunks; ++c) all += sh.mass[c];
-      at = (double)u * (double)all;
-      for (int c = 0; c < a.chunks; ++c) {
-        const uint64_t x = sh.mass[c];
-        if (!x) continue;
-        chunk = c, before = (double)sum;
-        sum += x;
-        if ((double)sum > at) break;
+    bool past = false;
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; ++i) {
+      if (64 * i >= a.chunks || past) break;
+      const double upto = wave_scan(share[i], Add()), from = c + upto - share[i];
+      const uint64_t over = __ballot(share[i] > 0.0 && c + upto > at), any = __ballot(share[i] > 0.0);
+      if (over | any) {
+        const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+        chunk = 64 * i + l, before = __shfl(from, l);
+        past = over != 0;
       }
-      at = fmax(at - before, 0.0) * (1.0 / (double)kUnit);
-    } else {
-      double sum = 0.0;
-      at = (double)u * r.total;
-      for (int c = 0; c < a.chunks; ++c) {
-        const double x = st[c].total * (double)any_weight(r.s, st[c].top, r.top);
-        if (!(x > 0.0)) continue;
-        chunk = c, before = sum;
-        sum += x;
-        if (sum > at) break;
-      }
-      at = fmax(at - before, 0.0);
+      c += __shfl(upto, 63);
     }
-    const uint32_t n = limited && chunk >= 0 ? sh.at_border[chunk] : 0;
-    if (chunk >= 0) token = draw_in(r, chunk, b, n, at, sh);
+    draw_in(a, id, r, chunk, b, 0, fmax(at - before, 0.0), sh);
+    return;
   }
-  if (t == 0) {
-    a.tokens[id] = token;
-    if (a.logp) {
-      float lp = 0.0f;
-      if (token >= 0) {
-        const float l = bf2f(r.logits[token]);
-        lp = (float)((l == r.top ? 0.0 : (double)(l - r.top) / (double)fminf(r.s.heat, kMaxHeat)) - log(r.total));
-      }
-      a.logp[id] = lp;
+  bool quick = r.counts != nullptr;
+  Bins<false> window{{0, 0}};
+  if (quick) {
+    // whether min-p's border is within the window: then no other that is further down matters (where top-p's may be within it
+    // though top-k's is not, that has to be known)
+    const bool cut = r.first < kWindow || key_weight(r.s, r.first - (kWindow - 1), r.top) < b.least;
+    bool found = false;
+    if (limit || p < 1.0f) {
+      window = count_window(r, first);
+      found = find(r, window, limit, p, b, sh);
     }
+    quick = found || (cut && !(limit && p < 1.0f));
+    if (!found) b.key = 0, b.n = 0;
   }
+  if (quick) {
+    chunk_masses(r, b, first, sh);
+  } else {
+    if (limit || p < 1.0f) {
+      if (count_all(r, r.counts ? &window : nullptr, sh))
+        (void)find(r, Bins<true>{}, limit, p, b, sh);  // (found nowhere: there is no border)
+      else
+        b = find_slowly(r, limit, p, b, sh);
+    }
+    chunk_masses(r, b, sh);
+  }
+  // the chunk, every wave by itself
+  const float border_weight = b.key ? key_weight(r.s, b.key, r.top) : 0.0f;
+  const uint64_t one = units(border_weight);
+  uint32_t left = border_weight >= b.least ? b.n : 0;
+  uint64_t mass[kLaneChunks], all = 0;
+  uint32_t mine[kLaneChunks];
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) {
+    mass[i] = 0, mine[i] = 0;
+    if (64 * i >= a.chunks) continue;
+    const int c = lane + 64 * i;
+    const uint32_t n = c < a.chunks ? sh.equal[c] : 0, upto = wave_scan(n, AddCounts()), from = upto - n;
+    mine[i] = min(n, left > from ? left - from : 0u);
+    mass[i] = (c < a.chunks ? sh.kept[c] : 0) + mine[i] * one;
+    const uint32_t used = last_lane(upto);
+    left = left > used ? left - used : 0;
+    all += units_sum(mass[i]);
+  }
+  const double at = (double)u * (double)all;
+  uint64_t c = 0;
+  double before = 0.0;
+  int chunk = -1;
+  uint32_t n = 0;
+  bool past = false;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) {
+    if (64 * i >= a.chunks || past) continue;
+    const uint64_t upto = wave_scan(mass[i], AddUnits());
+    const uint64_t over = __ballot(mass[i] && (double)(c + upto) > at), any = __ballot(mass[i] != 0);
+    if (over | any) {
+      const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+      chunk = 64 * i + l, past = over != 0;
+      before = (double)(c + (uint64_t)__shfl((unsigned long long)(upto - mass[i]), l));
+      n = __shfl(mine[i], l);
+    }
+    c += last_lane64(upto);
+  }
+  draw_in(a, id, r, chunk, b, n, fmax(at - before, 0.0) * (1.0 / (double)kUnit), sh);
 }
 
 SampleArgs from(SampleArgs a, int row) {
@@ -514,17 +794,17 @@ int launch(SampleArgs a, hipStream_t st) {
   std::lock_guard<std::mutex> lock(scratch_mutex(st));  // the launches that share the scratch stay together
   uint8_t* const z = call_scratch(st, per * each, ScratchOf::kOperators).data;
   if (!z) {
-    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)a.b), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)a.b), dim3(kDraw), 0, st, a);
     return (int)hipGetLastError();
   }
   a.stats = reinterpret_cast<ChunkStat*>(z);
-  a.counts = reinterpret_cast<uint16_t*>(a.stats + (size_t)each * a.chunks);
+  a.counts = reinterpret_cast<uint32_t*>(a.stats + (size_t)each * a.chunks);
   for (int i = 0; i < a.b; i += each) {
     const SampleArgs l = from(a, i);
     const unsigned n = (unsigned)(a.b - i < each ? a.b - i : each);
-    hipLaunchKernelGGL(sample_keys_kernel, dim3((unsigned)a.chunks, n), dim3(kThreads), 0, st, l);
+    hipLaunchKernelGGL(sample_keys_kernel, dim3((unsigned)a.chunks, n), dim3(kGroupThreads), 0, st, l);
     if (const int e = (int)hipGetLastError()) return e;
-    hipLaunchKernelGGL(sample_draw_kernel, dim3(n), dim3(kThreads), 0, st, l);
+    hipLaunchKernelGGL(sample_draw_kernel, dim3(n), dim3(kDraw), 0, st, l);
     if (const int e = (int)hipGetLastError()) return e;
   }
   return 0;

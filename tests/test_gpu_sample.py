@@ -117,6 +117,40 @@ def test_flat_rows_whose_border_is_far_down():
     r.compare(r.run(), least=0.7, tol=2e-6)
 
 
+@pytest.mark.parametrize("tiny", [0.0, 1e-6, 1e-15, 1e-30])
+@pytest.mark.parametrize("shift", [0.0, -1.0, 3.0])
+def test_borders_among_zeros_and_tiny_values(tiny, shift):
+    """Many logits of 0, -0 and magnitudes far below the largest: borders fall among them, where keys are far apart."""
+    rng = np.random.default_rng(19)
+    b, vocab = 40, 9000
+    x = rng.standard_normal((b, vocab)) + np.where(rng.random((b, vocab)) < 0.2, shift, 0.0)
+    kind = rng.random((b, vocab))
+    x = np.where(kind < 0.4, tiny * rng.standard_normal((b, vocab)), x)
+    bits = f2bf_array(x.astype(np.float32).ravel()).reshape(b, vocab)
+    bits[(kind > 0.4) & (kind < 0.45)] = 0x0000
+    bits[(kind > 0.45) & (kind < 0.5)] = 0x8000
+    bits[::7] |= 0x8000  # no positive logit
+    top_k = np.where(np.arange(b) % 3 == 0, rng.integers(1000, 8000, b), 0)
+    top_p = np.where(np.arange(b) % 3 != 0, 0.3 + 0.69 * rng.random(b), 1.0)
+    top_p[::4] = 0.9
+    min_p = np.where(np.arange(b) % 5 == 2, 0.03, 0.0)
+    r = Rows(bits, 0.5 + rng.random(b), top_k, top_p, min_p, rng.random(b))
+    # weights of |d / T| below 16: 8e-7 (as above)
+    r.compare(r.run(), least=0.7, tol=2e-6)
+
+
+@pytest.mark.parametrize("zero", list(range(1018, 1030)) + list(range(8186, 8198)) + [16382, 16384])
+def test_zeros_at_a_windows_end(zero):
+    """0 and -0 at every place around the last of the keys that are counted first."""
+    rng = np.random.default_rng(zero)
+    x = np.full((4, 600), 0xC000, dtype=np.uint16)
+    x[:, 300] = zero  # (the key of the largest logit is this far above 0's)
+    x[:, 301:340] = rng.integers(1, zero + 1, 39)
+    x[:, 100:200:2], x[:, 101:200:2] = 0x8000, 0x0000
+    r = Rows(x, 1e-38, [60, 0, 139, 140], [1.0, 0.8, 0.999, 0.6], None, rng.random(4))
+    r.compare(r.run(), least=1.0, tol=2e-6)
+
+
 @pytest.mark.parametrize("scale", [1e-30, 1e-3, 1.0, 1e30])
 def test_rows_of_any_size(scale):
     rng = np.random.default_rng(3)
