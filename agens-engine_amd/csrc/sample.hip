@@ -16,7 +16,7 @@
 //   sample_draw_kernel   a row a workgroup: the chunks' windows, shifted to the row's largest key and summed, give the border of
 //                        what is kept (one scan of counts and weights serves top-k and top-p, since top-p's border is not
 //                        behind top-k's), and what each chunk has of it; then the chunk that the draw falls into is read again.
-//                        A window goes down to 2^-8 of a positive largest logit; where the border is below it, the row's
+//                        A window goes down to 2^-4 of a positive largest logit; where the border is below it, the row's
 //                        keys are counted anew, all at once, and the chunks' shares summed up in another pass.
 // Both wait: for loads, and for each other's barriers.  Without scratch sample_draw_kernel takes the chunks' statistics itself
 // and does without their windows: the same tokens.
@@ -30,8 +30,9 @@ constexpr int kEach = 16, kGroupThreads = 256, kChunk = kGroupThreads * kEach;
 constexpr int kDraw = 512, kWaves = kDraw / 64, kGroups = kDraw / kGroupThreads;
 constexpr int kMaxChunks = 256, kLaneChunks = kMaxChunks / 64;  // of a row
 static_assert(kMaxChunks * kChunk == AK_SAMPLE_MAX_VOCAB, "the header's limit");
-constexpr int kWindow = 1024;
-static_assert(kWindow == 2 * kDraw && kChunk == 8 * kDraw, "two bins of the window and eight logits of a chunk a thread");
+constexpr int kWindow = 512;
+static_assert(kWindow == kDraw && kChunk == 8 * kDraw, "a bin of the window and eight logits of a chunk a thread");
+static_assert(kWindow == 2 * kGroupThreads, "two bins a thread");
 // Bins of all keys that matter: kSpan from the largest down, zero's, and the rest up from the least with any weight.
 constexpr int kSpan = 8192, kBins = 2 * kSpan, kBinsEach = kBins / kDraw;
 constexpr float kMaxHeat = 1.44e30f;  // (see heat_of)
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const Sample
   __shared__ __attribute__((aligned(16))) uint32_t bins[kWindow + 1];  // (one more: -0 behind 0)
   const int chunk = blockIdx.x, id = blockIdx.y, t = threadIdx.x;
   const Heat s = heat_of(a.temp ? a.temp[id] : 1.0f);
-  *reinterpret_cast<uint4*>(bins + 4 * t) = make_uint4(0, 0, 0, 0);  // (a barrier follows before the first count)
+  *reinterpret_cast<uint2*>(bins + 2 * t) = make_uint2(0, 0);  // (a barrier follows before the first count)
   if (t == 0) bins[kWindow] = 0;
   const ChunkStat r = chunk_stat(s, a.logits + (size_t)id * a.ld, chunk, a.vocab, bins, g);
   const size_t at = (size_t)id * a.chunks + chunk;
@@ -192,8 +193,8 @@ __global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const Sample
     if (r.top >= 0.0f && d < kWindow) bins[d] += bins[d + 1], bins[d + 1] = 0;
   }
   __syncthreads();
-  const uint4 n = *reinterpret_cast<const uint4*>(bins + 4 * t);
-  *reinterpret_cast<uint2*>(a.counts + at * (kWindow / 2) + 2 * t) = make_uint2(n.x | n.y << 16, n.z | n.w << 16);
+  const uint2 n = *reinterpret_cast<const uint2*>(bins + 2 * t);
+  a.counts[at * (kWindow / 2) + t] = n.x | n.y << 16;
 }
 
 // What is kept: keys above `key` and the first `n` tokens with it, of weights from `least` on.
@@ -233,13 +234,13 @@ struct Row {
 // Bins in order: two of the window a thread, or kBinsEach of all keys'.
 template <bool WIDE>
 struct Bins {
-  static constexpr int kCount = WIDE ? kBinsEach : 2;
-  uint32_t n[WIDE ? 1 : 2];
+  static constexpr int kCount = WIDE ? kBinsEach : 1;
+  uint32_t n;
   __device__ __forceinline__ uint32_t count(const Shared& sh, int i) const {
     if constexpr (WIDE)
       return sh.bins[threadIdx.x * kBinsEach + i];
     else
-      return n[i];
+      return n;
   }
   __device__ __forceinline__ uint32_t key(const Row& r, int i) const {
     const int at = (int)threadIdx.x * kCount + i;
@@ -252,23 +253,25 @@ struct Bins {
   }
 };
 
-// The two bins of the chunks' windows.
+// The thread's bin of the chunks' windows.
 __device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&first)[kLaneChunks]) {
-  Bins<false> b{{0, 0}};
-  for (int c0 = 0; c0 < r.chunks; c0 += 40) {
-    uint32_t v[40];
+  constexpr int kAt = 40;  // loads in flight
+  Bins<false> b{0};
+  const uint16_t* const counts = reinterpret_cast<const uint16_t*>(r.counts);
+  for (int c0 = 0; c0 < r.chunks; c0 += kAt) {
+    uint32_t v[kAt];
 #pragma unroll
-    for (int j = 0; j < 40; ++j) {
+    for (int j = 0; j < kAt; ++j) {
       const int c = min(c0 + j, r.chunks - 1);
       uint32_t f = first[0];
 #pragma unroll
       for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
-      const int at = (int)threadIdx.x - (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63)) / 2;
+      const int at = (int)threadIdx.x - (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
       v[j] = 0;
-      if (at >= 0 && c0 + j < r.chunks) v[j] = r.counts[(size_t)c * (kWindow / 2) + at];
+      if (at >= 0 && c0 + j < r.chunks) v[j] = counts[c * kWindow + at];
     }
 #pragma unroll
-    for (int j = 0; j < 40; ++j) b.n[0] += v[j] & 0xFFFFu, b.n[1] += v[j] >> 16;
+    for (int j = 0; j < kAt; ++j) b.n += v[j];
   }
   return b;
 }
@@ -296,6 +299,7 @@ __device__ __forceinline__ bool count_keys(const Row& r, uint32_t from, Shared& 
       }
     }
   };
+  // (loading the next 32 logits during these is slower: the atomics are what takes the time)
   for (int k0 = 8 * threadIdx.x; k0 < r.vocab; k0 += 4 * 8 * kDraw) {
     u32x4 v[4];
 #pragma unroll
@@ -330,7 +334,7 @@ __device__ __forceinline__ bool count_all(Row& r, const Bins<false>* window, Sha
   for (int i = threadIdx.x; i < kBins / 4; i += kDraw) reinterpret_cast<uint4*>(sh.bins)[i] = make_uint4(0, 0, 0, 0);
   if (threadIdx.x == 0) sh.between = 0;
   __syncthreads();
-  if (window) sh.bins[2 * threadIdx.x] = window->n[0], sh.bins[2 * threadIdx.x + 1] = window->n[1];
+  if (window) sh.bins[threadIdx.x] = window->n;
   if (r.straight ? count_keys<true>(r, from, sh) : count_keys<false>(r, from, sh)) sh.between = 1;
   __syncthreads();
   if (threadIdx.x == 0 && zeros_in(r)) {  // -0 counts as 0 (in the window, both are counted)
@@ -419,12 +423,9 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
 // Each chunk's weights above the border's key and its tokens with it, to sh.kept and sh.equal: from the windows;
 __device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, const uint32_t (&first)[kLaneChunks], Shared& sh) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t key = r.first - (2 * t + i);
-    const float x = key_weight(r.s, key, r.top);
-    sh.weight[2 * t + i] = key > b.key && x >= b.least ? units(x) : 0;
-  }
+  const uint32_t key = r.first - t;
+  const float x = key_weight(r.s, key, r.top);
+  sh.weight[t] = key > b.key && x >= b.least ? units(x) : 0;
   if (t < 2) sh.weight[kWindow + t] = 0;
   __syncthreads();
   // a wave kAt chunks at a time, lane by lane two neighbouring bins, 128 a step; steps past the border are not loaded
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     return;
   }
   bool quick = r.counts != nullptr;
-  Bins<false> window{{0, 0}};
+  Bins<false> window{0};
   if (quick) {
     // whether min-p's border is within the window: then no other that is further down matters (where top-p's may be within it
     // though top-k's is not, that has to be known)

@@ -357,7 +357,7 @@ int ak_rope_kv_write(int bits, const void* q, long ldq, const void* k, long ldk,
  * falling logit, the lower token first among equal ones: top_k keeps the first top_k; top_p the fewest of these, from the front,
  * whose p reach top_p of the sum of theirs (one at least); min_p drops those with p below min_p times the largest.  The token is
  * the first, in order of tokens, at which the cumulative p of those kept passes u times their sum.  temperature [b] (NULL: 1; 0
- * or less: greedy, the largest logit; more than 1.44e30 counts as that), top_k [b] (NULL, or 0 or less, or vocab and more: off), top_p [b]
+ * or less: greedy, the largest logit; below 2^-126 and above 1.44e30 it counts as these), top_k [b] (NULL, or 0 or less, or vocab and more: off), top_p [b]
  * (NULL, or 1 and more: off), min_p [b] (NULL, or 0 and less: off), u [b] uniform in [0, 1), all in device memory.
  * logp (may be NULL): log p of the token before any filter (greedy: at temperature 1).  NaN logits count as -inf; a row of
  * nothing else gives the token -1 and logp 0.  Without filters the tokens are ak_spec_verify's with t = 0, but for roundings.
