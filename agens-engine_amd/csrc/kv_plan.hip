@@ -9,11 +9,12 @@
 // numbers before the first barrier, and nothing is written before it.
 #include "agens_kernels.h"
 #include "kv_page.h"
+#include "logits.h"
 
 namespace agq {
 namespace {
 
-constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
+constexpr int kPlanThreads = 1024, kFewThreads = 256;
 static_assert(kPlanThreads >= AK_PLAN_MAX_SEQS, "a thread a sequence");
 
 struct PlanArgs {
@@ -22,19 +23,22 @@ struct PlanArgs {
   int b, m, npages, page_log2, ldt;
 };
 
-// the sum of x over the threads up to this one; *total: over all.  Sums below 2^31.
-__device__ __forceinline__ int block_scan(int x, int* red, int* total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int d = 1; d < 64; d *= 2) {
-    const int y = __shfl_up(x, d);
-    if (lane >= d) x += y;
+struct AddInt {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ int step(int x) const {
+    return x + (int)dpp<CTRL, ROWS>((uint32_t)x, 0);
   }
-  __syncthreads();
-  if (lane == 63) red[w] = x;
+};
+// the sum of x over the threads up to this one; *total: over all.  Sums below 2^31.  One barrier; red: this scan's own.
+template <int WAVES>
+__device__ __forceinline__ int block_scan(int x, int* red, int* total) {
+  const int w = threadIdx.x >> 6;
+  x = wave_scan(x, AddInt());
+  if ((threadIdx.x & 63) == 63) red[w] = x;
   __syncthreads();
   int all = 0;
 #pragma unroll
-  for (int i = 0; i < kPlanWaves; ++i) {
+  for (int i = 0; i < WAVES; ++i) {
     if (i < w) x += red[i];
     all += red[i];
   }
@@ -65,9 +69,11 @@ __device__ __forceinline__ void put_token(const PlanArgs& a, int t, int i, int f
   a.slots[t] = slot;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_seqs_kernel(const PlanArgs a, int tokens_too) {
-  __shared__ int red[kPlanWaves];
-  __shared__ int at[kPlanThreads + 1], from[kPlanThreads], to[kPlanThreads];
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) plan_seqs_kernel(const PlanArgs a, int tokens_too) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ int red[3][kWaves], granted;
+  __shared__ int at[THREADS], from[THREADS];
   const int i = threadIdx.x;
   const bool mine = i < a.b, pages = a.free_pages != nullptr;
   int count = 0, n = 0, h = 0, back = 0;
@@ -78,42 +84,57 @@ __global__ void __launch_bounds__(kPlanThreads) plan_seqs_kernel(const PlanArgs 
     if (a.drop && a.drop[i]) back = h, n = 0, h = 0;
   }
   const int stack = pages ? min(max(a.free_count[0], 0), a.npages) : 0;
-  // what ended sequences held
-  int total_back = 0;
-  if (pages) {
-    const int up = block_scan(back, red, &total_back);
-    at[i] = up - back;
-    __syncthreads();
-    for (int e = i; e < total_back; e += kPlanThreads) {
-      const int s = range_of(at, a.b, e);
-      if (stack + e < a.npages) a.free_pages[stack + e] = a.table[(size_t)s * a.ldt + e - at[s]];
+  if (i == 0) granted = 0;
+  int total, total_back = 0;
+  const int end = block_scan<kWaves>(count, red[0], &total), start = end - count;
+  if (pages && a.drop) {  // what ended sequences held
+    const int up = block_scan<kWaves>(back, red[1], &total_back);
+    if (total_back) {
+      at[i] = up - back;
+      __syncthreads();
+      for (int e0 = i; e0 < total_back; e0 += 4 * THREADS) {  // four on their way at a time
+        int page[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = min(e0 + j * THREADS, total_back - 1), s = range_of(at, a.b, e);
+          page[j] = a.table[(size_t)s * a.ldt + e - at[s]];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = e0 + j * THREADS;
+          if (e < total_back && stack + e < a.npages) a.free_pages[stack + e] = page[j];
+        }
+      }
     }
   }
   const int avail = min(stack + total_back, a.npages);
-  int total;
-  const int end = block_scan(count, red, &total), start = end - count;
   const long room = (long)a.ldt << a.page_log2, after = (long)n + count;
   bool no = after > room || end > a.m;
-  int want = 0;
-  if (pages && !no) want = max((int)((after + (1 << a.page_log2) - 1) >> a.page_log2) - h, 0);
-  int all;
-  const int upto = block_scan(want, red, &all);
-  no = no || (want > 0 && upto > avail);
-  const int take = no ? 0 : want;
-  int taken;
-  const int base = block_scan(take, red, &taken) - take;  // (= upto - want: those refused come after)
-  // (block_scan's barriers lie between the pages' way back and their way out)
-  at[i] = base, from[i] = h;
-  __syncthreads();
-  for (int e = i; e < taken; e += kPlanThreads) {
-    const int s = range_of(at, a.b, e);
-    a.table[(size_t)s * a.ldt + from[s] + e - at[s]] = a.free_pages[avail - 1 - e];
+  int want = 0, taken = 0;
+  if (pages) {
+    if (!no) want = max((int)((after + (1 << a.page_log2) - 1) >> a.page_log2) - h, 0);
+    int all;
+    const int upto = block_scan<kWaves>(want, red[2], &all);  // (its barrier: the pages given back are in the list)
+    if (all) {
+      at[i] = upto - want, from[i] = h;
+      no = no || (want > 0 && upto > avail);
+      if (no)
+        want = 0;
+      else if (want)
+        atomicMax(&granted, upto);  // (those refused for want of pages come after)
+      __syncthreads();
+      taken = granted;
+      for (int e = i; e < taken; e += THREADS) {
+        const int s = range_of(at, a.b, e);
+        a.table[(size_t)s * a.ldt + from[s] + e - at[s]] = a.free_pages[avail - 1 - e];
+      }
+    }
   }
   if (mine) {
     a.lens[i] = (int)(no ? n : after);
     a.refused[i] = no;
     a.qstart[i] = min(start, a.m);
-    if (pages) a.held_out[i] = h + take;
+    if (pages) a.held_out[i] = h + want;
   }
   if (i == 0) {
     a.qstart[a.b] = min(total, a.m);
@@ -121,12 +142,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_seqs_kernel(const PlanArgs 
   }
   if (!tokens_too) return;
   __syncthreads();
-  at[i] = min(start, a.m), to[i] = no ? -1 : n;
+  at[i] = min(start, a.m), from[i] = no ? -1 : n;
   __syncthreads();
-  for (int t = i; t < a.m; t += kPlanThreads) {
+  for (int t = i; t < a.m; t += THREADS) {
     const int s = a.b ? range_of(at, a.b, t) : 0;
-    const bool there = t < total && to[s] >= 0;
-    put_token(a, t, s, at[s], there ? to[s] + t - at[s] : -1);
+    const bool there = t < total && from[s] >= 0;
+    put_token(a, t, s, at[s], there ? from[s] + t - at[s] : -1);
   }
 }
 
@@ -160,7 +181,10 @@ extern "C" int ak_kv_plan(int b, int m, const int* counts, const int* drop, cons
                         slots, refused, b, m, npages, __builtin_ctz((unsigned)page), ldt};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool one = m <= agq::kTokensInOne;
-  hipLaunchKernelGGL(agq::plan_seqs_kernel, dim3(1), dim3(agq::kPlanThreads), 0, s, a, one ? 1 : 0);
+  if (b <= 64 && (!one || m <= 4 * agq::kFewThreads))  // barriers of four waves, but fewer pages and tokens at a time
+    hipLaunchKernelGGL(agq::plan_seqs_kernel<agq::kFewThreads>, dim3(1), dim3(agq::kFewThreads), 0, s, a, one ? 1 : 0);
+  else
+    hipLaunchKernelGGL(agq::plan_seqs_kernel<agq::kPlanThreads>, dim3(1), dim3(agq::kPlanThreads), 0, s, a, one ? 1 : 0);
   if (const int e = (int)hipGetLastError()) return e;
   if (one) return 0;
   hipLaunchKernelGGL(agq::plan_tokens_kernel, dim3((unsigned)(m + 255) / 256), dim3(256), 0, s, a);

@@ -63,13 +63,20 @@ __device__ __forceinline__ double2 turn(int pos, double f) {
   return make_double2(quarter == 1 || quarter == 2 ? -u : u, quarter & 2 ? -v : v);
 }
 
-// 64 bits -> the nearest bf16.  The step over 32 bits keeps as its last bit whether anything was cut off, so the second
-// rounding sees the side of a border that the value is on.
-__device__ __forceinline__ uint32_t d2bf(double d) {
+// 64 bits -> 32 on the way to bf16: the last bit kept says whether anything was cut off, so the rounding that follows sees the
+// side of a border that the value is on.
+__device__ __forceinline__ float narrow(double d) {
   const uint64_t u = (uint64_t)__double_as_longlong(d);
   uint32_t lo = (uint32_t)u;
   lo = (lo & 0xE0000000u) | ((lo & 0x1FFFFFFFu) ? 0x20000000u : 0u);
-  return f2bf((float)__longlong_as_double((long long)((u & 0xFFFFFFFF00000000ull) | lo)));
+  return (float)__longlong_as_double((long long)((u & 0xFFFFFFFF00000000ull) | lo));
+}
+// two values as bf16, rounded to nearest even
+__device__ __forceinline__ uint32_t two_bf16(double x, double y) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 f = {narrow(x), narrow(y)};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
 }
 
 __device__ __forceinline__ uint32_t value(const uint4& x, int i) {
@@ -84,41 +91,63 @@ __device__ __forceinline__ int spot(int j, int pairs) {
 }
 __host__ __device__ inline int spots(int pairs) { return (pairs + 7) / 8 * 8; }
 
-// The lane's 8 values of a row, rotated.  LAYOUT: 0 halves with rot % 16 == 0, 1 halves, 2 neighbours.
+// The lane's 8 values of a row, and those that they are paired with.  LAYOUT: 0 halves with rot % 16 == 0, 1 halves, 2
+// neighbours.
+struct Piece {
+  uint4 x, other;
+};
 template <int LAYOUT>
-__device__ __forceinline__ uint4 rotated(const RopeArgs& a, const uint16_t* row, int lane, const double2* cs) {
-  uint4 x = *reinterpret_cast<const uint4*>(row + 8 * lane);
+__device__ __forceinline__ Piece load_piece(const RopeArgs& a, const uint16_t* row, int lane) {
+  Piece p;
+  p.x = *reinterpret_cast<const uint4*>(row + 8 * lane);
+  p.other = p.x;
   const int at = 8 * lane, half = a.rot / 2;
-  if (at >= a.rot) return x;
-  uint32_t out[8];
-  if constexpr (LAYOUT == 2) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double u = bf2f(value(x, 2 * i)), v = bf2f(value(x, 2 * i + 1));
-      const double2 t = cs[spot<4>(min(at / 2 + i, half - 1), half)];
-      out[2 * i] = d2bf(__builtin_fma(u, t.x, -(v * t.y)));
-      out[2 * i + 1] = d2bf(__builtin_fma(v, t.x, u * t.y));
-    }
+  if (LAYOUT == 2 || at >= a.rot) return p;
+  if constexpr (LAYOUT == 0) {
+    p.other = *reinterpret_cast<const uint4*>(row + (at < half ? at + half : at - half));
   } else {
-    uint4 o = x;
-    if constexpr (LAYOUT == 0) o = *reinterpret_cast<const uint4*>(row + (at < half ? at + half : at - half));
+    uint32_t o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = min(at + i, a.rot - 1);
-      const bool low = e < half;
-      const int j = low ? e : e - half;
-      const uint32_t other = LAYOUT == 0 ? value(o, i) : row[low ? e + half : j];
-      const double u = bf2f(value(x, i)), v = bf2f(other);
-      const double2 t = cs[spot<8>(j, half)];
-      out[i] = d2bf(__builtin_fma(u, t.x, low ? -(v * t.y) : v * t.y));
+      o[i] = row[e < half ? e + half : e - half];
     }
+    p.other = make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[4] | o[5] << 16, o[6] | o[7] << 16);
+  }
+  return p;
+}
+template <int LAYOUT>
+__device__ __forceinline__ uint4 rotated(const RopeArgs& a, const Piece& p, int lane, const double2* cs) {
+  const int at = 8 * lane, half = a.rot / 2;
+  if (at >= a.rot) return p.x;
+  uint32_t out[4];
+  if constexpr (LAYOUT == 2) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double u = bf2f(value(p.x, 2 * i)), v = bf2f(value(p.x, 2 * i + 1));
+      const double2 t = cs[spot<4>(min(at / 2 + i, half - 1), half)];
+      out[i] = two_bf16(__builtin_fma(u, t.x, -(v * t.y)), __builtin_fma(v, t.x, u * t.y));
+    }
+  } else {
+    double r[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = LAYOUT == 0 ? at + i : min(at + i, a.rot - 1);
+      const bool low = LAYOUT == 0 ? at < half : e < half;
+      const double u = bf2f(value(p.x, i)), v = bf2f(value(p.other, i));
+      const double2 t = cs[LAYOUT == 0 ? i * (half / 8) + (low ? at : at - half) / 8 : spot<8>(low ? e : e - half, half)];
+      r[i] = __builtin_fma(u, t.x, low ? -(v * t.y) : v * t.y);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = two_bf16(r[2 * i], r[2 * i + 1]);
   }
   if constexpr (LAYOUT != 0) {  // a lane across rot's end
+    const uint32_t x[4] = {p.x.x, p.x.y, p.x.z, p.x.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (at + i >= a.rot) out[i] = value(x, i);
+    for (int i = 0; i < 4; ++i)
+      if (at + 2 * i >= a.rot) out[i] = x[i];  // (rot is even)
   }
-  return make_uint4(out[0] | out[1] << 16, out[2] | out[3] << 16, out[4] | out[5] << 16, out[6] | out[7] << 16);
+  return make_uint4(out[0], out[1], out[2], out[3]);
 }
 
 // One row of keys or values (part 0 or 1) into its slot.
@@ -139,33 +168,56 @@ __device__ __forceinline__ void store_row(const RopeArgs& a, const uint4 x, int 
   }
 }
 
-// BITS 0: heads of q alone.  Otherwise heads of q, then keys, then values of every token.
+// BITS 0: heads of q alone.  Otherwise heads of q, then keys, then values of every token; grid y: `each` of these rows.
 template <int BITS, int D, int LAYOUT>
-__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a, int lanes_log2) {
+__global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeArgs a, int lanes_log2, int each) {
   extern __shared__ double2 cs[];  // [tokens][spots(rot / 2)]
   const int first = blockIdx.x * a.tokens, n = min(a.tokens, a.m - first), half = a.rot / 2, per = spots(half);
-  for (int e = threadIdx.x; e < n * half; e += kRopeThreads) {
-    const int t = e / half, j = e - t * half;
+  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), groups = kRopeThreads >> lanes_log2;
+  const int row0 = blockIdx.y * each, rows = min(each, (BITS ? a.heads + 2 * a.s.heads : a.heads) - row0);
+  struct Item {
+    int t, h, pos, slot;
+    Piece p;
+  };
+  // the e-th of the workgroup's rows: of q where h < a.heads, then keys, values.  Nothing to do: pos < 0.
+  auto load = [&](int e) {
+    Item x;
+    const int lt = e / rows;
+    x.t = first + min(lt, n - 1), x.h = row0 + e - lt * rows, x.slot = 0;
+    x.pos = lt < n && 8 * lane < a.dim ? a.pos[x.t] : -1;
+    if (x.pos < 0) return x;
+    const size_t off = (size_t)x.h * a.dim;
+    if (BITS == 0 || x.h < a.heads) {
+      x.p = load_piece<LAYOUT>(a, a.q + x.t * a.ldq + off, lane);
+    } else {
+      const int kh = x.h - a.heads;
+      x.slot = a.slots[x.t];
+      if (kh < a.s.heads)
+        x.p = load_piece<LAYOUT>(a, a.k + x.t * a.ldk + (size_t)kh * D, lane);
+      else
+        x.p.x = *reinterpret_cast<const uint4*>(a.v + x.t * a.ldv + (size_t)(kh - a.s.heads) * D + 8 * lane);
+    }
+    return x;
+  };
+  int e = threadIdx.x >> lanes_log2;
+  Item x = load(e);  // (on its way while the sines and cosines are worked out)
+  for (int i = threadIdx.x; i < n * half; i += kRopeThreads) {
+    const int t = i / half, j = i - t * half;
     const double2 v = turn(max(a.pos[first + t], 0), a.freqs[j]);
     cs[t * per + (LAYOUT == 2 ? spot<4>(j, half) : spot<8>(j, half))] = make_double2(v.x * a.mag, v.y * a.mag);
   }
   __syncthreads();
-  const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), groups = kRopeThreads >> lanes_log2;
-  const int rows = BITS ? a.heads + 2 * a.s.heads : a.heads;
-  for (int e = threadIdx.x >> lanes_log2; e < n * rows; e += groups) {
-    const int lt = e / rows, h = e - lt * rows, t = first + lt;
-    if (a.pos[t] < 0 || 8 * lane >= a.dim) continue;
-    const double2* const c = cs + lt * per;
-    if (h < a.heads) {
-      const size_t off = (size_t)h * a.dim;
-      const uint4 r = rotated<LAYOUT>(a, a.q + t * a.ldq + off, lane, c);
-      *reinterpret_cast<uint4*>(a.y + t * a.ldy + off + 8 * lane) = r;
+  for (; e < n * rows; e += groups) {
+    const Item now = x;
+    if (e + groups < n * rows) x = load(e + groups);
+    if (now.pos < 0) continue;
+    const double2* const c = cs + (now.t - first) * per;
+    if (BITS == 0 || now.h < a.heads) {
+      *reinterpret_cast<uint4*>(a.y + now.t * a.ldy + (size_t)now.h * a.dim + 8 * lane) = rotated<LAYOUT>(a, now.p, lane, c);
     } else if constexpr (BITS != 0) {
-      const int slot = a.slots[t], part = h >= a.heads + a.s.heads, kh = h - a.heads - (part ? a.s.heads : 0);
-      if (slot < 0 || slot >> a.page_log2 >= a.s.npages) continue;  // (whole groups of lanes)
-      const uint4 x = part ? *reinterpret_cast<const uint4*>(a.v + t * a.ldv + (size_t)kh * D + 8 * lane)
-                           : rotated<LAYOUT>(a, a.k + t * a.ldk + (size_t)kh * D, lane, c);
-      store_row<BITS, D>(a, x, slot, kh, part, lane);
+      const int kh = now.h - a.heads, part = kh >= a.s.heads;
+      if (now.slot < 0 || now.slot >> a.page_log2 >= a.s.npages) continue;  // (whole groups of lanes)
+      store_row<BITS, D>(a, part ? now.p.x : rotated<LAYOUT>(a, now.p, lane, c), now.slot, part ? kh - a.s.heads : kh, part, lane);
     }
   }
 }
@@ -176,16 +228,25 @@ int launch(RopeArgs a, hipStream_t s) {
   while ((8 << lanes_log2) < a.dim) ++lanes_log2;
   const int rows = BITS ? a.heads + 2 * a.s.heads : a.heads;
   // tokens of a workgroup: three rounds of its lanes, while their sines and cosines fit 16 KB
-  const int per = spots(a.rot / 2) * 16;
-  int tokens = 3 * (kRopeThreads >> lanes_log2) / rows;
+  const int per = spots(a.rot / 2) * 16, groups = kRopeThreads >> lanes_log2;
+  int tokens = 3 * groups / rows;
   tokens = tokens < 1 ? 1 : tokens;
   while (tokens > 1 && tokens * per > 16384) --tokens;
+  // few tokens: one round, their sines and cosines worked out by several workgroups (one token of 48 heads 4.6 -> 3.4 us, 48 of
+  // 56 6.7 -> 4.5)
+  int each = rows;
+  if ((long)(a.m - 1) / tokens + 1 < 512) {
+    tokens = groups / rows < 1 ? 1 : groups / rows;
+    while (tokens > 1 && tokens * per > 16384) --tokens;
+    if (rows > groups) each = groups;
+  }
   a.tokens = tokens;
   const int m = a.m, most = (1 << 23) * (tokens < 64 ? tokens : 64);  // of a launch: its lanes are counted in 32 bits
   for (int t = 0; t < m; t += a.m) {
     a.m = m - t < most ? m - t : most;
-    hipLaunchKernelGGL((rope_kernel<BITS, D, LAYOUT>), dim3((unsigned)((a.m - 1) / tokens + 1)), dim3(kRopeThreads),
-                       (size_t)tokens * per, s, a, lanes_log2);
+    hipLaunchKernelGGL((rope_kernel<BITS, D, LAYOUT>),
+                       dim3((unsigned)((a.m - 1) / tokens + 1), (unsigned)((rows - 1) / each + 1)), dim3(kRopeThreads),
+                       (size_t)tokens * per, s, a, lanes_log2, each);
     if (const int e = (int)hipGetLastError()) return e;
     a.q += a.m * a.ldq, a.k += a.m * a.ldk, a.v += a.m * a.ldv, a.y += a.m * a.ldy, a.pos += a.m;
     if (BITS) a.slots += a.m;
