@@ -17,12 +17,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64, kChunk = 512, kGroup = 4;
-constexpr int kPlanThreads = 1024;
 
 struct Tile {
-  int adapter, start, count, pad;  // adapter -1: tokens without one
+  int adapter, count;  // adapter -1: tokens without one
 };
-// A plan's memory: this, tiles, the tokens in the tiles' order, then the products' parts.
+// A plan's memory: this, tiles, kTile places for each one's tokens, then the products' parts.  (Places of their own: the tokens are
+// loaded beside the tile, not after it.)
 struct PlanHead {
   int m, adapters, tiles, pad;
 };
@@ -38,10 +38,10 @@ __host__ __device__ inline int max_tiles(int m, int adapters) {
 }
 __host__ __device__ inline size_t tiles_at() { return sizeof(PlanHead); }
 __host__ __device__ inline size_t order_at(int m, int adapters) {
-  return tiles_at() + (size_t)max_tiles(m, adapters) * sizeof(Tile);
+  return (tiles_at() + (size_t)max_tiles(m, adapters) * sizeof(Tile) + 127) & ~(size_t)127;
 }
 __host__ __device__ inline size_t parts_at(int m, int adapters) {
-  return (order_at(m, adapters) + (size_t)m * 4 + 127) & ~(size_t)127;
+  return order_at(m, adapters) + (size_t)max_tiles(m, adapters) * kTile * 4;
 }
 __host__ __device__ inline PlanView view(void* plan, int m, int adapters) {
   uint8_t* const p = static_cast<uint8_t*>(plan);
@@ -69,49 +69,49 @@ __device__ __forceinline__ int next_place(int* n, int key, bool in) {
 // Counts the adapters' tokens, gives each adapter its places and tiles, then the tokens their places.  Up to kPlanEach tokens a
 // thread keep the place among their adapter's that the count gave them.
 constexpr int kPlanEach = 4;  // tokens of a thread at a time
-__global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int* ids, int m, int adapters, void* plan) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) lora_plan_kernel(const int* ids, int m, int adapters, void* plan) {
   extern __shared__ int n[];  // [adapters + 1] counts, then the next free places
-  __shared__ int red[2][kPlanThreads / 64], base[2];
+  __shared__ int red[THREADS / 64], base;
   const PlanView p = view(plan, m, adapters);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int key[kPlanEach], place[kPlanEach];
-  const bool once = m <= kPlanEach * kPlanThreads;
+  const bool once = m <= kPlanEach * THREADS;
   auto load = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i) {
-      const int t = t0 + tid + i * kPlanThreads;
+      const int t = t0 + tid + i * THREADS;
       key[i] = t < m ? adapter_of(ids, t, adapters) : -1;
     }
   };
   load(0);
-  for (int i = tid; i <= adapters; i += kPlanThreads) n[i] = 0;
-  if (tid == 0) base[0] = base[1] = 0;
+  for (int i = tid; i <= adapters; i += THREADS) n[i] = 0;
+  if (tid == 0) base = 0;
   __syncthreads();
-  for (int t0 = 0; t0 < m; t0 += kPlanEach * kPlanThreads) {
+  for (int t0 = 0; t0 < m; t0 += kPlanEach * THREADS) {
     if (t0) load(t0);
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i) place[i] = next_place(n, key[i], key[i] >= 0);
   }
   __syncthreads();
-  for (int i0 = 0; i0 <= adapters; i0 += kPlanThreads) {
+  for (int i0 = 0; i0 <= adapters; i0 += THREADS) {
     const int i = i0 + tid, count = i <= adapters ? n[i] : 0, tiles = (count + kTile - 1) / kTile;
-    int x = count, y = tiles;
+    int y = tiles;
     for (int d = 1; d < 64; d *= 2) {
-      const int u = __shfl_up(x, d), v = __shfl_up(y, d);
-      if (lane >= d) x += u, y += v;
+      const int v = __shfl_up(y, d);
+      if (lane >= d) y += v;
     }
-    if (lane == 63) red[0][w] = x, red[1][w] = y;
+    if (lane == 63) red[w] = y;
     __syncthreads();
-    int at = base[0] + x - count, tile = base[1] + y - tiles;
-    for (int j = 0; j < w; ++j) at += red[0][j], tile += red[1][j];
-    for (int j = 0; j < tiles; ++j)
-      p.tiles[tile + j] = Tile{i < adapters ? i : -1, at + j * kTile, min(kTile, count - j * kTile), 0};
-    if (i <= adapters) n[i] = at;
+    int tile = base + y - tiles;
+    for (int j = 0; j < w; ++j) tile += red[j];
+    for (int j = 0; j < tiles; ++j) p.tiles[tile + j] = Tile{i < adapters ? i : -1, min(kTile, count - j * kTile)};
+    if (i <= adapters) n[i] = tile * kTile;
     __syncthreads();
-    if (tid == kPlanThreads - 1) base[0] = at + count, base[1] = tile + tiles;
+    if (tid == THREADS - 1) base = tile + tiles;
     __syncthreads();
   }
-  for (int t0 = 0; t0 < m; t0 += kPlanEach * kPlanThreads) {
+  for (int t0 = 0; t0 < m; t0 += kPlanEach * THREADS) {
     if (!once) load(t0);
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i) {
@@ -119,10 +119,10 @@ __global__ void __launch_bounds__(kPlanThreads) lora_plan_kernel(const int* ids,
         place[i] = next_place(n, key[i], key[i] >= 0);
       else if (key[i] >= 0)
         place[i] += n[key[i]];
-      if (key[i] >= 0) p.order[place[i]] = t0 + tid + i * kPlanThreads;
+      if (key[i] >= 0) p.order[place[i]] = t0 + tid + i * THREADS;
     }
   }
-  if (tid == 0) *p.head = PlanHead{m, adapters, base[1], 0};
+  if (tid == 0) *p.head = PlanHead{m, adapters, base, 0};
 }
 
 struct LoraArgs {
@@ -153,8 +153,10 @@ __device__ __forceinline__ Tile tile_of(const PlanView& p, const LoraArgs& a, in
   if (head.m != a.m || head.adapters != a.adapters || i >= head.tiles) t.count = 0;
   return t;
 }
-// The token in place i of a tile, the last one's for places past it.
-__device__ __forceinline__ int token_of(const PlanView& p, const Tile& t, int i) { return p.order[t.start + min(i, t.count - 1)]; }
+// The token in place i of a tile; any token's where the tile has none.
+__device__ __forceinline__ int token_of(const PlanView& p, const LoraArgs& a, int tile, int i) {
+  return (int)min((unsigned)p.order[tile * kTile + i], (unsigned)a.m - 1);
+}
 
 // Few tokens: a workgroup takes 16 tokens of a tile (grid x), a group of chunks (y) and 16 ranks (z), a wave a chunk, all of whose
 // loads go out before its first product.  (z: the tiles' first sixteens before the second, which most tiles do not have.)
@@ -164,24 +166,25 @@ __global__ void __launch_bounds__(64 * kGroup) lora_down_few_kernel(const LoraAr
   const PlanView p = view(a.plan, a.m, a.adapters);
   const Tile t = tile_of(p, a, blockIdx.x);
   const int blocks = (a.ranks + 15) / 16, sub = blockIdx.z / blocks, r0 = (blockIdx.z - sub * blocks) * 16;
-  if (t.adapter < 0 || 16 * sub >= t.count) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
+  const int token = token_of(p, a, blockIdx.x, 16 * sub + col);
+  if (t.adapter < 0 || 16 * sub >= t.count) return;
+  const bool mine = 16 * sub + col < t.count;
   const int r = r0 + col, k0 = (blockIdx.y * kGroup + wave) * kChunk + 8 * quad;
   const uint16_t* const w = a.a + ((size_t)t.adapter * a.ranks + min(r, a.ranks - 1)) * a.k;
-  const int token = token_of(p, t, 16 * sub + col);
   const uint16_t* const x = a.x + token * a.ldx;
   uint4 av[kSteps], xv[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) av[i] = load_if(r < a.ranks && k0 + 32 * i < a.k, w + k0 + 32 * i);
 #pragma unroll
-  for (int i = 0; i < kSteps; ++i) xv[i] = load_if(k0 + 32 * i < a.k, x + k0 + 32 * i);
+  for (int i = 0; i < kSteps; ++i) xv[i] = load_if(mine && k0 + 32 * i < a.k, x + k0 + 32 * i);
   f32x4 acc = {};
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(av[i]), frag(xv[i]), acc, 0, 0, 0);
   sums[wave][lane] = acc;
   __syncthreads();
   const int row = r0 + 4 * quad, here = min((a.k - 1) / kChunk + 1 - (int)blockIdx.y * kGroup, kGroup);
-  if (wave || 16 * sub + col >= t.count || row >= a.ranks) return;
+  if (wave || !mine || row >= a.ranks) return;
   f32x4 part = {};
 #pragma unroll
   for (int j = 0; j < kGroup; ++j)
@@ -197,10 +200,10 @@ __global__ void __launch_bounds__(256, 2) lora_down_many_kernel(const LoraArgs a
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][16 * RT * kRow];
   const PlanView p = view(a.plan, a.m, a.adapters);
   const Tile t = tile_of(p, a, blockIdx.x);
-  if (t.adapter < 0 || t.count == 0) return;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4, sub = tid >> 6;
   const int r0 = blockIdx.z * 16 * RT;
-  const int token = token_of(p, t, 16 * sub + col);
+  const int token = token_of(p, a, blockIdx.x, 16 * sub + col);
+  if (t.adapter < 0 || t.count == 0) return;
   const uint16_t* const x = a.x + token * a.ldx;
   const bool mine = 16 * sub < t.count;
   const uint16_t* const w = a.a + (size_t)t.adapter * a.ranks * a.k;
@@ -334,7 +337,7 @@ __device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int se
 
 // Pieces [c0, c0 + width) of a tile's rows, eight in flight a thread.
 template <class T>
-__device__ __forceinline__ void copy_rows(const PlanView& p, const Tile& t, const void* from, void* to, int c0, int width, long ld) {
+__device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, const Tile& t, const void* from, void* to, int c0, int width, long ld) {
   const T* const src = static_cast<const T*>(from) + c0;
   T* const dst = static_cast<T*>(to) + c0;
   const int all = t.count * width;
@@ -344,7 +347,7 @@ __device__ __forceinline__ void copy_rows(const PlanView& p, const Tile& t, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = min(e0 + 256 * i, all - 1), row = e / width;
-      at[i] = token_of(p, t, row) * ld + (e - row * width);
+      at[i] = token_of(p, a, blockIdx.y, row) * ld + (e - row * width);
       v[i] = src[at[i]];
     }
 #pragma unroll
@@ -360,6 +363,10 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [hi, lo][kTile][rank + 8]
   const PlanView p = view(a.plan, a.m, a.adapters);
   const Tile t = tile_of(p, a, blockIdx.y);
+  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+  int tok[kTile / 16];
+#pragma unroll
+  for (int i = 0; i < kTile / 16; ++i) tok[i] = token_of(p, a, blockIdx.y, 16 * i + col);
   if (t.count == 0) return;
   int seg = 0;
   while (seg < a.nseg - 1 && (int)blockIdx.x >= a.end[seg]) ++seg;
@@ -370,13 +377,13 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   if (t.adapter < 0) {  // no products
     if (y0 != y) {
       if ((a.wide >> seg & 1) && (n1 - n0) % 8 == 0)
-        copy_rows<u32x4>(p, t, y0, y, n0 / 8, (n1 - n0) / 8, ldy / 8);
+        copy_rows<u32x4>(p, a, t, y0, y, n0 / 8, (n1 - n0) / 8, ldy / 8);
       else
-        copy_rows<uint16_t>(p, t, y0, y, n0, n1 - n0, ldy);
+        copy_rows<uint16_t>(p, a, t, y0, y, n0, n1 - n0, ldy);
     }
     return;
   }
-  const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, stride = a.rank + 8, subs = (t.count + 15) / 16;
+  const int stride = a.rank + 8, subs = (t.count + 15) / 16;
   const uint16_t* const w = a.b[seg] + (size_t)t.adapter * n * a.rank;
   // row of B for lane col of product i: the four products leave a lane 16 neighbouring outputs of a token
   auto load_b = [&](int wn, uint4(&bv)[KS][4]) {
@@ -392,9 +399,6 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   uint4 bv[KS][4];
   uint32_t v[kTile / 16][8];
   int wn = n0 + 64 * ((int)threadIdx.x >> 6);
-  int tok[kTile / 16];
-#pragma unroll
-  for (int i = 0; i < kTile / 16; ++i) tok[i] = token_of(p, t, 16 * i + col);
   const bool wide = a.wide >> seg & 1;
   auto load_y = [&](int wn) {
     const bool full = wide && wn + 64 <= n;
@@ -414,7 +418,7 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   const int fours = a.rank / 4;
   for (int e = threadIdx.x; e < 16 * subs * fours; e += 256) {  // 4 ranks of a token; kBatch of their parts at a time
     const int i = e / fours, r = 4 * (e - i * fours);
-    const float* const at = p.parts + (size_t)token_of(p, t, i) * a.ranks + seg * a.rank + r;
+    const float* const at = p.parts + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r;
     const f32x4 s = add_parts(at, a.parts, step);
     uint32_t hi[4], lo[4];
 #pragma unroll
@@ -467,8 +471,12 @@ extern "C" size_t ak_lora_plan_bytes(int m, int adapters, int ranks, int k) {
 
 extern "C" int ak_lora_plan(const int* ids, int m, int adapters, void* plan, void* stream) {
   if (!agq::sizes_ok(m, adapters) || !plan || (reinterpret_cast<uintptr_t>(plan) & 15) || (m && !ids)) return AK_INVALID;
-  hipLaunchKernelGGL(agq::lora_plan_kernel, dim3(1), dim3(agq::kPlanThreads), (size_t)(adapters + 1) * 4,
-                     static_cast<hipStream_t>(stream), ids, m, adapters, plan);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const size_t lds = (size_t)(adapters + 1) * 4;
+  if (m <= 256 && adapters < 256)  // barriers of four waves
+    hipLaunchKernelGGL(agq::lora_plan_kernel<256>, dim3(1), dim3(256), lds, s, ids, m, adapters, plan);
+  else
+    hipLaunchKernelGGL(agq::lora_plan_kernel<1024>, dim3(1), dim3(1024), lds, s, ids, m, adapters, plan);
   return (int)hipGetLastError();
 }
 
