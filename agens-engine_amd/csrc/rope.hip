@@ -102,10 +102,8 @@ __device__ __forceinline__ Piece load_piece(const RopeArgs& a, const uint16_t* r
   p.x = *reinterpret_cast<const uint4*>(row + 8 * lane);
   p.other = p.x;
   const int at = 8 * lane, half = a.rot / 2;
-  if (LAYOUT == 2 || at >= a.rot) return p;
-  if constexpr (LAYOUT == 0) {
-    p.other = *reinterpret_cast<const uint4*>(row + (at < half ? at + half : at - half));
-  } else {
+  if (LAYOUT != 1 || at >= a.rot) return p;
+  {
     uint32_t o[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -129,12 +127,17 @@ __device__ __forceinline__ uint4 rotated(const RopeArgs& a, const Piece& p, int 
       out[i] = two_bf16(__builtin_fma(u, t.x, -(v * t.y)), __builtin_fma(v, t.x, u * t.y));
     }
   } else {
+    uint4 other = p.other;
+    if constexpr (LAYOUT == 0) {  // from the lane that has it: loaded, it would come from L2 a second time
+      const int from = (int)(threadIdx.x & 63) + (at < half ? half / 8 : -half / 8);
+      other = make_uint4(__shfl(p.x.x, from), __shfl(p.x.y, from), __shfl(p.x.z, from), __shfl(p.x.w, from));
+    }
     double r[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int e = LAYOUT == 0 ? at + i : min(at + i, a.rot - 1);
       const bool low = LAYOUT == 0 ? at < half : e < half;
-      const double u = bf2f(value(p.x, i)), v = bf2f(value(p.other, i));
+      const double u = bf2f(value(p.x, i)), v = bf2f(value(other, i));
       const double2 t = cs[LAYOUT == 0 ? i * (half / 8) + (low ? at : at - half) / 8 : spot<8>(low ? e : e - half, half)];
       r[i] = __builtin_fma(u, t.x, low ? -(v * t.y) : v * t.y);
     }
