@@ -136,6 +136,7 @@ struct LoraArgs {
   long ldx;
   int m, adapters, k, rank, ranks, nseg;
   int parts;           // of the sums A x: one for each kGroup chunks
+  uint16_t* sums;      // these, behind the parts, or null: lora_up_kernel adds the parts up itself
   int rows, wide;      // output rows of a workgroup; bit i: segment i's rows of y and y0 are 16-byte aligned
 };
 
@@ -254,23 +255,57 @@ __global__ void __launch_bounds__(256, 2) lora_down_many_kernel(const LoraArgs a
   }
 }
 
-// Four sums: their parts from left to right, kBatch loads at a time.
-constexpr int kBatch = 8;
-__device__ __forceinline__ f32x4 add_parts(const float* at, int parts, size_t step) {
-  f32x4 s = {};
-  for (int c = 0; c < parts; c += kBatch) {
-    f32x4 x[kBatch];
+// N times four sums: their parts from left to right, kLoads loads at a time.
+constexpr int kLoads = 16;
+template <int N>
+__device__ __forceinline__ void add_parts(const float* const (&at)[N], int parts, size_t step, f32x4 (&s)[N]) {
+  constexpr int kAt = kLoads / N;
+  for (int c = 0; c < parts; c += kAt) {
+    f32x4 x[N][kAt];
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) x[j] = *reinterpret_cast<const f32x4*>(at + min(c + j, parts - 1) * step);
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (c + j < parts) s += x[j];
+      for (int j = 0; j < kAt; ++j) x[i][j] = *reinterpret_cast<const f32x4*>(at[i] + min(c + j, parts - 1) * step);
+#pragma unroll
+    for (int j = 0; j < kAt; ++j)
+      if (c + j < parts) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += x[i][j];
+      }
   }
-  return s;
 }
 
-// 16 outputs of a token, 8 from c on and 8 from c + 32 on: y = y0 + acc.  (A wave's 16-byte pieces of a token are neighbours:
-// with 16 outputs side by side in a lane no faster than 16 side by side, but fewer partial lines.)  WIDE: both 16-byte aligned and all within the row.
+// What fp32 holds of a sum in two bf16, to 16 bits (nothing in the second beside infinities and NaN).
+struct Halves {
+  uint32_t hi[2], lo[2];  // of four sums
+};
+__device__ __forceinline__ Halves halves(const f32x4 s) {
+  Halves h;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    h.hi[i] = f2bf2(s[2 * i], s[2 * i + 1]);
+    const float x = bf2f(h.hi[i] & 0xFFFFu), y = bf2f(h.hi[i] >> 16);
+    h.lo[i] = f2bf2(fabsf(x) < INFINITY ? s[2 * i] - x : 0.0f, fabsf(y) < INFINITY ? s[2 * i + 1] - y : 0.0f);
+  }
+  return h;
+}
+
+// The sums of every token from their parts: [token][first halves, second halves][ranks].
+__global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs a) {
+  const PlanView p = view(a.plan, a.m, a.adapters);
+  const size_t fours = a.ranks / 4, i = (size_t)blockIdx.x * 256 + threadIdx.x, token = i / fours, r = 4 * (i - token * fours);
+  if (token >= (size_t)a.m) return;
+  const float* const at[1] = {p.parts + token * a.ranks + r};
+  f32x4 s[1] = {};
+  add_parts(at, a.parts, (size_t)a.m * a.ranks, s);
+  const Halves h = halves(s[0]);
+  uint16_t* const out = a.sums + token * 2 * a.ranks + r;
+  *reinterpret_cast<uint2*>(out) = make_uint2(h.hi[0], h.hi[1]);
+  *reinterpret_cast<uint2*>(out + a.ranks) = make_uint2(h.lo[0], h.lo[1]);
+}
+
+// 16 outputs of a token, 8 from c on and 8 from c + 32 on: y = y0 + scale acc.  WIDE: both rows 16-byte aligned, all 64 outputs
+// of the wave within them.
 template <bool WIDE>
 __device__ __forceinline__ void load_out(const uint16_t* y0, int c, int n, uint32_t (&v)[8]) {
 #pragma unroll
@@ -288,12 +323,11 @@ __device__ __forceinline__ void load_out(const uint16_t* y0, int c, int n, uint3
   }
 }
 template <bool WIDE>
-__device__ __forceinline__ void store_out(uint16_t* y, int c, int n, const uint32_t (&v)[8], const f32x4 (&acc)[4]) {
+__device__ __forceinline__ void store_out(uint16_t* y, int c, int n, float scale, const uint32_t (&v)[8], const f32x4 (&acc)[4]) {
   uint32_t o[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    o[i] = (uint32_t)f2bf(bf2f(v[i] & 0xFFFFu) + acc[i / 2][2 * (i & 1)]) |
-           (uint32_t)f2bf(bf2f(v[i] >> 16) + acc[i / 2][2 * (i & 1) + 1]) << 16;
+    o[i] = f2bf2(bf2f(v[i] & 0xFFFFu) + scale * acc[i / 2][2 * (i & 1)], bf2f(v[i] >> 16) + scale * acc[i / 2][2 * (i & 1) + 1]);
 #pragma unroll
   for (int h = 0; h < 2; ++h, c += 32) {
     if constexpr (WIDE) {
@@ -306,10 +340,11 @@ __device__ __forceinline__ void store_out(uint16_t* y, int c, int n, const uint3
   }
 }
 
-// 64 output rows of a segment by one wave, for all tokens of a tile: KS steps of 32 ranks.  v: the outputs before.
-template <int KS, bool WIDE>
-__device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int seg, int wn, const uint16_t* sv, int stride,
-                                        const uint4 (&bv)[KS][4], const int (&tok)[kTile / 16], uint32_t (&v)[kTile / 16][8]) {
+// 64 output rows of a segment by one wave, for all tokens of a tile: KS steps of 32 ranks.  v: the outputs before; s(sub, lo, kk):
+// 8 halves of a token's sums.
+template <int KS, bool WIDE, class S>
+__device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int seg, int wn, float scale, S s,
+                                        const uint4 (&bv)[KS][4], const int (&tok)[kTile / 16], const uint32_t (&v)[kTile / 16][8]) {
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4, n = a.n[seg], c = wn + 8 * quad;
   uint16_t* const y = a.y[seg];
   const long ldy = a.ldy[seg];
@@ -318,20 +353,15 @@ __device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int se
     if (16 * sub >= t.count) break;
     f32x4 acc[4] = {};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int kk = 32 * s + 8 * quad;
-      uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-      if (kk < a.rank) {
-        hi = *reinterpret_cast<const uint4*>(sv + (16 * sub + col) * stride + kk);
-        lo = *reinterpret_cast<const uint4*>(sv + (kTile + 16 * sub + col) * stride + kk);
-      }
+    for (int k = 0; k < KS; ++k) {
+      const uint4 hi = s(sub, 0, 32 * k + 8 * quad), lo = s(sub, 1, 32 * k + 8 * quad);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[s][i]), frag(lo), acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[s][i]), frag(hi), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[k][i]), frag(lo), acc[i], 0, 0, 0);
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[k][i]), frag(hi), acc[i], 0, 0, 0);
       }
     }
-    if (16 * sub + col < t.count) store_out<WIDE>(y + tok[sub] * ldy, c, n, v[sub], acc);
+    if (16 * sub + col < t.count) store_out<WIDE>(y + tok[sub] * ldy, c, n, scale, v[sub], acc);
   }
 }
 
@@ -356,11 +386,12 @@ __device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, 
   }
 }
 
-// A workgroup: a tile's tokens (grid y) and a.rows output rows of a segment (x), 64 at a time a wave.
+// A workgroup: a tile's tokens (grid y) and a.rows output rows of a segment (x), 64 at a time a wave.  JOINED: the sums A x are
+// there; otherwise it adds up their parts, into LDS.
 constexpr int kUpRows = 256;
-template <int KS>
+template <int KS, bool JOINED>
 __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [hi, lo][kTile][rank + 8]
+  extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [halves][kTile][rank + 8]
   const PlanView p = view(a.plan, a.m, a.adapters);
   const Tile t = tile_of(p, a, blockIdx.y);
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
@@ -383,64 +414,60 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
     }
     return;
   }
-  const int stride = a.rank + 8, subs = (t.count + 15) / 16;
   const uint16_t* const w = a.b[seg] + (size_t)t.adapter * n * a.rank;
-  // row of B for lane col of product i: the four products leave a lane 16 neighbouring outputs of a token
-  auto load_b = [&](int wn, uint4(&bv)[KS][4]) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = wn + 32 * (i >> 1) + 8 * (col >> 2) + 4 * (i & 1) + (col & 3), kk = 32 * s + 8 * quad;
-        bv[s][i] = load_if(kk < a.rank && row < n, w + (size_t)row * a.rank + kk);
-      }
-  };
-  // the first rows' weights and outputs are on their way while the parts are added up
+  const bool wide = a.wide >> seg & 1;
   uint4 bv[KS][4];
   uint32_t v[kTile / 16][8];
-  int wn = n0 + 64 * ((int)threadIdx.x >> 6);
-  const bool wide = a.wide >> seg & 1;
-  auto load_y = [&](int wn) {
-    const bool full = wide && wn + 64 <= n;
+  auto load = [&](int wn) {
+    // row of B for lane col of product i: two products leave a lane 8 neighbouring outputs
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = wn + 32 * (i >> 1) + 8 * (col >> 2) + 4 * (i & 1) + (col & 3), kk = 32 * k + 8 * quad;
+        bv[k][i] = load_if(kk < a.rank && row < n, w + (size_t)row * a.rank + kk);
+      }
 #pragma unroll
     for (int i = 0; i < kTile / 16; ++i) {
       if (16 * i >= t.count) break;
-      if (full)
+      if (wide && wn + 64 <= n)
         load_out<true>(y0 + tok[i] * ldy, wn + 8 * quad, n, v[i]);
       else
         load_out<false>(y0 + tok[i] * ldy, wn + 8 * quad, n, v[i]);
     }
   };
-  load_b(wn, bv);
-  load_y(wn);
+  int wn = n0 + 64 * ((int)threadIdx.x >> 6);
+  load(wn);  // (on their way while the parts are added up)
   const float scale = a.scale ? a.scale[t.adapter] : 1.0f;
-  const size_t step = (size_t)a.m * a.ranks;
-  const int fours = a.rank / 4;
-  for (int e = threadIdx.x; e < 16 * subs * fours; e += 256) {  // 4 ranks of a token; kBatch of their parts at a time
-    const int i = e / fours, r = 4 * (e - i * fours);
-    const float* const at = p.parts + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r;
-    const f32x4 s = add_parts(at, a.parts, step);
-    uint32_t hi[4], lo[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f = i < t.count ? s[j] * scale : 0.0f;
-      hi[j] = f2bf(f);
-      lo[j] = (hi[j] & 0x7FFFu) < 0x7F80u ? f2bf(f - bf2f(hi[j])) : 0;  // (nothing beside infinities and NaN)
+  const int stride = a.rank + 8;
+  if constexpr (!JOINED) {
+    const size_t step = (size_t)a.m * a.ranks;
+    const int fours = a.rank / 4, subs = (t.count + 15) / 16;
+    for (int e = threadIdx.x; e < 16 * subs * fours; e += 256) {  // 4 ranks of a token
+      const int i = e / fours, r = 4 * (e - i * fours);
+      const float* const at[1] = {p.parts + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r};
+      f32x4 s[1] = {};
+      add_parts(at, a.parts, step, s);
+      if (i >= t.count) s[0] = f32x4{};
+      const Halves h = halves(s[0]);
+      *reinterpret_cast<uint2*>(sv + i * stride + r) = make_uint2(h.hi[0], h.hi[1]);
+      *reinterpret_cast<uint2*>(sv + (kTile + i) * stride + r) = make_uint2(h.lo[0], h.lo[1]);
     }
-    *reinterpret_cast<uint2*>(sv + i * stride + r) = make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
-    *reinterpret_cast<uint2*>(sv + (kTile + i) * stride + r) = make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+    __syncthreads();
   }
-  __syncthreads();
+  auto s = [&](int sub, int lo, int kk) {
+    if constexpr (JOINED)
+      return load_if(kk < a.rank, a.sums + (size_t)tok[sub] * 2 * a.ranks + lo * a.ranks + seg * a.rank + kk);
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (kk < a.rank) x = *reinterpret_cast<const uint4*>(sv + (lo * kTile + 16 * sub + col) * stride + kk);
+    return x;
+  };
   for (; wn < n1; wn += kUpRows) {
-    const bool full = wide && wn + 64 <= n;
-    if (wn >= n0 + kUpRows) {
-      load_b(wn, bv);
-      load_y(wn);
-    }
-    if (full)
-      up_rows<KS, true>(a, t, seg, wn, sv, stride, bv, tok, v);
+    if (wn >= n0 + kUpRows) load(wn);
+    if (wide && wn + 64 <= n)
+      up_rows<KS, true>(a, t, seg, wn, scale, s, bv, tok, v);
     else
-      up_rows<KS, false>(a, t, seg, wn, sv, stride, bv, tok, v);
+      up_rows<KS, false>(a, t, seg, wn, scale, s, bv, tok, v);
   }
 }
 
@@ -452,7 +479,10 @@ void down_many(const LoraArgs& l, unsigned tiles, hipStream_t s) {
 }
 template <int KS>
 void up(const LoraArgs& l, unsigned blocks, unsigned tiles, hipStream_t s) {
-  hipLaunchKernelGGL(lora_up_kernel<KS>, dim3(blocks, tiles), dim3(256), (size_t)2 * kTile * (l.rank + 8) * 2, s, l);
+  if (l.sums)
+    hipLaunchKernelGGL((lora_up_kernel<KS, true>), dim3(blocks, tiles), dim3(256), 0, s, l);
+  else
+    hipLaunchKernelGGL((lora_up_kernel<KS, false>), dim3(blocks, tiles), dim3(256), (size_t)2 * kTile * (l.rank + 8) * 2, s, l);
 }
 
 bool sizes_ok(int m, int adapters) {
@@ -466,7 +496,8 @@ extern "C" size_t ak_lora_plan_bytes(int m, int adapters, int ranks, int k) {
   if (!agq::sizes_ok(m, adapters) || ranks < 8 || ranks % 8 || ranks > AK_LORA_MAX_RANK * agq::kMaxSegs || k < 8 || k % 8 ||
       k > AK_LORA_MAX_INPUTS)
     return 0;
-  return agq::parts_at(m, adapters) + (size_t)((agq::chunks_of(k) - 1) / agq::kGroup + 1) * m * ranks * sizeof(float);
+  // (and the sums, once more)
+  return agq::parts_at(m, adapters) + (size_t)((agq::chunks_of(k) - 1) / agq::kGroup + 2) * m * ranks * sizeof(float);
 }
 
 extern "C" int ak_lora_plan(const int* ids, int m, int adapters, void* plan, void* stream) {
@@ -518,6 +549,13 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
   else
     agq::down_many<4>(l, tiles, s);
   if (const int e = (int)hipGetLastError()) return e;
+  // a launch more, but workgroups that read finished sums and need no LDS: 4001 tokens of 27648 inputs and 64 ranks 111 -> 104 us, 256
+  // 33 -> 31; of 5120 inputs and 16 ranks (3 parts) 54 -> 56
+  if (many && l.parts * l.rank >= 256) {
+    l.sums = reinterpret_cast<uint16_t*>(agq::view(plan, m, adapters).parts + (size_t)l.parts * m * l.ranks);
+    hipLaunchKernelGGL(agq::lora_join_kernel, dim3((unsigned)(((size_t)m * l.ranks / 4 - 1) / 256 + 1)), dim3(256), 0, s, l);
+    if (const int e = (int)hipGetLastError()) return e;
+  }
   // a workgroup adds up its tile's parts anew: more rows each where there are workgroups enough
   l.rows = agq::kUpRows;
   long rows = 0;

@@ -71,13 +71,7 @@ __device__ __forceinline__ float narrow(double d) {
   lo = (lo & 0xE0000000u) | ((lo & 0x1FFFFFFFu) ? 0x20000000u : 0u);
   return (float)__longlong_as_double((long long)((u & 0xFFFFFFFF00000000ull) | lo));
 }
-// two values as bf16, rounded to nearest even
-__device__ __forceinline__ uint32_t two_bf16(double x, double y) {
-  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f32x2 f = {narrow(x), narrow(y)};
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
-}
+__device__ __forceinline__ uint32_t two_bf16(double x, double y) { return f2bf2(narrow(x), narrow(y)); }
 
 __device__ __forceinline__ uint32_t value(const uint4& x, int i) {
   const uint32_t w = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;

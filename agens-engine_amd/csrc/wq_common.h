@@ -57,6 +57,14 @@ __device__ __forceinline__ uint16_t f2bf(float f) {
   return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
 }
 
+// two values as bf16, the first in the low half, rounded to nearest even by the hardware's conversion
+__device__ __forceinline__ uint32_t f2bf2(float x, float y) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 f = {x, y};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+}
+
 // segment of a global (padded, concatenated) row
 __device__ __forceinline__ int seg_of(const Segs& s, int grow) {
   int sg = 0;
