@@ -215,7 +215,7 @@ struct Shared {
   uint64_t kept[kMaxChunks];  // the chunks' weights above the border's key
   uint32_t equal[kMaxChunks]; // and their tokens with it
   uint64_t weight[kWindow + 2];  // of the window's keys; the last two are 0
-  uint32_t bins[kBins];
+  __attribute__((aligned(16))) uint32_t bins[kBins];
 };
 
 struct Row {
@@ -253,11 +253,28 @@ struct Bins {
   }
 };
 
+// The chunks' windows: in memory, or staged in LDS, where sh.bins has room for kStaged chunks' and nothing else is yet.
+constexpr int kStaged = kBins * 4 / (kWindow * 2);
+template <bool STAGED>
+struct Windows {
+  const uint32_t* memory;
+  const Shared& sh;
+  __device__ __forceinline__ uint32_t one(int c, int at) const {
+    const size_t i = (size_t)c * kWindow + at;
+    return STAGED ? reinterpret_cast<const uint16_t*>(sh.bins)[i] : reinterpret_cast<const uint16_t*>(memory)[i];
+  }
+  __device__ __forceinline__ uint32_t two(int c, int pair) const {
+    const size_t i = (size_t)c * (kWindow / 2) + pair;
+    return STAGED ? sh.bins[i] : memory[i];
+  }
+};
+
 // The thread's bin of the chunks' windows.
-__device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&first)[kLaneChunks]) {
+template <bool STAGED>
+__device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&first)[kLaneChunks], const Shared& sh) {
+  const Windows<STAGED> counts{r.counts, sh};
   constexpr int kAt = 40;  // loads in flight
   Bins<false> b{0};
-  const uint16_t* const counts = reinterpret_cast<const uint16_t*>(r.counts);
   for (int c0 = 0; c0 < r.chunks; c0 += kAt) {
     uint32_t v[kAt];
 #pragma unroll
@@ -268,7 +285,7 @@ __device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t
       for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
       const int at = (int)threadIdx.x - (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
       v[j] = 0;
-      if (at >= 0 && c0 + j < r.chunks) v[j] = counts[c * kWindow + at];
+      if (at >= 0 && c0 + j < r.chunks) v[j] = counts.one(c, at);
     }
 #pragma unroll
     for (int j = 0; j < kAt; ++j) b.n += v[j];
@@ -421,7 +438,9 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
 }
 
 // Each chunk's weights above the border's key and its tokens with it, to sh.kept and sh.equal: from the windows;
-__device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, const uint32_t (&first)[kLaneChunks], Shared& sh) {
+template <bool STAGED>
+__device__ __forceinline__ void window_masses(const Row& r, const Border& b, const uint32_t (&first)[kLaneChunks], Shared& sh) {
+  const Windows<STAGED> counts{r.counts, sh};
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   const uint32_t key = r.first - t;
   const float x = key_weight(r.s, key, r.top);
@@ -445,7 +464,7 @@ __device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, cons
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         pair[a][j] = 0;
-        if (128 * j <= last) pair[a][j] = r.counts[(size_t)c * (kWindow / 2) + 64 * j + lane];
+        if (128 * j <= last) pair[a][j] = counts.two(c, 64 * j + lane);
       }
     }
     uint64_t sum[kAt];
@@ -646,6 +665,18 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
   r.counts = a.counts ? a.counts + (size_t)id * a.chunks * (kWindow / 2) : nullptr;
   const int k = a.top_k ? a.top_k[id] : 0;
   const float p = a.top_p ? a.top_p[id] : 1.0f, least = a.min_p ? a.min_p[id] : 0.0f, u = a.u[id];
+  const int limit = k > 0 && k < a.vocab ? k : 0;
+  const bool filters = !r.s.greedy && (limit || p < 1.0f || least > 0.0f), staged = filters && r.counts && a.chunks <= kStaged;
+  if (staged) {  // beside the statistics
+    constexpr int kAt = kBins / 4 / kDraw;
+    const uint4* const src = reinterpret_cast<const uint4*>(r.counts);
+    const int all = a.chunks * (kWindow / 8);
+    uint4 v[kAt];
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) v[i] = src[min(t + i * kDraw, all - 1)];
+#pragma unroll
+    for (int i = 0; i < kAt; ++i) reinterpret_cast<uint4*>(sh.bins)[t + i * kDraw] = v[i];
+  }
   if (!a.stats) {
     for (int c0 = 0; c0 < a.chunks; c0 += kGroups) {
       const int c = c0 + t / kGroupThreads;
@@ -690,9 +721,8 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     if (t == 0) store(a, id, r, r.best);
     return;
   }
-  const int limit = k > 0 && k < a.vocab ? k : 0;
   Border b{0, 0, least > 0.0f ? fminf(least, 1.0f) : 0.0f};
-  if (!limit && !(p < 1.0f) && b.least == 0.0f) {  // no filter: the chunk from their own sums
+  if (!filters) {  // no filter: the chunk from their own sums
     double at = (double)u * r.total, before = 0.0, c = 0.0;
     int chunk = -1;
     bool past = false;
@@ -711,6 +741,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     draw_in(a, id, r, chunk, b, 0, fmax(at - before, 0.0), sh);
     return;
   }
+  if (staged) __syncthreads();
   bool quick = r.counts != nullptr;
   Bins<false> window{0};
   if (quick) {
@@ -719,14 +750,17 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     const bool cut = r.first < kWindow || key_weight(r.s, r.first - (kWindow - 1), r.top) < b.least;
     bool found = false;
     if (limit || p < 1.0f) {
-      window = count_window(r, first);
+      window = staged ? count_window<true>(r, first, sh) : count_window<false>(r, first, sh);
       found = find(r, window, limit, p, b, sh);
     }
     quick = found || (cut && !(limit && p < 1.0f));
     if (!found) b.key = 0, b.n = 0;
   }
   if (quick) {
-    chunk_masses(r, b, first, sh);
+    if (staged)
+      window_masses<true>(r, b, first, sh);
+    else
+      window_masses<false>(r, b, first, sh);
   } else {
     if (limit || p < 1.0f) {
       if (count_all(r, r.counts ? &window : nullptr, sh))
