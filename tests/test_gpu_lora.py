@@ -87,7 +87,8 @@ class Job:
 @pytest.mark.parametrize("m,adapters,rank,k,ns", [
     (1, 1, 8, 8, [1]), (1, 4, 16, 5120, [5120]), (2, 3, 24, 520, [17]), (17, 5, 64, 1000, [300, 33]), (64, 32, 16, 5120, [5120, 1024, 1024]),
     (100, 2, 128, 264, [257, 64, 1, 100]), (130, 1, 32, 4104, [64]), (333, 40, 8, 512, [129]), (700, 3, 48, 9000, [70]),
-    (5, 4096, 16, 64, [40]), (1500, 7, 16, 640, [2055])])
+    (5, 4096, 16, 64, [40]), (1500, 7, 16, 640, [2055]), (900, 3, 64, 9000, [70, 64]), (1000, 2, 128, 8200, [40]),
+    (3400, 5, 16, 520, [72])])
 def test_against_64_bits(m, adapters, rank, k, ns):
     j = Job(m + k, m, adapters, rank, k, ns, pad=m % 3)
     j.compare(j.run())
@@ -107,13 +108,14 @@ def test_groups_of_every_kind(ids, in_place):
     j.compare(j.run())
 
 
-def test_tokens_do_not_depend_on_the_call():
+@pytest.mark.parametrize("rank", [16, 64])
+def test_tokens_do_not_depend_on_the_call(rank):
     """Alone, in small batches and in large ones that take other launches: the same bits."""
     rng = np.random.default_rng(1)
-    big = Job(7, 2600, 3, 16, 9224, [96], ids=rng.integers(-1, 3, 2600))
+    big = Job(7, 2600, 3, rank, 9224, [96], ids=rng.integers(-1, 3, 2600))
     y = big.run()[0]
     for some in ([0], [5, 9], list(range(100, 140)), list(rng.integers(0, 2600, 300))):
-        j = Job(7, len(some), 3, 16, 9224, [96], ids=big.ids[some])
+        j = Job(7, len(some), 3, rank, 9224, [96], ids=big.ids[some])
         j.x, j.a, j.b, j.scale = big.x[some], big.a, big.b, big.scale
         j.X, j.A, j.B, j.S = Dev.of(j.x), big.A, big.B, big.S
         j.Z = [Dev.of(big.base[0][some])]
