@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS) plan_seqs_kernel(const PlanArgs a, in
   }
   const int avail = min(stack + total_back, a.npages);
   const long room = (long)a.ldt << a.page_log2, after = (long)n + count;
-  bool no = after > room || end > a.m;
+  bool no = after > room || after > 0x7FFFFFFF || end > a.m;
   int want = 0, taken = 0;
   if (pages) {
     if (!no) want = max((int)((after + (1 << a.page_log2) - 1) >> a.page_log2) - h, 0);

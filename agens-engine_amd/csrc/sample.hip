@@ -72,13 +72,14 @@ struct SampleArgs {
   float* logp;
   int b, vocab, chunks;
   ChunkStat* stats;  // [b][chunks]
-  uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys first_key - i
+  uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys from the chunk's largest down
 };
 
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // Keys of two logits: their bits, all inverted where the sign is set, else the sign alone.  -0 has a key of its own, kMinusZero,
 // which counts as kZero; NaN are above +inf's key or below -inf's, and never counted.
 __device__ __forceinline__ uint32_t two_keys(uint32_t bits) {
-  typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
   const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, bits) >> 15);
   return bits ^ (sign | 0x80008000u);
 }
@@ -90,9 +91,6 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
   return bf2f(key & 0x8000u ? key - 0x8000u : 0xFFFFu - key);
 }
 __device__ __forceinline__ uint32_t key_of_value(float l) { return key_of(__float_as_uint(l) >> 16); }
-// A window's first key: the largest, or the one above it, so that windows are shifted by whole pairs.
-__device__ __forceinline__ uint32_t first_key(float top) { return key_of_value(top) | 1u; }
-
 // in whole numbers of 2^-40
 __device__ __forceinline__ uint64_t units(float w) {
   const float x = w * kUnit, hi = __builtin_truncf(x * 0x1p-32f);
@@ -114,6 +112,12 @@ struct AddCounts {
     return x + dpp<CTRL, ROWS>(x, 0);
   }
 };
+struct MaxCounts {
+  template <int CTRL, int ROWS>
+  __device__ __forceinline__ uint32_t step(uint32_t x) const {
+    return max(x, dpp<CTRL, ROWS>(x, 0));
+  }
+};
 __device__ __forceinline__ uint64_t last_lane64(uint64_t x) {
   return (uint64_t)last_lane((uint32_t)(x >> 32)) << 32 | last_lane((uint32_t)x);
 }
@@ -122,6 +126,7 @@ __device__ __forceinline__ uint32_t counts_sum(uint32_t x) { return last_lane(wa
 
 // What kGroupThreads threads share over a chunk
 struct Group {
+  uint32_t high[kGroupThreads / 64];
   double red[kGroupThreads / 64];
   int best[kGroupThreads / 64];
 };
@@ -134,24 +139,28 @@ __device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* r
   float l[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) l[i] = value(v[i >> 3], i & 7);
-  float mine = l[0];
+  // the largest by its key, with what is above an infinity's, NaN, wrapped to the lowest (fmaxf loses what it has to a signalling
+  // NaN)
+  u16x2 keys = {0, 0};
 #pragma unroll
-  for (int i = 1; i < kEach; ++i) mine = fmaxf(mine, l[i]);
-  float top = wave_max(mine);
+  for (int i = 0; i < kEach / 2; ++i)
+    keys = __builtin_elementwise_max(keys, __builtin_bit_cast(u16x2, two_keys(v[i >> 2][i & 3])) + (uint16_t)kLowest);
+  uint32_t high = last_lane(wave_scan((uint32_t)max(keys.x, keys.y), MaxCounts()));
   __syncthreads();
-  if ((t & 63) == 0) g.red[w] = top;
+  if ((t & 63) == 0) g.high[w] = high;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kGroupThreads / 64; ++i) top = fmaxf(top, (float)g.red[i]);
+  for (int i = 0; i < kGroupThreads / 64; ++i) high = max(high, g.high[i]);
+  const float top = high <= 2 * kLowest ? -INFINITY : logit_of(high - kLowest);
   int best = 0x7FFFFFFF;
-  if (mine == top && top > -INFINITY) {
+  if (top > -INFINITY) {
 #pragma unroll
     for (int i = kEach - 1; i >= 0; --i)
       if (l[i] == top) best = (i < 8 ? at0 : at1 - 8) + i;
   }
   best = wave_min(best);
   if (bins && top > -INFINITY) {
-    const uint32_t first = first_key(top), span = min((uint32_t)kWindow + 1, first - kLowest);  // (-inf weighs nothing)
+    const uint32_t first = key_of_value(top), span = min((uint32_t)kWindow + 1, first - kLowest);  // (-inf weighs nothing)
 #pragma unroll
     for (int i = 0; i < kEach / 2; ++i) {
       const uint32_t keys = two_keys(v[i >> 2][i & 3]), d0 = first - (keys & 0xFFFFu), d1 = first - (keys >> 16);
@@ -189,7 +198,7 @@ __global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const Sample
   const size_t at = (size_t)id * a.chunks + chunk;
   if (t == 0) {
     a.stats[at] = r;
-    const uint32_t d = first_key(r.top) - kZero;  // the counts of -0
+    const uint32_t d = key_of_value(r.top) - kZero;  // the counts of -0
     if (r.top >= 0.0f && d < kWindow) bins[d] += bins[d + 1], bins[d + 1] = 0;
   }
   __syncthreads();
@@ -225,7 +234,7 @@ struct Row {
   float top;
   int best, vocab, chunks;
   double total;
-  uint32_t first;  // first_key(top)
+  uint32_t first;  // the key of top
   uint32_t least;  // the lowest key that weighs anything
   uint32_t low;    // the first key of the bins past zero's
   bool straight;   // or the bins go on below kSpan without a gap, and without a bin for zero alone
@@ -343,7 +352,7 @@ __device__ __forceinline__ bool zeros_in(const Row& r) {
 __device__ __forceinline__ bool count_all(Row& r, const Bins<false>* window, Shared& sh) {
   // what lies 31 T below the largest weighs less than 2^-44; a key less, since the value loses its low bits
   const float heat = fminf(fmaxf(r.s.heat, FLT_MIN), kMaxHeat);
-  r.least = r.top == INFINITY ? r.first - 1 : max((int)key_of_value(r.top - 31.0f * heat), (int)kLowest + 2) - 1;
+  r.least = r.top == INFINITY ? r.first : max((int)key_of_value(r.top - 31.0f * heat), (int)kLowest + 2) - 1;
   r.low = r.least + (kSpan - 2);
   r.straight = r.low + kSpan >= r.first;
   const uint32_t from = window ? kWindow : 0;
@@ -696,7 +705,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     if (lane + 64 * i < a.chunks) st[i] = stats[lane + 64 * i];
   }
 #pragma unroll
-  for (int i = 0; i < kLaneChunks; ++i) r.top = fmaxf(r.top, st[i].top), first[i] = first_key(st[i].top);
+  for (int i = 0; i < kLaneChunks; ++i) r.top = fmaxf(r.top, st[i].top), first[i] = key_of_value(st[i].top);
   r.top = wave_max(r.top);
   if (r.top == -INFINITY) {
     if (t == 0) {
@@ -716,7 +725,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
   for (int i = 0; i < kLaneChunks; ++i) total += share[i];
   r.total = wave_sum(total);
   r.best = wave_min(best);
-  r.first = first_key(r.top);
+  r.first = key_of_value(r.top);
   if (r.s.greedy) {
     if (t == 0) store(a, id, r, r.best);
     return;
@@ -738,7 +747,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
       }
       c += __shfl(upto, 63);
     }
-    draw_in(a, id, r, chunk, b, 0, fmax(at - before, 0.0), sh);
+    draw_in(a, id, r, max(chunk, 0), b, 0, fmax(at - before, 0.0), sh);  // (the largest has a weight: there is a chunk)
     return;
   }
   if (staged) __syncthreads();
@@ -807,7 +816,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
     }
     c += last_lane64(upto);
   }
-  draw_in(a, id, r, chunk, b, n, fmax(at - before, 0.0) * (1.0 / (double)kUnit), sh);
+  draw_in(a, id, r, max(chunk, 0), b, n, fmax(at - before, 0.0) * (1.0 / (double)kUnit), sh);
 }
 
 SampleArgs from(SampleArgs a, int row) {

@@ -310,7 +310,7 @@ int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, co
  * list, and these tokens' ranges, positions and slots.  Sequence i has cached[i] tokens in the cache, held[i] pages in
  * table[i * ldt ...], and counts[i] new tokens; drop[i] (drop may be NULL) other than 0: it has ended, its pages go to the end of
  * the free list, in order, and the row begins anew with counts[i] tokens.  Missing pages come off the end of the list, in the
- * order of the sequences.  A sequence that does not fit its ldt pages, or whose range passes m, is refused, as is one whose
+ * order of the sequences.  A sequence that does not fit its ldt pages (or 2^31 - 1 tokens), or whose range passes m, is refused, as is one whose
  * pages are not all there, and then every later one that wants any; it keeps what it had.  free_pages [npages] with
  * free_count[0] pages in it; NULL: the table's pages are taken as they are (held, held_out, free_count, free_out unused).
  *   lens [b]       cached and new tokens (refused: cached);       held_out [b], free_out [1]   as held and free_count, after;
@@ -335,7 +335,8 @@ int ak_kv_plan(int b, int m, const int* counts, const int* drop, const int* cach
  *   ak_rope   heads of x (token t at x + t * ldx, heads contiguous; 16-byte aligned, multiples of 8) to y, which may be x (with
  *             the same stride) but overlap it in no other way.  dim a multiple of 8 up to 512, heads up to 4096;
  *   ak_rope_kv_write   q to y likewise, the keys turned, and keys and values into slots (the paged cache's): what ak_rope of q,
- *             ak_rope of k and ak_kv_write leave, bit for bit, in one launch and without the turned keys' way through memory;
+ *             ak_rope of k and ak_kv_write leave, bit for bit, in one launch and without the turned keys' way through memory
+ *             (tokens with a negative position are not written either);
  *   ak_rope_freqs      host memory, no device: freqs[j] = theta^(-2j / rot) and *mag = 1, for contexts `factor` times the
  *             trained one: LINEAR divides all by factor; BASE takes theta * factor^(rot / (rot - 2)); BANDS divides those that
  *             make fewer than `slow` turns in `trained` tokens, leaves those of more than `fast`, mixes those between in
@@ -361,8 +362,8 @@ int ak_rope_kv_write(int bits, const void* q, long ldq, const void* k, long ldk,
  * (NULL, or 1 and more: off), min_p [b] (NULL, or 0 and less: off), u [b] uniform in [0, 1), all in device memory.
  * logp (may be NULL): log p of the token before any filter (greedy: at temperature 1).  NaN logits count as -inf; a row of
  * nothing else gives the token -1 and logp 0.  Without filters the tokens are ak_spec_verify's with t = 0, but for roundings.
- * Weights are fp32; sums of what filters keep count whole 2^-42 of the largest weight, so a token below that is not drawn.
- * Rows need no alignment beyond bf16's.  Library scratch (above; inside a capture the graph's own): 2064 bytes for each 16384
+ * Weights are fp32; sums of what filters keep count whole 2^-40 of the largest weight, so a token below that is not drawn where a filter is on.
+ * Rows need no alignment beyond bf16's.  Library scratch (above; inside a capture the graph's own): 1040 bytes for each 4096
  * logits, 64 MB at most; without it one workgroup takes a row, with the same tokens. */
 #define AK_SAMPLE_MAX_VOCAB 1048576
 int ak_sample(const void* logits, long ld, const float* temperature, const int* top_k, const float* top_p,

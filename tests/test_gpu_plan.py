@@ -146,6 +146,20 @@ def test_table_as_it_is(b, longest):
     same(g, w)
 
 
+def test_lengths_end_at_31_bits():
+    """Room for more than 2^31 tokens: a sequence that would pass them is refused, its neighbour is not."""
+    x = Batch(8, 2, 256, 8, 3, drops=0.0)
+    x.ldt = (1 << 23) + 5
+    x.cached, x.counts = np.array([2 ** 31 - 3, 2 ** 31 - 6]), np.array([3, 5])
+    x.table = np.zeros((2, x.ldt), dtype=np.int32)
+    x.m = 10
+    x.device()
+    check(x.call(drop=False, alloc=False))
+    g = x.got(alloc=False)
+    assert g["refused"].tolist() == [1, 0] and g["lens"].tolist() == [2 ** 31 - 3, 2 ** 31 - 1]
+    assert g["pos"][3:8].tolist() == [2 ** 31 - 6 + j for j in range(5)] and (g["pos"][:3] == -1).all()
+
+
 def test_no_sequences_and_no_tokens():
     x = Batch(3, 1, 16, 4, 0)
     x.m = 6

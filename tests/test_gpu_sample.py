@@ -215,6 +215,33 @@ def test_masked_infinite_and_empty_rows():
     assert tok[:4].tolist() == [-1, -1, 17, 100] and tok[6] == 0
 
 
+@pytest.mark.parametrize("nan", [0x7F81, 0x7FFF, 0xFF81, 0xFFFF])
+@pytest.mark.parametrize("top", [0x7F80, 0x7F7F, 0x4000])
+def test_nan_next_to_the_largest(nan, top):
+    """The bits of a NaN are neighbours of an infinity's: it is never counted, let alone drawn."""
+    rng = np.random.default_rng(21)
+    x = f2bf_array(rng.standard_normal(6 * 9000).astype(np.float32)).reshape(6, 9000)
+    x[:, 40::9] = nan
+    x[:, 4500] = top
+    r = Rows(x, 1.0, [1, 0, 3, 0, 8999, 0], [1.0, 0.4, 0.9, 1.0, 0.9999, 1.0], [0, 0, 0, 0.5, 0, 0], [0.0, 0.99, 0.5, 0.3, 0.7, 0.5])
+    tok, lp = r.run()
+    assert all(t < 40 or (t - 40) % 9 for t in tok)
+    if top != 0x4000:  # (2: others are larger)
+        assert (tok == 4500).all() and (lp == 0).all()
+    else:
+        r.compare((tok, lp), least=0.5)
+
+
+@pytest.mark.parametrize("u", [1.0, float("nan"), 2.0, -1.0])
+def test_numbers_that_are_none(u):
+    """u outside [0, 1): one of the tokens that are kept."""
+    rng = np.random.default_rng(22)
+    x = logits(rng, 3, 5000)
+    tok, _ = Rows(x, 1.0, [0, 10, 0], [1.0, 1.0, 0.5], None, u).run()
+    l = bf2f_array(x).astype(np.float64)
+    assert ((tok >= 0) & (tok < 5000)).all() and l[1, tok[1]] >= np.sort(l[1])[-10] and l[2, tok[2]] >= np.sort(l[2])[-2000]
+
+
 def test_settings_out_of_their_ranges():
     """NaN and what is beyond a filter's range: off, or the most it can do."""
     rng = np.random.default_rng(8)
