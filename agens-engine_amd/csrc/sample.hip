@@ -147,18 +147,20 @@ __device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* r
     keys = __builtin_elementwise_max(keys, __builtin_bit_cast(u16x2, two_keys(v[i >> 2][i & 3])) + (uint16_t)kLowest);
   uint32_t high = last_lane(wave_scan((uint32_t)max(keys.x, keys.y), MaxCounts()));
   __syncthreads();
+  const uint32_t mine = high;
   if ((t & 63) == 0) g.high[w] = high;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kGroupThreads / 64; ++i) high = max(high, g.high[i]);
   const float top = high <= 2 * kLowest ? -INFINITY : logit_of(high - kLowest);
   int best = 0x7FFFFFFF;
-  if (top > -INFINITY) {
+  // (whole waves; where it is 0, a wave with -0 alone has it too)
+  if (top > -INFINITY && (mine == high || top == 0.0f)) {
 #pragma unroll
     for (int i = kEach - 1; i >= 0; --i)
       if (l[i] == top) best = (i < 8 ? at0 : at1 - 8) + i;
+    best = wave_min(best);
   }
-  best = wave_min(best);
   if (bins && top > -INFINITY) {
     const uint32_t first = key_of_value(top), span = min((uint32_t)kWindow + 1, first - kLowest);  // (-inf weighs nothing)
 #pragma unroll
