@@ -7,8 +7,8 @@
 //
 // A logit has 16 bits, so equal ones are many and its bits, made to ascend with the value (`key`), index everything: a
 // histogram of a row's keys holds all counts, and all weights as counts times the weight of a key.  The weights enter sums as
-// whole numbers of 2^-40 of the largest (2^20 of them fit 64 bits, 2^12 a double's 53): sums are exact, in any order, so which way they were
-// reached does not show in the tokens.
+// whole numbers of 2^-40 of the largest (2^20 of them fit 64 bits, 2^12 a double's 53): sums are exact, in any
+// order, so which way they were reached does not show in the tokens.
 //
 //   sample_keys_kernel   a chunk of 4096 logits a workgroup, held in registers: its largest, its lowest token with that, the
 //                        sum of its weights (16 in 32 bits, then 64), and how often each of the kWindow keys up to its
@@ -16,10 +16,14 @@
 //   sample_draw_kernel   a row a workgroup: the chunks' windows, shifted to the row's largest key and summed, give the border of
 //                        what is kept (one scan of counts and weights serves top-k and top-p, since top-p's border is not
 //                        behind top-k's), and what each chunk has of it; then the chunk that the draw falls into is read again.
-//                        A window goes down to 2^-4 of a positive largest logit; where the border is below it, the row's
-//                        keys are counted anew, all at once, and the chunks' shares summed up in another pass.
-// Both wait: for loads, and for each other's barriers.  Without scratch sample_draw_kernel takes the chunks' statistics itself
-// and does without their windows: the same tokens.
+//                        A window goes down to 2^-4 of a positive largest logit.  Where the border is below it, a sample of the
+//                        row leaves few keys for it and one pass lists the logits with these (find_sampled); where that does not
+//                        do, the row's keys are counted anew, all at once, and the chunks' shares summed up in another pass.
+// Without scratch sample_draw_kernel takes the chunks' statistics itself and does without their windows: the same tokens.
+//
+// What bounds them: loads' and barriers' latency, one after another (1 row of 152064: 4.2 + 4.1 us without a filter; 32 rows: 5.7 +
+// 13.8 us, 9.7 MB at 7 TB/s would be 1.4), and instructions for rows whose border is far down: 25 a logit by one workgroup, 1 row of
+// 152064 52 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 62 us and 87.
 #include "agens_kernels.h"
 #include "logits.h"
 
@@ -34,7 +38,10 @@ constexpr int kWindow = 512;
 static_assert(kWindow == kDraw && kChunk == 8 * kDraw, "a bin of the window and eight logits of a chunk a thread");
 static_assert(kWindow == 2 * kGroupThreads, "two bins a thread");
 // Bins of all keys that matter: kSpan from the largest down, zero's, and the rest up from the least with any weight.
-constexpr int kSpan = 8192, kBins = 2 * kSpan, kBinsEach = kBins / kDraw;
+constexpr int kSpan = 4096, kBins = 2 * kSpan, kBinsEach = kBins / kDraw;
+// Where a sample narrows the border down: its logits and its bins, and how many logits a wave lists.
+constexpr int kSample = 16 * kDraw, kSampleBins = 4 * kDraw, kPiece = kChunk / 2, kList = 2048 - 64, kListed = kList - 512,
+              kPool = kBins + kWaves * (kList + 64) / 2;
 constexpr float kMaxHeat = 1.44e30f;  // (see heat_of)
 constexpr float kUnit = 0x1p40f;
 constexpr size_t kMaxScratch = (size_t)64 << 20;
@@ -223,10 +230,14 @@ struct Shared {
   Border border;
   uint64_t border_mass;  // in front of it, its own tokens included
   uint32_t between;
+  int after, upto;            // bins of a sample
+  float low[kWaves];
+  double square[kWaves];
+  uint16_t ends[2 * kMaxChunks];  // of the pieces' parts of their waves' lists
   uint64_t kept[kMaxChunks];  // the chunks' weights above the border's key
   uint32_t equal[kMaxChunks]; // and their tokens with it
   uint64_t weight[kWindow + 2];  // of the window's keys; the last two are 0
-  __attribute__((aligned(16))) uint32_t bins[kBins];
+  __attribute__((aligned(16))) uint32_t bins[kPool];  // (lists behind the bins)
 };
 
 struct Row {
@@ -242,7 +253,7 @@ struct Row {
   bool straight;   // or the bins go on below kSpan without a gap, and without a bin for zero alone
 };
 
-// Bins in order: two of the window a thread, or kBinsEach of all keys'.
+// Bins in order: one of the window a thread, or kBinsEach of all keys'.
 template <bool WIDE>
 struct Bins {
   static constexpr int kCount = WIDE ? kBinsEach : 1;
@@ -265,7 +276,7 @@ struct Bins {
 };
 
 // The chunks' windows: in memory, or staged in LDS, where sh.bins has room for kStaged chunks' and nothing else is yet.
-constexpr int kStaged = kBins * 4 / (kWindow * 2);
+constexpr int kStaged = kPool * 4 / (kWindow * 2);
 template <bool STAGED>
 struct Windows {
   const uint32_t* memory;
@@ -400,13 +411,16 @@ __device__ __forceinline__ Sums sum_bins(const Row& r, const Bins<WIDE>& b, Shar
   return s;
 }
 
-// The borders of top-k (k > 0) and top-p (p < 1) among bins that hold all in front of them.  False: these do not.
+// The borders of top-k (k > 0) and top-p (p < 1) among bins that hold all in front of them, but for `counts` tokens that weigh
+// `masses`.  False: these do not.
 template <bool WIDE>
-__device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, float p, Border& out, Shared& sh) {
-  const Sums s = sum_bins(r, b, sh);
+__device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, float p, Border& out, Shared& sh, uint32_t counts = 0,
+                                     uint64_t masses = 0) {
+  Sums s = sum_bins(r, b, sh);
+  s.count += counts, s.counts += counts, s.mass += masses, s.masses += masses;
   double all = r.total * (double)kUnit;
   bool found = false;
-  if (k > 0 && s.counts >= (uint32_t)k) {
+  if (k > 0 && counts < (uint32_t)k && s.counts >= (uint32_t)k) {
     uint32_t n = s.count;
     uint64_t m = s.mass;
     for (int i = 0; i < b.kCount && n < (uint32_t)k && s.count + s.own_count >= (uint32_t)k; ++i) {
@@ -428,7 +442,7 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
   if (p < 1.0f) {
     const double want = ceil((double)fmaxf(p, 0.0f) * all);
     const uint64_t goal = want > 1.0 ? (uint64_t)want : 1;
-    if (s.masses < goal) return found;
+    if (s.masses < goal || masses >= goal) return found;
     __syncthreads();  // (border was read)
     uint64_t m = s.mass;
     for (int i = 0; i < b.kCount && m < goal && s.mass + s.own_mass >= goal; ++i) {
@@ -533,8 +547,187 @@ __device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, Shar
   __syncthreads();
 }
 
+// One border, top-k's or top-p's, past the window of a long row: the weights (or tokens) behind a logit, estimated by those of a
+// sample, leave few keys for it, within four standard deviations.  One pass over the row adds up the weights in front of these
+// and lists the logits between; that list has the border, and what is missing of the chunks' weights.  False: it has not.
+__device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Border& out, Shared& sh) {
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  uint16_t* const list = reinterpret_cast<uint16_t*>(sh.bins + kBins) + w * (kList + 64);
+  __syncthreads();
+  reinterpret_cast<uint4*>(sh.bins)[t] = make_uint4(0, 0, 0, 0);
+  if (t == 0) sh.after = -1, sh.upto = kSampleBins, sh.between = 0;
+  if (t < kMaxChunks) sh.kept[t] = 0, sh.equal[t] = 0;
+  float l[16], low = r.top;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const u32x4 v = load_bits(r.logits, (2 * t + j) * (r.vocab / 8) / (2 * kDraw) * 8, r.vocab);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) l[8 * j + i] = value(v, i);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (l[i] > -INFINITY) low = fminf(low, l[i]);
+  const float farthest = wave_max(r.top - low);
+  if (lane == 0) sh.low[w] = farthest;
+  __syncthreads();
+  float span = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) span = fmaxf(span, sh.low[i]);
+  span = fminf(span, 31.0f * fminf(fmaxf(r.s.heat, FLT_MIN), kMaxHeat));
+  const float fine = (float)kSampleBins / span;  // bins from the least up
+  if (!(span < INFINITY && fine < 0x1p100f)) return false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const float at = span - (r.top - l[i]);
+    if (at >= 0.0f && at <= span) atomicAdd(&sh.bins[min((int)(at * fine), kSampleBins - 1)], 1u);
+  }
+  __syncthreads();
+  const uint4 bins = reinterpret_cast<const uint4*>(sh.bins)[t];
+  const uint32_t n[4] = {bins.x, bins.y, bins.z, bins.w};
+  float x[4];
+  double sum = 0.0, square = 0.0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[i] = k > 0 ? 1.0f : weight(r.s, r.top - span + (4 * t + i + 0.5f) / fine, r.top);
+    sum += (double)(n[i] * x[i]), square += (double)(n[i] * x[i] * x[i]);
+  }
+  const double upto = wave_scan(sum, Add()), upto2 = wave_scan(square, Add());
+  if (lane == 63) sh.sum[w] = upto, sh.square[w] = upto2;
+  __syncthreads();
+  double behind = upto - sum, behind2 = upto2 - square, all = 0.0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) behind += sh.sum[i], behind2 += sh.square[i];
+    all += sh.sum[i];
+  }
+  const double part = (double)kSample / r.vocab;
+  const float goal = (float)(k > 0 ? all - k * part : (1.0 - (double)fmaxf(p, 0.0f)) * r.total * part);
+  int after = -1, end = kSampleBins;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    behind += (double)(n[i] * x[i]), behind2 += (double)(n[i] * x[i] * x[i]);
+    const double var = k > 0 ? (all - behind) * (1.0 - (all - behind) / kSample) : behind2;
+    const float far = 4.0f * sqrtf((float)fmax(var, 0.0)) + 2.0f * x[i], b = (float)behind;
+    if (b + far < goal) after = 4 * t + i;
+    if (b - far > goal) end = min(end, 4 * t + i);
+  }
+  after = -wave_min(-after), end = wave_min(end);
+  if (lane == 0) atomicMax(&sh.after, after), atomicMin(&sh.upto, end);
+  __syncthreads();
+  after = sh.after, end = sh.upto;
+  uint32_t count = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) count += 4 * t + i > after && 4 * t + i <= end ? n[i] : 0;
+  count = counts_sum(count);
+  if (lane == 0) sh.count[w] = count;
+  for (int i = t; i < kBins / 4; i += kDraw) reinterpret_cast<uint4*>(sh.bins)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  count = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) count += sh.count[i];
+  Row q = r;
+  if (end < kSampleBins) q.first = min(r.first, key_of_value(r.top - span + (end + 1) / fine) + 1);
+  if (q.first == kMinusZero) q.first = kZero;
+  q.least = max(key_of_value(r.top - span + (after + 1) / fine), kLowest + 2) - 1;
+  q.low = q.least + (kSpan - 2);
+  q.straight = q.low + kSpan >= q.first;
+  if (count > 0.8 * part * (kWaves * kListed) || q.least > q.first || key_weight(r.s, q.least, r.top) < out.least) return false;
+
+  const float highest = logit_of(q.first), lowest = logit_of(q.least);
+  const int pieces = (r.vocab + kPiece - 1) / kPiece;
+  uint32_t listed = 0;
+  count = 0;
+  u32x4 v[kPiece / 512], next[kPiece / 512];
+  auto load = [&](int piece) {
+#pragma unroll
+    for (int j = 0; j < kPiece / 512; ++j) next[j] = load_bits(r.logits, min(piece * kPiece + 512 * j + 8 * lane, r.vocab), r.vocab);
+  };
+  load(w);
+  for (int c = w; c < pieces; c += kWaves) {
+#pragma unroll
+    for (int j = 0; j < kPiece / 512; ++j) v[j] = next[j];
+    if (c + kWaves < pieces) load(c + kWaves);
+    double mass = 0.0;
+#pragma unroll
+    for (int j = 0; j < kPiece / 512; ++j) {
+      if (listed > kListed) break;  // (the next 512 may not fit: the row is counted instead)
+      float x[8];
+      uint64_t over[8], in[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = value(v[j], i), d = y - r.top;  // (no clamp: what is over is near enough)
+        x[i] = __builtin_truncf(__builtin_amdgcn_exp2f(__builtin_fmaf(d, r.s.scale, d * r.s.scale_lo)) * kUnit);
+        over[i] = __ballot(y > highest), in[i] = __ballot(y >= lowest) & ~over[i];
+        x[i] = y > highest ? x[i] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mass += (double)x[i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        count += __builtin_popcountll(over[i]);
+        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[i], listed));
+        // (what is not listed goes behind the list: a branch takes longer)
+        list[__builtin_amdgcn_inverse_ballot_w64(in[i]) ? at : (uint32_t)kList + lane] = (uint16_t)(i & 1 ? v[j][i >> 1] >> 16 : v[j][i >> 1]);
+        listed += __builtin_popcountll(in[i]);
+      }
+    }
+    mass = wave_sum(mass);
+    if (lane == 0) {
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.kept[c / 2]), (unsigned long long)mass);
+      sh.ends[c] = (uint16_t)listed;
+    }
+  }
+  bool between = listed > kListed;
+  for (uint32_t i = lane; i < listed; i += 64) {
+    const uint32_t key = key_of(list[i]), d = q.first - key, e = q.low - key;
+    list[i] = (uint16_t)key;
+    if (q.straight || d < kSpan)
+      atomicAdd(&sh.bins[d], 1u);
+    else if (e < kSpan - 1)
+      atomicAdd(&sh.bins[kSpan + 1 + e], 1u);
+    else if (key == kZero)
+      atomicAdd(&sh.bins[kSpan], 1u);
+    else
+      between = true;
+  }
+  if (between) sh.between = 1;
+  __syncthreads();
+  if (lane == 0) sh.same[w] = count;
+  uint64_t mass = 0;
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i) mass += sh.kept[64 * i + lane];
+  mass = units_sum(mass);
+  __syncthreads();
+  if (sh.between) return false;
+  count = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) count += sh.same[i];
+  Border b = out;
+  if (!find(q, Bins<true>{}, k, p, b, sh, count, mass)) return false;
+  uint32_t begin = 0;
+  for (int c = w; c < pieces; c += kWaves) {
+    const uint32_t stop = sh.ends[c];
+    uint64_t kept = 0;
+    uint32_t same = 0;
+    for (uint32_t i = begin + lane; i < stop; i += 64) {
+      const uint32_t key = list[i];
+      kept += key > b.key ? units(key_weight(r.s, key, r.top)) : 0;
+      same += key == b.key;
+    }
+    kept = units_sum(kept), same = counts_sum(same);
+    if (lane == 0) {
+      atomicAdd(reinterpret_cast<unsigned long long*>(&sh.kept[c / 2]), (unsigned long long)kept);
+      atomicAdd(&sh.equal[c / 2], same);
+    }
+    begin = stop;
+  }
+  out = b;
+  __syncthreads();
+  return true;
+}
+
 // Keys of a row that has some between the bins: down from the largest, kBins at a time and over empty stretches at once, first to
-// top-k's border, then to top-p's.  Slow, for rows with logits of 2^-58 of the largest and less.
+// top-k's border, then to top-p's.  Slow, for rows with logits of 2^-31 of the largest and less.
 __device__ __attribute__((noinline)) Border find_slowly(Row r, int k, float p, Border out, Shared& sh) {
   const uint32_t top = r.first;
   r.straight = true;
@@ -602,7 +795,7 @@ __device__ __forceinline__ void store(const SampleArgs& a, int id, const Row& r,
   float lp = 0.0f;
   if (token >= 0) {
     const float l = bf2f(r.logits[token]);
-    lp = (float)((l == r.top ? 0.0 : (double)(l - r.top) / (double)fminf(r.s.heat, kMaxHeat)) - log(r.total));
+    lp = (float)((l == r.top ? 0.0 : (double)(l - r.top) / (double)fminf(fmaxf(r.s.heat, FLT_MIN), kMaxHeat)) - log(r.total));
   }
   a.logp[id] = lp;
 }
@@ -666,7 +859,7 @@ __device__ __forceinline__ void draw_in(const SampleArgs& a, int id, const Row& 
   store(a, id, r, token);
 }
 
-__global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs a) {
   __shared__ Shared sh;
   const int id = blockIdx.x, t = threadIdx.x, lane = t & 63;
   Row r;
@@ -679,7 +872,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
   const int limit = k > 0 && k < a.vocab ? k : 0;
   const bool filters = !r.s.greedy && (limit || p < 1.0f || least > 0.0f), staged = filters && r.counts && a.chunks <= kStaged;
   if (staged) {  // beside the statistics
-    constexpr int kAt = kBins / 4 / kDraw;
+    constexpr int kAt = kPool / 4 / kDraw;
     const uint4* const src = reinterpret_cast<const uint4*>(r.counts);
     const int all = a.chunks * (kWindow / 8);
     uint4 v[kAt];
@@ -772,7 +965,7 @@ __global__ void __launch_bounds__(kDraw) sample_draw_kernel(const SampleArgs a) 
       window_masses<true>(r, b, first, sh);
     else
       window_masses<false>(r, b, first, sh);
-  } else {
+  } else if (a.vocab < kSample || (limit != 0) == (p < 1.0f) || r.top == INFINITY || !find_sampled(r, limit, p, b, sh)) {
     if (limit || p < 1.0f) {
       if (count_all(r, r.counts ? &window : nullptr, sh))
         (void)find(r, Bins<true>{}, limit, p, b, sh);  // (found nowhere: there is no border)
@@ -840,8 +1033,11 @@ int launch(SampleArgs a, hipStream_t st) {
   std::lock_guard<std::mutex> lock(scratch_mutex(st));  // the launches that share the scratch stay together
   uint8_t* const z = call_scratch(st, per * each, ScratchOf::kOperators).data;
   if (!z) {
-    hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)a.b), dim3(kDraw), 0, st, a);
-    return (int)hipGetLastError();
+    for (int i = 0; i < a.b; i += 65535) {
+      hipLaunchKernelGGL(sample_draw_kernel, dim3((unsigned)(a.b - i < 65535 ? a.b - i : 65535)), dim3(kDraw), 0, st, from(a, i));
+      if (const int e = (int)hipGetLastError()) return e;
+    }
+    return 0;
   }
   a.stats = reinterpret_cast<ChunkStat*>(z);
   a.counts = reinterpret_cast<uint32_t*>(a.stats + (size_t)each * a.chunks);

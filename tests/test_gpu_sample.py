@@ -118,6 +118,56 @@ def test_flat_rows_whose_border_is_far_down():
     r.compare(r.run(), least=0.7, tol=2e-6)
 
 
+def far_borders(rng, b, vocab):
+    """Top-k or top-p of each row, never both, that keeps a large part of a flat row."""
+    ks = np.arange(b) % 2 == 0
+    return np.where(ks, rng.integers(vocab // 10, vocab - vocab // 50, b), 0), np.where(ks, 1.0, 0.5 + 0.4999 * rng.random(b))
+
+
+@pytest.mark.parametrize("zeros", [0.0, 0.2])
+@pytest.mark.parametrize("vocab", [8191, 8192, 8199, 16385, 100277])
+def test_long_flat_rows(vocab, zeros):
+    """One border far down, which a sample of the row finds: also among zeros of either sign, and with min-p below it."""
+    rng = np.random.default_rng(vocab)
+    b = 20
+    x = rng.standard_normal((b, vocab)) * (0.5 + 0.5 * rng.random((b, 1)))
+    x = np.where(rng.random((b, vocab)) < zeros, np.where(rng.random((b, vocab)) < 0.5, 0.0, -0.0), x)
+    bits = f2bf_array(x.astype(np.float32).ravel()).reshape(b, vocab)
+    top_k, top_p = far_borders(rng, b, vocab)
+    min_p = np.where(np.arange(b) % 5 == 1, 1e-6, 0.0)
+    r = Rows(bits, None, top_k, top_p, min_p, rng.random(b))
+    # (as above.  A draw is within 2e-6 of one of n tokens' ends with a chance of 4e-6 n, 0.40 of 100277 and 0.07 of 16385; top-p's
+    # border, in the half of the rows, is so with about twice that.  Of the most, 0.6 (0.5 + 0.5 0.5) = 0.45 of 20 rows are left,
+    # give or take 0.11 a standard deviation; of 16385 0.87 0.93 = 0.8.)
+    r.compare(r.run(), least=0.15 if vocab > 20000 else 0.5, tol=2e-6)
+
+
+@pytest.mark.parametrize("kind", ["ascending", "descending", "blocks", "masked", "nan", "equal", "shifted"])
+@pytest.mark.parametrize("vocab", [16384, 65536])
+def test_long_rows_that_a_sample_misjudges(kind, vocab):
+    rng = np.random.default_rng(vocab)
+    b = 16
+    x = rng.standard_normal((b, vocab)) * 0.8
+    # every (vocab / 8192)th eight logits are those that a sample of 8192 in eights takes
+    eights = np.arange(vocab) // 8 % (vocab // 8192) == 0
+    if kind in ("ascending", "descending"):
+        x = np.sort(x, axis=1)[:, :: 1 if kind == "ascending" else -1]
+    elif kind == "blocks":
+        x[:, eights] -= 4.0
+    elif kind == "masked":
+        x[:, eights] = -np.inf
+    elif kind == "nan":
+        x[:, eights] = np.nan
+    elif kind == "equal":
+        x[:, ~eights] = -0.25
+    else:
+        x[:, eights] += 0.5
+    bits = f2bf_array(x.astype(np.float32).ravel()).reshape(b, vocab)
+    top_k, top_p = far_borders(rng, b, vocab)
+    r = Rows(bits, None, top_k, top_p, None, rng.random(b))
+    r.compare(r.run(), least=0.5, tol=2e-6)
+
+
 @pytest.mark.parametrize("tiny", [0.0, 1e-6, 1e-15, 1e-30])
 @pytest.mark.parametrize("shift", [0.0, -1.0, 3.0])
 def test_borders_among_zeros_and_tiny_values(tiny, shift):
