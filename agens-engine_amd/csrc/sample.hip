@@ -12,7 +12,7 @@
 //
 //   sample_keys_kernel   a chunk of 4096 logits a workgroup, held in registers: its largest, its lowest token with that, the
 //                        sum of its weights (16 in 32 bits, then 64), and how often each of the kWindow keys up to its
-//                        largest occurs;
+//                        largest, or to the one above where that is even, occurs: windows are shifted by whole pairs;
 //   sample_draw_kernel   a row a workgroup: the chunks' windows, shifted to the row's largest key and summed, give the border of
 //                        what is kept (one scan of counts and weights serves top-k and top-p, since top-p's border is not
 //                        behind top-k's), and what each chunk has of it; then the chunk that the draw falls into is read again.
@@ -21,9 +21,10 @@
 //                        do, the row's keys are counted anew, all at once, and the chunks' shares summed up in another pass.
 // Without scratch sample_draw_kernel takes the chunks' statistics itself and does without their windows: the same tokens.
 //
-// What bounds them: loads' and barriers' latency, one after another (1 row of 152064: 4.2 + 4.1 us without a filter; 32 rows: 5.7 +
-// 13.8 us, 9.7 MB at 7 TB/s would be 1.4), and instructions for rows whose border is far down: 25 a logit by one workgroup, 1 row of
-// 152064 52 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 62 us and 87.
+// What bounds them: latency, of loads, barriers and one wave's instructions one after another (1 row of 152064: 4.2 us, and then 4.1
+// without a filter, 8.6 with one, of which 1.4 the first loads, 1.3 the windows, 1.1 the border, 1.4 the chunks' shares and 2 the
+// draw; 32 rows: 5.7 + 11 us, where 9.7 MB at 7 TB/s are 1.4); and instructions where a border is far down: 25 a logit by one
+// workgroup, 1 row of 152064 50 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 61 us and 87.
 #include "agens_kernels.h"
 #include "logits.h"
 
@@ -79,7 +80,7 @@ struct SampleArgs {
   float* logp;
   int b, vocab, chunks;
   ChunkStat* stats;  // [b][chunks]
-  uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys from the chunk's largest down
+  uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys from the chunk's largest down, the first one odd
 };
 
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
@@ -169,12 +170,13 @@ __device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* r
     best = wave_min(best);
   }
   if (bins && top > -INFINITY) {
-    const uint32_t first = key_of_value(top), span = min((uint32_t)kWindow + 1, first - kLowest);  // (-inf weighs nothing)
+    const uint32_t first = key_of_value(top), even = ~first & 1;
+    const uint32_t span = min((uint32_t)kWindow + 1 - even, first - kLowest);  // (-inf weighs nothing)
 #pragma unroll
     for (int i = 0; i < kEach / 2; ++i) {
       const uint32_t keys = two_keys(v[i >> 2][i & 3]), d0 = first - (keys & 0xFFFFu), d1 = first - (keys >> 16);
-      if (d0 < span) atomicAdd(&bins[d0], 1u);
-      if (d1 < span) atomicAdd(&bins[d1], 1u);
+      if (d0 < span) atomicAdd(&bins[even + d0], 1u);
+      if (d1 < span) atomicAdd(&bins[even + d1], 1u);
     }
   }
   float sum = 0.0f;
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const Sample
   const size_t at = (size_t)id * a.chunks + chunk;
   if (t == 0) {
     a.stats[at] = r;
-    const uint32_t d = key_of_value(r.top) - kZero;  // the counts of -0
+    const uint32_t d = (key_of_value(r.top) | 1) - kZero;  // the counts of -0
     if (r.top >= 0.0f && d < kWindow) bins[d] += bins[d + 1], bins[d + 1] = 0;
   }
   __syncthreads();
@@ -236,7 +238,7 @@ struct Shared {
   uint16_t ends[2 * kMaxChunks];  // of the pieces' parts of their waves' lists
   uint64_t kept[kMaxChunks];  // the chunks' weights above the border's key
   uint32_t equal[kMaxChunks]; // and their tokens with it
-  uint64_t weight[kWindow + 2];  // of the window's keys; the last two are 0
+  __attribute__((aligned(16))) double weight[kWindow + 2];  // of the window's keys, in units; the last two are 0
   __attribute__((aligned(16))) uint32_t bins[kPool];  // (lists behind the bins)
 };
 
@@ -248,6 +250,7 @@ struct Row {
   int best, vocab, chunks;
   double total;
   uint32_t first;  // the key of top
+  uint32_t base;   // the first of the window: that, or the one above where that is even
   uint32_t least;  // the lowest key that weighs anything
   uint32_t low;    // the first key of the bins past zero's
   bool straight;   // or the bins go on below kSpan without a gap, and without a bin for zero alone
@@ -266,7 +269,8 @@ struct Bins {
   }
   __device__ __forceinline__ uint32_t key(const Row& r, int i) const {
     const int at = (int)threadIdx.x * kCount + i;
-    if (!WIDE || at < kSpan || r.straight) return r.first - at;
+    if (!WIDE) return r.base - at;
+    if (at < kSpan || r.straight) return r.first - at;
     return at == kSpan ? kZero : r.low - (at - kSpan - 1);
   }
   __device__ __forceinline__ uint64_t mass(const Row& r, const Shared& sh, int i) const {
@@ -275,43 +279,62 @@ struct Bins {
   }
 };
 
-// The chunks' windows: in memory, or staged in LDS, where sh.bins has room for kStaged chunks' and nothing else is yet.
-constexpr int kStaged = kPool * 4 / (kWindow * 2);
-template <bool STAGED>
-struct Windows {
-  const uint32_t* memory;
-  const Shared& sh;
-  __device__ __forceinline__ uint32_t one(int c, int at) const {
-    const size_t i = (size_t)c * kWindow + at;
-    return STAGED ? reinterpret_cast<const uint16_t*>(sh.bins)[i] : reinterpret_cast<const uint16_t*>(memory)[i];
-  }
-  __device__ __forceinline__ uint32_t two(int c, int pair) const {
-    const size_t i = (size_t)c * (kWindow / 2) + pair;
-    return STAGED ? sh.bins[i] : memory[i];
-  }
+// The chunks' windows, in LDS where sh.bins, which holds nothing else yet, has room for all: slots of kSlot pairs, for the banks, the
+// first one unused, so that what is in front of a window can be loaded too.
+constexpr int kSlot = kWindow / 2 + 4, kStaged = kPool / kSlot - 1;
+static_assert(kStaged < 64 && kSlot % 4 == 0 && (kStaged + 1) * kSlot <= kPool - 4, "a chunk a lane, windows of whole 16 bytes, 16 left");
+struct Slot {
+  int at, begin;  // of the pair that lines up with the row's first; of the window's first
 };
+// of the chunk of the lane, whose window begins with key `base`
+__device__ __forceinline__ Slot slot_of(const Row& r, uint32_t base) {
+  const int lane = threadIdx.x & 63, begin = kSlot * (min(lane, r.chunks - 1) + 1);
+  return Slot{begin - (int)min(r.base - base, (uint32_t)kWindow) / 2, lane < r.chunks ? begin : INT_MAX};
+}
 
-// The thread's bin of the chunks' windows.
-template <bool STAGED>
-__device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&first)[kLaneChunks], const Shared& sh) {
-  const Windows<STAGED> counts{r.counts, sh};
-  constexpr int kAt = 40;  // loads in flight
-  Bins<false> b{0};
-  for (int c0 = 0; c0 < r.chunks; c0 += kAt) {
-    uint32_t v[kAt];
+// The thread's bin of the row's window, from the staged ones: one half of the threads adds up every other chunk's pairs.
+__device__ __forceinline__ Bins<false> count_staged(const Row& r, uint32_t base, Shared& sh) {
+  const int t = threadIdx.x, pair = t % (kDraw / 2), half = __builtin_amdgcn_readfirstlane(t / (kDraw / 2));
+  const Slot slot = slot_of(r, base);
+  uint32_t even = 0, odd = 0;
+  for (int c0 = half; c0 < r.chunks; c0 += 16) {
+    uint32_t v[8], sum = 0;  // (eight chunks' counts fit 16 bits)
 #pragma unroll
-    for (int j = 0; j < kAt; ++j) {
-      const int c = min(c0 + j, r.chunks - 1);
-      uint32_t f = first[0];
-#pragma unroll
-      for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
-      const int at = (int)threadIdx.x - (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
-      v[j] = 0;
-      if (at >= 0 && c0 + j < r.chunks) v[j] = counts.one(c, at);
+    for (int j = 0; j < 8; ++j) {
+      const int c = min(c0 + 2 * j, r.chunks - 1), at = pair + __builtin_amdgcn_readlane(slot.at, c);
+      v[j] = sh.bins[at];
+      v[j] = at >= (c0 + 2 * j < r.chunks ? kSlot * (c + 1) : INT_MAX) ? v[j] : 0;
     }
 #pragma unroll
-    for (int j = 0; j < kAt; ++j) b.n += v[j];
+    for (int j = 0; j < 8; ++j) sum += v[j];
+    even += sum & 0xFFFFu, odd += sum >> 16;
   }
+  uint32_t* const halves = reinterpret_cast<uint32_t*>(sh.weight);
+  reinterpret_cast<uint2*>(halves)[t] = make_uint2(even, odd);
+  __syncthreads();
+  return Bins<false>{halves[t] + halves[kDraw + t]};
+}
+
+// and from memory
+__device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t (&base)[kLaneChunks]) {
+  const uint16_t* const counts = reinterpret_cast<const uint16_t*>(r.counts);
+  constexpr int kAt = 32;  // loads in flight
+  Bins<false> b{0};
+#pragma unroll
+  for (int i = 0; i < kLaneChunks; ++i)
+    for (int c0 = 0; c0 < min(r.chunks - 64 * i, 64); c0 += kAt) {
+      uint32_t v[kAt];
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) {
+        const int c = min(64 * i + c0 + j, r.chunks - 1);
+        // how far the window is from the row's; past the last chunk as far as can be
+        const int shift = c0 + j < r.chunks - 64 * i ? (int)(r.base - (uint32_t)__builtin_amdgcn_readlane((int)base[i], c & 63)) : kWindow;
+        v[j] = counts[(size_t)c * kWindow + max((int)threadIdx.x - shift, 0)];
+        v[j] = (int)threadIdx.x >= shift ? v[j] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < kAt; ++j) b.n += v[j];
+    }
   return b;
 }
 
@@ -368,12 +391,12 @@ __device__ __forceinline__ bool count_all(Row& r, const Bins<false>* window, Sha
   r.least = r.top == INFINITY ? r.first : max((int)key_of_value(r.top - 31.0f * heat), (int)kLowest + 2) - 1;
   r.low = r.least + (kSpan - 2);
   r.straight = r.low + kSpan >= r.first;
-  const uint32_t from = window ? kWindow : 0;
+  const uint32_t from = window ? kWindow - (r.base - r.first) : 0;
   __syncthreads();
   for (int i = threadIdx.x; i < kBins / 4; i += kDraw) reinterpret_cast<uint4*>(sh.bins)[i] = make_uint4(0, 0, 0, 0);
   if (threadIdx.x == 0) sh.between = 0;
   __syncthreads();
-  if (window) sh.bins[threadIdx.x] = window->n;
+  if (window && threadIdx.x >= r.base - r.first) sh.bins[threadIdx.x - (r.base - r.first)] = window->n;
   if (r.straight ? count_keys<true>(r, from, sh) : count_keys<false>(r, from, sh)) sh.between = 1;
   __syncthreads();
   if (threadIdx.x == 0 && zeros_in(r)) {  // -0 counts as 0 (in the window, both are counted)
@@ -411,6 +434,12 @@ __device__ __forceinline__ Sums sum_bins(const Row& r, const Bins<WIDE>& b, Shar
   return s;
 }
 
+// What top-p's front weighs at least, of a sum.
+__device__ __forceinline__ uint64_t goal_of(float p, double all) {
+  const double want = ceil((double)fmaxf(p, 0.0f) * all);
+  return want > 1.0 ? (uint64_t)want : 1;
+}
+
 // The borders of top-k (k > 0) and top-p (p < 1) among bins that hold all in front of them, but for `counts` tokens that weigh
 // `masses`.  False: these do not.
 template <bool WIDE>
@@ -440,8 +469,7 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
     return false;
   }
   if (p < 1.0f) {
-    const double want = ceil((double)fmaxf(p, 0.0f) * all);
-    const uint64_t goal = want > 1.0 ? (uint64_t)want : 1;
+    const uint64_t goal = goal_of(p, all);
     if (s.masses < goal || masses >= goal) return found;
     __syncthreads();  // (border was read)
     uint64_t m = s.mass;
@@ -462,16 +490,47 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
   return found;
 }
 
-// Each chunk's weights above the border's key and its tokens with it, to sh.kept and sh.equal: from the windows;
-template <bool STAGED>
-__device__ __forceinline__ void window_masses(const Row& r, const Border& b, const uint32_t (&first)[kLaneChunks], Shared& sh) {
-  const Windows<STAGED> counts{r.counts, sh};
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
-  const uint32_t key = r.first - t;
+// The weights of the window's keys above the border, to sh.weight: in doubles, where a chunk's counts times these are whole (4096 of
+// 2^40 units), and whose products take a quarter of the time of those in 64 bits.
+__device__ __forceinline__ void window_weights(const Row& r, const Border& b, Shared& sh) {
+  const int t = threadIdx.x;
+  const uint32_t key = r.base - t;
   const float x = key_weight(r.s, key, r.top);
-  sh.weight[t] = key > b.key && x >= b.least ? units(x) : 0;
-  if (t < 2) sh.weight[kWindow + t] = 0;
+  sh.weight[t] = key <= r.first && key > b.key && x >= b.least ? (double)__builtin_truncf(x * kUnit) : 0.0;
+  if (t < 2) sh.weight[kWindow + t] = 0.0;
   __syncthreads();
+}
+// Each chunk's weights above the border's key and its tokens with it: from the staged windows, a lane a chunk, every eighth pair a
+// wave;
+__device__ __forceinline__ void staged_masses(const Row& r, const Border& b, uint32_t base, uint64_t& kept, uint32_t& equal, Shared& sh) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  window_weights(r, b, sh);
+  const Slot slot = slot_of(r, base);
+  const int down = (int)min(r.base - b.key, (uint32_t)kWindow - 1);
+  double sum = 0.0;
+#pragma unroll 4
+  for (int pair = w; pair <= down / 2; pair += kWaves) {
+    uint32_t n = sh.bins[slot.at + pair];
+    n = slot.at + pair >= slot.begin ? n : 0;
+    const double2 x = *reinterpret_cast<const double2*>(&sh.weight[2 * pair]);
+    sum = __builtin_fma((double)(n & 0xFFFFu), x.x, sum);
+    sum = __builtin_fma((double)(n >> 16), x.y, sum);
+  }
+  double* const parts = reinterpret_cast<double*>(sh.stats);
+  static_assert(sizeof(sh.stats) >= kDraw * sizeof(double), "a part a thread");
+  parts[threadIdx.x] = sum;
+  const uint32_t n = sh.bins[slot.at + down / 2];
+  equal = b.key && slot.at + down / 2 >= slot.begin ? n >> (16 * (down & 1)) & 0xFFFFu : 0;
+  __syncthreads();
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) sum += parts[64 * i + lane];
+  kept = (uint64_t)sum;
+}
+// to sh.kept and sh.equal from those in memory,
+__device__ __forceinline__ void window_masses(const Row& r, const Border& b, const uint32_t (&base)[kLaneChunks], Shared& sh) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  window_weights(r, b, sh);
   // a wave kAt chunks at a time, lane by lane two neighbouring bins, 128 a step; steps past the border are not loaded
   constexpr int kAt = 5, kSteps = kWindow / 128;
   for (int c0 = w; c0 < r.chunks; c0 += kAt * kWaves) {
@@ -480,38 +539,40 @@ __device__ __forceinline__ void window_masses(const Row& r, const Border& b, con
 #pragma unroll
     for (int a = 0; a < kAt; ++a) {
       const int c = min(c0 + a * kWaves, r.chunks - 1);
-      uint32_t f = first[0];
+      uint32_t f = base[0];
 #pragma unroll
-      for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? first[i] : f;
-      shift[a] = (int)(r.first - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
-      border[a] = (int)(r.first - b.key) - shift[a];
+      for (int i = 1; i < kLaneChunks; ++i) f = c >> 6 == i ? base[i] : f;
+      shift[a] = (int)(r.base - (uint32_t)__builtin_amdgcn_readlane((int)f, c & 63));
+      border[a] = (int)(r.base - b.key) - shift[a];
       const int last = min(border[a], kWindow - 1 - shift[a]);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         pair[a][j] = 0;
-        if (128 * j <= last) pair[a][j] = counts.two(c, 64 * j + lane);
+        if (128 * j <= last) pair[a][j] = r.counts[(size_t)c * (kWindow / 2) + 64 * j + lane];
       }
     }
-    uint64_t sum[kAt];
+    double sum[kAt];
     uint32_t same[kAt];
 #pragma unroll
     for (int a = 0; a < kAt; ++a) {
-      sum[a] = 0, same[a] = 0;
+      sum[a] = 0.0, same[a] = 0;
       const int last = min(border[a], kWindow - 1 - shift[a]);
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
         if (128 * j > last) break;
-        const int at = 128 * j + 2 * lane, in = min(at + shift[a], kWindow);  // (past the window the weights are 0)
-        sum[a] += (pair[a][j] & 0xFFFFu) * sh.weight[in] + (pair[a][j] >> 16) * sh.weight[in + 1];
-        if (at == (border[a] & ~1)) same[a] = pair[a][j] >> (16 * (border[a] & 1)) & 0xFFFFu;
+        const int in = min(128 * j + 2 * lane + shift[a], kWindow);  // (past the window the weights are 0)
+        sum[a] = __builtin_fma((double)(pair[a][j] & 0xFFFFu), sh.weight[in], sum[a]);
+        sum[a] = __builtin_fma((double)(pair[a][j] >> 16), sh.weight[in + 1], sum[a]);
+        if (border[a] >> 7 == j)
+          same[a] = (uint32_t)__builtin_amdgcn_readlane((int)pair[a][j], border[a] >> 1 & 63) >> (16 * (border[a] & 1)) & 0xFFFFu;
       }
     }
 #pragma unroll
-    for (int a = 0; a < kAt; ++a) sum[a] = units_sum(sum[a]), same[a] = counts_sum(same[a]);
+    for (int a = 0; a < kAt; ++a) sum[a] = wave_sum(sum[a]);
 #pragma unroll
     for (int a = 0; a < kAt; ++a)
       if (lane == 0 && c0 + a * kWaves < r.chunks)
-        sh.kept[c0 + a * kWaves] = sum[a], sh.equal[c0 + a * kWaves] = b.key ? same[a] : 0;
+        sh.kept[c0 + a * kWaves] = (uint64_t)sum[a], sh.equal[c0 + a * kWaves] = b.key ? same[a] : 0;
   }
   __syncthreads();
 }
@@ -549,8 +610,9 @@ __device__ __forceinline__ void chunk_masses(const Row& r, const Border& b, Shar
 
 // One border, top-k's or top-p's, past the window of a long row: the weights (or tokens) behind a logit, estimated by those of a
 // sample, leave few keys for it, within four standard deviations.  One pass over the row adds up the weights in front of these
-// and lists the logits between; that list has the border, and what is missing of the chunks' weights.  False: it has not.
-__device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Border& out, Shared& sh) {
+// and lists the logits between; that list has the border, and what is missing of the chunks' weights.
+enum class Sampled { kFound, kBehind, kNot };  // kBehind: behind min-p's border, it seems; kNot: not in the list
+__device__ __forceinline__ Sampled find_sampled(const Row& r, int k, float p, Border& out, Shared& sh) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   uint16_t* const list = reinterpret_cast<uint16_t*>(sh.bins + kBins) + w * (kList + 64);
   __syncthreads();
@@ -575,7 +637,7 @@ __device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Borde
   for (int i = 0; i < kWaves; ++i) span = fmaxf(span, sh.low[i]);
   span = fminf(span, 31.0f * fminf(fmaxf(r.s.heat, FLT_MIN), kMaxHeat));
   const float fine = (float)kSampleBins / span;  // bins from the least up
-  if (!(span < INFINITY && fine < 0x1p100f)) return false;
+  if (!(span < INFINITY && fine < 0x1p100f)) return Sampled::kNot;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float at = span - (r.top - l[i]);
@@ -631,7 +693,8 @@ __device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Borde
   q.least = max(key_of_value(r.top - span + (after + 1) / fine), kLowest + 2) - 1;
   q.low = q.least + (kSpan - 2);
   q.straight = q.low + kSpan >= q.first;
-  if (count > 0.8 * part * (kWaves * kListed) || q.least > q.first || key_weight(r.s, q.least, r.top) < out.least) return false;
+  if (key_weight(r.s, q.first, r.top) < out.least) return Sampled::kBehind;
+  if (count > 0.8 * part * (kWaves * kListed) || q.least > q.first) return Sampled::kNot;
 
   const float highest = logit_of(q.first), lowest = logit_of(q.least);
   const int pieces = (r.vocab + kPiece - 1) / kPiece;
@@ -698,12 +761,12 @@ __device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Borde
   for (int i = 0; i < kLaneChunks; ++i) mass += sh.kept[64 * i + lane];
   mass = units_sum(mass);
   __syncthreads();
-  if (sh.between) return false;
+  if (sh.between) return Sampled::kNot;
   count = 0;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) count += sh.same[i];
   Border b = out;
-  if (!find(q, Bins<true>{}, k, p, b, sh, count, mass)) return false;
+  if (!find(q, Bins<true>{}, k, p, b, sh, count, mass)) return Sampled::kNot;
   uint32_t begin = 0;
   for (int c = w; c < pieces; c += kWaves) {
     const uint32_t stop = sh.ends[c];
@@ -711,7 +774,8 @@ __device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Borde
     uint32_t same = 0;
     for (uint32_t i = begin + lane; i < stop; i += 64) {
       const uint32_t key = list[i];
-      kept += key > b.key ? units(key_weight(r.s, key, r.top)) : 0;
+      const float x = key_weight(r.s, key, r.top);
+      kept += key > b.key && x >= b.least ? units(x) : 0;
       same += key == b.key;
     }
     kept = units_sum(kept), same = counts_sum(same);
@@ -723,7 +787,7 @@ __device__ __forceinline__ bool find_sampled(const Row& r, int k, float p, Borde
   }
   out = b;
   __syncthreads();
-  return true;
+  return Sampled::kFound;
 }
 
 // Keys of a row that has some between the bins: down from the largest, kBins at a time and over empty stretches at once, first to
@@ -734,8 +798,7 @@ __device__ __attribute__((noinline)) Border find_slowly(Row r, int k, float p, B
   double all = r.total * (double)kUnit;
   bool found = false;
   for (int turn = k > 0 ? 0 : 1; turn < (p < 1.0f ? 2 : 1); ++turn) {
-    const double want = turn ? ceil((double)fmaxf(p, 0.0f) * all) : (double)k;
-    const uint64_t goal = want > 1.0 ? (uint64_t)want : 1;
+    const uint64_t goal = turn ? goal_of(p, all) : (uint64_t)k;
     uint32_t counts = 0;
     uint64_t masses = 0;
     r.first = top;
@@ -871,6 +934,15 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   const float p = a.top_p ? a.top_p[id] : 1.0f, least = a.min_p ? a.min_p[id] : 0.0f, u = a.u[id];
   const int limit = k > 0 && k < a.vocab ? k : 0;
   const bool filters = !r.s.greedy && (limit || p < 1.0f || least > 0.0f), staged = filters && r.counts && a.chunks <= kStaged;
+  ChunkStat st[kLaneChunks];
+  auto load_stats = [&](const ChunkStat* stats) {
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; ++i) {
+      st[i] = ChunkStat{-INFINITY, -1, 0.0};
+      if (lane + 64 * i < a.chunks) st[i] = stats[lane + 64 * i];
+    }
+  };
+  if (a.stats) load_stats(a.stats + (size_t)id * a.chunks);
   if (staged) {  // beside the statistics
     constexpr int kAt = kPool / 4 / kDraw;
     const uint4* const src = reinterpret_cast<const uint4*>(r.counts);
@@ -879,7 +951,10 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
 #pragma unroll
     for (int i = 0; i < kAt; ++i) v[i] = src[min(t + i * kDraw, all - 1)];
 #pragma unroll
-    for (int i = 0; i < kAt; ++i) reinterpret_cast<uint4*>(sh.bins)[t + i * kDraw] = v[i];
+    for (int i = 0; i < kAt; ++i) {
+      const int e = t + i * kDraw, c = e / (kWindow / 8);
+      reinterpret_cast<uint4*>(sh.bins)[e < all ? (c + 1) * (kSlot / 4) + e % (kWindow / 8) : kPool / 4 - 1] = v[i];  // (or nowhere)
+    }
   }
   if (!a.stats) {
     for (int c0 = 0; c0 < a.chunks; c0 += kGroups) {
@@ -888,19 +963,13 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
       if (t % kGroupThreads == 0 && c < a.chunks) sh.stats[c] = x;
     }
     __syncthreads();
+    load_stats(sh.stats);
   }
   // every wave by itself: the row from its chunks (lane by lane, then over the lanes)
-  const ChunkStat* const stats = a.stats ? a.stats + (size_t)id * a.chunks : sh.stats;
-  ChunkStat st[kLaneChunks];
-  uint32_t first[kLaneChunks];
+  uint32_t base[kLaneChunks];
   r.top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kLaneChunks; ++i) {
-    st[i] = ChunkStat{-INFINITY, -1, 0.0};
-    if (lane + 64 * i < a.chunks) st[i] = stats[lane + 64 * i];
-  }
-#pragma unroll
-  for (int i = 0; i < kLaneChunks; ++i) r.top = fmaxf(r.top, st[i].top), first[i] = key_of_value(st[i].top);
+  for (int i = 0; i < kLaneChunks; ++i) r.top = fmaxf(r.top, st[i].top), base[i] = key_of_value(st[i].top) | 1;
   r.top = wave_max(r.top);
   if (r.top == -INFINITY) {
     if (t == 0) {
@@ -920,7 +989,7 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   for (int i = 0; i < kLaneChunks; ++i) total += share[i];
   r.total = wave_sum(total);
   r.best = wave_min(best);
-  r.first = key_of_value(r.top);
+  r.first = key_of_value(r.top), r.base = r.first | 1;
   if (r.s.greedy) {
     if (t == 0) store(a, id, r, r.best);
     return;
@@ -951,28 +1020,43 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   if (quick) {
     // whether min-p's border is within the window: then no other that is further down matters (where top-p's may be within it
     // though top-k's is not, that has to be known)
-    const bool cut = r.first < kWindow || key_weight(r.s, r.first - (kWindow - 1), r.top) < b.least;
+    const bool cut = r.first < kWindow || key_weight(r.s, r.base - (kWindow - 1), r.top) < b.least;
     bool found = false;
     if (limit || p < 1.0f) {
-      window = staged ? count_window<true>(r, first, sh) : count_window<false>(r, first, sh);
+      window = staged ? count_staged(r, base[0], sh) : count_window(r, base);
       found = find(r, window, limit, p, b, sh);
     }
     quick = found || (cut && !(limit && p < 1.0f));
     if (!found) b.key = 0, b.n = 0;
   }
-  if (quick) {
-    if (staged)
-      window_masses<true>(r, b, first, sh);
-    else
-      window_masses<false>(r, b, first, sh);
-  } else if (a.vocab < kSample || (limit != 0) == (p < 1.0f) || r.top == INFINITY || !find_sampled(r, limit, p, b, sh)) {
-    if (limit || p < 1.0f) {
-      if (count_all(r, r.counts ? &window : nullptr, sh))
-        (void)find(r, Bins<true>{}, limit, p, b, sh);  // (found nowhere: there is no border)
-      else
-        b = find_slowly(r, limit, p, b, sh);
+  uint64_t kept[kLaneChunks];
+  uint32_t equal[kLaneChunks];
+  if (quick && !staged) {
+    window_masses(r, b, base, sh);
+  } else if (quick) {
+    staged_masses(r, b, base[0], kept[0], equal[0], sh);
+  } else {
+    const bool one = (limit != 0) != (p < 1.0f) && a.vocab >= kSample && r.top < INFINITY;
+    Sampled how = one ? find_sampled(r, limit, p, b, sh) : Sampled::kNot;
+    if (how == Sampled::kBehind) {
+      chunk_masses(r, b, sh);
+      uint64_t all = 0;
+      for (int i = lane; i < a.chunks; i += 64) all += sh.kept[i];
+      if (!limit && units_sum(all) < goal_of(p, r.total * (double)kUnit)) how = Sampled::kFound;  // so it is: no border but min-p's
     }
-    chunk_masses(r, b, sh);
+    if (how != Sampled::kFound) {
+      if (limit || p < 1.0f) {
+        if (count_all(r, r.counts ? &window : nullptr, sh))
+          (void)find(r, Bins<true>{}, limit, p, b, sh);  // (found nowhere: there is no border)
+        else
+          b = find_slowly(r, limit, p, b, sh);
+      }
+      chunk_masses(r, b, sh);
+    }
+  }
+  if (!(quick && staged)) {
+#pragma unroll
+    for (int i = 0; i < kLaneChunks; ++i) kept[i] = sh.kept[lane + 64 * i], equal[i] = sh.equal[lane + 64 * i];
   }
   // the chunk, every wave by itself
   const float border_weight = b.key ? key_weight(r.s, b.key, r.top) : 0.0f;
@@ -985,9 +1069,9 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
     mass[i] = 0, mine[i] = 0;
     if (64 * i >= a.chunks) continue;
     const int c = lane + 64 * i;
-    const uint32_t n = c < a.chunks ? sh.equal[c] : 0, upto = wave_scan(n, AddCounts()), from = upto - n;
+    const uint32_t n = c < a.chunks ? equal[i] : 0, upto = wave_scan(n, AddCounts()), from = upto - n;
     mine[i] = min(n, left > from ? left - from : 0u);
-    mass[i] = (c < a.chunks ? sh.kept[c] : 0) + mine[i] * one;
+    mass[i] = (c < a.chunks ? kept[i] : 0) + mine[i] * one;
     const uint32_t used = last_lane(upto);
     left = left > used ? left - used : 0;
     all += units_sum(mass[i]);

@@ -93,6 +93,19 @@ def test_against_64_bits(vocab, peaks):
     x.compare(x.run(), least=0.7)
 
 
+@pytest.mark.parametrize("vocab", [253951, 253953, 262144, 1048576])
+def test_large_vocabularies(vocab):
+    """Where the chunks' windows fit into LDS and where they do not, up to the limit."""
+    rng = np.random.default_rng(vocab)
+    b = 10
+    s = settings(rng, b, vocab)
+    s["temp"] = np.full(b, 0.8)
+    s["top_k"][:4] = [50, 1, 400, 0]
+    x = Rows(logits(rng, b, vocab, peaks=30), pad=3, **s)
+    # 4e-6 n of the draws without a filter are too near where all n tokens weigh the same; the peaks weigh e^7 and more of the rest
+    x.compare(x.run(), least=0.3, tol=2e-6)
+
+
 @pytest.mark.parametrize("one", ["top_k", "top_p", "min_p", None])
 def test_each_filter_alone(one):
     rng = np.random.default_rng(7)
@@ -127,14 +140,14 @@ def far_borders(rng, b, vocab):
 @pytest.mark.parametrize("zeros", [0.0, 0.2])
 @pytest.mark.parametrize("vocab", [8191, 8192, 8199, 16385, 100277])
 def test_long_flat_rows(vocab, zeros):
-    """One border far down, which a sample of the row finds: also among zeros of either sign, and with min-p below it."""
+    """One border far down, which a sample of the row finds: also among zeros of either sign, and with min-p's around it."""
     rng = np.random.default_rng(vocab)
     b = 20
     x = rng.standard_normal((b, vocab)) * (0.5 + 0.5 * rng.random((b, 1)))
     x = np.where(rng.random((b, vocab)) < zeros, np.where(rng.random((b, vocab)) < 0.5, 0.0, -0.0), x)
     bits = f2bf_array(x.astype(np.float32).ravel()).reshape(b, vocab)
     top_k, top_p = far_borders(rng, b, vocab)
-    min_p = np.where(np.arange(b) % 5 == 1, 1e-6, 0.0)
+    min_p = np.where(np.arange(b) % 5 == 1, 1e-6, np.where(np.arange(b) % 5 > 2, 0.003 + 0.04 * rng.random(b), 0.0))
     r = Rows(bits, None, top_k, top_p, min_p, rng.random(b))
     # (as above.  A draw is within 2e-6 of one of n tokens' ends with a chance of 4e-6 n, 0.40 of 100277 and 0.07 of 16385; top-p's
     # border, in the half of the rows, is so with about twice that.  Of the most, 0.6 (0.5 + 0.5 0.5) = 0.45 of 20 rows are left,
