@@ -10,8 +10,11 @@
 //
 // A workgroup takes a few tokens: it works out their sines and cosines once, into LDS, for all heads.  Then every group of
 // dim / 8 lanes (a power of two: 80 values take 16 lanes, 10 of them at work) takes one head of one token, 16 bytes a lane; a
-// lane loads its pairs' other halves itself, which are in the same lines.  A head stays within one wave's instructions, so
-// that rotating in place is safe: all of its loads come before its stores.
+// lane has its pairs' other halves from the lane that loaded them (where rot is no multiple of 16, it loads them itself).  A head
+// stays within one wave's instructions, so that rotating in place is safe: all of its loads come before its stores.
+//
+// Memory bounds long batches: 8191 tokens of 48 heads of 128 (201 MB) 40.5 us, 5.0 TB/s, as fast as a copy; 8192 tokens of 40 + 16
+// heads into pages (235 MB) 51 us, 4.6 TB/s.  One token, 2.9 us, waits for one load after another.
 #include <math.h>
 
 #include "agens_kernels.h"
