@@ -342,7 +342,8 @@ __device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t
 // bins.
 template <bool STRAIGHT>
 __device__ __forceinline__ bool count_keys(const Row& r, uint32_t from, Shared& sh) {
-  const uint32_t top = r.first - from, span = (STRAIGHT ? r.first - r.least + 1 : kSpan) - from, all = r.first - r.least + 1 - from;
+  // (the last key that weighs anything may be within the window: nothing is left then)
+  const uint32_t top = r.first - from, all = (uint32_t)max((int)(r.first - r.least + 1) - (int)from, 0), span = STRAIGHT ? all : kSpan - from;
   bool between = false;
   auto add = [&](uint32_t key) {
     const uint32_t d = top - key;

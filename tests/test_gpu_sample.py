@@ -155,6 +155,32 @@ def test_long_flat_rows(vocab, zeros):
     r.compare(r.run(), least=0.15 if vocab > 20000 else 0.5, tol=2e-6)
 
 
+@pytest.mark.parametrize("vocab", [1000, 2617, 8199, 40000])
+def test_borders_behind_all_weights(vocab):
+    """Cold rows: what weighs anything ends within the keys that are counted first, the border of top-k (or of a top-p of all but
+    nothing) is far behind."""
+    rng = np.random.default_rng(vocab)
+    b = 60
+    kind = np.arange(b) % 4
+    top_k = np.where(kind < 3, rng.integers(vocab // 2, vocab, b), 0)
+    top_p = np.where(kind < 2, 0.3 + 0.69 * rng.random(b), np.where(kind == 2, 1.0, np.float32(1 - 2.0 ** -24)))
+    min_p = np.where(kind == 1, 0.01, 0.0)
+    x = logits(rng, b, vocab, peaks=40)
+    x[kind == 2, vocab // 3:] = 0xFF80  # fewer tokens than top-k keeps
+    r = Rows(x, 0.1 + 0.4 * rng.random(b), top_k, top_p, min_p, rng.random(b))
+    r.compare(r.run(), least=0.7, tol=2e-6)
+
+
+def test_top_k_of_more_than_there_are_far_below_zero():
+    """Logits at the lowest finite numbers, below which there are fewer keys than are counted first."""
+    rng = np.random.default_rng(23)
+    b, vocab = 12, 700
+    x = rng.integers(0xFF00, 0xFF80, (b, vocab)).astype(np.uint16)
+    x[:, 50:] = 0xFF80
+    r = Rows(x, 1e37, np.where(np.arange(b) % 2 == 0, 300, 0), np.where(np.arange(b) % 3 == 0, 1.0, 0.7), None, rng.random(b))
+    r.compare(r.run(), least=0.7, tol=2e-6)
+
+
 @pytest.mark.parametrize("kind", ["ascending", "descending", "blocks", "masked", "nan", "equal", "shifted"])
 @pytest.mark.parametrize("vocab", [16384, 65536])
 def test_long_rows_that_a_sample_misjudges(kind, vocab):
