@@ -108,6 +108,13 @@ __device__ __forceinline__ float key_weight(const Heat& s, uint32_t key, float t
   return any_weight(s, logit_of(key), top);
 }
 
+// What a chunk's sum counts in its row's: in 64 bits, since 32 would move all of the chunk's tokens the same way (by 2^-22 of their
+// weight, 2 10^-8 of a row's in all, within which one row of 10^4 has its draw).  0 where its tokens' own weights are.
+__device__ __forceinline__ double chunk_weight(const Heat& s, float l, float top) {
+  const float x = any_weight(s, l, top);
+  return x > 0.0f && l < top ? exp2(((double)l - (double)top) * ((double)s.scale + (double)s.scale_lo)) : (double)x;
+}
+
 struct AddUnits {
   template <int CTRL, int ROWS>
   __device__ __forceinline__ uint64_t step(uint64_t x) const {
@@ -984,7 +991,7 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
 #pragma unroll
   for (int i = kLaneChunks - 1; i >= 0; --i) {
     if (st[i].top == r.top) best = st[i].best;
-    share[i] = st[i].total * (double)any_weight(r.s, st[i].top, r.top);
+    share[i] = 64 * i < a.chunks ? st[i].total * chunk_weight(r.s, st[i].top, r.top) : 0.0;
   }
 #pragma unroll
   for (int i = 0; i < kLaneChunks; ++i) total += share[i];
