@@ -83,6 +83,19 @@ struct SampleArgs {
   uint32_t* counts;  // [b][chunks][kWindow / 2]: pairs of 16 bits, of keys from the chunk's largest down, the first one odd
 };
 
+// A row's.
+struct Settings {
+  float temp, p, least;
+  int limit;     // of top-k; 0: none
+  bool filters;  // any
+};
+__device__ __forceinline__ Settings settings_of(const SampleArgs& a, int id) {
+  const int k = a.top_k ? a.top_k[id] : 0;
+  Settings s{a.temp ? a.temp[id] : 1.0f, a.top_p ? a.top_p[id] : 1.0f, a.min_p ? a.min_p[id] : 0.0f, k > 0 && k < a.vocab ? k : 0, false};
+  s.filters = s.temp > 0.0f && (s.limit || s.p < 1.0f || s.least > 0.0f);
+  return s;
+}
+
 typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 // Keys of two logits: their bits, all inverted where the sign is set, else the sign alone.  -0 has a key of its own, kMinusZero,
@@ -148,9 +161,16 @@ struct Group {
 
 // A chunk, by a group of kGroupThreads threads: see ChunkStat.  bins: where to count its keys (kWindow + 1 zeros), or null.  All
 // threads of the workgroup come here together; a chunk past the last is empty.
-__device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const uint16_t* row, int chunk, int vocab, uint32_t* bins, Group& g) {
+struct ChunkBits {
+  u32x4 v[2];
+};
+__device__ __forceinline__ ChunkBits load_chunk(const uint16_t* row, int chunk, int vocab) {
+  const int at = chunk * kChunk + 8 * (threadIdx.x % kGroupThreads);
+  return ChunkBits{{load_bits(row, at, vocab), load_bits(row, at + kChunk / 2, vocab)}};
+}
+__device__ __forceinline__ ChunkStat chunk_stat(const Heat& s, const ChunkBits& bits, int chunk, uint32_t* bins, Group& g) {
   const int t = threadIdx.x % kGroupThreads, w = t >> 6, at0 = chunk * kChunk + 8 * t, at1 = at0 + kChunk / 2;
-  const u32x4 v[2] = {load_bits(row, at0, vocab), load_bits(row, at1, vocab)};
+  const u32x4 (&v)[2] = bits.v;
   float l[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i) l[i] = value(v[i >> 3], i & 7);
@@ -209,13 +229,16 @@ __global__ void __launch_bounds__(kGroupThreads) sample_keys_kernel(const Sample
   __shared__ Group g;
   __shared__ __attribute__((aligned(16))) uint32_t bins[kWindow + 1];  // (one more: -0 behind 0)
   const int chunk = blockIdx.x, id = blockIdx.y, t = threadIdx.x;
-  const Heat s = heat_of(a.temp ? a.temp[id] : 1.0f);
+  const ChunkBits v = load_chunk(a.logits + (size_t)id * a.ld, chunk, a.vocab);
+  const Settings set = settings_of(a, id);
+  const Heat s = heat_of(set.temp);  // (a division in 64 bits, while these are on their way)
   *reinterpret_cast<uint2*>(bins + 2 * t) = make_uint2(0, 0);  // (a barrier follows before the first count)
   if (t == 0) bins[kWindow] = 0;
-  const ChunkStat r = chunk_stat(s, a.logits + (size_t)id * a.ld, chunk, a.vocab, bins, g);
+  const ChunkStat r = chunk_stat(s, v, chunk, set.filters ? bins : nullptr, g);
   const size_t at = (size_t)id * a.chunks + chunk;
+  if (t == 0) a.stats[at] = r;
+  if (!set.filters) return;  // (nobody reads counts)
   if (t == 0) {
-    a.stats[at] = r;
     const uint32_t d = (key_of_value(r.top) | 1) - kZero;  // the counts of -0
     if (r.top >= 0.0f && d < kWindow) bins[d] += bins[d + 1], bins[d + 1] = 0;
   }
@@ -934,14 +957,12 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   __shared__ Shared sh;
   const int id = blockIdx.x, t = threadIdx.x, lane = t & 63;
   Row r;
-  r.s = heat_of(a.temp ? a.temp[id] : 1.0f);
   r.logits = a.logits + (size_t)id * a.ld;
   r.vocab = a.vocab, r.chunks = a.chunks;
   r.counts = a.counts ? a.counts + (size_t)id * a.chunks * (kWindow / 2) : nullptr;
-  const int k = a.top_k ? a.top_k[id] : 0;
-  const float p = a.top_p ? a.top_p[id] : 1.0f, least = a.min_p ? a.min_p[id] : 0.0f, u = a.u[id];
-  const int limit = k > 0 && k < a.vocab ? k : 0;
-  const bool filters = !r.s.greedy && (limit || p < 1.0f || least > 0.0f), staged = filters && r.counts && a.chunks <= kStaged;
+  const auto [temp, p, least, limit, filters] = settings_of(a, id);
+  const float u = a.u[id];
+  const bool staged = filters && r.counts && a.chunks <= kStaged;
   ChunkStat st[kLaneChunks];
   auto load_stats = [&](const ChunkStat* stats) {
 #pragma unroll
@@ -954,20 +975,22 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   if (staged) {  // beside the statistics
     constexpr int kAt = kPool / 4 / kDraw;
     const uint4* const src = reinterpret_cast<const uint4*>(r.counts);
-    const int all = a.chunks * (kWindow / 8);
+    const int pieces = a.chunks * (kWindow / 8);
     uint4 v[kAt];
 #pragma unroll
-    for (int i = 0; i < kAt; ++i) v[i] = src[min(t + i * kDraw, all - 1)];
+    for (int i = 0; i < kAt; ++i) v[i] = src[min(t + i * kDraw, pieces - 1)];
+    r.s = heat_of(temp);  // (a division in 64 bits, while these are on their way)
 #pragma unroll
     for (int i = 0; i < kAt; ++i) {
       const int e = t + i * kDraw, c = e / (kWindow / 8);
-      reinterpret_cast<uint4*>(sh.bins)[e < all ? (c + 1) * (kSlot / 4) + e % (kWindow / 8) : kPool / 4 - 1] = v[i];  // (or nowhere)
+      reinterpret_cast<uint4*>(sh.bins)[e < pieces ? (c + 1) * (kSlot / 4) + e % (kWindow / 8) : kPool / 4 - 1] = v[i];  // (or nowhere)
     }
   }
+  if (!staged) r.s = heat_of(temp);
   if (!a.stats) {
     for (int c0 = 0; c0 < a.chunks; c0 += kGroups) {
       const int c = c0 + t / kGroupThreads;
-      const ChunkStat x = chunk_stat(r.s, r.logits, min(c, a.chunks), a.vocab, nullptr, sh.g[t / kGroupThreads]);
+      const ChunkStat x = chunk_stat(r.s, load_chunk(r.logits, min(c, a.chunks), a.vocab), min(c, a.chunks), nullptr, sh.g[t / kGroupThreads]);
       if (t % kGroupThreads == 0 && c < a.chunks) sh.stats[c] = x;
     }
     __syncthreads();
