@@ -14,7 +14,7 @@
 // token, row), 2.9 + 4.6 + 5.4 us.  64 tokens of 24 adapters beside q, k and v: the same, 2.9 + 7.5 + 5.5, where the weights' 17 MB
 // are 2.5 at 7 TB/s.  4001 tokens of 27648 inputs and 64 ranks: A x reads 193 MB of x in 56 us (3.4 TB/s) and the weights from L2 as
 // often; without the latter it takes 41, without x 33, and the two do not overlap fully behind one barrier a stage.  The second
-// product moves 82 MB of outputs in 31 us.
+// product moves 82 MB of outputs in 24 us.
 #include "agens_kernels.h"
 #include "wq_common.h"
 
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(256, 2) lora_down_many_kernel(const LoraArgs a
 // N times four sums: their parts from left to right, kLoads loads at a time.
 constexpr int kLoads = 16;
 template <int N>
-__device__ __forceinline__ void add_parts(const float* const (&at)[N], int parts, size_t step, f32x4 (&s)[N]) {
+__device__ __forceinline__ void add_parts(const float* (&at)[N], int parts, size_t step, f32x4 (&s)[N]) {
   constexpr int kAt = kLoads / N;
   for (int c = 0; c < parts; c += kAt) {
     f32x4 x[N][kAt];
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs a) {
   const PlanView p = view(a.plan, a.m, a.adapters);
   const size_t fours = a.ranks / 4, i = (size_t)blockIdx.x * 256 + threadIdx.x, token = i / fours, r = 4 * (i - token * fours);
   if (token >= (size_t)a.m) return;
-  const float* const at[1] = {p.parts + token * a.ranks + r};
+  const float* at[1] = {p.parts + token * a.ranks + r};
   f32x4 s[1] = {};
   add_parts(at, a.parts, (size_t)a.m * a.ranks, s);
   const Halves h = halves(s[0]);
@@ -395,7 +395,7 @@ __device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, 
 }
 
 // A workgroup: a tile's tokens (grid y) and a.rows output rows of a segment (x), 64 at a time a wave.  JOINED: the sums A x are
-// there; otherwise it adds up their parts, into LDS.
+// there; otherwise it adds up their parts.  Into LDS, several loads at a time (16 bytes at a time where they are used: 31 us, not 24).
 constexpr int kUpRows = 256;
 template <int KS, bool JOINED>
 __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
@@ -450,22 +450,50 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   const int stride = a.rank + 8;
   if constexpr (!JOINED) {
     const size_t step = (size_t)a.m * a.ranks;
-    const int fours = a.rank / 4, subs = (t.count + 15) / 16;
-    for (int e = threadIdx.x; e < 16 * subs * fours; e += 256) {  // 4 ranks of a token
-      const int i = e / fours, r = 4 * (e - i * fours);
-      const float* const at[1] = {p.parts + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r};
-      f32x4 s[1] = {};
+    const int fours = a.rank / 4, all = 16 * ((t.count + 15) / 16) * fours;
+    auto some = [&]<int N>(int e0) {  // N times 4 ranks of a token
+      const float* at[N];
+      int to[N];
+      f32x4 s[N] = {};
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int e = min(e0 + 256 * j, all - 1), i = e / fours, r = 4 * (e - i * fours);
+        at[j] = p.parts + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r;
+        to[j] = i * stride + r;
+      }
       add_parts(at, a.parts, step, s);
-      if (i >= t.count) s[0] = f32x4{};
-      const Halves h = halves(s[0]);
-      *reinterpret_cast<uint2*>(sv + i * stride + r) = make_uint2(h.hi[0], h.hi[1]);
-      *reinterpret_cast<uint2*>(sv + (kTile + i) * stride + r) = make_uint2(h.lo[0], h.lo[1]);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (to[j] / stride >= t.count) s[j] = f32x4{};
+        const Halves h = halves(s[j]);
+        *reinterpret_cast<uint2*>(sv + to[j]) = make_uint2(h.hi[0], h.hi[1]);
+        *reinterpret_cast<uint2*>(sv + kTile * stride + to[j]) = make_uint2(h.lo[0], h.lo[1]);
+      }
+    };
+    // four at a time: 256 tokens of 64 ranks 11.8 -> 7.8 us; up to 32 ranks they cost more in registers than they bring (5.9 -> 7.6)
+    if (KS == 1 || all <= 256) {
+      for (int e0 = threadIdx.x; e0 < all; e0 += 256) some.template operator()<1>(e0);
+    } else if constexpr (KS > 1) {
+      for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) some.template operator()<4>(e0);
+    }
+    __syncthreads();
+  } else {
+    const int eights = a.rank / 8, all = 2 * 16 * ((t.count + 15) / 16) * eights;
+    for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) {  // 8 halves of a token, four times
+      u32x4 x[4];
+      int at[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = min(e0 + 256 * j, all - 1), h = e / eights, r = 8 * (e - h * eights), lo = h & 1, i = h >> 1;
+        at[j] = (lo * kTile + i) * stride + r;
+        x[j] = *reinterpret_cast<const u32x4*>(a.sums + (size_t)token_of(p, a, blockIdx.y, i) * 2 * a.ranks + lo * a.ranks + seg * a.rank + r);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(sv + at[j]) = x[j];
     }
     __syncthreads();
   }
   auto s = [&](int sub, int lo, int kk) {
-    if constexpr (JOINED)
-      return load_if(kk < a.rank, a.sums + (size_t)tok[sub] * 2 * a.ranks + lo * a.ranks + seg * a.rank + kk);
     uint4 x = make_uint4(0, 0, 0, 0);
     if (kk < a.rank) x = *reinterpret_cast<const uint4*>(sv + (lo * kTile + 16 * sub + col) * stride + kk);
     return x;
@@ -487,10 +515,11 @@ void down_many(const LoraArgs& l, unsigned tiles, hipStream_t s) {
 }
 template <int KS>
 void up(const LoraArgs& l, unsigned blocks, unsigned tiles, hipStream_t s) {
-  if (l.sums)
-    hipLaunchKernelGGL((lora_up_kernel<KS, true>), dim3(blocks, tiles), dim3(256), 0, s, l);
+  const size_t lds = (size_t)2 * kTile * (l.rank + 8) * 2;
+  if (KS > 1 && l.sums)
+    hipLaunchKernelGGL((lora_up_kernel<KS, (KS > 1)>), dim3(blocks, tiles), dim3(256), lds, s, l);
   else
-    hipLaunchKernelGGL((lora_up_kernel<KS, false>), dim3(blocks, tiles), dim3(256), (size_t)2 * kTile * (l.rank + 8) * 2, s, l);
+    hipLaunchKernelGGL((lora_up_kernel<KS, false>), dim3(blocks, tiles), dim3(256), lds, s, l);
 }
 
 bool sizes_ok(int m, int adapters) {
@@ -557,9 +586,10 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
   else
     agq::down_many<4>(l, tiles, s);
   if (const int e = (int)hipGetLastError()) return e;
-  // a launch more, but workgroups that read finished sums and need no LDS: 4001 tokens of 27648 inputs and 64 ranks 111 -> 104 us, 256
-  // 33 -> 31; of 5120 inputs and 16 ranks (3 parts) 54 -> 56
-  if (many && l.parts * l.rank >= 256) {
+  // A launch more, but parts that are read once and not by every workgroup of outputs.  The two kernels against the one: 4001 tokens
+  // of 27648 inputs and 64 ranks (14 parts) 29 us and 46, 4096 of 5120 and 48 (3 parts) 25 and 28; 2048 of these 17.4 and 18, less
+  // than the launch; 1100 of 5120 and 128 18.7 and 17.6; up to 32 ranks, whose parts are few loads, 28 and 29 at 4096 of 27648.
+  if (many && rank > 32 && l.parts > 1 && (long)m * l.parts * rank >= 500000) {
     l.sums = reinterpret_cast<uint16_t*>(agq::view(plan, m, adapters).parts + (size_t)l.parts * m * l.ranks);
     hipLaunchKernelGGL(agq::lora_join_kernel, dim3((unsigned)(((size_t)m * l.ranks / 4 - 1) / 256 + 1)), dim3(256), 0, s, l);
     if (const int e = (int)hipGetLastError()) return e;

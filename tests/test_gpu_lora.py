@@ -94,6 +94,13 @@ def test_against_64_bits(m, adapters, rank, k, ns):
     j.compare(j.run())
 
 
+@pytest.mark.parametrize("m,adapters,rank,k,ns", [(1800, 3, 64, 9000, [70, 64]), (2600, 2, 40, 9000, [33]), (700, 5, 72, 27648, [17, 1, 80])])
+def test_sums_of_many_tokens_and_parts(m, adapters, rank, k, ns):
+    """Parts that are added up once, ahead of the second product: segments, ranks of no multiple of 32, odd outputs."""
+    j = Job(m + rank, m, adapters, rank, k, ns, pad=m % 3)
+    j.compare(j.run())
+
+
 @pytest.mark.parametrize("pad", [0, 1, 8])
 def test_in_place_and_without_scales(pad):
     j = Job(5, 90, 4, 16, 1024, [500, 40], pad=pad, scale=False, in_place=True)
