@@ -470,8 +470,9 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
         *reinterpret_cast<uint2*>(sv + kTile * stride + to[j]) = make_uint2(h.lo[0], h.lo[1]);
       }
     };
-    // four at a time: 256 tokens of 64 ranks 11.8 -> 7.8 us; up to 32 ranks they cost more in registers than they bring (5.9 -> 7.6)
-    if (KS == 1 || all <= 256) {
+    // four at a time where all their parts are on their way at once: 256 tokens of 64 ranks and 3 parts 11.8 -> 7.8 us (64 of 14 parts
+    // would take 10 and not 8); up to 32 ranks that costs more in registers than it brings (5.9 -> 7.6)
+    if (KS == 1 || all <= 256 || a.parts > kLoads / 4) {
       for (int e0 = threadIdx.x; e0 < all; e0 += 256) some.template operator()<1>(e0);
     } else if constexpr (KS > 1) {
       for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) some.template operator()<4>(e0);
