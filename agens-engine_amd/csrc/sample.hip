@@ -21,10 +21,10 @@
 //                        do, the row's keys are counted anew, all at once, and the chunks' shares summed up in another pass.
 // Without scratch sample_draw_kernel takes the chunks' statistics itself and does without their windows: the same tokens.
 //
-// What bounds them: latency, of loads, barriers and one wave's instructions one after another (1 row of 152064: 4.2 us, and then 4.1
+// What bounds them: latency, of loads, barriers and one wave's instructions one after another (1 row of 152064: 3.7 us, and then 4.2
 // without a filter, 8.6 with one, of which 1.4 the first loads, 1.3 the windows, 1.1 the border, 1.4 the chunks' shares and 2 the
-// draw; 32 rows: 5.7 + 11 us, where 9.7 MB at 7 TB/s are 1.4); and instructions where a border is far down: 25 a logit by one
-// workgroup, 1 row of 152064 50 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 61 us and 87.
+// draw; 32 rows: 5.8 + 11 us, where 9.7 MB at 7 TB/s are 1.4); and instructions where a border is far down: 25 a logit by one
+// workgroup, 1 row of 152064 50 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 63 us and 87.
 #include "agens_kernels.h"
 #include "logits.h"
 
