@@ -6,8 +6,8 @@
 // page, which finds its sequence by bisecting the sums.  So do tokens.
 //
 // All of it is a chain of round trips to memory and barriers: 2.1 us for one sequence, 7.2 and 3.7 for 200 with 20000 new tokens,
-// whose 0.2 MB are nothing.  Few sequences take four waves instead of sixteen, whose barriers are shorter.  Inputs and outputs may be the same arrays: every thread has read its sequence's
-// numbers before the first barrier, and nothing is written before it.
+// whose 0.2 MB are nothing.  Few sequences take four waves instead of sixteen, whose barriers are shorter.  Inputs and outputs may be
+// the same arrays: every thread has read its sequence's numbers before the first barrier, and nothing is written before it.
 #include "agens_kernels.h"
 #include "kv_page.h"
 #include "logits.h"

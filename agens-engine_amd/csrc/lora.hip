@@ -375,7 +375,8 @@ __device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int se
 
 // Pieces [c0, c0 + width) of a tile's rows, eight in flight a thread.
 template <class T>
-__device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, const Tile& t, const void* from, void* to, int c0, int width, long ld) {
+__device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, const Tile& t, const void* from, void* to, int c0,
+                                          int width, long ld) {
   const T* const src = static_cast<const T*>(from) + c0;
   T* const dst = static_cast<T*>(to) + c0;
   const int all = t.count * width;
@@ -487,7 +488,8 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
       for (int j = 0; j < 4; ++j) {
         const int e = min(e0 + 256 * j, all - 1), h = e / eights, r = 8 * (e - h * eights), lo = h & 1, i = h >> 1;
         at[j] = (lo * kTile + i) * stride + r;
-        x[j] = *reinterpret_cast<const u32x4*>(a.sums + (size_t)token_of(p, a, blockIdx.y, i) * 2 * a.ranks + lo * a.ranks + seg * a.rank + r);
+        const size_t row = (size_t)token_of(p, a, blockIdx.y, i) * 2 * a.ranks;
+        x[j] = *reinterpret_cast<const u32x4*>(a.sums + row + lo * a.ranks + seg * a.rank + r);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(sv + at[j]) = x[j];

@@ -373,7 +373,8 @@ __device__ __forceinline__ Bins<false> count_window(const Row& r, const uint32_t
 template <bool STRAIGHT>
 __device__ __forceinline__ bool count_keys(const Row& r, uint32_t from, Shared& sh) {
   // (the last key that weighs anything may be within the window: nothing is left then)
-  const uint32_t top = r.first - from, all = (uint32_t)max((int)(r.first - r.least + 1) - (int)from, 0), span = STRAIGHT ? all : kSpan - from;
+  const uint32_t top = r.first - from, all = (uint32_t)max((int)(r.first - r.least + 1) - (int)from, 0);
+  const uint32_t span = STRAIGHT ? all : kSpan - from;
   bool between = false;
   auto add = [&](uint32_t key) {
     const uint32_t d = top - key;
@@ -515,7 +516,8 @@ __device__ __forceinline__ bool find(const Row& r, const Bins<WIDE>& b, int k, f
     }
     __syncthreads();
     // (top-k's own border where a rounding of the goal would go past it)
-    if (!found || sh.border.key > out.key || (sh.border.key == out.key && sh.border.n < out.n)) out.key = sh.border.key, out.n = sh.border.n;
+    if (!found || sh.border.key > out.key || (sh.border.key == out.key && sh.border.n < out.n))
+      out.key = sh.border.key, out.n = sh.border.n;
     found = true;
   }
   return found;
@@ -761,7 +763,8 @@ __device__ __forceinline__ Sampled find_sampled(const Row& r, int k, float p, Bo
         count += __builtin_popcountll(over[i]);
         const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in[i] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[i], listed));
         // (what is not listed goes behind the list: a branch takes longer)
-        list[__builtin_amdgcn_inverse_ballot_w64(in[i]) ? at : (uint32_t)kList + lane] = (uint16_t)(i & 1 ? v[j][i >> 1] >> 16 : v[j][i >> 1]);
+        const uint32_t bits = v[j][i >> 1] >> (16 * (i & 1));
+        list[__builtin_amdgcn_inverse_ballot_w64(in[i]) ? at : (uint32_t)kList + lane] = (uint16_t)bits;
         listed += __builtin_popcountll(in[i]);
       }
     }
@@ -989,8 +992,8 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   if (!staged) r.s = heat_of(temp);
   if (!a.stats) {
     for (int c0 = 0; c0 < a.chunks; c0 += kGroups) {
-      const int c = c0 + t / kGroupThreads;
-      const ChunkStat x = chunk_stat(r.s, load_chunk(r.logits, min(c, a.chunks), a.vocab), min(c, a.chunks), nullptr, sh.g[t / kGroupThreads]);
+      const int c = min(c0 + t / kGroupThreads, a.chunks);
+      const ChunkStat x = chunk_stat(r.s, load_chunk(r.logits, c, a.vocab), c, nullptr, sh.g[t / kGroupThreads]);
       if (t % kGroupThreads == 0 && c < a.chunks) sh.stats[c] = x;
     }
     __syncthreads();
