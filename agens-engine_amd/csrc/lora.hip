@@ -5,8 +5,8 @@
 //   lora_down_few_kernel, lora_down_many_kernel   s = A x on MFMA (bf16, sums in fp32), a part for every kGroup chunks of kChunk
 //                      inputs: 16 tokens and ranks a workgroup, or a tile and up to 64 ranks with the weights through LDS;
 //   lora_join_kernel   the parts' sums, where there are many tokens and parts; otherwise
-//   lora_up_kernel     adds the parts up, and y = y0 + scale (B s): s enters the MFMA as two bf16 operands, which hold 16 bits of
-//                      it (one alone would move y by 2^-9 of what is added).
+//   lora_up_kernel     adds the parts up, and y = y0 + scale (B s): s enters the MFMA as three bf16 operands, which hold all 24 bits
+//                      of it (one alone would move y by 2^-9 of what is added, two by 2^-17).
 // A chunk's products are one chain of MFMA, the chunks' sums are added up by fours and then from left to right, whoever does it: a
 // token's bits do not depend on the other tokens of the call.
 //
@@ -144,7 +144,7 @@ struct LoraArgs {
   long ldx;
   int m, adapters, k, rank, ranks, nseg;
   int parts;           // of the sums A x: one for each kGroup chunks
-  uint16_t* sums;      // these, behind the parts, or null: lora_up_kernel adds the parts up itself
+  float* sums;         // these, behind the parts, or null: lora_up_kernel adds the parts up itself
   int rows, wide;      // output rows of a workgroup; bit i: segment i's rows of y and y0 are 16-byte aligned
 };
 
@@ -283,22 +283,23 @@ __device__ __forceinline__ void add_parts(const float* (&at)[N], int parts, size
   }
 }
 
-// What fp32 holds of a sum in two bf16, to 16 bits (nothing in the second beside infinities and NaN).
-struct Halves {
-  uint32_t hi[2], lo[2];  // of four sums
-};
-__device__ __forceinline__ Halves halves(const f32x4 s) {
-  Halves h;
+// What fp32 holds of four sums in kSplit bf16 each (nothing past the first beside infinities and NaN), into rows `step` apart.
+constexpr int kSplit = 3;
+__device__ __forceinline__ void split(f32x4 s, uint16_t* to, int step) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    h.hi[i] = f2bf2(s[2 * i], s[2 * i + 1]);
-    const float x = bf2f(h.hi[i] & 0xFFFFu), y = bf2f(h.hi[i] >> 16);
-    h.lo[i] = f2bf2(fabsf(x) < INFINITY ? s[2 * i] - x : 0.0f, fabsf(y) < INFINITY ? s[2 * i + 1] - y : 0.0f);
+  for (int j = 0; j < kSplit; ++j) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = f2bf2(s[2 * i], s[2 * i + 1]);
+      const float x = bf2f(w[i] & 0xFFFFu), y = bf2f(w[i] >> 16);
+      s[2 * i] = fabsf(x) < INFINITY ? s[2 * i] - x : 0.0f, s[2 * i + 1] = fabsf(y) < INFINITY ? s[2 * i + 1] - y : 0.0f;
+    }
+    *reinterpret_cast<uint2*>(to + j * step) = make_uint2(w[0], w[1]);
   }
-  return h;
 }
 
-// The sums of every token from their parts: [token][first halves, second halves][ranks].
+// The sums of every token from their parts: [token][ranks].
 __global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs a) {
   const PlanView p = view(a.plan, a.m, a.adapters);
   const size_t fours = a.ranks / 4, i = (size_t)blockIdx.x * 256 + threadIdx.x, token = i / fours, r = 4 * (i - token * fours);
@@ -306,10 +307,7 @@ __global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs a) {
   const float* at[1] = {p.parts + token * a.ranks + r};
   f32x4 s[1] = {};
   add_parts(at, a.parts, (size_t)a.m * a.ranks, s);
-  const Halves h = halves(s[0]);
-  uint16_t* const out = a.sums + token * 2 * a.ranks + r;
-  *reinterpret_cast<uint2*>(out) = make_uint2(h.hi[0], h.hi[1]);
-  *reinterpret_cast<uint2*>(out + a.ranks) = make_uint2(h.lo[0], h.lo[1]);
+  *reinterpret_cast<f32x4*>(a.sums + token * a.ranks + r) = s[0];
 }
 
 // 16 outputs of a token, 8 from c on and 8 from c + 32 on: y = y0 + scale acc.  WIDE: both rows 16-byte aligned, all 64 outputs
@@ -348,8 +346,8 @@ __device__ __forceinline__ void store_out(uint16_t* y, int c, int n, float scale
   }
 }
 
-// 64 output rows of a segment by one wave, for all tokens of a tile: KS steps of 32 ranks.  v: the outputs before; s(sub, lo, kk):
-// 8 halves of a token's sums.
+// 64 output rows of a segment by one wave, for all tokens of a tile: KS steps of 32 ranks.  v: the outputs before; s(sub, j, kk):
+// the j-th bf16 of 8 of a token's sums.
 template <int KS, bool WIDE, class S>
 __device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int seg, int wn, float scale, S s,
                                         const uint4 (&bv)[KS][4], const int (&tok)[kTile / 16], const uint32_t (&v)[kTile / 16][8]) {
@@ -362,12 +360,13 @@ __device__ __forceinline__ void up_rows(const LoraArgs& a, const Tile& t, int se
     f32x4 acc[4] = {};
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const uint4 hi = s(sub, 0, 32 * k + 8 * quad), lo = s(sub, 1, 32 * k + 8 * quad);
+      uint4 x[kSplit];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[k][i]), frag(lo), acc[i], 0, 0, 0);
-        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[k][i]), frag(hi), acc[i], 0, 0, 0);
-      }
+      for (int j = 0; j < kSplit; ++j) x[j] = s(sub, j, 32 * k + 8 * quad);
+#pragma unroll
+      for (int j = kSplit - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(frag(bv[k][i]), frag(x[j]), acc[i], 0, 0, 0);
     }
     if (16 * sub + col < t.count) store_out<WIDE>(y + tok[sub] * ldy, c, n, scale, v[sub], acc);
   }
@@ -400,7 +399,7 @@ __device__ __forceinline__ void copy_rows(const PlanView& p, const LoraArgs& a, 
 constexpr int kUpRows = 256;
 template <int KS, bool JOINED>
 __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [halves][kTile][rank + 8]
+  extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [kSplit][kTile][rank + 8]
   const PlanView p = view(a.plan, a.m, a.adapters);
   const Tile t = tile_of(p, a, blockIdx.y);
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
@@ -466,9 +465,7 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         if (to[j] / stride >= t.count) s[j] = f32x4{};
-        const Halves h = halves(s[j]);
-        *reinterpret_cast<uint2*>(sv + to[j]) = make_uint2(h.hi[0], h.hi[1]);
-        *reinterpret_cast<uint2*>(sv + kTile * stride + to[j]) = make_uint2(h.lo[0], h.lo[1]);
+        split(s[j], sv + to[j], kTile * stride);
       }
     };
     // four at a time where all their parts are on their way at once: 256 tokens of 64 ranks and 3 parts 11.8 -> 7.8 us (64 of 14 parts
@@ -480,25 +477,24 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
     }
     __syncthreads();
   } else {
-    const int eights = a.rank / 8, all = 2 * 16 * ((t.count + 15) / 16) * eights;
-    for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) {  // 8 halves of a token, four times
-      u32x4 x[4];
-      int at[4];
+    const int fours = a.rank / 4, all = 16 * ((t.count + 15) / 16) * fours;
+    for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) {  // 4 sums of a token, four times
+      f32x4 x[4];
+      int to[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = min(e0 + 256 * j, all - 1), h = e / eights, r = 8 * (e - h * eights), lo = h & 1, i = h >> 1;
-        at[j] = (lo * kTile + i) * stride + r;
-        const size_t row = (size_t)token_of(p, a, blockIdx.y, i) * 2 * a.ranks;
-        x[j] = *reinterpret_cast<const u32x4*>(a.sums + row + lo * a.ranks + seg * a.rank + r);
+        const int e = min(e0 + 256 * j, all - 1), i = e / fours, r = 4 * (e - i * fours);
+        to[j] = i * stride + r;
+        x[j] = *reinterpret_cast<const f32x4*>(a.sums + (size_t)token_of(p, a, blockIdx.y, i) * a.ranks + seg * a.rank + r);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) *reinterpret_cast<u32x4*>(sv + at[j]) = x[j];
+      for (int j = 0; j < 4; ++j) split(x[j], sv + to[j], kTile * stride);
     }
     __syncthreads();
   }
-  auto s = [&](int sub, int lo, int kk) {
+  auto s = [&](int sub, int j, int kk) {
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (kk < a.rank) x = *reinterpret_cast<const uint4*>(sv + (lo * kTile + 16 * sub + col) * stride + kk);
+    if (kk < a.rank) x = *reinterpret_cast<const uint4*>(sv + (j * kTile + 16 * sub + col) * stride + kk);
     return x;
   };
   for (; wn < n1; wn += kUpRows) {
@@ -518,7 +514,7 @@ void down_many(const LoraArgs& l, unsigned tiles, hipStream_t s) {
 }
 template <int KS>
 void up(const LoraArgs& l, unsigned blocks, unsigned tiles, hipStream_t s) {
-  const size_t lds = (size_t)2 * kTile * (l.rank + 8) * 2;
+  const size_t lds = (size_t)kSplit * kTile * (l.rank + 8) * 2;
   if (KS > 1 && l.sums)
     hipLaunchKernelGGL((lora_up_kernel<KS, (KS > 1)>), dim3(blocks, tiles), dim3(256), lds, s, l);
   else
@@ -593,7 +589,7 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
   // of 27648 inputs and 64 ranks (14 parts) 29 us and 46, 4096 of 5120 and 48 (3 parts) 25 and 28; 2048 of these 17.4 and 18, less
   // than the launch; 1100 of 5120 and 128 18.7 and 17.6; up to 32 ranks, whose parts are few loads, 28 and 29 at 4096 of 27648.
   if (many && rank > 32 && l.parts > 1 && (long)m * l.parts * rank >= 500000) {
-    l.sums = reinterpret_cast<uint16_t*>(agq::view(plan, m, adapters).parts + (size_t)l.parts * m * l.ranks);
+    l.sums = agq::view(plan, m, adapters).parts + (size_t)l.parts * m * l.ranks;
     hipLaunchKernelGGL(agq::lora_join_kernel, dim3((unsigned)(((size_t)m * l.ranks / 4 - 1) / 256 + 1)), dim3(256), 0, s, l);
     if (const int e = (int)hipGetLastError()) return e;
   }

@@ -376,7 +376,7 @@ int ak_sample(const void* logits, long ld, const float* temperature, const int* 
  * [adapters][n[i]][rank]; rank a multiple of 8 up to AK_LORA_MAX_RANK (pad with zeros), k a multiple of 8; x bf16 [m] rows of
  * stride ldx (a multiple of 8); a, b[i] and x 16-byte aligned; y[i] and base[i] bf16 of row stride ldy[i] (0, or ldy NULL:
  * n[i]).  base (the linear's outputs) NULL, or base[i] the same as y[i]: added in place; they may overlap in no other way.
- * scale [adapters] fp32 in device memory (NULL: 1).  Sums are fp32; A x is rounded to 16 bits before B, y once to bf16; a
+ * scale [adapters] fp32 in device memory (NULL: 1).  Sums are fp32, A x among them, y is rounded once to bf16; a
  * token's bits do not depend on the other tokens.
  * ak_lora_plan groups the tokens by adapter, once for all linears of a step, into `plan`: 16-byte aligned device memory of
  * ak_lora_plan_bytes(m, adapters, nseg * rank, k) bytes, the most over these linears (0: refused).  It also holds what

@@ -199,3 +199,29 @@ def test_two_streams_with_plans_of_their_own():
             check(j.add(st.h))
     for j in jobs:
         j.compare(j.got())
+
+
+@pytest.mark.parametrize("m,rank,k", [(1, 16, 64), (3, 16, 5120), (70, 8, 1024), (700, 32, 9224), (700, 64, 9224), (1800, 64, 9000),
+                                      (1800, 72, 9000)])
+def test_sums_enter_the_second_product_with_24_bits(m, rank, k):
+    """A sum s = p0 + p1 + p2 of three bf16, from which the second product takes p1 and the base takes p0: p2 is left, which lies
+    below the 16 bits of two bf16.  All of it is exact in fp32 but for the last sums' order: four roundings of s at most."""
+    rng = np.random.default_rng(m + rank)
+    s = (np.float32(1) + rng.random(m).astype(np.float32) * np.float32(0.9)) * np.float32(2) ** rng.integers(-20, 20, m).astype(np.float32)
+    part, left = [], s
+    for _ in range(3):
+        part.append(f2bf_array(left))
+        left = left - bf2f_array(part[-1])
+    assert (left == 0).all() and (np.abs(bf2f_array(part[2])) > 8 * 2.0 ** -24 * s).any()
+    j = Job(30, m, 2, rank, k, [9], ids=[t % 2 for t in range(m)], scale=False)
+    x, a, b = np.zeros((m, k), dtype=np.uint16), np.zeros((2, rank, k), dtype=np.uint16), np.zeros((2, 9, rank), dtype=np.uint16)
+    one, at = 0x3F80, [0, k // 3, k // 2, k - 1]
+    for i, p in zip(at, part + [part[1] ^ 0x8000]):
+        x[:, i] = p
+    a[:, 0, at[:3]], a[:, rank - 1, at[3]] = one, one
+    b[:, :, 0], b[:, :, rank - 1] = one, one
+    base = np.repeat((part[0] ^ 0x8000)[:, None], 9, axis=1)
+    j.X, j.A, j.B, j.Z = Dev.of(x), Dev.of(a), [Dev.of(b)], [Dev.of(base)]
+    y = bf2f_array(j.run()[0]).astype(np.float64).reshape(m, 9)
+    want = bf2f_array(part[2]).astype(np.float64)[:, None]
+    assert (np.abs(y - want) <= 4 * 2.0 ** -24 * s[:, None]).all()
