@@ -155,12 +155,14 @@ __device__ __forceinline__ uint4 load_if(bool in, const uint16_t* p) {
 }
 __device__ __forceinline__ bf16x8 frag(uint4 v) { return __builtin_bit_cast(bf16x8, v); }
 
-// A tile of a plan that was made for this call; count 0 past the last.  (Both loads go out at once.)
-__device__ __forceinline__ Tile tile_of(const PlanView& p, const LoraArgs& a, int i) {
+// Whether a plan was made for a call of these sizes; nothing else of another one's memory is read or written, which may be shorter.
+__device__ __forceinline__ bool made_for(const PlanHead& head, const LoraArgs& a) {
+  return head.m == a.m && head.adapters == a.adapters;
+}
+// Whether it has a tile.
+__device__ __forceinline__ bool has_tile(const PlanView& p, const LoraArgs& a, int tile) {
   const PlanHead head = *p.head;
-  Tile t = p.tiles[i];
-  if (head.m != a.m || head.adapters != a.adapters || i >= head.tiles) t.count = 0;
-  return t;
+  return made_for(head, a) && tile < head.tiles;
 }
 // The token in place i of a tile; any token's where the tile has none.
 __device__ __forceinline__ int token_of(const PlanView& p, const LoraArgs& a, int tile, int i) {
@@ -173,7 +175,8 @@ __global__ void __launch_bounds__(64 * kGroup) lora_down_few_kernel(const LoraAr
   constexpr int kSteps = kChunk / 32;
   __shared__ f32x4 sums[kGroup][64];
   const PlanView p = view(a.plan, a.m, a.adapters);
-  const Tile t = tile_of(p, a, blockIdx.x);
+  if (!has_tile(p, a, blockIdx.x)) return;
+  const Tile t = p.tiles[blockIdx.x];
   const int blocks = (a.ranks + 15) / 16, sub = blockIdx.z / blocks, r0 = (blockIdx.z - sub * blocks) * 16;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, quad = lane >> 4;
   const int token = token_of(p, a, blockIdx.x, 16 * sub + col);
@@ -208,11 +211,12 @@ template <int RT>
 __global__ void __launch_bounds__(256, 2) lora_down_many_kernel(const LoraArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][16 * RT * kRow];
   const PlanView p = view(a.plan, a.m, a.adapters);
-  const Tile t = tile_of(p, a, blockIdx.x);
+  if (!has_tile(p, a, blockIdx.x)) return;
+  const Tile t = p.tiles[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quad = lane >> 4, sub = tid >> 6;
   const int r0 = blockIdx.z * 16 * RT;
   const int token = token_of(p, a, blockIdx.x, 16 * sub + col);
-  if (t.adapter < 0 || t.count == 0) return;
+  if (t.adapter < 0) return;
   const uint16_t* const x = a.x + token * a.ldx;
   const bool mine = 16 * sub < t.count;
   const uint16_t* const w = a.a + (size_t)t.adapter * a.ranks * a.k;
@@ -303,7 +307,7 @@ __device__ __forceinline__ void split(f32x4 s, uint16_t* to, int step) {
 __global__ void __launch_bounds__(256) lora_join_kernel(const LoraArgs a) {
   const PlanView p = view(a.plan, a.m, a.adapters);
   const size_t fours = a.ranks / 4, i = (size_t)blockIdx.x * 256 + threadIdx.x, token = i / fours, r = 4 * (i - token * fours);
-  if (token >= (size_t)a.m) return;
+  if (token >= (size_t)a.m || !made_for(*p.head, a)) return;
   const float* at[1] = {p.parts + token * a.ranks + r};
   f32x4 s[1] = {};
   add_parts(at, a.parts, (size_t)a.m * a.ranks, s);
@@ -401,12 +405,12 @@ template <int KS, bool JOINED>
 __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint16_t sv[];  // [kSplit][kTile][rank + 8]
   const PlanView p = view(a.plan, a.m, a.adapters);
-  const Tile t = tile_of(p, a, blockIdx.y);
+  if (!has_tile(p, a, blockIdx.y)) return;
+  const Tile t = p.tiles[blockIdx.y];
   const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
   int tok[kTile / 16];
 #pragma unroll
   for (int i = 0; i < kTile / 16; ++i) tok[i] = token_of(p, a, blockIdx.y, 16 * i + col);
-  if (t.count == 0) return;
   int seg = 0;
   while (seg < a.nseg - 1 && (int)blockIdx.x >= a.end[seg]) ++seg;
   const int n = a.n[seg], n0 = ((int)blockIdx.x - (seg ? a.end[seg - 1] : 0)) * a.rows, n1 = min(n0 + a.rows, n);

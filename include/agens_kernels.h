@@ -381,7 +381,7 @@ int ak_sample(const void* logits, long ld, const float* temperature, const int* 
  * ak_lora_plan groups the tokens by adapter, once for all linears of a step, into `plan`: 16-byte aligned device memory of
  * ak_lora_plan_bytes(m, adapters, nseg * rank, k) bytes, the most over these linears (0: refused).  It also holds what
  * ak_lora_add's launches hand on, so calls with one plan must follow one another; ak_lora_add with other m or adapters than
- * the plan's leaves y alone.  Only launches, allocates nothing, can be captured. */
+ * the plan's leaves y alone, and reads and writes nothing of the plan's memory but its first 16 bytes.  Only launches, allocates nothing, can be captured. */
 #define AK_LORA_MAX_RANK 128
 #define AK_LORA_MAX_ADAPTERS 4096
 #define AK_LORA_MAX_TOKENS 1048576

@@ -225,3 +225,24 @@ def test_sums_enter_the_second_product_with_24_bits(m, rank, k):
     y = bf2f_array(j.run()[0]).astype(np.float64).reshape(m, 9)
     want = bf2f_array(part[2]).astype(np.float64)[:, None]
     assert (np.abs(y - want) <= 4 * 2.0 ** -24 * s[:, None]).all()
+
+
+@pytest.mark.parametrize("m,adapters", [(40, 3), (1, 3), (0, 3), (1799, 3), (1801, 3), (1800, 2), (1800, 600), (3000, 3)])
+@pytest.mark.parametrize("calls", [(1800, 64, 9000), (700, 16, 9224), (30, 16, 256)])
+def test_memory_past_a_plan_of_other_sizes_stays(m, adapters, calls):
+    """A plan of m tokens and `adapters`, and a call of other sizes in all of its launches' forms (joined sums, many tokens, few):
+    the outputs stay, and so does all behind the plan's own memory, which here goes on for the call's needs."""
+    n, rank, k = calls
+    j = Job(40, n, 3, rank, k, [70])
+    own = step().ak_lora_plan_bytes(m, adapters, rank, k)
+    room = max(own, j.size) + 64
+    j.P = Dev.of(np.full(room, 0xA5, dtype=np.uint8))
+    ids = Dev.of(i32(np.arange(max(m, 1)) % adapters))
+    check(step().ak_lora_plan(ids.p, m, adapters, j.P.p, None))
+    check(step().ak_synchronize())
+    before = j.P.get(np.uint8, room)
+    assert (before[own:] == 0xA5).all()
+    check(j.add())
+    check(step().ak_synchronize())
+    assert np.array_equal(j.P.get(np.uint8, room), before)
+    assert (j.Y[0].get(np.uint16, n * j.ldy[0]) == FILL).all()
