@@ -1028,7 +1028,7 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
     if (t == 0) store(a, id, r, r.best);
     return;
   }
-  Border b{0, 0, least > 0.0f ? fminf(least, 1.0f) : 0.0f};
+  Border b{0, 0, 0.0f};
   if (!filters) {  // no filter: the chunk from their own sums
     double at = (double)u * r.total, before = 0.0, c = 0.0;
     int chunk = -1;
@@ -1048,12 +1048,14 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
     draw_in(a, id, r, max(chunk, 0), b, 0, fmax(at - before, 0.0), sh);  // (the largest has a weight: there is a chunk)
     return;
   }
+  // (weights below a unit are nothing in the sums, so their tokens are not drawn either, whatever shares their chunk)
+  b.least = fmaxf(least > 0.0f ? fminf(least, 1.0f) : 0.0f, 1.0f / kUnit);
   if (staged) __syncthreads();
   bool quick = r.counts != nullptr;
   Bins<false> window{0};
   if (quick) {
-    // whether min-p's border is within the window: then no other that is further down matters (where top-p's may be within it
-    // though top-k's is not, that has to be known)
+    // whether min-p's border, or the end of what weighs a unit, is within the window: then no border that is further down matters
+    // (where top-p's may be within it though top-k's is not, that has to be known)
     const bool cut = r.first < kWindow || key_weight(r.s, r.base - (kWindow - 1), r.top) < b.least;
     bool found = false;
     if (limit || p < 1.0f) {

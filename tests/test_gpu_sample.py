@@ -429,3 +429,41 @@ def test_captured_without_and_with_scratch():
     r = subprocess.run([sys.executable, "-c", "import test_gpu_sample as t; t.captured_before_any_call()"], cwd=HERE,
                        capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr
+
+
+def faint_tokens(vocab):
+    """Rows of a token that weighs 2^-45 of the largest at either end, the largest, and, in every other row, one of 2^-39.5 beside
+    it, with u at either end and each filter; the tokens drawn."""
+    faint, some, top = f2bf_array(np.array([8.8125, 12.625, 40.0], dtype=np.float32))
+    filters = [(5, 1.0, 0.0), (0, 1 - 2.0 ** -24, 0.0), (0, 1.0, 1e-20), (vocab - 1, 0.9999999, 1e-25), (0, 1.0, 0.0)]
+    x, at = np.full((4 * len(filters), vocab), 0xFF80, dtype=np.uint16), vocab // 2
+    x[:, 0], x[:, -1], x[:, at] = faint, faint, top
+    x[1::2, at - 1] = some
+    k, p, m = (np.repeat(v, 4) for v in zip(*filters))
+    u = np.tile(np.float32([0, 0, 1 - 2.0 ** -24, 1 - 2.0 ** -24]), len(filters))
+    # (top-p's front, all but 2^-24 of the weights, is the largest alone)
+    return Rows(x, None, k, p, m, u), [t for f in filters[:-1] for t in (at, at if f[1] < 1 else at - 1, at, at)] + [0, 0, at, at]
+
+
+@pytest.mark.parametrize("vocab", [10, 1000, 4097, 9000, 300001])
+def test_tokens_below_a_unit_are_not_drawn_where_a_filter_is_on(vocab):
+    """Below 2^-40 of the largest weight, whether the token shares a chunk with heavier ones or not.  Without a filter u = 0 draws it."""
+    r, want = faint_tokens(vocab)
+    assert r.run()[0].tolist() == want
+
+
+def faint_tokens_before_any_call():
+    for vocab in (1000, 9000, 300001):
+        r, want = faint_tokens(vocab)
+        s = Stream()
+        g = Graph(s, r.call)
+        g.launch()
+        s.sync()
+        assert r.got()[0].tolist() == want, vocab
+    print("captured: the same")
+
+
+def test_tokens_below_a_unit_without_scratch():
+    r = subprocess.run([sys.executable, "-c", "import test_gpu_sample as t; t.faint_tokens_before_any_call()"], cwd=HERE,
+                       capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr
