@@ -435,6 +435,9 @@ __device__ __forceinline__ bool count_all(Row& r, const Bins<false>* window, Sha
     const uint32_t zero = bin_of(r, kZero);
     if (zero >= from) sh.bins[zero] += sh.bins[zero + 1];
     if (zero + 1 >= from) sh.bins[zero + 1] = 0;
+  } else if (threadIdx.x == 0 && !r.straight && r.low == kMinusZero) {  // and where its bin is the first past zero's own
+    sh.bins[kSpan] += sh.bins[kSpan + 1];
+    sh.bins[kSpan + 1] = 0;
   }
   __syncthreads();
   return sh.between == 0;

@@ -467,3 +467,24 @@ def test_tokens_below_a_unit_without_scratch():
     r = subprocess.run([sys.executable, "-c", "import test_gpu_sample as t; t.faint_tokens_before_any_call()"], cwd=HERE,
                        capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "the same" in r.stdout, r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("step", range(-3, 4))
+@pytest.mark.parametrize("top_k", [700, 2500])
+def test_zeros_where_the_bins_of_the_least_keys_begin(step, top_k):
+    """Logits and temperatures so small that all keys do not fit the bins, 4096 keys and more between the largest and 0, and the
+    keys around -0 the first of the bins of the least: borders among zeros of either sign."""
+    rng = np.random.default_rng(24)
+    vocab = 4000
+    x = np.full(vocab, 0x9000, dtype=np.uint16)  # (-2^-95, 0 but for one in 2^44)
+    x[10:3000] = np.where(rng.random(2990) < 0.5, 0x8000, 0x0000)
+    x[5] = 0x1020
+    top, least = bf2f_array(x[5:6])[0].astype(np.float64), 0x0FFD + step
+    temp = np.float32((top + bf2f_array(np.uint16([least]))[0] * (1 + 2.0 ** -9)) / 31)
+    # zeros weigh e^-17.3 of the largest each, their kept ones (top_k - 1) times that; u is a multiple of 2^-24, two of them
+    w = np.exp(-top / np.float64(temp))
+    u = np.float32([1 - f * (top_k - 1) * w for f in (0.9, 0.77, 0.6, 0.47, 0.34, 0.2, 0.1, 0.04)] + [0.1])
+    b = len(u)
+    r = Rows(np.tile(x, (b, 1)), temp, top_k, np.where(np.arange(b) % 4 == 1, 1 - 2.0 ** -24, 1.0), None, u)
+    # weights lose less than a unit of 2^-40 each: 2500 of them 2.3e-9, a tenth of a token
+    r.compare(r.run(), least=0.5, tol=3e-9)
