@@ -729,7 +729,7 @@ __device__ __forceinline__ Sampled find_sampled(const Row& r, int k, float p, Bo
   q.least = max(key_of_value(r.top - span + (after + 1) / fine), kLowest + 2) - 1;
   q.low = q.least + (kSpan - 2);
   q.straight = q.low + kSpan >= q.first;
-  if (key_weight(r.s, q.first, r.top) < out.least) return Sampled::kBehind;
+  if (out.least > 1.0f / kUnit && key_weight(r.s, q.first, r.top) < out.least) return Sampled::kBehind;
   if (count > 0.8 * part * (kWaves * kListed) || q.least > q.first) return Sampled::kNot;
 
   const float highest = logit_of(q.first), lowest = logit_of(q.least);
