@@ -1077,11 +1077,11 @@ __global__ void __launch_bounds__(kDraw, 4) sample_draw_kernel(const SampleArgs 
   } else {
     const bool one = (limit != 0) != (p < 1.0f) && a.vocab >= kSample && r.top < INFINITY;
     Sampled how = one ? find_sampled(r, limit, p, b, sh) : Sampled::kNot;
-    if (how == Sampled::kBehind) {
+    if (how == Sampled::kBehind && !limit) {  // (of top-k's, weights do not say it)
       chunk_masses(r, b, sh);
       uint64_t all = 0;
       for (int i = lane; i < a.chunks; i += 64) all += sh.kept[i];
-      if (!limit && units_sum(all) < goal_of(p, r.total * (double)kUnit)) how = Sampled::kFound;  // so it is: no border but min-p's
+      if (units_sum(all) < goal_of(p, r.total * (double)kUnit)) how = Sampled::kFound;  // so it is: no border but min-p's
     }
     if (how != Sampled::kFound) {
       if (limit || p < 1.0f) {

@@ -488,3 +488,19 @@ def test_zeros_where_the_bins_of_the_least_keys_begin(step, top_k):
     r = Rows(np.tile(x, (b, 1)), temp, top_k, np.where(np.arange(b) % 4 == 1, 1 - 2.0 ** -24, 1.0), None, u)
     # weights lose less than a unit of 2^-40 each: 2500 of them 2.3e-9, a tenth of a token
     r.compare(r.run(), least=0.5, tol=3e-9)
+
+
+@pytest.mark.parametrize("vocab", [8192, 33000, 100277])
+def test_top_k_behind_min_p_in_flat_rows(vocab):
+    """min-p's border beyond the keys counted first, and top-k's further down, or beside it: a sample says which may come first."""
+    rng = np.random.default_rng(vocab + 1)
+    b = 16
+    bits = f2bf_array((rng.standard_normal(b * vocab) * 0.5).astype(np.float32)).reshape(b, vocab)
+    min_p = 0.1 + 0.1 * rng.random(b)
+    l = np.sort(bf2f_array(bits).reshape(b, vocab), axis=1)[:, ::-1]
+    left = (l >= l[:, :1] + np.log(min_p)[:, None]).sum(1)
+    assert (left > vocab // 20).all() and (left < vocab - 1500).all()
+    top_k = left + np.where(np.arange(b) % 2 == 0, 1500, [-40, -3, -1, 0, 1, 3, 40, 400] * (b // 8))
+    r = Rows(bits, None, top_k, None, min_p, rng.random(b))
+    # (as of other flat rows: 4e-6 n of the draws are too near)
+    r.compare(r.run(), least=0.3, tol=2e-6)
