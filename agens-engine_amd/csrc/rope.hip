@@ -66,13 +66,15 @@ __device__ __forceinline__ double2 turn(int pos, double f) {
   return make_double2(quarter == 1 || quarter == 2 ? -u : u, quarter & 2 ? -v : v);
 }
 
-// 64 bits -> 32 on the way to bf16: the last bit kept says whether anything was cut off, so the rounding that follows sees the
-// side of a border that the value is on.
+// 64 bits -> 32 on the way to bf16: the last of 15 bits kept says whether anything was cut off, so the rounding that follows sees the
+// side of a border that the value is on.  (15 and not 23: of a value between 2^-134, half of bf16's least, and 2^-126 fp32 still holds
+// as many.  The low word may stay: five zeros are between it and that bit.)
 __device__ __forceinline__ float narrow(double d) {
   const uint64_t u = (uint64_t)__double_as_longlong(d);
-  uint32_t lo = (uint32_t)u;
-  lo = (lo & 0xE0000000u) | ((lo & 0x1FFFFFFFu) ? 0x20000000u : 0u);
-  return (float)__longlong_as_double((long long)((u & 0xFFFFFFFF00000000ull) | lo));
+  const uint32_t lo = (uint32_t)u;
+  uint32_t hi = (uint32_t)(u >> 32);
+  hi = (hi & ~0x1Fu) | (((hi & 0x1Fu) | lo) ? 0x20u : 0u);
+  return (float)__longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 __device__ __forceinline__ uint32_t two_bf16(double x, double y) { return f2bf2(narrow(x), narrow(y)); }
 

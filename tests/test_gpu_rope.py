@@ -197,3 +197,20 @@ def test_queries_in_place_and_captured():
         g.launch()
         s.sync()
         assert np.array_equal(Y.get(np.uint16, 30 * 1024), want_q) and np.array_equal(D.get(np.uint8, a.pool.mem.size), want_pool)
+
+
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("rot", [64, 60])
+def test_results_below_the_normal_numbers_are_rounded_once(rot, interleaved):
+    """Products a little above, at and below the middles between bf16's numbers below 2^-126, which fp32 has not the bits to tell."""
+    rng = np.random.default_rng(9)
+    x = np.zeros((24, 4, 64), dtype=np.uint16)
+    x[:] = f2bf_array((rng.integers(1, 256, x.size) * 2.0 ** rng.integers(-18, 2, x.size)).astype(np.float32)).reshape(x.shape)
+    x |= (rng.random(x.shape) < 0.5).astype(np.uint16) << 15
+    f, _ = freqs64(1e4, rot)
+    for part in (1.0, 1 + 2.0 ** -23, 1 - 2.0 ** -24):
+        mag = np.float32(2.0 ** -125 * part)
+        for pos in (np.zeros(24, dtype=int), rng.integers(0, 1000, 24)):
+            got = rotate(x, pos, f, rot, interleaved, float(mag))
+            w = want(x, pos, f, rot, interleaved, mag, x)
+            assert np.array_equal(got, w), (part, (got != w).sum())
