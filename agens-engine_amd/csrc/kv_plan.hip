@@ -182,7 +182,11 @@ extern "C" int ak_kv_plan(int b, int m, const int* counts, const int* drop, cons
                         slots, refused, b, m, npages, __builtin_ctz((unsigned)page), ldt};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool one = m <= agq::kTokensInOne;
-  if (b <= 64 && (!one || m <= 4 * agq::kFewThreads))  // barriers of four waves, but fewer pages and tokens at a time
+  // Four waves: shorter barriers, but fewer pages and tokens at a time.  One sequence of 8192 new tokens, 512 pages, 5.5 us and 5.9 with
+  // sixteen; 16 of 4096, 16384 pages, 12.2 and 8.3; 64 of 8192, 32768 pages, 76 and 27.  How many pages come back nobody knows here: an
+  // eighth of what the rows can hold counts (64 rows of 1024 pages, some of them ended, 17 and 11 us), in steps of few tokens none.
+  const bool few = one ? m <= 4 * agq::kFewThreads : m / page + (drop ? (long)b * ldt / 8 : 0) <= 4 * agq::kFewThreads;
+  if (b <= 64 && few)
     hipLaunchKernelGGL(agq::plan_seqs_kernel<agq::kFewThreads>, dim3(1), dim3(agq::kFewThreads), 0, s, a, one ? 1 : 0);
   else
     hipLaunchKernelGGL(agq::plan_seqs_kernel<agq::kPlanThreads>, dim3(1), dim3(agq::kPlanThreads), 0, s, a, one ? 1 : 0);

@@ -198,3 +198,28 @@ def test_captured_steps_follow_the_device():
         s.sync()
         same(x.got(), w)
         x.cached, x.held, x.table, x.free, x.nfree = w["lens"], w["held"], w["table"], w["free"], w["nfree"][0]
+
+
+@pytest.mark.parametrize("drop", [False, True])
+@pytest.mark.parametrize("b,page,ldt,longest", [(1, 16, 700, 11000), (3, 16, 400, 6000), (20, 16, 90, 1400), (64, 32, 60, 1800),
+                                                (64, 16, 300, 4700), (5, 256, 100, 25000)])
+def test_few_sequences_with_long_prompts(b, page, ldt, longest, drop):
+    """More tokens than one launch writes, fewer pages than 1024 and more, and those that ended sequences give back."""
+    x = Batch(b + page, b, page, ldt, longest, drops=0.3 if drop else 0.0)
+    x.cached = np.where(np.arange(b) % 3 == 1, x.cached, x.cached % 50)
+    x.held = np.maximum(-(-x.cached // page), np.minimum(x.held, 5))
+    x.counts = np.random.default_rng(b).integers(longest // 2, longest, b)
+    x.counts = np.minimum(x.counts, ldt * page - x.cached)
+    ids = np.random.default_rng(page).permutation(x.b * ldt + 9)
+    x.npages, x.free, at = len(ids), np.full(len(ids), -1, dtype=np.int32), int(x.held.sum())
+    x.table = np.full((b, ldt), -1, dtype=np.int32)
+    x.table[np.arange(ldt)[None] < x.held[:, None]] = ids[:at]
+    x.nfree = len(ids) - at
+    x.free[:x.nfree] = ids[at:]
+    x.m = int(x.counts.sum()) + 3
+    assert x.m > 4096
+    x.device()
+    check(x.call(drop=drop))
+    w = x.want(drop=drop)
+    assert (w["nfree"][0] < x.nfree or drop) and not w["refused"].any()
+    same(x.got(), w)
