@@ -246,3 +246,13 @@ def test_memory_past_a_plan_of_other_sizes_stays(m, adapters, calls):
     check(step().ak_synchronize())
     assert np.array_equal(j.P.get(np.uint8, room), before)
     assert (j.Y[0].get(np.uint16, n * j.ldy[0]) == FILL).all()
+
+
+@pytest.mark.parametrize("m,adapters,used,rank,ns,in_place", [(4200, 4096, 3, 8, [700, 70], False), (4200, 4096, 3, 8, [700, 70], True),
+                                                              (2000, 2000, 2000, 8, [1300], False), (8192, 3, 3, 64, [5120], True),
+                                                              (300, 600, 40, 40, [2055, 1030], False)])
+def test_many_output_rows_of_a_workgroup(m, adapters, used, rank, ns, in_place):
+    """512 and 1024 output rows a workgroup, full tiles and tiles of a token, rows that end within a turn."""
+    ids = np.random.default_rng(m).integers(-1, used, m)
+    j = Job(50 + m, m, adapters, rank, 64, ns, ids=ids, in_place=in_place)
+    j.compare(j.run())

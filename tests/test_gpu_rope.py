@@ -214,3 +214,41 @@ def test_results_below_the_normal_numbers_are_rounded_once(rot, interleaved):
             got = rotate(x, pos, f, rot, interleaved, float(mag))
             w = want(x, pos, f, rot, interleaved, mag, x)
             assert np.array_equal(got, w), (part, (got != w).sum())
+
+
+# ------------------------------------------------------------------------------------------------ prompts
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("m,heads,dim,rot,interleaved", [(530, 48, 128, 128, 0), (530, 48, 128, 120, 0), (530, 48, 128, 64, 1),
+                                                         (517, 20, 256, 250, 0), (520, 40, 80, 80, 1), (8500, 6, 64, 64, 0),
+                                                         (9800, 5, 64, 36, 0), (8500, 6, 64, 64, 1)])
+def test_prompts(m, heads, dim, rot, interleaved, in_place):
+    """512 workgroups and more: each turns several times, the next heads' values on their way before these are stored."""
+    rng = np.random.default_rng(m + dim + rot)
+    x = rows(rng, m, heads, dim)
+    pos = rng.integers(-1, 1 << 20, m)
+    f, _ = freqs64(1e4, rot)
+    got = rotate(x, pos, f, rot, interleaved, 0.75, pad_in=8 * (heads % 3), pad_out=24, in_place=in_place)
+    assert np.array_equal(got, want(x, pos, f, rot, interleaved, np.float32(0.75), x if in_place else np.full_like(x, FILL)))
+
+
+PROMPTS = [(530, 40, 8, 128, 128, 0, 16), (530, 40, 8, 128, 128, 1, 64), (530, 40, 8, 128, 100, 0, 256), (520, 16, 4, 256, 256, 0, 32),
+           (3100, 9, 3, 64, 64, 0, 128), (1030, 30, 9, 64, 44, 0, 16)]
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("m,heads,kv,dim,rot,interleaved,page", PROMPTS)
+def test_prompts_into_the_cache(bits, m, heads, kv, dim, rot, interleaved, page):
+    test_into_the_cache_as_the_calls_apart(bits, m, heads, kv, dim, rot, interleaved, page)
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("m,heads,kv,dim,rot,interleaved,page", PROMPTS)
+def test_prompts_into_the_cache_with_queries_in_place(bits, m, heads, kv, dim, rot, interleaved, page):
+    a = Merged(m + bits, bits, m, heads, kv, dim, rot, interleaved, page, pad=8)
+    q, pool = a.apart()
+    X, D, w = Dev.of(a.x), Dev.of(a.pool.mem), heads * dim
+    check(a.fused(X, a.w, D, X=X))
+    check(step().ak_synchronize())
+    got = X.get(np.uint16, a.x.size).reshape(a.x.shape)
+    assert np.array_equal(got[:, :w], np.where((a.pos < 0)[:, None], a.x[:, :w], q.reshape(m, w)))
+    assert np.array_equal(got[:, w:], a.x[:, w:]) and np.array_equal(D.get(np.uint8, a.pool.mem.size), pool)
