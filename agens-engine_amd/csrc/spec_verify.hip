@@ -132,9 +132,9 @@ __device__ __forceinline__ RowStat chunk_stat(const Seq& s, const uint16_t* row,
   float l[kEach];
   load8(row, at0, vocab, l);
   load8(row, at1, vocab, l + 8);
-  float mine = l[0];
+  float mine = -INFINITY;  // (of quiet NaN: fmaxf loses what it has to a signalling one)
 #pragma unroll
-  for (int i = 1; i < kEach; ++i) mine = fmaxf(mine, l[i]);
+  for (int i = 0; i < kEach; ++i) mine = fmaxf(mine, __builtin_canonicalizef(l[i]));
   float top = wave_max(mine);
   __syncthreads();
   if ((t & 63) == 0) sh.red[t >> 6] = top;

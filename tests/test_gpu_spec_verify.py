@@ -221,3 +221,25 @@ def test_graph_replays():
 
 def test_no_sequences():
     assert ops().ak_spec_verify(None, 8, None, 8, None, None, None, None, 0, 0, 8, None, None, None, None) == 0
+
+
+@pytest.mark.parametrize("nan", [0x7F81, 0x7FBF, 0x7FC0, 0xFF81, 0xFFFF])
+@pytest.mark.parametrize("drafted", [False, True])
+def test_nan_of_any_bits_beside_the_largest(nan, drafted):
+    """NaN logits count as -inf, signalling ones too, before and behind the largest, in its eight and in others."""
+    rng = np.random.default_rng(21)
+    b, t, vocab = 16, 2, 9000
+    target = logits(rng, (b, t + 1, vocab), peaks=0)
+    draft = logits(rng, (b, t, vocab), peaks=0)
+    at = 4500 + np.arange(b)
+    for x in (target, draft):
+        x[np.arange(b)[:, None], :, at[:, None]] = f2bf_array(np.array([9.0], dtype=np.float32))[0]
+        for i in range(b):
+            x[i, :, [at[i] - 3, at[i] - 1, at[i] + 1, at[i] + 2]] = nan
+        x[:, :, 5::7] = np.where(x[:, :, 5::7] == f2bf_array(np.array([9.0], dtype=np.float32))[0], x[:, :, 5::7], nan)
+    ids = np.stack([at, at + 11], axis=1)
+    temp = np.where(np.arange(b) % 2 == 0, 0.0, 0.7)
+    u = rng.random((b, t + 1))
+    args = (target, draft if drafted else None, ids, None, u, temp, b, t)
+    with np.errstate(invalid="ignore"):
+        compare(run(*args[:6], b, t, vocab), *args, least=0.7)
