@@ -15,6 +15,8 @@
 // are 2.5 at 7 TB/s.  4001 tokens of 27648 inputs and 64 ranks: A x reads 193 MB of x in 56 us (3.4 TB/s) and the weights from L2 as
 // often; without the latter it takes 41, without x 33, and the two do not overlap fully behind one barrier a stage.  The second
 // product moves 82 MB of outputs in 24 us.
+#include <type_traits>
+
 #include "agens_kernels.h"
 #include "wq_common.h"
 
@@ -455,7 +457,8 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
   if constexpr (!JOINED) {
     const size_t step = (size_t)a.m * a.ranks;
     const int fours = a.rank / 4, all = 16 * ((t.count + 15) / 16) * fours;
-    auto some = [&]<int N>(int e0) {  // N times 4 ranks of a token
+    auto some = [&](auto times, int e0) {  // so many times 4 ranks of a token
+      constexpr int N = decltype(times)::value;
       const float* at[N];
       int to[N];
       f32x4 s[N] = {};
@@ -475,9 +478,9 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
     // four at a time where all their parts are on their way at once: 256 tokens of 64 ranks and 3 parts 11.8 -> 7.8 us (64 of 14 parts
     // would take 10 and not 8); up to 32 ranks that costs more in registers than it brings (5.9 -> 7.6)
     if (KS == 1 || all <= 256 || a.parts > kLoads / 4) {
-      for (int e0 = threadIdx.x; e0 < all; e0 += 256) some.template operator()<1>(e0);
+      for (int e0 = threadIdx.x; e0 < all; e0 += 256) some(std::integral_constant<int, 1>(), e0);
     } else if constexpr (KS > 1) {
-      for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) some.template operator()<4>(e0);
+      for (int e0 = threadIdx.x; e0 < all; e0 += 4 * 256) some(std::integral_constant<int, 4>(), e0);
     }
     __syncthreads();
   } else {
