@@ -5,16 +5,16 @@
 //   lora_down_few_kernel, lora_down_many_kernel   s = A x on MFMA (bf16, sums in fp32), a part for every kGroup chunks of kChunk
 //                      inputs: 16 tokens and ranks a workgroup, or a tile and up to 64 ranks with the weights through LDS;
 //   lora_join_kernel   the parts' sums, where there are many tokens and parts; otherwise
-//   lora_up_kernel     adds the parts up, and y = y0 + scale (B s): s enters the MFMA as three bf16 operands, which hold all 24 bits
-//                      of it (one alone would move y by 2^-9 of what is added, two by 2^-17).
+//   lora_up_kernel     adds the parts up, and y = y0 + scale (B s): s enters the MFMA as three bf16 operands, which hold all 24
+//                      bits of it (one alone would move y by 2^-9 of what is added, two by 2^-17).
 // A chunk's products are one chain of MFMA, the chunks' sums are added up by fours and then from left to right, whoever does it: a
 // token's bits do not depend on the other tokens of the call.
 //
-// What bounds them.  One token of 5120 inputs, 16 ranks and 5120 outputs: three chains of loads that wait for one another (tile,
-// token, row), 2.9 + 4.6 + 5.4 us.  64 tokens of 24 adapters beside q, k and v: the same, 2.9 + 7.5 + 5.5, where the weights' 17 MB
-// are 2.5 at 7 TB/s.  4001 tokens of 27648 inputs and 64 ranks: A x reads 193 MB of x in 56 us (3.4 TB/s) and the weights from L2 as
-// often; without the latter it takes 41, without x 33, and the two do not overlap fully behind one barrier a stage.  The second
-// product moves 82 MB of outputs in 24 us.
+// What bounds them.  One token of 5120 inputs, 16 ranks and 5120 outputs: three chains of loads that wait for one another (head and
+// tile, token, row), 2.8 + 4.6 + 4.9 us.  64 tokens of 24 adapters beside q, k and v: the same, 2.8 + 7.3 + 6.2, where the weights'
+// 16 MB are 2.3 at 7 TB/s.  4001 tokens of 27648 inputs and 64 ranks: A x reads 193 MB of x in 57 us (3.4 TB/s) and the weights from
+// L2 as often; without the latter it takes 41, without x 33, and the two do not overlap fully behind one barrier a stage.  The second
+// product moves 82 MB of outputs in 28 us (24 with two bf16 of a sum and not three).
 #include <type_traits>
 
 #include "agens_kernels.h"
@@ -475,8 +475,8 @@ __global__ void __launch_bounds__(256) lora_up_kernel(const LoraArgs a) {
         split(s[j], sv + to[j], kTile * stride);
       }
     };
-    // four at a time where all their parts are on their way at once: 256 tokens of 64 ranks and 3 parts 11.8 -> 7.8 us (64 of 14 parts
-    // would take 10 and not 8); up to 32 ranks that costs more in registers than it brings (5.9 -> 7.6)
+    // four at a time where all their parts are on their way at once: 256 tokens of 64 ranks and 3 parts 11.8 -> 7.8 us (64 of 14
+    // parts would take 10 and not 8); up to 32 ranks that costs more in registers than it brings (5.9 -> 7.6).  (Of sums in two bf16.)
     if (KS == 1 || all <= 256 || a.parts > kLoads / 4) {
       for (int e0 = threadIdx.x; e0 < all; e0 += 256) some(std::integral_constant<int, 1>(), e0);
     } else if constexpr (KS > 1) {
@@ -592,10 +592,13 @@ extern "C" int ak_lora_add(void* plan, const void* x, int m, long ldx, int k, in
   else
     agq::down_many<4>(l, tiles, s);
   if (const int e = (int)hipGetLastError()) return e;
-  // A launch more, but parts that are read once and not by every workgroup of outputs.  The two kernels against the one: 4001 tokens
-  // of 27648 inputs and 64 ranks (14 parts) 29 us and 46, 4096 of 5120 and 48 (3 parts) 25 and 28; 2048 of these 17.4 and 18, less
-  // than the launch; 1100 of 5120 and 128 18.7 and 17.6; up to 32 ranks, whose parts are few loads, 28 and 29 at 4096 of 27648.
-  if (many && rank > 32 && l.parts > 1 && (long)m * l.parts * rank >= 500000) {
+  // A launch more, but parts that are read once and not by every workgroup of outputs.  The two kernels against the one, to 5120
+  // outputs: 4001 tokens of 27648 inputs and 64 ranks (14 parts) 34 us and 48, 1024 of these 16.3 and 17.6, 4000 of 9224 and 64 (5
+  // parts) 33 and 45, 1500 of these 17.2 and 18.2.  Few parts are on their way at once and cost less: 3000 tokens of 5120 inputs and
+  // 64 ranks (3 parts) 29 and 25, 4096 33 and 34.5, with 128 ranks 45 and 48; 1100 with 128 22 and 19.  Up to 32 ranks the parts are
+  // few loads: 28 and 29 at 4096 of 27648.
+  const long joined = l.parts > agq::kLoads / 4 ? 500000 : 700000;
+  if (many && rank > 32 && l.parts > 1 && (long)m * l.parts * rank >= joined) {
     l.sums = agq::view(plan, m, adapters).parts + (size_t)l.parts * m * l.ranks;
     hipLaunchKernelGGL(agq::lora_join_kernel, dim3((unsigned)(((size_t)m * l.ranks / 4 - 1) / 256 + 1)), dim3(256), 0, s, l);
     if (const int e = (int)hipGetLastError()) return e;

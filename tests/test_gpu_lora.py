@@ -202,7 +202,7 @@ def test_two_streams_with_plans_of_their_own():
 
 
 @pytest.mark.parametrize("m,rank,k", [(1, 16, 64), (3, 16, 5120), (70, 8, 1024), (700, 32, 9224), (700, 64, 9224), (1800, 64, 9000),
-                                      (1800, 72, 9000)])
+                                      (1800, 72, 9000), (3700, 64, 5120)])
 def test_sums_enter_the_second_product_with_24_bits(m, rank, k):
     """A sum s = p0 + p1 + p2 of three bf16, from which the second product takes p1 and the base takes p0: p2 is left, which lies
     below the 16 bits of two bf16.  All of it is exact in fp32 but for the last sums' order: four roundings of s at most."""
