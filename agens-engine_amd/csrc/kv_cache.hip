@@ -1,6 +1,7 @@
 // Writing keys and values into the pages of the cache, and reading them back (kv_page.h has the layout).
 //
-// kv_codes.h has the codes.  Quantisation of a row x of dim values (one token, one head, keys or values), Q = 127 (8 bits) or 7 (4 bits):
+// Quantisation of a row x of dim values (one token, one head, keys or values), Q = 127 (8 bits) or 7 (4 bits; kv_codes.h has
+// the code):
 //   s = bf16(max|x| / Q), q = rint(x / s) clamped to +-Q, the value held is q * s.
 // The codes are those of the rounded scale that readers multiply with, so the rounding of s costs no accuracy beyond the
 // clamped end (x / s <= Q (1 + 2^-9), less than half a step).  The codes are those of exact arithmetic: two bf16's quotient is

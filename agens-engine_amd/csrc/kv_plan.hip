@@ -5,9 +5,10 @@
 // the first that goes short leaves all later ones without new pages too.  Pages move as one flat list each way, a thread a
 // page, which finds its sequence by bisecting the sums.  So do tokens.
 //
-// All of it is a chain of round trips to memory and barriers: 2.1 us for one sequence, 7.2 and 3.7 for 200 with 20000 new tokens,
-// whose 0.2 MB are nothing.  Few sequences take four waves instead of sixteen, whose barriers are shorter.  Inputs and outputs may be
-// the same arrays: every thread has read its sequence's numbers before the first barrier, and nothing is written before it.
+// All of it is a chain of round trips to memory and barriers: 2.2 us for one sequence, 7.3 and 3.4 for 200 with 20000 new tokens,
+// whose 0.2 MB are nothing.  Few sequences with few pages take four waves instead of sixteen, whose barriers are shorter.  Inputs and
+// outputs may be the same arrays: every thread has read its sequence's numbers before the first barrier, and nothing is written
+// before it.
 #include "agens_kernels.h"
 #include "kv_page.h"
 #include "logits.h"
@@ -182,9 +183,10 @@ extern "C" int ak_kv_plan(int b, int m, const int* counts, const int* drop, cons
                         slots, refused, b, m, npages, __builtin_ctz((unsigned)page), ldt};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool one = m <= agq::kTokensInOne;
-  // Four waves: shorter barriers, but fewer pages and tokens at a time.  One sequence of 8192 new tokens, 512 pages, 5.5 us and 5.9 with
-  // sixteen; 16 of 4096, 16384 pages, 12.2 and 8.3; 64 of 8192, 32768 pages, 76 and 27.  How many pages come back nobody knows here: an
-  // eighth of what the rows can hold counts (64 rows of 1024 pages, some of them ended, 17 and 11 us), in steps of few tokens none.
+  // Four waves: shorter barriers, but fewer pages and tokens at a time.  One sequence of 8192 new tokens, 512 pages, 5.5 us and
+  // 5.9 with sixteen; 16 of 4096, 4096 pages, 12.2 and 8.3; 64 of 8192, 32768 pages, 76 and 27.  How many pages come back nobody
+  // knows here: an eighth of what the rows can hold counts (64 rows of 1024 pages, some of them ended, 17 and 11 us), in steps of
+  // few tokens none.
   const bool few = one ? m <= 4 * agq::kFewThreads : m / page + (drop ? (long)b * ldt / 8 : 0) <= 4 * agq::kFewThreads;
   if (b <= 64 && few)
     hipLaunchKernelGGL(agq::plan_seqs_kernel<agq::kFewThreads>, dim3(1), dim3(agq::kFewThreads), 0, s, a, one ? 1 : 0);

@@ -13,8 +13,8 @@
 // lane has its pairs' other halves from the lane that loaded them (where rot is no multiple of 16, it loads them itself).  A head
 // stays within one wave's instructions, so that rotating in place is safe: all of its loads come before its stores.
 //
-// Memory bounds long batches: 8191 tokens of 48 heads of 128 (201 MB) 40.5 us, 5.0 TB/s, as fast as a copy; 8192 tokens of 40 + 16
-// heads into pages (235 MB) 51 us, 4.6 TB/s.  One token, 2.9 us, waits for one load after another.
+// Memory bounds long batches: 8191 tokens of 48 heads of 128, half of each, neighbours paired (201 MB) 40 us, 5.0 TB/s, as fast as a
+// copy; 8192 tokens of 40 + 16 heads into pages (235 MB) 52 us, 4.5 TB/s.  One token, 2.8 us, waits for one load after another.
 #include <math.h>
 
 #include "agens_kernels.h"
@@ -66,9 +66,9 @@ __device__ __forceinline__ double2 turn(int pos, double f) {
   return make_double2(quarter == 1 || quarter == 2 ? -u : u, quarter & 2 ? -v : v);
 }
 
-// 64 bits -> 32 on the way to bf16: the last of 15 bits kept says whether anything was cut off, so the rounding that follows sees the
-// side of a border that the value is on.  (15 and not 23: of a value between 2^-134, half of bf16's least, and 2^-126 fp32 still holds
-// as many.  The low word may stay: five zeros are between it and that bit.)
+// 64 bits -> 32 on the way to bf16: the last of 15 bits kept says whether anything was cut off, so the rounding that follows sees
+// the side of a border that the value is on.  (15 and not 23: of a value between 2^-134, half of bf16's least, and 2^-126 fp32
+// still holds as many.  The low word may stay: five zeros are between it and that bit.)
 __device__ __forceinline__ float narrow(double d) {
   const uint64_t u = (uint64_t)__double_as_longlong(d);
   const uint32_t lo = (uint32_t)u;

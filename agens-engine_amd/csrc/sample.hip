@@ -24,7 +24,8 @@
 // What bounds them: latency, of loads, barriers and one wave's instructions one after another (1 row of 152064: 3.7 us, and then 4.2
 // without a filter, 8.6 with one, of which 1.4 the first loads, 1.3 the windows, 1.1 the border, 1.4 the chunks' shares and 2 the
 // draw; 32 rows: 5.8 + 11 us, where 9.7 MB at 7 TB/s are 1.4); and instructions where a border is far down: 25 a logit by one
-// workgroup, 1 row of 152064 50 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 of 100277 63 us and 87.
+// workgroup, 1 row of 152064 with top-k 50000 52 us where counting all keys in LDS takes 88 (40 cycles for 64 counts), 250 flat rows
+// of 100277 63 us and 87 (59 with settings of which a part reaches so far down).
 #include "agens_kernels.h"
 #include "logits.h"
 

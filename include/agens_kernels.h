@@ -310,9 +310,10 @@ int ak_spec_verify(const void* target, long ldt, const void* draft, long ldd, co
  * list, and these tokens' ranges, positions and slots.  Sequence i has cached[i] tokens in the cache, held[i] pages in
  * table[i * ldt ...], and counts[i] new tokens; drop[i] (drop may be NULL) other than 0: it has ended, its pages go to the end of
  * the free list, in order, and the row begins anew with counts[i] tokens.  Missing pages come off the end of the list, in the
- * order of the sequences.  A sequence that does not fit its ldt pages (or 2^31 - 1 tokens), or whose range passes m, is refused, as is one whose
- * pages are not all there, and then every later one that wants any; it keeps what it had.  free_pages [npages] with
- * free_count[0] pages in it; NULL: the table's pages are taken as they are (held, held_out, free_count, free_out unused).
+ * order of the sequences.  A sequence that does not fit its ldt pages (or 2^31 - 1 tokens), or whose range passes m, is
+ * refused, as is one whose pages are not all there, and then every later one that wants any; it keeps what it had.
+ * free_pages [npages] with free_count[0] pages in it; NULL: the table's pages are taken as they are (held, held_out, free_count,
+ * free_out unused).
  *   lens [b]       cached and new tokens (refused: cached);       held_out [b], free_out [1]   as held and free_count, after;
  *   qstart [b + 1] the ranges of the new tokens, side by side (ak_paged_attn's; at most m);       refused [b]  0 or 1;
  *   pos [m], slots [m]   position of each token, and its slot (ak_kv_write's); -1 past the last and for refused sequences, and
@@ -340,7 +341,9 @@ int ak_kv_plan(int b, int m, const int* counts, const int* drop, const int* cach
  *   ak_rope_freqs      host memory, no device: freqs[j] = theta^(-2j / rot) and *mag = 1, for contexts `factor` times the
  *             trained one: LINEAR divides all by factor; BASE takes theta * factor^(rot / (rot - 2)); BANDS divides those that
  *             make fewer than `slow` turns in `trained` tokens, leaves those of more than `fast`, mixes those between in
- *             proportion, and gives *mag = 0.1 ln factor + 1. */
+ *             proportion to their turns, and gives *mag = 0.1 ln factor + 1.  (A model whose bands go without a factor takes
+ *             these frequencies and a mag of 1.  One whose mix goes by a pair's place between the bands' ends, not by its turns,
+ *             has its own rule for freqs: ak_rope takes any.) */
 #define AK_ROPE_PLAIN 0
 #define AK_ROPE_LINEAR 1
 #define AK_ROPE_BASE 2
@@ -358,13 +361,14 @@ int ak_rope_kv_write(int bits, const void* q, long ldq, const void* k, long ldk,
  * falling logit, the lower token first among equal ones: top_k keeps the first top_k; top_p the fewest of these, from the front,
  * whose p reach top_p of the sum of theirs (one at least); min_p drops those with p below min_p times the largest.  The token is
  * the first, in order of tokens, at which the cumulative p of those kept passes u times their sum.  temperature [b] (NULL: 1; 0
- * or less: greedy, the largest logit; below 2^-126 and above 1.44e30 it counts as these), top_k [b] (NULL, or 0 or less, or vocab and more: off), top_p [b]
- * (NULL, or 1 and more: off), min_p [b] (NULL, or 0 and less: off), u [b] uniform in [0, 1), all in device memory.
+ * or less: greedy, the largest logit; below 2^-126 and above 1.44e30 it counts as these), top_k [b] (NULL, or 0 or less, or
+ * vocab and more: off), top_p [b] (NULL, or 1 and more: off), min_p [b] (NULL, or 0 and less: off), u [b] uniform in [0, 1), all
+ * in device memory.
  * logp (may be NULL): log p of the token before any filter (greedy: at temperature 1).  NaN logits count as -inf; a row of
  * nothing else gives the token -1 and logp 0.  Without filters the tokens are ak_spec_verify's with t = 0, but for roundings.
- * Weights are fp32; sums of what filters keep count whole 2^-40 of the largest weight, so a token below that is not drawn where a filter is on.
- * Rows need no alignment beyond bf16's.  Library scratch (above; inside a capture the graph's own): 1040 bytes for each 4096
- * logits, 64 MB at most; without it one workgroup takes a row, with the same tokens. */
+ * Weights are fp32; sums of what filters keep count whole 2^-40 of the largest weight, and a token below that is not drawn where
+ * a filter is on.  Rows need no alignment beyond bf16's.  Library scratch (above; inside a capture the graph's own): 1040 bytes
+ * for each 4096 logits, 64 MB at most; without it one workgroup takes a row, with the same tokens. */
 #define AK_SAMPLE_MAX_VOCAB 1048576
 int ak_sample(const void* logits, long ld, const float* temperature, const int* top_k, const float* top_p,
               const float* min_p, const float* u, int b, int vocab, int* tokens, float* logp, void* stream);
@@ -381,7 +385,8 @@ int ak_sample(const void* logits, long ld, const float* temperature, const int* 
  * ak_lora_plan groups the tokens by adapter, once for all linears of a step, into `plan`: 16-byte aligned device memory of
  * ak_lora_plan_bytes(m, adapters, nseg * rank, k) bytes, the most over these linears (0: refused).  It also holds what
  * ak_lora_add's launches hand on, so calls with one plan must follow one another; ak_lora_add with other m or adapters than
- * the plan's leaves y alone, and reads and writes nothing of the plan's memory but its first 16 bytes.  Only launches, allocates nothing, can be captured. */
+ * the plan's leaves y and the plan alone, whatever the plan's length: it reads the first 16 bytes.  Only launches, allocates
+ * nothing, can be captured. */
 #define AK_LORA_MAX_RANK 128
 #define AK_LORA_MAX_ADAPTERS 4096
 #define AK_LORA_MAX_TOKENS 1048576
