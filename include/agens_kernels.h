@@ -381,7 +381,8 @@ int ak_sample(const void* logits, long ld, const float* temperature, const int* 
  * stride ldx (a multiple of 8); a, b[i] and x 16-byte aligned; y[i] and base[i] bf16 of row stride ldy[i] (0, or ldy NULL:
  * n[i]).  base (the linear's outputs) NULL, or base[i] the same as y[i]: added in place; they may overlap in no other way.
  * scale [adapters] fp32 in device memory (NULL: 1).  Sums are fp32, A x among them, y is rounded once to bf16; a
- * token's bits do not depend on the other tokens.
+ * token's bits do not depend on the other tokens.  Infinities and NaN of x and a act as in fp32; an infinite value of b gives its
+ * output NaN or an infinity, which of them is not told.
  * ak_lora_plan groups the tokens by adapter, once for all linears of a step, into `plan`: 16-byte aligned device memory of
  * ak_lora_plan_bytes(m, adapters, nseg * rank, k) bytes, the most over these linears (0: refused).  It also holds what
  * ak_lora_add's launches hand on, so calls with one plan must follow one another; ak_lora_add with other m or adapters than

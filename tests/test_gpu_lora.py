@@ -256,3 +256,16 @@ def test_many_output_rows_of_a_workgroup(m, adapters, used, rank, ns, in_place):
     ids = np.random.default_rng(m).integers(-1, used, m)
     j = Job(50 + m, m, adapters, rank, 64, ns, ids=ids, in_place=in_place)
     j.compare(j.run())
+
+
+@pytest.mark.parametrize("m", [40, 1800])
+def test_infinite_weights_of_the_second_product_stay_in_their_output(m):
+    j = Job(60, m, 2, 64, 9000, [70], ids=np.arange(m) % 2)
+    want = j.run()[0]
+    b = j.b[0].copy()
+    b[1, 33, 5], b[1, 64, 9] = 0x7F80, 0xFF80
+    j.B = [Dev.of(b)]
+    y = j.run()[0]
+    bad = np.zeros(y.shape, dtype=bool)
+    bad[1::2, [33, 64]] = True
+    assert np.array_equal(y[~bad], want[~bad]) and not np.isfinite(bf2f_array(y[bad])).any()
